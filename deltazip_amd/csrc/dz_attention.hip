@@ -1,0 +1,468 @@
+// Attention of one new token per row over a paged key/value cache.
+//
+//   o = sum_t 2^(s_t - m) v_t / sum_t 2^(s_t - m),   s_t = scale log2(e) q.k_t,   max(0, n - window) <= t < n
+//
+// for every row (a sequence with its length n and its table of pages) and head; the heads / kv_heads heads that
+// share a key head are taken together, up to 16 at once, so that every key and value is read once.  What bounds it
+// is the reading of keys and values: 4 flops per byte and head against the 300 that the card has.
+//
+// A wavefront walks 32 tokens at a time and holds all of it in registers:
+//   scores   C[token, head] = K[token, dim] Q[dim, head] on v_mfma_f32_16x16x32, two tiles of 16 tokens: lane l has
+//            head l % 16 and tokens 4 (l / 16) + i of each tile
+//   weights  those 8 values are just what the second product's operand wants of lane l if its k index 8 (l / 16) + e
+//            stands for token 4 (l / 16) + e % 4 of tile e / 4: nothing crosses lanes but the maximum
+//   values   C[dim, head] += V^T[dim, token] P[token, head]: a lane loads 8 dims (16 bytes) of its 8 tokens and
+//            turns the 8 x 8 block with 32 byte permutes; row r of product j stands for dim 8 r + j, so rows are
+//            read whole
+// The unused columns of the matrix instructions cost nothing: they are under a tenth of the time at one head per key.
+//
+// The running maximum moves only where a score is more than twice above it (in 2^s): weights are held times 2^14
+// (fp16) so that they use the type's range, at most 2^15, and are split in two values of the type, high and low: a
+// weight then has 16 (bf16) or 22 (fp16) bits, and the output's error is its own rounding.  Sums are fp32.
+//
+// The work is cut on the device, which alone knows the lengths: every wavefront reads the lengths of the launch's
+// rows (up to 256, four a lane), and takes for the tiles of a workgroup as many as make about `target` workgroups.
+// Parts of a row are joined by a second kernel in the order of the tokens, so results do not depend on timing.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <atomic>
+
+#include "../../include/dz_amd.h"
+#include "dz_device.h"
+
+namespace {
+
+typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
+
+constexpr int WAVES = 4;               // wavefronts of a workgroup
+constexpr int TILE = 32;               // tokens of a step
+constexpr int HEADS = 16;              // heads taken together: columns of a matrix instruction
+constexpr int GROUP_ROWS = 256;        // rows of a launch: four lengths a lane
+constexpr int TARGET = 1024;           // workgroups that the work is cut into, rows' last parts apart
+
+struct AttnParams {
+  const char *q, *k, *v;
+  const int *tables, *lengths;
+  uint16_t* out;
+  float* parts;
+  unsigned* status;
+  long long q_row, q_head, k_page, k_head, k_token, v_page, v_head, v_token, out_row, out_head, table_row;   // bytes; out, table: elements
+  unsigned num_pages;
+  int rows, heads, kv_heads, share, head_tiles, dim, shift, pages_per_row, window, part_floats;
+  float scale;
+};
+
+template <bool BF>
+struct Type;
+template <>
+struct Type<false> {
+  typedef h8_t v8;
+  static constexpr float BIAS = 14.0f;
+  static __device__ __forceinline__ f4_t mma(v8 a, v8 b, f4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+  static __device__ __forceinline__ uint16_t round(float x) { return __builtin_bit_cast(uint16_t, (_Float16)x); }
+  static __device__ __forceinline__ _Float16 one(float x) { return (_Float16)x; }
+};
+template <>
+struct Type<true> {
+  typedef b8_t v8;
+  static constexpr float BIAS = 0.0f;
+  static __device__ __forceinline__ f4_t mma(v8 a, v8 b, f4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+  static __device__ __forceinline__ uint16_t round(float x) { return __builtin_bit_cast(uint16_t, (__bf16)x); }
+  static __device__ __forceinline__ __bf16 one(float x) { return (__bf16)x; }
+};
+
+// Tokens [first, end) of a row, end <= the table's room.
+__device__ __forceinline__ void span(const AttnParams& P, int length, int& first, int& end) {
+  const int room = P.pages_per_row << P.shift;
+  end = length < 0 ? 0 : length > room ? room : length;
+  first = P.window > 0 && end > P.window ? end - P.window : 0;
+}
+
+__device__ __forceinline__ int tiles_of(const AttnParams& P, int length) {
+  int first, end;
+  span(P, length, first, end);
+  return end > first ? (end + TILE - 1) / TILE - first / TILE : 0;
+}
+
+// The parts of the launch's rows, as every wavefront works them out for itself.  Lane l has rows 4 l .. 4 l + 3.
+struct Plan {
+  int tiles[4], before[4];             // tiles of a row; parts of the rows in front of it
+  int each;                            // most tiles of a part
+  __device__ __forceinline__ int parts(int r) const { return tiles[r] ? (tiles[r] + each - 1) / each : 1; }   // (an empty row has its zeros written)
+};
+
+__device__ __forceinline__ Plan make_plan(const AttnParams& P, int lane) {
+  Plan p;
+  int mine = 0;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int row = 4 * lane + r;
+    p.tiles[r] = row < P.rows ? tiles_of(P, P.lengths[row]) : 0;
+    mine += p.tiles[r];
+  }
+  long long total = mine;
+#pragma unroll
+  for (int d = 32; d; d >>= 1) total += __shfl_xor(total, d);
+  const long long items = (long long)P.kv_heads * P.head_tiles;
+  long long each = (total * items + TARGET - 1) / TARGET;
+  each = (each + WAVES - 1) / WAVES * WAVES;
+  p.each = each < WAVES ? WAVES : (int)each;
+  int sum = 0;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    p.before[r] = sum;
+    sum += 4 * lane + r < P.rows ? p.parts(r) : 0;
+  }
+  int upto = sum;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int o = __shfl_up(upto, d);
+    if (lane >= d) upto += o;
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r) p.before[r] += upto - sum;
+  return p;
+}
+
+template <int KC, bool BF>
+__global__ __launch_bounds__(64 * WAVES) void dz_attention_kernel(const AttnParams P) {
+  typedef Type<BF> Ty;
+  typedef typename Ty::v8 v8;
+  constexpr int NB = (KC + 3) / 4;     // blocks of 128 dims
+  extern __shared__ float lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
+  const int items = P.kv_heads * P.head_tiles;
+  const int part = blockIdx.x / items, item = blockIdx.x % items;
+  const int kvh = item / P.head_tiles, head0 = kvh * P.share + item % P.head_tiles * HEADS;
+  const int nheads = min(HEADS, (kvh + 1) * P.share - head0);
+
+  // the row whose part this is
+  const Plan plan = make_plan(P, lane);
+  int row = -1, nth = 0, nparts = 0;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int n = plan.parts(r), at = part - plan.before[r];
+    const unsigned long long hit = __ballot(4 * lane + r < P.rows && at >= 0 && at < n);
+    if (hit) {
+      const int src = __builtin_ctzll(hit);
+      row = 4 * src + r;
+      nth = __builtin_amdgcn_readlane(at, src);
+      nparts = __builtin_amdgcn_readlane(n, src);
+    }
+  }
+  if (row < 0) return;
+  const int length = P.lengths[row];
+  int first, end;
+  span(P, length, first, end);
+  if (length > end && nth == 0 && item == 0 && threadIdx.x == 0) atomicOr(P.status, 4u);
+  const int tiles = end > first ? (end + TILE - 1) / TILE - first / TILE : 0, tile0 = first / TILE;
+  // this part's tiles, and this wavefront's of them
+  const int lo = (int)((long long)tiles * nth / nparts), hi = (int)((long long)tiles * (nth + 1) / nparts);
+  int t0 = tile0 + lo + (hi - lo) * wave / WAVES;
+  const int t1 = tile0 + lo + (hi - lo) * (wave + 1) / WAVES;
+
+  // queries: lane holds dims 32 c + 8 g .. + 7 of head `col`
+  v8 q[KC];
+#pragma unroll
+  for (int c = 0; c < KC; ++c) {
+    u4_t w = {0, 0, 0, 0};
+    if (col < nheads && 32 * c + 8 * g < P.dim)
+      w = *(const u4_t*)(P.q + row * P.q_row + (head0 + col) * P.q_head + (32 * c + 8 * g) * 2);
+    q[c] = __builtin_bit_cast(v8, w);
+  }
+
+  f4_t acc[8 * NB];
+#pragma unroll
+  for (int j = 0; j < 8 * NB; ++j) acc[j] = f4_t{0, 0, 0, 0};
+  float top = -INFINITY, sum = 0.0f;   // of head `col`: the reference maximum, this lane's share of the sum
+
+  const int* table = P.tables + row * P.table_row;
+  const int last_page = (end - 1) >> P.shift;
+  int page0 = t0 * TILE >> P.shift;    // of the 64 page numbers that the lanes hold
+  auto fetch = [&](int base) {
+    const int at = base + lane;
+    unsigned id = at <= last_page && at >= first >> P.shift ? (unsigned)table[at] : 0u;
+    if (id >= P.num_pages) {
+      atomicOr(P.status, 4u);
+      id = 0;
+    }
+    return id;
+  };
+  unsigned ids = 0, next_ids = 0;
+  if (t0 < t1) {
+    ids = fetch(page0);
+    next_ids = fetch(page0 + 64);
+  }
+  const int in_page = (1 << P.shift) - 1;
+
+  for (; t0 < t1; ++t0) {
+    const int tok = t0 * TILE;
+    const bool edge = tok < first || tok + TILE > end;
+    if (((tok + TILE - 1) >> P.shift) >= page0 + 64) {     // (pages hold 8 tokens or more: a tile has 4 pages at most)
+      const int base = tok >> P.shift;
+      ids = base == page0 + 64 ? next_ids : fetch(base);
+      page0 = base;
+      next_ids = fetch(page0 + 64);
+    }
+    u4_t kw[2][KC], vw[NB][8];
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      int t = tok + 16 * a + col;
+      t = max(first, min(t, end - 1));
+      const unsigned id = __shfl(ids, (t >> P.shift) - page0);
+      const char* at = P.k + id * P.k_page + kvh * P.k_head + (t & in_page) * P.k_token + 16 * g;
+#pragma unroll
+      for (int c = 0; c < KC; ++c) {
+        kw[a][c] = u4_t{0, 0, 0, 0};
+        if (32 * c + 8 * g < P.dim) kw[a][c] = *(const u4_t*)(at + 64 * c);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      int t = tok + 16 * (e >> 2) + 4 * g + (e & 3);
+      const bool out = t < first || t >= end;
+      t = max(first, min(t, end - 1));
+      const unsigned id = __shfl(ids, (t >> P.shift) - page0);
+      const char* at = P.v + id * P.v_page + kvh * P.v_head + (t & in_page) * P.v_token + 16 * col;
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        vw[b][e] = u4_t{0, 0, 0, 0};       // (what is masked may be anything: it has no part in the product)
+        if (!out && 128 * b + 8 * col < P.dim) vw[b][e] = *(const u4_t*)(at + 256 * b);
+      }
+    }
+    float s[8];
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      f4_t c4 = {0, 0, 0, 0};
+#pragma unroll
+      for (int c = 0; c < KC; ++c) c4 = Ty::mma(__builtin_bit_cast(v8, kw[a][c]), q[c], c4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[4 * a + i] = c4[i] * P.scale;
+    }
+    if (edge) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int t = tok + 16 * (e >> 2) + 4 * g + (e & 3);
+        if (t < first || t >= end) s[e] = -INFINITY;
+      }
+    }
+    float most = s[0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) most = fmaxf(most, s[e]);
+    most = fmaxf(most, __shfl_xor(most, 16));
+    most = fmaxf(most, __shfl_xor(most, 32));
+    if (__any(most > top + 1.0f)) {
+      const float up = fmaxf(most, top);
+      const float f = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - up);
+      top = up;
+      sum *= f;
+#pragma unroll
+      for (int j = 0; j < 8 * NB; ++j) acc[j] *= f;
+    }
+    const float ref = top == -INFINITY ? 0.0f : top - Ty::BIAS;
+    v8 ph, pl;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float p = __builtin_amdgcn_exp2f(s[e] - ref);
+      sum += p;
+      ph[e] = Ty::one(p);
+      pl[e] = Ty::one(p - (float)ph[e]);
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const unsigned sel = j & 1 ? 0x07060302u : 0x05040100u;
+        u4_t w;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) w[x] = __builtin_amdgcn_perm(vw[b][2 * x + 1][j >> 1], vw[b][2 * x][j >> 1], sel);
+        const v8 vt = __builtin_bit_cast(v8, w);
+        acc[8 * b + j] = Ty::mma(vt, pl, Ty::mma(vt, ph, acc[8 * b + j]));
+      }
+  }
+  sum += __shfl_xor(sum, 16);
+  sum += __shfl_xor(sum, 32);
+
+  // the four wavefronts' sums joined: [wave][head][dim], then maxima and sums
+  const int ld = P.dim + 4;
+  float* mine = lds + wave * nheads * ld;
+  float* stat = lds + WAVES * nheads * ld;
+  if (col < nheads) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int d = 128 * b + 8 * (4 * g + i);
+        if (d < P.dim) {
+          *(f4_t*)(mine + col * ld + d) = f4_t{acc[8 * b][i], acc[8 * b + 1][i], acc[8 * b + 2][i], acc[8 * b + 3][i]};
+          *(f4_t*)(mine + col * ld + d + 4) = f4_t{acc[8 * b + 4][i], acc[8 * b + 5][i], acc[8 * b + 6][i], acc[8 * b + 7][i]};
+        }
+      }
+    if (g == 0) {
+      stat[(wave * HEADS + col) * 2] = top;
+      stat[(wave * HEADS + col) * 2 + 1] = sum;
+    }
+  }
+  __syncthreads();
+  float* to = nparts > 1 ? P.parts + (size_t)blockIdx.x * P.part_floats : nullptr;
+  for (int x = threadIdx.x; x < nheads * (P.dim / 4); x += 64 * WAVES) {
+    const int h = x / (P.dim / 4), d = x % (P.dim / 4) * 4;
+    float m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) m = fmaxf(m, stat[(w * HEADS + h) * 2]);
+    float l = 0.0f;
+    f4_t o = {0, 0, 0, 0};
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      const float lw = stat[(w * HEADS + h) * 2 + 1], mw = stat[(w * HEADS + h) * 2];
+      const float f = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw - m);
+      l += mw == -INFINITY ? 0.0f : lw * f;
+      o += mw == -INFINITY ? f4_t{0, 0, 0, 0} : *(const f4_t*)(lds + (w * nheads + h) * ld + d) * f;
+    }
+    if (to) {
+      *(f4_t*)(to + h * P.dim + d) = o;
+      if (d == 0) {
+        to[nheads * P.dim + 2 * h] = m;
+        to[nheads * P.dim + 2 * h + 1] = l;
+      }
+    } else {
+      const f4_t y = tiles ? o / l : f4_t{0, 0, 0, 0};
+      uint16_t* at = P.out + row * P.out_row + (head0 + h) * P.out_head + d;
+      const u2_t w = {(unsigned)Ty::round(y[0]) | (unsigned)Ty::round(y[1]) << 16,
+                      (unsigned)Ty::round(y[2]) | (unsigned)Ty::round(y[3]) << 16};
+      *(u2_t*)at = w;
+    }
+  }
+}
+
+// Joins the parts of a row's heads, in the order of the tokens.
+template <bool BF>
+__global__ __launch_bounds__(256) void dz_attention_join_kernel(const AttnParams P) {
+  typedef Type<BF> Ty;
+  const int lane = threadIdx.x & 63;
+  const int items = P.kv_heads * P.head_tiles;
+  const int row = blockIdx.x / items, item = blockIdx.x % items;
+  const int kvh = item / P.head_tiles, head0 = kvh * P.share + item % P.head_tiles * HEADS;
+  const int nheads = min(HEADS, (kvh + 1) * P.share - head0);
+  const Plan plan = make_plan(P, lane);
+  int n = 1, before = 0;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int a = __shfl(plan.parts(r), row >> 2), b = __shfl(plan.before[r], row >> 2);
+    if ((row & 3) == r) n = a, before = b;
+  }
+  if (n <= 1) return;
+  const size_t step = (size_t)items * P.part_floats;
+  const float* from = P.parts + ((size_t)before * items + item) * P.part_floats;
+  for (int x = threadIdx.x; x < nheads * (P.dim / 4); x += 256) {
+    const int h = x / (P.dim / 4), d = x % (P.dim / 4) * 4;
+    float m = -INFINITY, l = 0.0f;
+    f4_t o = {0, 0, 0, 0};
+    for (int s = 0; s < n; ++s) {
+      const float* p = from + s * step;
+      const float ms = p[nheads * P.dim + 2 * h], ls = p[nheads * P.dim + 2 * h + 1];
+      if (ms == -INFINITY) continue;
+      const float up = fmaxf(m, ms), f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - up), fs = __builtin_amdgcn_exp2f(ms - up);
+      l = l * f + ls * fs;
+      o = o * f + *(const f4_t*)(p + h * P.dim + d) * fs;
+      m = up;
+    }
+    const f4_t y = o / l;
+    uint16_t* at = P.out + row * P.out_row + (head0 + h) * P.out_head + d;
+    const u2_t w = {(unsigned)Ty::round(y[0]) | (unsigned)Ty::round(y[1]) << 16,
+                    (unsigned)Ty::round(y[2]) | (unsigned)Ty::round(y[3]) << 16};
+    *(u2_t*)at = w;
+  }
+}
+
+// Workgroups that a launch of so many rows can come to.
+inline long long most_groups(int rows, int items, long long room) {
+  const long long whole = (room + TILE - 1) / TILE + 1;          // tiles of the longest row (a window may cut two)
+  const long long parts = (whole + WAVES - 1) / WAVES;
+  const long long all = parts * rows * items, cut = TARGET + (long long)rows * items;
+  return all < cut ? all : cut;
+}
+
+typedef void (*kernel_t)(const AttnParams);
+template <bool BF>
+kernel_t kernel_for(int dim) {
+  return dim <= 64 ? dz_attention_kernel<2, BF> : dim <= 96 ? dz_attention_kernel<3, BF> : dim <= 128 ? dz_attention_kernel<4, BF>
+         : dim <= 192 ? dz_attention_kernel<6, BF> : dz_attention_kernel<8, BF>;
+}
+
+inline bool shapes_fit(int rows, int heads, int kv_heads, int dim, int page_size, int pages_per_row) {
+  return rows >= 0 && heads >= 1 && kv_heads >= 1 && heads <= 4096 && heads % kv_heads == 0 && dim >= 8 && dim <= 256 && dim % 8 == 0 &&
+         page_size >= 8 && page_size <= 1024 && (page_size & (page_size - 1)) == 0 && pages_per_row >= 0 &&
+         (long long)pages_per_row * page_size <= (1ll << 30);
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t dz_paged_attention_bytes(int rows, int heads, int kv_heads, int dim, int page_size, int pages_per_row) {
+  if (!shapes_fit(rows, heads, kv_heads, dim, page_size, pages_per_row)) return 0;
+  const int share = heads / kv_heads, items = kv_heads * ((share + HEADS - 1) / HEADS);
+  const int most = share < HEADS ? share : HEADS;
+  return (size_t)most_groups(rows < GROUP_ROWS ? rows : GROUP_ROWS, items, (long long)pages_per_row * page_size) * most * (dim + 4) * 4;
+}
+
+int dz_paged_attention(const dz_attention_args* a, void* stream) {
+  if (!a || a->bytes != (int64_t)sizeof(*a)) return DZ_EINVAL;
+  if (!shapes_fit(a->rows, a->heads, a->kv_heads, a->dim, a->page_size, a->pages_per_row)) return DZ_EPAGES;
+  if (a->dtype != DZ_F16 && a->dtype != DZ_BF16) return DZ_EINVAL;
+  if (a->rows == 0) return DZ_OK;
+  if (!a->q || !a->k_pages || !a->v_pages || (!a->tables && a->pages_per_row) || !a->lengths || !a->out || !a->status || a->window < 0)
+    return DZ_EINVAL;
+  if (a->num_pages < 1 || a->num_pages > 0x7fffffffll) return DZ_EPAGES;
+  const int64_t strides[] = {a->q_row, a->q_head, a->k_page, a->k_head, a->k_token, a->v_page, a->v_head, a->v_token, a->out_row, a->out_head};
+  for (int64_t s : strides)
+    if (s < 0 || s % 8) return DZ_EALIGN;
+  if (((uintptr_t)a->q | (uintptr_t)a->k_pages | (uintptr_t)a->v_pages | (uintptr_t)a->out) & 15) return DZ_EALIGN;
+  if (((uintptr_t)a->tables | (uintptr_t)a->lengths | (uintptr_t)a->status) & 3) return DZ_EALIGN;
+  if (a->table_row < 0) return DZ_EPAGES;
+  const size_t need = dz_paged_attention_bytes(a->rows, a->heads, a->kv_heads, a->dim, a->page_size, a->pages_per_row);
+  if (!a->work || (size_t)a->work_bytes < need || ((uintptr_t)a->work & 15)) return DZ_EWORKSPACE;
+
+  AttnParams P;
+  P.k = (const char*)a->k_pages;
+  P.v = (const char*)a->v_pages;
+  P.parts = (float*)a->work;
+  P.status = a->status;
+  P.q_row = 2 * a->q_row, P.q_head = 2 * a->q_head;
+  P.k_page = 2 * a->k_page, P.k_head = 2 * a->k_head, P.k_token = 2 * a->k_token;
+  P.v_page = 2 * a->v_page, P.v_head = 2 * a->v_head, P.v_token = 2 * a->v_token;
+  P.out_row = a->out_row, P.out_head = a->out_head, P.table_row = a->table_row;
+  P.num_pages = (unsigned)a->num_pages;
+  P.heads = a->heads, P.kv_heads = a->kv_heads, P.share = a->heads / a->kv_heads;
+  P.head_tiles = (P.share + HEADS - 1) / HEADS;
+  P.dim = a->dim, P.shift = __builtin_ctz(a->page_size), P.pages_per_row = a->pages_per_row, P.window = a->window;
+  const int most = P.share < HEADS ? P.share : HEADS, items = P.kv_heads * P.head_tiles;
+  P.part_floats = most * (a->dim + 4);
+  P.scale = a->scale * 1.44269504088896340736f;
+  const size_t lds = ((size_t)WAVES * most * (a->dim + 4) + 2 * WAVES * HEADS) * 4;
+  const kernel_t kern = a->dtype == DZ_BF16 ? kernel_for<true>(a->dim) : kernel_for<false>(a->dim);
+  const int which = (a->dim <= 64 ? 0 : a->dim <= 96 ? 1 : a->dim <= 128 ? 2 : a->dim <= 192 ? 3 : 4) * 2 + a->dtype;
+  static std::atomic<unsigned long long> attr_done[10];
+  if (lds > 65536 && !dz_lds_limit_once(attr_done[which], (const void*)kern, (WAVES * HEADS * (256 + 4) + 2 * WAVES * HEADS) * 4)) return DZ_ELAUNCH;
+  const hipStream_t st = (hipStream_t)stream;
+  for (int row = 0; row < a->rows; row += GROUP_ROWS) {
+    P.rows = a->rows - row < GROUP_ROWS ? a->rows - row : GROUP_ROWS;
+    P.q = (const char*)a->q + row * P.q_row;
+    P.out = (uint16_t*)a->out + row * P.out_row;
+    P.tables = a->tables + row * P.table_row;
+    P.lengths = a->lengths + row;
+    const long long groups = most_groups(P.rows, items, (long long)a->pages_per_row * a->page_size);
+    hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(64 * WAVES), lds, st, P);
+    if (groups > (long long)P.rows * items) {
+      if (a->dtype == DZ_BF16)
+        hipLaunchKernelGGL(dz_attention_join_kernel<true>, dim3(P.rows * items), dim3(256), 0, st, P);
+      else
+        hipLaunchKernelGGL(dz_attention_join_kernel<false>, dim3(P.rows * items), dim3(256), 0, st, P);
+    }
+  }
+  return hipGetLastError() == hipSuccess ? DZ_OK : DZ_ELAUNCH;
+}
+
+}  // extern "C"

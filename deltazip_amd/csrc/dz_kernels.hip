@@ -789,6 +789,7 @@ const char* dz_strerror(int code) {
     case DZ_ELAUNCH: return "HIP launch failed";
     case DZ_EALIGN: return "pointer or leading dimension not aligned";
     case DZ_ESTATICMAX: return "N exceeds DZ_STATIC_MAX_N, the largest layer the library's built-in workspace serves";
+    case DZ_EPAGES: return "sizes not supported by the operators on a paged cache";
     default: return "unknown error";
   }
 }

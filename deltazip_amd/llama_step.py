@@ -5,8 +5,9 @@ reference's serving model (serving/vllm/model_executor/models/llama.py:58-89 Lla
 LlamaAttention, :175-235 LlamaDecoderLayer, :238-290 LlamaModel, :293-339 the delta module tables)
 with the fused projections held as plain `torch.nn.Linear` modules, which
 `create_delta_manager` (serving/vllm/delta/models.py:450-488, 606-626) replaces by delta layers.
-RMSNorm, rotary embedding and attention over the KV context are plain PyTorch ops: they are not
-part of the path this library accelerates and are here so that a step has its real shape.
+RMSNorm and activation are plain PyTorch ops.  `decode_step` takes sequences that all stand at one position,
+over a padded cache with plain rotary positions and attention; `paged_step` takes sequences at
+positions of their own over a `PagedKVCache`, with the package's operators for both.
 
 Nothing in the package depends on this module.
 """
@@ -18,6 +19,9 @@ from typing import List, Optional, Tuple
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+
+from .kv_cache import PagedBatch, PagedKVCache
+from .paged import RotaryPositions, append_kv, paged_attention
 
 
 @dataclass
@@ -79,6 +83,15 @@ class LlamaAttention(nn.Module):
         out, _ = self.o_proj(out.reshape(B, -1))
         return out
 
+    def paged(self, hidden: torch.Tensor, rope: RotaryPositions, batch: PagedBatch, keys: torch.Tensor,
+              values: torch.Tensor) -> torch.Tensor:
+        qkv, _ = self.qkv_proj(hidden)
+        q, k, v = (t.unflatten(1, (self.num_heads, self.head_dim)) for t in qkv.chunk(3, dim=-1))
+        q = append_kv(q, k, v, batch.positions, batch.slots, rope, keys, values)
+        out = paged_attention(q, keys, values, batch.block_tables, batch.lengths)
+        out, _ = self.o_proj(out.flatten(1))
+        return out
+
 
 class LlamaMLP(nn.Module):
     def __init__(self, cfg: LlamaStepConfig, device=None) -> None:
@@ -104,12 +117,18 @@ class LlamaDecoderLayer(nn.Module):
         self.post_attention_layernorm = RMSNorm(cfg.hidden_size, cfg.rms_norm_eps, device)
 
     def forward(self, hidden, residual, cos, sin, kv_cache, context_len):
+        return self._around(hidden, residual, self.self_attn, cos, sin, kv_cache, context_len)
+
+    def paged(self, hidden, residual, rope, batch, keys, values):
+        return self._around(hidden, residual, self.self_attn.paged, rope, batch, keys, values)
+
+    def _around(self, hidden, residual, attention, *context):
         if residual is None:
             residual = hidden
             hidden = self.input_layernorm(hidden)
         else:
             hidden, residual = self.input_layernorm(hidden, residual)
-        hidden = self.self_attn(hidden, cos, sin, kv_cache, context_len)
+        hidden = attention(hidden, *context)
         hidden, residual = self.post_attention_layernorm(hidden, residual)
         hidden = self.mlp(hidden)
         return hidden, residual
@@ -166,6 +185,7 @@ class LlamaForDecodeStep(nn.Module):
         hd = cfg.hidden_size // cfg.num_attention_heads
         inv = 1.0 / (cfg.rope_theta ** (torch.arange(0, hd, 2, device=device).float() / hd))
         self.register_buffer("inv_freq", inv, persistent=False)
+        self.rope = RotaryPositions(hd, base=cfg.rope_theta, max_position=cfg.max_position_embeddings)
 
     def projections(self) -> List[Tuple[str, nn.Module]]:
         """(name, module) of every projection, in execution order."""
@@ -200,6 +220,26 @@ class LlamaForDecodeStep(nn.Module):
         residual = None
         for layer, kv in zip(self.model.layers, kv_caches):
             hidden, residual = layer(hidden, residual, cos, sin, kv, context_len)
+        hidden, _ = self.model.norm(hidden, residual)
+        if sample_rows is not None:
+            hidden = hidden.index_select(0, sample_rows)
+        return self.logits_processor._get_logits(hidden, self.lm_head.weight)
+
+    def make_paged_cache(self, num_pages: int, page_size: int = 16, device="cuda") -> PagedKVCache:
+        cfg = self.config
+        return PagedKVCache(cfg.num_hidden_layers, num_pages, page_size, cfg.num_attention_heads,
+                            cfg.hidden_size // cfg.num_attention_heads, cfg.max_position_embeddings, device=device)
+
+    @torch.no_grad()
+    def paged_step(self, input_ids: torch.Tensor, cache: PagedKVCache, batch: PagedBatch,
+                   sample_rows: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """One decode step of sequences that stand where `batch` says (`cache.extend(seqs)`, then `cache.batch(seqs)`): their
+        new tokens' keys and values go into the cache.  Returns the logits [rows, vocab] of `sample_rows` (default: all)."""
+        emb = self.model.embed_tokens(input_ids.view(-1))
+        hidden = emb if not isinstance(emb, tuple) else emb[0]
+        residual = None
+        for layer, keys, values in zip(self.model.layers, cache.keys, cache.values):
+            hidden, residual = layer.paged(hidden, residual, self.rope, batch, keys, values)
         hidden, _ = self.model.norm(hidden, residual)
         if sample_rows is not None:
             hidden = hidden.index_select(0, sample_rows)

@@ -838,6 +838,7 @@ WS_HEADER_BYTES = 256          # the status word sits in front of the token orde
 
 STATUS_BAD_ID = 1              # a delta id outside [-1, S) was met and treated as -1
 STATUS_SUM_MISSING = 2         # a partial sum of a K-slice did not arrive: that call's output is invalid
+STATUS_BAD_PAGE = 4            # a page, slot or length outside the key/value cache: that call's output is invalid
 
 
 @lru_cache(maxsize=4096)
@@ -863,7 +864,7 @@ def _workspace(device: torch.device, T: int, K: int, N: int) -> torch.Tensor:
 
 def workspace_status(device=None) -> int:
     """Status words of the device's workspaces, OR-ed (bit 0: a delta id outside [-1, S) was seen
-    and treated as -1; bit 1: a partial sum did not arrive).  Synchronises; meant for debugging
+    and treated as -1; bit 1: a partial sum did not arrive; bit 2: a page, slot or length outside the cache).  Synchronises; meant for debugging
     and tests -- the serving path uses `poll_status`."""
     idx = torch.cuda.current_device() if device is None else torch.device(device).index
     status = 0
@@ -881,7 +882,7 @@ _warned_bad_id = False
 
 
 def raise_for_status(word: int, where: str = "multi-delta linear") -> None:
-    """What a status word means to the caller.  Bit 1 -> DeltaKernelError (a RuntimeError, as every
+    """What a status word means to the caller.  Bits 1 and 2 -> DeltaKernelError (a RuntimeError, as every
     failure of the reference's ops is a Python exception); bit 0 -> one warning per process."""
     global _warned_bad_id
     if word & STATUS_SUM_MISSING:
@@ -889,6 +890,10 @@ def raise_for_status(word: int, where: str = "multi-delta linear") -> None:
             f"{where}: a partial sum of a K dimension split over workgroups did not arrive within the kernel's "
             "bounded wait; the outputs of the calls since the last check are invalid (status bit 1). The "
             "workspace has been cleared; repeat the step.")
+    if word & STATUS_BAD_PAGE:
+        raise DeltaKernelError(
+            "paged cache: a page number or slot outside the pool, or a length beyond its table, was met; the outputs of "
+            "the calls since the last check are invalid (status bit 2).")
     if word & STATUS_BAD_ID and not _warned_bad_id:
         _warned_bad_id = True
         import warnings

@@ -43,6 +43,7 @@ extern "C" {
 #define DZ_ELAUNCH      -9   /* the HIP runtime refused the launch                         */
 #define DZ_EALIGN      -10   /* pointer not aligned as required                            */
 #define DZ_ESTATICMAX  -11   /* dz_multi_delta_linear_static: N above DZ_STATIC_MAX_N       */
+#define DZ_EPAGES      -12   /* sizes that the operators on a paged cache do not take       */
 
 #define DZ_MAX_TOKENS_FUSED 128   /* largest T the fused decode kernel takes in one launch   */
 #define DZ_MAX_BATCH_CALLS 4      /* layer calls dz_multi_delta_linear_batch takes at once    */
@@ -55,6 +56,9 @@ extern "C" {
 #define DZ_MIXED_SMALL_DELTAS 2   /* deltas */
 #define DZ_MIXED_HEADER 4         /* words in front of the blocks of a table; the first: how many there are */
 #define DZ_MAX_SLOTS_MAP 4096      /* largest S dz_map_ids takes (the slot table lives in LDS) */
+
+#define DZ_F16  0                 /* element types of the operators on a paged cache */
+#define DZ_BF16 1
 
 /* Library version (major*10000 + minor*100 + patch). */
 int dz_version(void);
@@ -465,6 +469,70 @@ int dz_multi_delta_gemm_tiled(const uint16_t* x, const uint16_t* w_base_tiled, c
                               const void* meta_stacked, const void* scales_stacked, int S, int bits,
                               int group_size, const dz_gemm_tile* tiles, int ntiles, const int32_t* perm,
                               uint16_t* y, int T, int K, int N, int accumulate, int ldy, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * A paged key/value cache.  Pages are those of the reference's serving engine
+ * (serving/csrc/attention, serving/csrc/cache_kernels, serving/csrc/pos_encoding): a pool of pages of page_size
+ * tokens, a table of page numbers per sequence.  Strides are in elements; the values of a head are
+ * contiguous.  Element types: DZ_F16, DZ_BF16.  `bytes` is the structure's size.
+ * ------------------------------------------------------------------------------------------- */
+
+/* One new token per row over the tokens in front of it:
+ *   out[r, h] = softmax_t(scale q[r, h] . k[t, h / (heads / kv_heads)]) v[t, ...],  max(0, n - window) <= t < n = lengths[r]
+ * where token t is at page tables[r, t / page_size], place t % page_size.  window 0: all tokens.  A row of length 0 (or
+ * less) gives zeros; nothing behind a row's length is read, in its table or in the pages.  A length beyond the
+ * table's room is cut there, and a page number outside [0, num_pages) read as page 0: either sets bit 2 of *status.
+ * dim is a multiple of 8 up to 256, page_size a power of two from 8 to 1024, heads a multiple of kv_heads; pointers are aligned
+ * to 16 bytes and strides multiples of 8.  work: dz_paged_attention_bytes() bytes, any contents; calls that
+ * overlap in time need one each.  The sums of a row go in the order of its tokens, cut by the lengths of all rows: results are the
+ * same for the same lengths. */
+typedef struct dz_attention_args {
+  int64_t bytes;
+  const void *q, *k_pages, *v_pages;      /* q [rows, heads, dim]; pages [num_pages, kv_heads, page_size, dim] */
+  const int32_t *tables, *lengths;        /* [rows, pages_per_row], [rows] */
+  void *out;                              /* [rows, heads, dim] */
+  void *work;
+  uint32_t *status;
+  int64_t work_bytes, num_pages;
+  int64_t q_row, q_head, k_page, k_head, k_token, v_page, v_head, v_token, out_row, out_head, table_row;
+  int32_t rows, heads, kv_heads, dim, page_size, pages_per_row, window, dtype;
+  float scale;
+  int32_t reserved;
+} dz_attention_args;
+
+size_t dz_paged_attention_bytes(int rows, int heads, int kv_heads, int dim, int page_size, int pages_per_row);
+int dz_paged_attention(const dz_attention_args* args, void* stream);
+
+/* The first `rot` values of every head of q and k turned to their token's position: pair i is (i, i + rot / 2), or with
+ * neighbours != 0 (2 i, 2 i + 1), its angle positions[t] * turns[i] full turns, the turned values times `factor`;
+ * the others are copied.  Without slots: k_out [tokens, kv_heads, dim] (strides k_out_token, k_out_head), and
+ * the outputs may be the inputs.  With slots: token t's key and value go to place slots[t] % page_size of page slots[t] / page_size
+ * of k_out and v_out [num_pages, kv_heads, page_size, dim]; a negative slot stores nothing, one beyond the pages
+ * nothing either and sets bit 2 of *status.  Slots are distinct: of two tokens with one slot either may end up
+ * there, in part.  k and v may be NULL.  rot 0: nothing is turned.  dim is even, up to 256; pointers and
+ * strides are aligned to 4 bytes (16 and sizes in whole requests: fewer instructions). */
+typedef struct dz_rotary_args {
+  int64_t bytes;
+  const void *q, *k, *v;                  /* [tokens, heads or kv_heads, dim] */
+  void *q_out, *k_out, *v_out;
+  const int64_t *positions, *slots;       /* [tokens]; slots or NULL */
+  const double *turns;                    /* [rot / 2] */
+  uint32_t *status;
+  int64_t num_pages;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head, q_out_row, q_out_head;
+  int64_t k_out_page, k_out_head, k_out_token, v_out_page, v_out_head, v_out_token;
+  int32_t tokens, heads, kv_heads, dim, rot, neighbours, page_size, dtype;
+  float factor;
+  int32_t reserved;
+} dz_rotary_args;
+
+int dz_rotary(const dz_rotary_args* args, void* stream);
+
+/* Page pairs[2 i] copied over page pairs[2 i + 1], i < npairs, in every one of npools pools (host arrays, read before the
+ * call returns).  No page may be written twice, or be read and written: the copies run side by side.  Pages are
+ * page_bytes bytes every page_stride bytes, both multiples of 16. */
+int dz_copy_pages(void* const* pools, int npools, long long page_stride, long long page_bytes, int num_pages,
+                  const int32_t* pairs, int npairs, void* stream);
 
 #ifdef __cplusplus
 }
