@@ -22,34 +22,44 @@
 //
 // The work is cut on the device, which alone knows the lengths: every wavefront reads the lengths of the launch's
 // rows (up to 256, four a lane), and takes for the tiles of a workgroup as many as make about `target` workgroups.
-// Parts of a row are joined by a second kernel in the order of the tokens, so results do not depend on timing.
+// Parts of a row are joined by the workgroup that is done last of them (a counter per row and item says which),
+// in the order of the tokens, so results do not depend on timing.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "../../include/dz_amd.h"
 #include "dz_device.h"
 
 namespace {
 
+typedef float f2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
 
 constexpr int WAVES = 4;               // wavefronts of a workgroup
 constexpr int TILE = 32;               // tokens of a step
 constexpr int HEADS = 16;              // heads taken together: columns of a matrix instruction
 constexpr int GROUP_ROWS = 256;        // rows of a launch: four lengths a lane
-constexpr int TARGET = 1024;           // workgroups that the work is cut into, rows' last parts apart
+#ifndef TGT
+#define TGT 768
+#endif
+constexpr int TARGET = TGT;           // workgroups that the work is cut into, rows' last parts apart
+constexpr int COUNTERS = DZ_ATTENTION_COUNTERS;   // rows of a launch times their items, at most
+constexpr size_t LDS_MOST = 96 << 10;
+constexpr long long CACHED = 64ll << 20;   // bytes of keys and values
 
 struct AttnParams {
   const char *q, *k, *v;
   const int *tables, *lengths;
   uint16_t* out;
   float* parts;
+  unsigned* counters;
   unsigned* status;
   long long q_row, q_head, k_page, k_head, k_token, v_page, v_head, v_token, out_row, out_head, table_row;   // bytes; out, table: elements
   unsigned num_pages;
-  int rows, heads, kv_heads, share, head_tiles, dim, shift, pages_per_row, window, part_floats;
+  int rows, heads, kv_heads, share, head_tiles, dim, shift, pages_per_row, window, part_floats, stat_at;
   float scale;
 };
 
@@ -89,6 +99,7 @@ __device__ __forceinline__ int tiles_of(const AttnParams& P, int length) {
 struct Plan {
   int tiles[4], before[4];             // tiles of a row; parts of the rows in front of it
   int each;                            // most tiles of a part
+  long long total;                     // tiles of all rows and items
   __device__ __forceinline__ int parts(int r) const { return tiles[r] ? (tiles[r] + each - 1) / each : 1; }   // (an empty row has its zeros written)
 };
 
@@ -105,7 +116,8 @@ __device__ __forceinline__ Plan make_plan(const AttnParams& P, int lane) {
 #pragma unroll
   for (int d = 32; d; d >>= 1) total += __shfl_xor(total, d);
   const long long items = (long long)P.kv_heads * P.head_tiles;
-  long long each = (total * items + TARGET - 1) / TARGET;
+  p.total = total * items;
+  long long each = (p.total + TARGET - 1) / TARGET;
   each = (each + WAVES - 1) / WAVES * WAVES;
   p.each = each < WAVES ? WAVES : (int)each;
   int sum = 0;
@@ -125,8 +137,27 @@ __device__ __forceinline__ Plan make_plan(const AttnParams& P, int lane) {
   return p;
 }
 
+// Keys and values of a call pass through once: loads that keep nothing in the caches read 7.1 TB/s where others read 6.2.
+template <bool ONCE>
+__device__ __forceinline__ u4_t load16(const char* at) {
+  return ONCE ? __builtin_nontemporal_load((const u4_t*)at) : *(const u4_t*)at;
+}
+
+// Sums of parts go from one workgroup to another past the caches of the eight dies (agent scope, relaxed): a fence
+// there writes back and empties a whole cache, which took six times as long as the attention itself.
+__device__ __forceinline__ void put(float* at, f2_t x) {
+  __hip_atomic_store((unsigned long long*)at, __builtin_bit_cast(unsigned long long, x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ f2_t get(const float* at) {
+  return __builtin_bit_cast(f2_t, __hip_atomic_load((const unsigned long long*)at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
+__device__ __forceinline__ f4_t get4(const float* at) {
+  const f2_t a = get(at), b = get(at + 2);
+  return f4_t{a[0], a[1], b[0], b[1]};
+}
+
 template <int KC, bool BF>
-__global__ __launch_bounds__(64 * WAVES) void dz_attention_kernel(const AttnParams P) {
+__global__ __launch_bounds__(64 * WAVES, 2) void dz_attention_kernel(const AttnParams P) {
   typedef Type<BF> Ty;
   typedef typename Ty::v8 v8;
   constexpr int NB = (KC + 3) / 4;     // blocks of 128 dims
@@ -196,6 +227,8 @@ __global__ __launch_bounds__(64 * WAVES) void dz_attention_kernel(const AttnPara
   }
   const int in_page = (1 << P.shift) - 1;
 
+  auto walk = [&](auto once) __attribute__((always_inline)) {
+  constexpr bool ONCE = decltype(once)::value;
   for (; t0 < t1; ++t0) {
     const int tok = t0 * TILE;
     const bool edge = tok < first || tok + TILE > end;
@@ -215,7 +248,7 @@ __global__ __launch_bounds__(64 * WAVES) void dz_attention_kernel(const AttnPara
 #pragma unroll
       for (int c = 0; c < KC; ++c) {
         kw[a][c] = u4_t{0, 0, 0, 0};
-        if (32 * c + 8 * g < P.dim) kw[a][c] = *(const u4_t*)(at + 64 * c);
+        if (32 * c + 8 * g < P.dim) kw[a][c] = load16<ONCE>(at + 64 * c);
       }
     }
 #pragma unroll
@@ -228,7 +261,7 @@ __global__ __launch_bounds__(64 * WAVES) void dz_attention_kernel(const AttnPara
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
         vw[b][e] = u4_t{0, 0, 0, 0};       // (what is masked may be anything: it has no part in the product)
-        if (!out && 128 * b + 8 * col < P.dim) vw[b][e] = *(const u4_t*)(at + 256 * b);
+        if (!out && 128 * b + 8 * col < P.dim) vw[b][e] = load16<ONCE>(at + 256 * b);
       }
     }
     float s[8];
@@ -281,13 +314,18 @@ __global__ __launch_bounds__(64 * WAVES) void dz_attention_kernel(const AttnPara
         acc[8 * b + j] = Ty::mma(vt, pl, Ty::mma(vt, ph, acc[8 * b + j]));
       }
   }
+  };
+  if (plan.total * (TILE * 4ll * P.dim) > CACHED)
+    walk(std::integral_constant<bool, true>());
+  else
+    walk(std::integral_constant<bool, false>());
   sum += __shfl_xor(sum, 16);
   sum += __shfl_xor(sum, 32);
 
   // the four wavefronts' sums joined: [wave][head][dim], then maxima and sums
   const int ld = P.dim + 4;
   float* mine = lds + wave * nheads * ld;
-  float* stat = lds + WAVES * nheads * ld;
+  float* stat = lds + P.stat_at;
   if (col < nheads) {
 #pragma unroll
     for (int b = 0; b < NB; ++b)
@@ -306,8 +344,16 @@ __global__ __launch_bounds__(64 * WAVES) void dz_attention_kernel(const AttnPara
   }
   __syncthreads();
   float* to = nparts > 1 ? P.parts + (size_t)blockIdx.x * P.part_floats : nullptr;
-  for (int x = threadIdx.x; x < nheads * (P.dim / 4); x += 64 * WAVES) {
-    const int h = x / (P.dim / 4), d = x % (P.dim / 4) * 4;
+  const int quads = P.dim / 4, spots = nheads * quads;
+  auto store = [&](int h, int d, f4_t o, float l) {
+    const f4_t y = tiles ? o / l : f4_t{0, 0, 0, 0};
+    uint16_t* at = P.out + row * P.out_row + (head0 + h) * P.out_head + d;
+    const u2_t w = {(unsigned)Ty::round(y[0]) | (unsigned)Ty::round(y[1]) << 16,
+                    (unsigned)Ty::round(y[2]) | (unsigned)Ty::round(y[3]) << 16};
+    *(u2_t*)at = w;
+  };
+  for (int x = threadIdx.x; x < spots; x += 64 * WAVES) {
+    const int h = x / quads, d = x % quads * 4;
     float m = -INFINITY;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) m = fmaxf(m, stat[(w * HEADS + h) * 2]);
@@ -321,62 +367,91 @@ __global__ __launch_bounds__(64 * WAVES) void dz_attention_kernel(const AttnPara
       o += mw == -INFINITY ? f4_t{0, 0, 0, 0} : *(const f4_t*)(lds + (w * nheads + h) * ld + d) * f;
     }
     if (to) {
-      *(f4_t*)(to + h * P.dim + d) = o;
-      if (d == 0) {
-        to[nheads * P.dim + 2 * h] = m;
-        to[nheads * P.dim + 2 * h + 1] = l;
-      }
+      put(to + h * P.dim + d, f2_t{o[0], o[1]});
+      put(to + h * P.dim + d + 2, f2_t{o[2], o[3]});
+      if (d == 0) put(to + nheads * P.dim + 2 * h, f2_t{m, l});
     } else {
-      const f4_t y = tiles ? o / l : f4_t{0, 0, 0, 0};
-      uint16_t* at = P.out + row * P.out_row + (head0 + h) * P.out_head + d;
-      const u2_t w = {(unsigned)Ty::round(y[0]) | (unsigned)Ty::round(y[1]) << 16,
-                      (unsigned)Ty::round(y[2]) | (unsigned)Ty::round(y[3]) << 16};
-      *(u2_t*)at = w;
+      store(h, d, o, l);
     }
   }
-}
+  if (!to) return;
 
-// Joins the parts of a row's heads, in the order of the tokens.
-template <bool BF>
-__global__ __launch_bounds__(256) void dz_attention_join_kernel(const AttnParams P) {
-  typedef Type<BF> Ty;
-  const int lane = threadIdx.x & 63;
-  const int items = P.kv_heads * P.head_tiles;
-  const int row = blockIdx.x / items, item = blockIdx.x % items;
-  const int kvh = item / P.head_tiles, head0 = kvh * P.share + item % P.head_tiles * HEADS;
-  const int nheads = min(HEADS, (kvh + 1) * P.share - head0);
-  const Plan plan = make_plan(P, lane);
-  int n = 1, before = 0;
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int a = __shfl(plan.parts(r), row >> 2), b = __shfl(plan.before[r], row >> 2);
-    if ((row & 3) == r) n = a, before = b;
+  // the last of a row's parts to be done joins them
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this wavefront's sums have arrived
+  __syncthreads();
+  int* flag = (int*)(stat + 2 * WAVES * HEADS);
+  if (threadIdx.x == 0) {
+    unsigned* counter = P.counters + row * items + item;
+    const bool last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)nparts - 1;
+    if (last) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // as the next call wants it
+    *flag = last;
   }
-  if (n <= 1) return;
+  __syncthreads();
+  if (!*flag) return;
   const size_t step = (size_t)items * P.part_floats;
-  const float* from = P.parts + ((size_t)before * items + item) * P.part_floats;
-  for (int x = threadIdx.x; x < nheads * (P.dim / 4); x += 256) {
-    const int h = x / (P.dim / 4), d = x % (P.dim / 4) * 4;
-    float m = -INFINITY, l = 0.0f;
-    f4_t o = {0, 0, 0, 0};
-    for (int s = 0; s < n; ++s) {
-      const float* p = from + s * step;
-      const float ms = p[nheads * P.dim + 2 * h], ls = p[nheads * P.dim + 2 * h + 1];
-      if (ms == -INFINITY) continue;
-      const float up = fmaxf(m, ms), f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - up), fs = __builtin_amdgcn_exp2f(ms - up);
-      l = l * f + ls * fs;
-      o = o * f + *(const f4_t*)(p + h * P.dim + d) * fs;
-      m = up;
+  const float* from = P.parts + ((size_t)(part - nth) * items + item) * P.part_floats;
+  // factors of the parts, [head][part], and behind them the heads' sums
+  float* factor = lds;
+  float* total = stat;
+  for (int h = wave; h < nheads; h += WAVES) {
+    const float* p = from + nheads * P.dim + 2 * h;
+    float m = -INFINITY;
+    for (int s = lane; s < nparts; s += 64) m = fmaxf(m, get(p + s * step)[0]);
+#pragma unroll
+    for (int d = 32; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+    float l = 0.0f;
+    for (int s = lane; s < nparts; s += 64) {
+      const f2_t ml = get(p + s * step);
+      const float f = ml[0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[0] - m);
+      factor[h * nparts + s] = f;
+      l += ml[0] == -INFINITY ? 0.0f : f * ml[1];
     }
-    const f4_t y = o / l;
-    uint16_t* at = P.out + row * P.out_row + (head0 + h) * P.out_head + d;
-    const u2_t w = {(unsigned)Ty::round(y[0]) | (unsigned)Ty::round(y[1]) << 16,
-                    (unsigned)Ty::round(y[2]) | (unsigned)Ty::round(y[3]) << 16};
-    *(u2_t*)at = w;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) l += __shfl_xor(l, d);
+    if (lane == 0) total[h] = l;
+  }
+  __syncthreads();
+  // threads that have no values of their own share the parts of others': slice c of `slices`
+  int slices = 1;
+  while (2 * slices * spots <= 64 * WAVES) slices *= 2;
+  float* shared = lds + (nheads * nparts + 3) / 4 * 4;   // [slice][spot]
+  for (int x = threadIdx.x; x < spots * slices; x += 64 * WAVES) {
+    const int spot = x % spots, c = x / spots, h = spot / quads, d = spot % quads * 4;
+    const float *p = from + h * P.dim + d, *f = factor + h * nparts;
+    f4_t o = {0, 0, 0, 0};
+    int s = c;
+    for (; s + 7 * slices < nparts; s += 8 * slices) {
+      f4_t w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = get4(p + (s + i * slices) * step);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float fs = f[s + i * slices];
+        o += fs == 0.0f ? f4_t{0, 0, 0, 0} : w[i] * fs;
+      }
+    }
+    for (; s < nparts; s += slices) {
+      const float fs = f[s];
+      o += fs == 0.0f ? f4_t{0, 0, 0, 0} : get4(p + s * step) * fs;
+    }
+    if (slices == 1)
+      store(h, d, o, total[h]);
+    else
+      *(f4_t*)(shared + 4 * x) = o;
+  }
+  if (slices == 1) return;
+  __syncthreads();
+  for (int spot = threadIdx.x; spot < spots; spot += 64 * WAVES) {
+    f4_t o = {0, 0, 0, 0};
+    for (int c = 0; c < slices; ++c) o += *(const f4_t*)(shared + 4 * (c * spots + spot));
+    store(spot / quads, spot % quads * 4, o, total[spot / quads]);
   }
 }
 
 // Workgroups that a launch of so many rows can come to.
+// Rows that go in one launch.
+inline int group_rows(int items) { return COUNTERS / items < GROUP_ROWS ? COUNTERS / items : GROUP_ROWS; }
+
 inline long long most_groups(int rows, int items, long long room) {
   const long long whole = (room + TILE - 1) / TILE + 1;          // tiles of the longest row (a window may cut two)
   const long long parts = (whole + WAVES - 1) / WAVES;
@@ -405,7 +480,9 @@ size_t dz_paged_attention_bytes(int rows, int heads, int kv_heads, int dim, int 
   if (!shapes_fit(rows, heads, kv_heads, dim, page_size, pages_per_row)) return 0;
   const int share = heads / kv_heads, items = kv_heads * ((share + HEADS - 1) / HEADS);
   const int most = share < HEADS ? share : HEADS;
-  return (size_t)most_groups(rows < GROUP_ROWS ? rows : GROUP_ROWS, items, (long long)pages_per_row * page_size) * most * (dim + 4) * 4;
+  const int together = group_rows(items) < rows ? group_rows(items) : rows;
+  const long long groups = most_groups(together, items, (long long)pages_per_row * page_size);
+  return groups > (long long)together * items ? (size_t)groups * most * (dim + 4) * 4 : 0;   // (no row has parts)
 }
 
 int dz_paged_attention(const dz_attention_args* a, void* stream) {
@@ -423,12 +500,14 @@ int dz_paged_attention(const dz_attention_args* a, void* stream) {
   if (((uintptr_t)a->tables | (uintptr_t)a->lengths | (uintptr_t)a->status) & 3) return DZ_EALIGN;
   if (a->table_row < 0) return DZ_EPAGES;
   const size_t need = dz_paged_attention_bytes(a->rows, a->heads, a->kv_heads, a->dim, a->page_size, a->pages_per_row);
-  if (!a->work || (size_t)a->work_bytes < need || ((uintptr_t)a->work & 15)) return DZ_EWORKSPACE;
+  if (need && (!a->work || (size_t)a->work_bytes < need || ((uintptr_t)a->work & 15) || !a->counters || ((uintptr_t)a->counters & 3)))
+    return DZ_EWORKSPACE;
 
   AttnParams P;
   P.k = (const char*)a->k_pages;
   P.v = (const char*)a->v_pages;
   P.parts = (float*)a->work;
+  P.counters = a->counters;
   P.status = a->status;
   P.q_row = 2 * a->q_row, P.q_head = 2 * a->q_head;
   P.k_page = 2 * a->k_page, P.k_head = 2 * a->k_head, P.k_token = 2 * a->k_token;
@@ -441,26 +520,24 @@ int dz_paged_attention(const dz_attention_args* a, void* stream) {
   const int most = P.share < HEADS ? P.share : HEADS, items = P.kv_heads * P.head_tiles;
   P.part_floats = most * (a->dim + 4);
   P.scale = a->scale * 1.44269504088896340736f;
-  const size_t lds = ((size_t)WAVES * most * (a->dim + 4) + 2 * WAVES * HEADS) * 4;
+  // the wavefronts' sums; or the factors of all parts that a row can have, and what threads add up for others
+  const size_t sums = (size_t)WAVES * most * (a->dim + 4), joins = (size_t)most * (TARGET / items + 2) + 4 * 64 * WAVES;
+  const size_t lds = ((sums > joins ? sums : joins + 3) / 4 * 4 + 2 * WAVES * HEADS + 4) * 4;
+  P.stat_at = (int)(lds / 4) - (2 * WAVES * HEADS + 4);
   const kernel_t kern = a->dtype == DZ_BF16 ? kernel_for<true>(a->dim) : kernel_for<false>(a->dim);
   const int which = (a->dim <= 64 ? 0 : a->dim <= 96 ? 1 : a->dim <= 128 ? 2 : a->dim <= 192 ? 3 : 4) * 2 + a->dtype;
   static std::atomic<unsigned long long> attr_done[10];
-  if (lds > 65536 && !dz_lds_limit_once(attr_done[which], (const void*)kern, (WAVES * HEADS * (256 + 4) + 2 * WAVES * HEADS) * 4)) return DZ_ELAUNCH;
+  if (lds > 65536 && !dz_lds_limit_once(attr_done[which], (const void*)kern, (int)LDS_MOST)) return DZ_ELAUNCH;
   const hipStream_t st = (hipStream_t)stream;
-  for (int row = 0; row < a->rows; row += GROUP_ROWS) {
-    P.rows = a->rows - row < GROUP_ROWS ? a->rows - row : GROUP_ROWS;
+  const int together = group_rows(items);
+  for (int row = 0; row < a->rows; row += together) {
+    P.rows = a->rows - row < together ? a->rows - row : together;
     P.q = (const char*)a->q + row * P.q_row;
     P.out = (uint16_t*)a->out + row * P.out_row;
     P.tables = a->tables + row * P.table_row;
     P.lengths = a->lengths + row;
     const long long groups = most_groups(P.rows, items, (long long)a->pages_per_row * a->page_size);
     hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(64 * WAVES), lds, st, P);
-    if (groups > (long long)P.rows * items) {
-      if (a->dtype == DZ_BF16)
-        hipLaunchKernelGGL(dz_attention_join_kernel<true>, dim3(P.rows * items), dim3(256), 0, st, P);
-      else
-        hipLaunchKernelGGL(dz_attention_join_kernel<false>, dim3(P.rows * items), dim3(256), 0, st, P);
-    }
   }
   return hipGetLastError() == hipSuccess ? DZ_OK : DZ_ELAUNCH;
 }

@@ -27,9 +27,10 @@ import torch
 from . import _lib, ops
 
 _TYPES = {torch.float16: 0, torch.bfloat16: 1}
-_ATTENTION = struct.Struct("=q8Q2q11q8ifi")       # dz_attention_args
+_ATTENTION = struct.Struct("=q9Q2q11q8ifi")       # dz_attention_args
 _ROTARY = struct.Struct("=q10Qq14q8ifi")          # dz_rotary_args
 MAX_DIM = 256
+COUNTERS = 16384                  # DZ_ATTENTION_COUNTERS
 
 
 class RotaryPositions:
@@ -181,6 +182,23 @@ def _attention_bytes(rows: int, heads: int, kv_heads: int, dim: int, page_size: 
     return _lib.lib().dz_paged_attention_bytes(rows, heads, kv_heads, dim, page_size, pages_per_row)
 
 
+# (device, stream) -> counters, all zero between calls, and room for the sums of parts
+_spaces: Dict[Tuple[int, int], Tuple[torch.Tensor, torch.Tensor]] = {}
+
+
+def _parts_space(device: torch.device, need: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Calls on one stream follow each other and share theirs.  A captured call has its own: its graph may be replayed beside
+    anything."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.zeros(COUNTERS, dtype=torch.int32, device=device), torch.empty(need, dtype=torch.uint8, device=device)
+    key = device.index, ops._stream()
+    space = _spaces.get(key)
+    if space is None or space[1].numel() < need:
+        counters = torch.zeros(COUNTERS, dtype=torch.int32, device=device) if space is None else space[0]
+        space = _spaces[key] = counters, torch.empty(max(need, 1 << 20), dtype=torch.uint8, device=device)
+    return space
+
+
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_tables: torch.Tensor,
                     lengths: torch.Tensor, scale: Optional[float] = None, window: int = 0,
                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -232,11 +250,11 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if rows == 0:
         return out
     need = _attention_bytes(rows, heads, kv_heads, dim, page_size, width)
-    work = torch.empty(need, dtype=torch.uint8, device=q.device)
+    counters, work = _parts_space(q.device, need) if need else (None, None)
     ks, vs = k_pages.stride(), v_pages.stride()
     args = _ATTENTION.pack(
         _ATTENTION.size, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), block_tables.data_ptr(), lengths.data_ptr(),
-        out.data_ptr(), work.data_ptr(), _status(q.device), need, pages, _stride(q, 0), _stride(q, 1),
+        out.data_ptr(), work.data_ptr() if need else 0, counters.data_ptr() if need else 0, _status(q.device), need, pages, _stride(q, 0), _stride(q, 1),
         ks[0] if pages > 1 else 0, ks[1] if kv_heads > 1 else 0, ks[2], vs[0] if pages > 1 else 0, vs[1] if kv_heads > 1 else 0,
         vs[2], _stride(out, 0), _stride(out, 1), block_tables.stride(0) if rows > 1 else 0, rows, heads, kv_heads, dim, page_size,
         width, min(int(window), (1 << 31) - 1), _TYPES[q.dtype], dim ** -0.5 if scale is None else scale, 0)

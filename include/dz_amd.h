@@ -59,6 +59,7 @@ extern "C" {
 
 #define DZ_F16  0                 /* element types of the operators on a paged cache */
 #define DZ_BF16 1
+#define DZ_ATTENTION_COUNTERS 16384
 
 /* Library version (major*10000 + minor*100 + patch). */
 int dz_version(void);
@@ -483,8 +484,9 @@ int dz_multi_delta_gemm_tiled(const uint16_t* x, const uint16_t* w_base_tiled, c
  * less) gives zeros; nothing behind a row's length is read, in its table or in the pages.  A length beyond the
  * table's room is cut there, and a page number outside [0, num_pages) read as page 0: either sets bit 2 of *status.
  * dim is a multiple of 8 up to 256, page_size a power of two from 8 to 1024, heads a multiple of kv_heads; pointers are aligned
- * to 16 bytes and strides multiples of 8.  work: dz_paged_attention_bytes() bytes, any contents; calls that
- * overlap in time need one each.  The sums of a row go in the order of its tokens, cut by the lengths of all rows: results are the
+ * to 16 bytes and strides multiples of 8.  work: dz_paged_attention_bytes() bytes, any contents; counters: DZ_ATTENTION_COUNTERS
+ * words, zero before the first call and after every one (either may be NULL where that is 0); calls that overlap in time need
+ * both of their own.  The sums of a row go in the order of its tokens, cut by the lengths of all rows: results are the
  * same for the same lengths. */
 typedef struct dz_attention_args {
   int64_t bytes;
@@ -492,7 +494,7 @@ typedef struct dz_attention_args {
   const int32_t *tables, *lengths;        /* [rows, pages_per_row], [rows] */
   void *out;                              /* [rows, heads, dim] */
   void *work;
-  uint32_t *status;
+  uint32_t *counters, *status;
   int64_t work_bytes, num_pages;
   int64_t q_row, q_head, k_page, k_head, k_token, v_page, v_head, v_token, out_row, out_head, table_row;
   int32_t rows, heads, kv_heads, dim, page_size, pages_per_row, window, dtype;

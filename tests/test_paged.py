@@ -246,10 +246,10 @@ def test_c_entry_points_check_their_arguments(dzlib):
     """On the host, before anything is launched: no pointer below is dereferenced."""
     from deltazip_amd import paged
     P = 0x1000
-    names = ("bytes q k v tables lengths out work status work_bytes num_pages q_row q_head k_page k_head k_token v_page v_head v_token "
+    names = ("bytes q k v tables lengths out work counters status work_bytes num_pages q_row q_head k_page k_head k_token v_page v_head v_token "
              "out_row out_head table_row rows heads kv_heads dim page_size pages_per_row window dtype scale reserved").split()
-    ok = dict(zip(names, [paged._ATTENTION.size] + [P] * 8 + [1 << 30, 10] + [4096, 128, 65536, 2048, 128, 65536, 2048, 128, 4096, 128, 4]
-                  + [2, 32, 32, 128, 16, 4, 0, 0, 0.1, 0]))
+    ok = dict(zip(names, [paged._ATTENTION.size] + [P] * 9 + [1 << 30, 10] + [4096, 128, 65536, 2048, 128, 65536, 2048, 128, 4096, 128, 4]
+                  + [2, 32, 32, 128, 16, 40, 0, 0, 0.1, 0]))
     attend = lambda **kw: dzlib.dz_paged_attention(paged._ATTENTION.pack(*{**ok, **kw}.values()), None)
     assert dzlib.dz_paged_attention(None, None) == -1 and attend(bytes=8) == -1
     for name in ("q", "k", "v", "tables", "lengths", "out", "status"):
@@ -261,9 +261,9 @@ def test_c_entry_points_check_their_arguments(dzlib):
     for kw in (dict(q=P + 8), dict(k=P + 2), dict(out=P + 4), dict(lengths=P + 2), dict(k_token=132), dict(v_page=-8)):
         assert attend(**kw) == -10, kw
     assert attend(dtype=2) == -1 and attend(window=-1) == -1
-    assert attend(work=0) == -8 and attend(work_bytes=64) == -8
+    assert attend(work=0) == -8 and attend(work_bytes=64) == -8 and attend(counters=0) == -8 and attend(counters=P + 2) == -8
     assert attend(rows=0, q=0) == 0
-    assert dzlib.dz_paged_attention_bytes(2, 32, 32, 128, 16, 4) > 0 and dzlib.dz_paged_attention_bytes(2, 33, 32, 128, 16, 4) == 0
+    assert dzlib.dz_paged_attention_bytes(2, 32, 32, 128, 16, 40) > 0 == dzlib.dz_paged_attention_bytes(2, 32, 32, 128, 16, 4) and dzlib.dz_paged_attention_bytes(2, 33, 32, 128, 16, 4) == 0
 
     names = ("bytes q k v q_out k_out v_out positions slots turns status num_pages q_row q_head k_row k_head v_row v_head q_out_row "
              "q_out_head k_out_page k_out_head k_out_token v_out_page v_out_head v_out_token tokens heads kv_heads dim rot neighbours "
