@@ -102,6 +102,22 @@ def lib():
     return _lib
 
 
+_host = None
+
+
+def host():
+    """The Python extension over the library (csrc/dz_host.cpp).  Raises RuntimeError when it has not been built."""
+    global _host
+    if _host is None:
+        lib()
+        try:
+            from . import _host as made
+        except ImportError as e:
+            raise RuntimeError("deltazip_amd/_host.so is missing or does not fit: build it with `python -m deltazip_amd.build`") from e
+        _host = made
+    return _host
+
+
 def check(code: int, what: str) -> None:
     """Turn a negative return code into the exception the reference API would raise:
     ValueError for argument problems, RuntimeError for launch failures."""

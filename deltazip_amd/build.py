@@ -1,4 +1,4 @@
-"""Builds libdz_amd.so (HIP kernels + C ABI) in-tree for gfx950 with hipcc.
+"""Builds libdz_amd.so (HIP kernels + C ABI) in-tree for gfx950 with hipcc, and _host.so (a Python extension over it).
 
 Run as `python -m deltazip_amd.build`.  The library is written next to this file so that it
 travels with the source tree; nothing is installed into site-packages.
@@ -9,10 +9,12 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libdz_amd.so")
+HOST = os.path.join(HERE, "_host.so")
 
 SOURCES = ["dz_repack.cpp", "dz_kernels.hip", "dz_mdl32.hip", "dz_gemm.hip", "dz_gemm24.hip", "dz_gemm24_rows.hip",
            "dz_gemm24_mixed.hip", "dz_obs.hip", "dz_probe.hip", "dz_attention.hip", "dz_kv.hip"]
@@ -26,7 +28,7 @@ HIPCC_FLAGS = [
 
 
 def build_library(verbose: bool = False, extra_flags=()) -> str:
-    """Compiles every source (one hipcc process each, side by side) and links libdz_amd.so."""
+    """Compiles every source (one hipcc process each, side by side), links libdz_amd.so and builds _host.so."""
     from concurrent.futures import ThreadPoolExecutor
     hipcc = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
     objdir = os.path.join(HERE, "build")
@@ -64,7 +66,18 @@ def build_library(verbose: bool = False, extra_flags=()) -> str:
     with ThreadPoolExecutor(max_workers=min(len(srcs), os.cpu_count() or 4)) as pool:
         objs = list(pool.map(compile_one, srcs))
     run([hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", *objs, "-o", LIB])
+    run(host_command())
     return LIB
+
+
+def host_command():
+    """The compiler's line for the Python extension (plain C++ over torch's headers, linked with libdz_amd.so)."""
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+    libs = [f"-L{d}" for d in library_paths()] + ["-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10"]
+    return [shutil.which("g++") or "c++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{d}" for d in include_paths()),
+            f"-I{sysconfig.get_paths()['include']}", os.path.join(CSRC, "dz_host.cpp"), LIB, *libs, "-Wl,-rpath,$ORIGIN", "-o", HOST]
 
 
 if __name__ == "__main__":

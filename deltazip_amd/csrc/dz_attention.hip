@@ -43,7 +43,7 @@ constexpr int TILE = 32;               // tokens of a step
 constexpr int HEADS = 16;              // heads taken together: columns of a matrix instruction
 constexpr int GROUP_ROWS = 256;        // rows of a launch: four lengths a lane
 #ifndef TGT
-#define TGT 768
+#define TGT 512
 #endif
 constexpr int TARGET = TGT;           // workgroups that the work is cut into, rows' last parts apart
 constexpr int COUNTERS = DZ_ATTENTION_COUNTERS;   // rows of a launch times their items, at most
@@ -156,11 +156,12 @@ __device__ __forceinline__ f4_t get4(const float* at) {
   return f4_t{a[0], a[1], b[0], b[1]};
 }
 
-template <int KC, bool BF>
+template <int KC, bool FULL, bool BF>
 __global__ __launch_bounds__(64 * WAVES, 2) void dz_attention_kernel(const AttnParams P) {
   typedef Type<BF> Ty;
   typedef typename Ty::v8 v8;
   constexpr int NB = (KC + 3) / 4;     // blocks of 128 dims
+  constexpr bool AHEAD = KC <= 6;      // (heads of 256: no registers for it)
   extern __shared__ float lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
   const int items = P.kv_heads * P.head_tiles;
@@ -228,92 +229,110 @@ __global__ __launch_bounds__(64 * WAVES, 2) void dz_attention_kernel(const AttnP
   const int in_page = (1 << P.shift) - 1;
 
   auto walk = [&](auto once) __attribute__((always_inline)) {
-  constexpr bool ONCE = decltype(once)::value;
-  for (; t0 < t1; ++t0) {
-    const int tok = t0 * TILE;
-    const bool edge = tok < first || tok + TILE > end;
-    if (((tok + TILE - 1) >> P.shift) >= page0 + 64) {     // (pages hold 8 tokens or more: a tile has 4 pages at most)
-      const int base = tok >> P.shift;
-      ids = base == page0 + 64 ? next_ids : fetch(base);
-      page0 = base;
-      next_ids = fetch(page0 + 64);
-    }
+    constexpr bool ONCE = decltype(once)::value;
     u4_t kw[2][KC], vw[NB][8];
-#pragma unroll
-    for (int a = 0; a < 2; ++a) {
-      int t = tok + 16 * a + col;
-      t = max(first, min(t, end - 1));
+    // a token's page number, of those that the lanes hold; behind the ends: the nearest token that the row sees
+    auto place = [&](const char* pages, long long page, long long head, long long token, int t, bool edge) {
+      if (edge) t = max(first, min(t, end - 1));
       const unsigned id = __shfl(ids, (t >> P.shift) - page0);
-      const char* at = P.k + id * P.k_page + kvh * P.k_head + (t & in_page) * P.k_token + 16 * g;
+      return pages + id * page + kvh * head + (t & in_page) * token;
+    };
+    auto load_keys = [&](int tok, bool edge) {
 #pragma unroll
-      for (int c = 0; c < KC; ++c) {
-        kw[a][c] = u4_t{0, 0, 0, 0};
-        if (32 * c + 8 * g < P.dim) kw[a][c] = load16<ONCE>(at + 64 * c);
+      for (int a = 0; a < 2; ++a) {
+        const char* at = place(P.k, P.k_page, P.k_head, P.k_token, tok + 16 * a + col, edge);
+#pragma unroll
+        for (int c = 0; c < KC; ++c) {
+          const bool in = FULL || 32 * c + 8 * g < P.dim;
+          kw[a][c] = load16<ONCE>(at + (in ? 64 * c + 16 * g : 0));
+          if (!in) kw[a][c] = u4_t{0, 0, 0, 0};
+        }
       }
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      int t = tok + 16 * (e >> 2) + 4 * g + (e & 3);
-      const bool out = t < first || t >= end;
-      t = max(first, min(t, end - 1));
-      const unsigned id = __shfl(ids, (t >> P.shift) - page0);
-      const char* at = P.v + id * P.v_page + kvh * P.v_head + (t & in_page) * P.v_token + 16 * col;
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        vw[b][e] = u4_t{0, 0, 0, 0};       // (what is masked may be anything: it has no part in the product)
-        if (!out && 128 * b + 8 * col < P.dim) vw[b][e] = load16<ONCE>(at + 256 * b);
+    };
+    auto at_edge = [&](int tok) { return tok < first || tok + TILE > end; };
+    auto turn_page = [&](int tok) {
+      if (((tok + TILE - 1) >> P.shift) >= page0 + 64) {       // (a tile has 4 pages at most)
+        ids = next_ids;
+        page0 += 64;
+        next_ids = fetch(page0 + 64);
       }
-    }
-    float s[8];
-#pragma unroll
-    for (int a = 0; a < 2; ++a) {
-      f4_t c4 = {0, 0, 0, 0};
-#pragma unroll
-      for (int c = 0; c < KC; ++c) c4 = Ty::mma(__builtin_bit_cast(v8, kw[a][c]), q[c], c4);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s[4 * a + i] = c4[i] * P.scale;
-    }
-    if (edge) {
+    };
+    if (AHEAD && t0 < t1) load_keys(t0 * TILE, at_edge(t0 * TILE));
+    for (; t0 < t1; ++t0) {
+      const int tok = t0 * TILE;
+      const bool edge = at_edge(tok);
+      if (!AHEAD) {
+        turn_page(tok);
+        load_keys(tok, edge);
+      }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const int t = tok + 16 * (e >> 2) + 4 * g + (e & 3);
-        if (t < first || t >= end) s[e] = -INFINITY;
+        const char* at = place(P.v, P.v_page, P.v_head, P.v_token, tok + 16 * (e >> 2) + 4 * g + (e & 3), edge);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          const int d = 128 * b + 8 * col;             // (a lane behind the head's end makes values that no one stores)
+          vw[b][e] = load16<ONCE>(at + (FULL && KC % 4 == 0 || d < P.dim ? 2 * d : 0));
+        }
       }
-    }
-    float most = s[0];
+      float s[8];
 #pragma unroll
-    for (int e = 1; e < 8; ++e) most = fmaxf(most, s[e]);
-    most = fmaxf(most, __shfl_xor(most, 16));
-    most = fmaxf(most, __shfl_xor(most, 32));
-    if (__any(most > top + 1.0f)) {
-      const float up = fmaxf(most, top);
-      const float f = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - up);
-      top = up;
-      sum *= f;
+      for (int a = 0; a < 2; ++a) {
+        f4_t c4 = {0, 0, 0, 0};
 #pragma unroll
-      for (int j = 0; j < 8 * NB; ++j) acc[j] *= f;
-    }
-    const float ref = top == -INFINITY ? 0.0f : top - Ty::BIAS;
-    v8 ph, pl;
+        for (int c = 0; c < KC; ++c) c4 = Ty::mma(__builtin_bit_cast(v8, kw[a][c]), q[c], c4);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float p = __builtin_amdgcn_exp2f(s[e] - ref);
-      sum += p;
-      ph[e] = Ty::one(p);
-      pl[e] = Ty::one(p - (float)ph[e]);
-    }
-#pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const unsigned sel = j & 1 ? 0x07060302u : 0x05040100u;
-        u4_t w;
-#pragma unroll
-        for (int x = 0; x < 4; ++x) w[x] = __builtin_amdgcn_perm(vw[b][2 * x + 1][j >> 1], vw[b][2 * x][j >> 1], sel);
-        const v8 vt = __builtin_bit_cast(v8, w);
-        acc[8 * b + j] = Ty::mma(vt, pl, Ty::mma(vt, ph, acc[8 * b + j]));
+        for (int i = 0; i < 4; ++i) s[4 * a + i] = c4[i] * P.scale;
       }
-  }
+      // the next step's keys are on their way while this one's values come in
+      if (AHEAD && t0 + 1 < t1) {
+        turn_page(tok + TILE);
+        load_keys(tok + TILE, at_edge(tok + TILE));
+      }
+      if (edge) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int t = tok + 16 * (e >> 2) + 4 * g + (e & 3);
+          if (t < first || t >= end) {
+            s[e] = -INFINITY;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) vw[b][e] = u4_t{0, 0, 0, 0};   // (what is masked has no part in the product)
+          }
+        }
+      }
+      float most = s[0];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) most = fmaxf(most, s[e]);
+      most = fmaxf(most, __shfl_xor(most, 16));
+      most = fmaxf(most, __shfl_xor(most, 32));
+      if (__any(most > top + 1.0f)) {
+        const float up = fmaxf(most, top);
+        const float f = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - up);
+        top = up;
+        sum *= f;
+#pragma unroll
+        for (int j = 0; j < 8 * NB; ++j) acc[j] *= f;
+      }
+      const float ref = top == -INFINITY ? 0.0f : top - Ty::BIAS;
+      v8 ph, pl;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float p = __builtin_amdgcn_exp2f(s[e] - ref);
+        sum += p;
+        ph[e] = Ty::one(p);
+        pl[e] = Ty::one(p - (float)ph[e]);
+      }
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const unsigned sel = j & 1 ? 0x07060302u : 0x05040100u;
+          u4_t w;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) w[x] = __builtin_amdgcn_perm(vw[b][2 * x + 1][j >> 1], vw[b][2 * x][j >> 1], sel);
+          const v8 vt = __builtin_bit_cast(v8, w);
+          acc[8 * b + j] = Ty::mma(vt, pl, Ty::mma(vt, ph, acc[8 * b + j]));
+        }
+    }
   };
   if (plan.total * (TILE * 4ll * P.dim) > CACHED)
     walk(std::integral_constant<bool, true>());
@@ -460,10 +479,16 @@ inline long long most_groups(int rows, int items, long long room) {
 }
 
 typedef void (*kernel_t)(const AttnParams);
+template <int KC, bool BF>
+kernel_t kernel_of(int dim) {
+  return dim == 32 * KC ? dz_attention_kernel<KC, true, BF> : dz_attention_kernel<KC, false, BF>;
+}
+inline int chunks_of(int dim) { return dim <= 64 ? 2 : dim <= 96 ? 3 : dim <= 128 ? 4 : dim <= 192 ? 6 : 8; }
 template <bool BF>
 kernel_t kernel_for(int dim) {
-  return dim <= 64 ? dz_attention_kernel<2, BF> : dim <= 96 ? dz_attention_kernel<3, BF> : dim <= 128 ? dz_attention_kernel<4, BF>
-         : dim <= 192 ? dz_attention_kernel<6, BF> : dz_attention_kernel<8, BF>;
+  const int kc = chunks_of(dim);
+  return kc == 2 ? kernel_of<2, BF>(dim) : kc == 3 ? kernel_of<3, BF>(dim) : kc == 4 ? kernel_of<4, BF>(dim)
+         : kc == 6 ? kernel_of<6, BF>(dim) : kernel_of<8, BF>(dim);
 }
 
 inline bool shapes_fit(int rows, int heads, int kv_heads, int dim, int page_size, int pages_per_row) {
@@ -525,8 +550,8 @@ int dz_paged_attention(const dz_attention_args* a, void* stream) {
   const size_t lds = ((sums > joins ? sums : joins + 3) / 4 * 4 + 2 * WAVES * HEADS + 4) * 4;
   P.stat_at = (int)(lds / 4) - (2 * WAVES * HEADS + 4);
   const kernel_t kern = a->dtype == DZ_BF16 ? kernel_for<true>(a->dim) : kernel_for<false>(a->dim);
-  const int which = (a->dim <= 64 ? 0 : a->dim <= 96 ? 1 : a->dim <= 128 ? 2 : a->dim <= 192 ? 3 : 4) * 2 + a->dtype;
-  static std::atomic<unsigned long long> attr_done[10];
+  const int kc = chunks_of(a->dim), which = kc * 4 + (a->dim == 32 * kc) * 2 + a->dtype;
+  static std::atomic<unsigned long long> attr_done[36];        // one per kernel
   if (lds > 65536 && !dz_lds_limit_once(attr_done[which], (const void*)kern, (int)LDS_MOST)) return DZ_ELAUNCH;
   const hipStream_t st = (hipStream_t)stream;
   const int together = group_rows(items);

@@ -19,7 +19,7 @@ import ctypes as C
 import math
 import struct
 from functools import lru_cache
-from typing import Dict, Mapping, Optional, Sequence, Tuple, Union
+from typing import Dict, Mapping, NamedTuple, Optional, Sequence, Tuple, Union
 
 import numpy as np
 import torch
@@ -87,6 +87,7 @@ class RotaryPositions:
             raise ValueError(f"entries of the scaling that {kind!r} has no use for: {sorted(scaling)}")
         self.frequencies = torch.from_numpy(freq)                         # radians per position, float64
         self._turns: Dict[torch.device, torch.Tensor] = {}
+        self._packed: Dict[int, tuple] = {}                               # device index -> what the host's half takes
         if device is not None:
             self.on(device)
 
@@ -100,6 +101,7 @@ class RotaryPositions:
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("RotaryPositions.on(device) has to be called before the capture")
             t = self._turns[device] = (self.frequencies / (2 * math.pi)).to(device)
+            self._packed[device.index] = (t.data_ptr(), self.rotary_dim, int(self.interleaved), self.attention_factor, self.head_dim)
         return t
 
 
@@ -168,6 +170,16 @@ def _pages(name: str, t: torch.Tensor, q: torch.Tensor) -> None:
         raise ValueError(f"{name} holds no pages")
 
 
+_UNPACKED = object()
+
+
+def _place() -> Tuple[int, int, int]:
+    """(current device, current stream, status word of its workspace)."""
+    dev, stream = ops._current_device(), ops._stream()
+    ws = ops._workspaces.get((dev, stream))
+    return dev, stream, (ops._workspace(torch.device("cuda", dev), 1, 256, 32) if ws is None else ws).data_ptr()
+
+
 def _status(device: torch.device) -> int:
     return ops._workspace(device, 1, 256, 32).data_ptr()
 
@@ -182,20 +194,33 @@ def _attention_bytes(rows: int, heads: int, kv_heads: int, dim: int, page_size: 
     return _lib.lib().dz_paged_attention_bytes(rows, heads, kv_heads, dim, page_size, pages_per_row)
 
 
-# (device, stream) -> counters, all zero between calls, and room for the sums of parts
-_spaces: Dict[Tuple[int, int], Tuple[torch.Tensor, torch.Tensor]] = {}
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
 
 
-def _parts_space(device: torch.device, need: int) -> Tuple[torch.Tensor, torch.Tensor]:
+class _Space(NamedTuple):
+    """What rows that are split over workgroups need: counters, all zero between calls, and room for the parts' sums."""
+    counters: torch.Tensor
+    work: torch.Tensor
+    counters_at: int
+    work_at: int
+    work_bytes: int
+
+
+_spaces: Dict[Tuple[int, int], _Space] = {}       # (device, stream)
+
+
+def _parts_space(device: torch.device, need: int) -> _Space:
     """Calls on one stream follow each other and share theirs.  A captured call has its own: its graph may be replayed beside
     anything."""
-    if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(COUNTERS, dtype=torch.int32, device=device), torch.empty(need, dtype=torch.uint8, device=device)
     key = device.index, ops._stream()
-    space = _spaces.get(key)
-    if space is None or space[1].numel() < need:
-        counters = torch.zeros(COUNTERS, dtype=torch.int32, device=device) if space is None else space[0]
-        space = _spaces[key] = counters, torch.empty(max(need, 1 << 20), dtype=torch.uint8, device=device)
+    space = None if _capturing() else _spaces.get(key)
+    if space is None or space.work_bytes < need:
+        counters = torch.zeros(COUNTERS, dtype=torch.int32, device=device) if space is None else space.counters
+        size = need if _capturing() else max(need, 1 << 20)
+        work = torch.empty(size, dtype=torch.uint8, device=device)
+        space = _Space(counters, work, counters.data_ptr(), work.data_ptr(), size)
+        if not _capturing():
+            _spaces[key] = space
     return space
 
 
@@ -216,6 +241,13 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     tokens.  A length beyond its table is cut; a page number outside the pool is read as page 0; either is reported through the
     status word.  The order of a row's sums follows the lengths of all rows of the call (the work is cut by them,
     256 rows at a time): the same lengths give the same bits."""
+    if out is None and q.is_cuda:
+        dev, stream, status = _place()
+        space = None if _capturing() else _spaces.get((dev, stream))
+        out = _lib.host().attend(q, k_pages, v_pages, block_tables, lengths, scale, window, dev, stream, status,
+                                 *((0, 0, 0) if space is None else space[2:]))
+        if out is not None:
+            return out
     ops._need_cuda(q, k_pages, v_pages, block_tables, lengths, out)
     if _elsewhere(q):
         with torch.cuda.device(q.device):
@@ -250,11 +282,11 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if rows == 0:
         return out
     need = _attention_bytes(rows, heads, kv_heads, dim, page_size, width)
-    counters, work = _parts_space(q.device, need) if need else (None, None)
+    space = _parts_space(q.device, need) if need else None
     ks, vs = k_pages.stride(), v_pages.stride()
     args = _ATTENTION.pack(
         _ATTENTION.size, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), block_tables.data_ptr(), lengths.data_ptr(),
-        out.data_ptr(), work.data_ptr() if need else 0, counters.data_ptr() if need else 0, _status(q.device), need, pages, _stride(q, 0), _stride(q, 1),
+        out.data_ptr(), space.work_at if need else 0, space.counters_at if need else 0, _status(q.device), need, pages, _stride(q, 0), _stride(q, 1),
         ks[0] if pages > 1 else 0, ks[1] if kv_heads > 1 else 0, ks[2], vs[0] if pages > 1 else 0, vs[1] if kv_heads > 1 else 0,
         vs[2], _stride(out, 0), _stride(out, 1), block_tables.stride(0) if rows > 1 else 0, rows, heads, kv_heads, dim, page_size,
         width, min(int(window), (1 << 31) - 1), _TYPES[q.dtype], dim ** -0.5 if scale is None else scale, 0)
@@ -273,7 +305,7 @@ def _rotate(q, k, v, positions, slots, rope, q_out, k_out, v_out, page_size, num
         num_pages, _stride(q, 0), _stride(q, 1), *((0, 0) if k is None else (_stride(k, 0), _stride(k, 1))),
         *((0, 0) if v is None else (_stride(v, 0), _stride(v, 1))), _stride(q_out, 0), _stride(q_out, 1),
         *((0, 0, 0) if k is None else strides(k_out)), *((0, 0, 0) if v is None else strides(v_out)),
-        tokens, heads, 0 if k is None else k.shape[1], dim, 0 if rope is None else rope.rotary_dim,
+        tokens, 0 if rope is None and q_out is q else heads, 0 if k is None else k.shape[1], dim, 0 if rope is None else rope.rotary_dim,
         0 if rope is None else int(rope.interleaved), page_size, _TYPES[q.dtype], 1.0 if rope is None else rope.attention_factor, 0)
     _lib.check(_lib.lib().dz_rotary(args, ops._stream()), "dz_rotary")
 
@@ -284,6 +316,11 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     value); returns new tensors, or writes `out` = (q, k): the inputs themselves (in place, as
     serving/csrc/pos_encoding does) or memory of their own.  Rows and heads may have any stride of an even number of values;
     with strides, sizes and half of rotary_dim multiples of eight, requests are four times as wide."""
+    if out is None and q.is_cuda:
+        dev, stream = ops._current_device(), ops._stream()
+        made = _lib.host().rotate(q, k, None, positions, None, rope._packed.get(dev), None, None, False, dev, stream, 0)
+        if made is not None:
+            return made
     ops._need_cuda(q, k, positions)
     if _elsewhere(q):
         with torch.cuda.device(q.device):
@@ -327,6 +364,12 @@ def append_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torc
     same); one beyond the pages neither, and is reported through the status word.  rope None: nothing is turned, and q is
     returned as it is.  No two tokens may have one slot: what is there afterwards may be parts of either.  Strides as
     for `rotary`."""
+    if q.is_cuda and (out is None or out is q):
+        dev, stream, status = _place()
+        turns = None if rope is None else rope._packed.get(dev, _UNPACKED)
+        made = _lib.host().rotate(q, k, v, positions, slots, turns, k_pages, v_pages, out is q or rope is None, dev, stream, status)
+        if made is not None:
+            return made
     ops._need_cuda(q, k, v, positions, slots, k_pages, v_pages, out)
     if _elsewhere(q):
         with torch.cuda.device(q.device):
@@ -371,7 +414,13 @@ def copy_pages(pools: Union[torch.Tensor, Sequence[torch.Tensor]], pairs) -> Non
     [pages, ...] of one shape, type and stride, pages contiguous and of a multiple of 16 bytes.  pairs: host integers [n, 2],
     a tensor or a sequence; they are read before the call returns (a graph that captures the call copies the same
     pages at every replay).  All copies run side by side: no page may be written twice, or be both read and written."""
+    if isinstance(pairs, list):
+        pairs = np.asarray(pairs)
+    if isinstance(pairs, np.ndarray) and pairs.dtype == np.int64:
+        pairs = torch.from_numpy(pairs)
     stacked = isinstance(pools, torch.Tensor)
+    if stacked and pools.is_cuda and _lib.host().copy(pools, pairs, ops._current_device(), ops._stream()):
+        return
     if stacked:
         if pools.dim() < 2:
             raise ValueError("pools must be [pools, pages, ...]")
