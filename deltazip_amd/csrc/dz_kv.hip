@@ -38,25 +38,35 @@ __device__ __forceinline__ uint16_t narrow(float x) {
 }
 
 template <int N>
-struct Words;
-template <>
-struct Words<8> {
-  typedef uint16_t type __attribute__((ext_vector_type(8)));
+struct Words {
+  typedef uint16_t type __attribute__((ext_vector_type(N)));
 };
 template <>
-struct Words<2> {
-  typedef uint16_t type __attribute__((ext_vector_type(2)));
+struct Words<1> {
+  typedef uint16_t type;
 };
+// Stores keep nothing in the caches: 2047 tokens of 40 heads of 80 9.7 -> 9.1 us, 128 of 96 heads of 128 3.42 -> 3.28, heads of 192
+// of which 20 are turned 48 -> 35; attention right behind them takes what it took.
+template <typename W>
+__device__ __forceinline__ void put(const W& w, char* to) {
+  __builtin_nontemporal_store(w, (W*)to);
+}
+template <typename W>
+__device__ __forceinline__ uint16_t part(const W& w, int e) {
+  if constexpr (sizeof(W) == 2)
+    return w;
+  else
+    return w[e];
+}
 
-// One head's share of thread x of X.  VEC: values of a request, 8 where the sizes and strides allow it, or 2
-// (of a pair of halves: 1).
-template <bool BF, bool NEIGHBOURS, bool WIDE>
+// One head's turned values, thread x of X: V values of a request, or with halves apart V of either half.
+template <bool BF, bool NEIGHBOURS, int V>
 __device__ __forceinline__ void turn_head(const RotaryParams& P, const char* from, char* to, const float2* table, int x, int X) {
-  if (NEIGHBOURS) {
-    constexpr int V = WIDE ? 8 : 2;
-    typedef typename Words<V>::type W;
+  typedef typename Words<V>::type W;
+  if constexpr (NEIGHBOURS) {
     for (int c = x; c < P.rot / V; c += X) {
-      W w = *(const W*)(from + c * V * 2), o;
+      const W w = *(const W*)(from + c * V * 2);
+      W o;
 #pragma unroll
       for (int e = 0; e < V; e += 2) {
         const float2 cs = table[(c * V + e) / 2];
@@ -64,47 +74,43 @@ __device__ __forceinline__ void turn_head(const RotaryParams& P, const char* fro
         o[e] = narrow<BF>(a * cs.x - b * cs.y);
         o[e + 1] = narrow<BF>(b * cs.x + a * cs.y);
       }
-      *(W*)(to + c * V * 2) = o;
-    }
-  } else if (WIDE) {
-    typedef typename Words<8>::type W;
-    const int half = P.rot / 2;
-    for (int c = x; c < half / 8; c += X) {
-      const W w = *(const W*)(from + c * 16), u = *(const W*)(from + half * 2 + c * 16);
-      W o, r;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float2 cs = table[c * 8 + e];
-        const float a = wide<BF>(w[e]), b = wide<BF>(u[e]);
-        o[e] = narrow<BF>(a * cs.x - b * cs.y);
-        r[e] = narrow<BF>(b * cs.x + a * cs.y);
-      }
-      *(W*)(to + c * 16) = o;
-      *(W*)(to + half * 2 + c * 16) = r;
+      put(o, to + c * V * 2);
     }
   } else {
     const int half = P.rot / 2;
-    for (int i = x; i < half; i += X) {
-      const float2 cs = table[i];
-      const float a = wide<BF>(((const uint16_t*)from)[i]), b = wide<BF>(((const uint16_t*)from)[half + i]);
-      ((uint16_t*)to)[i] = narrow<BF>(a * cs.x - b * cs.y);
-      ((uint16_t*)to)[half + i] = narrow<BF>(b * cs.x + a * cs.y);
+    for (int c = x; c < half / V; c += X) {
+      const W w = *(const W*)(from + c * V * 2), u = *(const W*)(from + (half + c * V) * 2);
+      W o, r;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float2 cs = table[c * V + e];
+        const float a = wide<BF>(part(w, e)), b = wide<BF>(part(u, e));
+        const uint16_t y = narrow<BF>(a * cs.x - b * cs.y), z = narrow<BF>(b * cs.x + a * cs.y);
+        if constexpr (V == 1)
+          o = y, r = z;
+        else
+          o[e] = y, r[e] = z;
+      }
+      put(o, to + c * V * 2);
+      put(r, to + (half + c * V) * 2);
     }
   }
 }
 
-// Values [lo, dim) of a head, as they are; the threads that have turned none begin.
-template <bool WIDE>
+// Values [lo, dim) of a head, as they are; the threads behind the `used` that have turned some begin.
+template <int V>
 __device__ __forceinline__ void copy_head(const char* from, char* to, int lo, int dim, int used, int x, int X) {
-  constexpr int V = WIDE ? 8 : 2;
+  typedef typename Words<V>::type W;
+  typedef typename Words<2>::type W2;
   x -= used % X;
   if (x < 0) x += X;
-  typedef typename Words<V>::type W;
-  for (int c = lo / V + x; c < dim / V; c += X) *(W*)(to + c * V * 2) = *(const W*)(from + c * V * 2);
+  const int begin = (lo + V - 1) / V;                  // (whole requests from here)
+  for (int c = begin + x; c < dim / V; c += X) put(*(const W*)(from + c * V * 2), to + c * V * 2);
+  for (int d = lo + 2 * x; d < begin * V; d += 2 * X) put(*(const W2*)(from + d * 2), to + d * 2);
 }
 
 // A workgroup takes one token and every gridDim.y-th of its groups of blockDim.y heads.
-template <bool BF, bool NEIGHBOURS, bool WIDE>
+template <bool BF, bool NEIGHBOURS, int TURN, int COPY>
 __global__ __launch_bounds__(256) void dz_rotary_kernel(const RotaryParams P) {
   __shared__ float2 table[128];
   const int t = blockIdx.x, tid = threadIdx.y * blockDim.x + threadIdx.x;
@@ -127,13 +133,13 @@ __global__ __launch_bounds__(256) void dz_rotary_kernel(const RotaryParams P) {
   __syncthreads();
   const long long page = slot >> P.shift, at = slot & ((1 << P.shift) - 1);
   const int total = P.heads + (P.k ? P.kv_heads : 0) + (P.v ? P.kv_heads : 0);
-  const int turned = NEIGHBOURS ? P.rot / (WIDE ? 8 : 2) : P.rot / (WIDE ? 16 : 2);       // requests (or pairs of them) of a head
+  const int turned = P.rot / (NEIGHBOURS ? TURN : 2 * TURN);       // requests (or pairs of them) of a head
   for (int h = blockIdx.y * blockDim.y + threadIdx.y; h < total; h += gridDim.y * blockDim.y) {
     if (h < P.heads) {
       const char* from = P.q + t * P.q_row + h * P.q_head;
       char* to = P.q_out + t * P.qo_row + h * P.qo_head;
-      turn_head<BF, NEIGHBOURS, WIDE>(P, from, to, table, threadIdx.x, blockDim.x);
-      copy_head<WIDE>(from, to, P.rot, P.dim, turned, threadIdx.x, blockDim.x);
+      turn_head<BF, NEIGHBOURS, TURN>(P, from, to, table, threadIdx.x, blockDim.x);
+      copy_head<COPY>(from, to, P.rot, P.dim, turned, threadIdx.x, blockDim.x);
     } else if (P.k && h < P.heads + P.kv_heads) {
       const int kh = h - P.heads;
       const char* from = P.k + t * P.k_row + kh * P.k_head;
@@ -144,12 +150,12 @@ __global__ __launch_bounds__(256) void dz_rotary_kernel(const RotaryParams P) {
       } else {
         to = P.k_out + t * P.ko_token + kh * P.ko_head;
       }
-      turn_head<BF, NEIGHBOURS, WIDE>(P, from, to, table, threadIdx.x, blockDim.x);
-      copy_head<WIDE>(from, to, P.rot, P.dim, turned, threadIdx.x, blockDim.x);
+      turn_head<BF, NEIGHBOURS, TURN>(P, from, to, table, threadIdx.x, blockDim.x);
+      copy_head<COPY>(from, to, P.rot, P.dim, turned, threadIdx.x, blockDim.x);
     } else {
       if (slot < 0) continue;
       const int vh = h - P.heads - (P.k ? P.kv_heads : 0);
-      copy_head<WIDE>(P.v + t * P.v_row + vh * P.v_head, P.v_out + page * P.vo_page + vh * P.vo_head + at * P.vo_token, 0, P.dim, 0,
+      copy_head<COPY>(P.v + t * P.v_row + vh * P.v_head, P.v_out + page * P.vo_page + vh * P.vo_head + at * P.vo_token, 0, P.dim, 0,
                       threadIdx.x, blockDim.x);
     }
   }
@@ -165,21 +171,17 @@ struct CopyParams {
 };
 static_assert(sizeof(CopyParams) <= 4000, "kernel arguments");
 
-constexpr int COPY_EACH = 4;           // requests of a thread
-
+// A request of 16 bytes a thread: 2 and 4 of them took 6 and 25 % longer (16 pages of 64 pools of 128 KiB: 43.6, 46, 54 us;
+// the stores kept in the caches as well: 54).  ONCE: loads that keep nothing either, 555 -> 541 us for 700 pages of 32 KiB, but
+// 2.7 -> 3.7 for 4 pages of 48 pools, which were in the caches.
+template <bool ONCE>
 __global__ __launch_bounds__(256) void dz_copy_pages_kernel(const CopyParams P) {
   char* pool = P.pools[blockIdx.z];
   const int2 pair = P.pairs[blockIdx.y];
-  const u4_t* from = (const u4_t*)(pool + pair.x * P.page_stride);
-  u4_t* to = (u4_t*)(pool + pair.y * P.page_stride);
-  const int c = blockIdx.x * (256 * COPY_EACH) + threadIdx.x;
-  u4_t w[COPY_EACH];
-#pragma unroll
-  for (int i = 0; i < COPY_EACH; ++i)
-    if (c + 256 * i < P.chunks) w[i] = from[c + 256 * i];
-#pragma unroll
-  for (int i = 0; i < COPY_EACH; ++i)
-    if (c + 256 * i < P.chunks) to[c + 256 * i] = w[i];
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= P.chunks) return;
+  const u4_t* from = (const u4_t*)(pool + pair.x * P.page_stride) + c;
+  __builtin_nontemporal_store(ONCE ? __builtin_nontemporal_load(from) : *from, (u4_t*)(pool + pair.y * P.page_stride) + c);
 }
 
 }  // namespace
@@ -211,7 +213,7 @@ int dz_rotary(const dz_rotary_args* a, void* stream) {
   P.capacity = a->slots ? a->num_pages * a->page_size : 0;
   P.heads = a->heads, P.kv_heads = a->kv_heads, P.dim = a->dim, P.rot = a->rot, P.factor = a->factor;
 
-  // requests of 16 bytes where every row and every half of the turned values begins on one
+  // requests of 16 bytes where every row, and every half of the turned values, begins on one
   uintptr_t bits = (uintptr_t)P.q | (uintptr_t)P.k | (uintptr_t)P.v | (uintptr_t)P.q_out | (uintptr_t)P.k_out | (uintptr_t)P.v_out;
   const long long strides[] = {P.q_row, P.q_head, P.k_row, P.k_head, P.v_row, P.v_head, P.qo_row, P.qo_head,
                                P.ko_page, P.ko_head, P.ko_token, P.vo_page, P.vo_head, P.vo_token};
@@ -220,19 +222,22 @@ int dz_rotary(const dz_rotary_args* a, void* stream) {
     bits |= (uintptr_t)s;
   }
   if (bits & 3) return DZ_EALIGN;
-  const bool whole = !(bits & 15) && a->dim % 8 == 0 && a->rot % (a->neighbours ? 8 : 16) == 0;
-  int units = whole ? (a->neighbours ? a->dim / 8 : a->dim / 8 - a->rot / 16) : a->dim / 2;
+  const int copy = !(bits & 15) && a->dim % 8 == 0;
+  const int turn = a->neighbours ? (copy && a->rot % 8 == 0 ? 8 : 2) : copy && a->rot % 16 == 0 ? 8 : a->rot % 4 == 0 ? 2 : 1;
+  // a thread per request of a head
+  int units = a->rot / (a->neighbours ? turn : 2 * turn) + (a->dim - a->rot) / (copy ? 8 : 2);
   units = units < 1 ? 1 : units > 64 ? 64 : units;
   const int each = 256 / units, total = P.heads + (P.k ? P.kv_heads : 0) + (P.v ? P.kv_heads : 0);
   if (total == 0) return DZ_OK;
-  int slices = (total + each - 1) / each;
-  if (slices > 65535) slices = 65535;
+  const int slices = (total + each - 1) / each;
   typedef void (*kernel_t)(const RotaryParams);
-  static const kernel_t kernels[8] = {dz_rotary_kernel<false, false, false>, dz_rotary_kernel<false, false, true>,
-                                      dz_rotary_kernel<false, true, false>,  dz_rotary_kernel<false, true, true>,
-                                      dz_rotary_kernel<true, false, false>,  dz_rotary_kernel<true, false, true>,
-                                      dz_rotary_kernel<true, true, false>,   dz_rotary_kernel<true, true, true>};
-  const kernel_t kern = kernels[(a->dtype == DZ_BF16) * 4 + (a->neighbours != 0) * 2 + whole];
+  static const kernel_t kernels[2][8] = {
+      {dz_rotary_kernel<false, false, 8, 8>, dz_rotary_kernel<false, false, 2, 8>, dz_rotary_kernel<false, false, 1, 8>, dz_rotary_kernel<false, false, 2, 2>,
+       dz_rotary_kernel<false, false, 1, 2>, dz_rotary_kernel<false, true, 8, 8>, dz_rotary_kernel<false, true, 2, 8>, dz_rotary_kernel<false, true, 2, 2>},
+      {dz_rotary_kernel<true, false, 8, 8>, dz_rotary_kernel<true, false, 2, 8>, dz_rotary_kernel<true, false, 1, 8>, dz_rotary_kernel<true, false, 2, 2>,
+       dz_rotary_kernel<true, false, 1, 2>, dz_rotary_kernel<true, true, 8, 8>, dz_rotary_kernel<true, true, 2, 8>, dz_rotary_kernel<true, true, 2, 2>}};
+  const int which = a->neighbours ? (turn == 8 ? 5 : copy ? 6 : 7) : turn == 8 ? 0 : copy ? (turn == 2 ? 1 : 2) : turn == 2 ? 3 : 4;
+  const kernel_t kern = kernels[a->dtype == DZ_BF16][which];
   hipLaunchKernelGGL(kern, dim3(a->tokens, slices), dim3(units, each), 0, (hipStream_t)stream, P);
   return hipGetLastError() == hipSuccess ? DZ_OK : DZ_ELAUNCH;
 }
@@ -242,11 +247,12 @@ int dz_copy_pages(void* const* pools, int npools, long long page_stride, long lo
   if (npools < 0 || npairs < 0 || num_pages < 0 || page_bytes < 0) return DZ_EPAGES;
   if (npools == 0 || npairs == 0 || page_bytes == 0) return DZ_OK;
   if (!pools || !pairs) return DZ_EINVAL;
-  if (page_bytes % 16 || page_stride % 16 || page_stride < page_bytes || page_bytes / 16 > 0x7fffffff - 256 * COPY_EACH) return DZ_EPAGES;
+  if (page_bytes % 16 || page_stride % 16 || page_stride < page_bytes || page_bytes / 16 > 0x7fffffff - 256) return DZ_EPAGES;
   for (int i = 0; i < npools; ++i)
     if (!pools[i] || ((uintptr_t)pools[i] & 15)) return DZ_EALIGN;
   for (int i = 0; i < 2 * npairs; ++i)
     if (pairs[i] < 0 || pairs[i] >= num_pages) return DZ_EINVAL;
+  const bool once = (double)page_bytes * npools * npairs > (double)(256 << 20);     // (more than the last cache holds)
   CopyParams P;
   P.page_stride = page_stride;
   P.chunks = (int)(page_bytes / 16);
@@ -256,8 +262,8 @@ int dz_copy_pages(void* const* pools, int npools, long long page_stride, long lo
     for (int l0 = 0; l0 < npools; l0 += COPY_POOLS) {
       const int nl = npools - l0 < COPY_POOLS ? npools - l0 : COPY_POOLS;
       for (int i = 0; i < nl; ++i) P.pools[i] = (char*)pools[l0 + i];
-      const int blocks = (P.chunks + 256 * COPY_EACH - 1) / (256 * COPY_EACH);
-      hipLaunchKernelGGL(dz_copy_pages_kernel, dim3(blocks, np, nl), dim3(256), 0, (hipStream_t)stream, P);
+      const int blocks = (P.chunks + 255) / 256;
+      hipLaunchKernelGGL(once ? dz_copy_pages_kernel<true> : dz_copy_pages_kernel<false>, dim3(blocks, np, nl), dim3(256), 0, (hipStream_t)stream, P);
     }
   }
   return hipGetLastError() == hipSuccess ? DZ_OK : DZ_ELAUNCH;
