@@ -21,7 +21,7 @@
 // weight then has 16 (bf16) or 22 (fp16) bits, and the output's error is its own rounding.  Sums are fp32.
 //
 // The work is cut on the device, which alone knows the lengths: every wavefront reads the lengths of the launch's
-// rows (up to 256, four a lane), and takes for the tiles of a workgroup as many as make about `target` workgroups.
+// rows (up to 256, up to four a lane), and takes for the tiles of a workgroup as many as make about `target` workgroups.
 // Parts of a row are joined by the workgroup that is done last of them (a counter per row and item says which),
 // in the order of the tokens, so results do not depend on timing.
 #include <hip/hip_runtime.h>
@@ -48,7 +48,8 @@ constexpr int GROUP_ROWS = 256;        // rows of a launch: four lengths a lane
 constexpr int TARGET = TGT;           // workgroups that the work is cut into, rows' last parts apart
 constexpr int COUNTERS = DZ_ATTENTION_COUNTERS;   // rows of a launch times their items, at most
 constexpr size_t LDS_MOST = 96 << 10;
-constexpr long long CACHED = 64ll << 20;   // bytes of keys and values
+constexpr float CACHED = 64 << 20;     // bytes of keys and values
+constexpr int AT_ONCE = 16;            // parts that a join asks for at a time
 
 struct AttnParams {
   const char *q, *k, *v;
@@ -59,7 +60,7 @@ struct AttnParams {
   unsigned* status;
   long long q_row, q_head, k_page, k_head, k_token, v_page, v_head, v_token, out_row, out_head, table_row;   // bytes; out, table: elements
   unsigned num_pages;
-  int rows, heads, kv_heads, share, head_tiles, dim, shift, pages_per_row, window, part_floats, stat_at;
+  int rows, heads, kv_heads, share, head_tiles, dim, shift, pages_per_row, window, part_floats, stat_at, single;
   float scale;
 };
 
@@ -95,46 +96,78 @@ __device__ __forceinline__ int tiles_of(const AttnParams& P, int length) {
   return end > first ? (end + TILE - 1) / TILE - first / TILE : 0;
 }
 
-// The parts of the launch's rows, as every wavefront works them out for itself.  Lane l has rows 4 l .. 4 l + 3.
-struct Plan {
-  int tiles[4], before[4];             // tiles of a row; parts of the rows in front of it
-  int each;                            // most tiles of a part
-  long long total;                     // tiles of all rows and items
-  __device__ __forceinline__ int parts(int r) const { return tiles[r] ? (tiles[r] + each - 1) / each : 1; }   // (an empty row has its zeros written)
+// Sums over the lanes in front of and at each, by shifts within the wavefront's rows of 16 lanes and broadcasts of their last ones.
+template <typename T>
+__device__ __forceinline__ T scan_add(T x) {
+  auto add = [&](auto ctrl, auto mask) {
+    x += __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(ctrl)::value, decltype(mask)::value, 0xf, false));
+  };
+  using std::integral_constant;
+  add(integral_constant<int, 0x111>(), integral_constant<int, 0xf>());     // row_shr:1, 2, 4, 8
+  add(integral_constant<int, 0x112>(), integral_constant<int, 0xf>());
+  add(integral_constant<int, 0x114>(), integral_constant<int, 0xf>());
+  add(integral_constant<int, 0x118>(), integral_constant<int, 0xf>());
+  add(integral_constant<int, 0x142>(), integral_constant<int, 0xa>());     // row_bcast:15
+  add(integral_constant<int, 0x143>(), integral_constant<int, 0xc>());     // row_bcast:31
+  return x;
+}
+
+// The part of the launch that a workgroup is, as each of its wavefronts works it out: part `nth` of `nparts` of `row`.
+struct Part {
+  int row, length, nth, nparts;
+  bool once;                           // whether the launch's keys and values are more than the caches keep
 };
 
-__device__ __forceinline__ Plan make_plan(const AttnParams& P, int lane) {
-  Plan p;
-  int mine = 0;
+__device__ __forceinline__ Part find_part(const AttnParams& P, int part, int items, int lane) {
+  Part found = {-1, 0, 0, 1, false};
+  if (P.single) {                      // (no row can have a second part)
+    found.row = part;
+    found.length = P.lengths[part];
+    return found;
+  }
+  // lane l has rows l * each_lane .. ; their tiles, and the parts in front of them
+  const int each_lane = (P.rows + 63) / 64, row0 = lane * each_lane;
+  int length[4], tiles[4], before[4];
+  float mine = 0.0f;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) length[r] = r < each_lane && row0 + r < P.rows ? P.lengths[row0 + r] : 0;
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
-    const int row = 4 * lane + r;
-    p.tiles[r] = row < P.rows ? tiles_of(P, P.lengths[row]) : 0;
-    mine += p.tiles[r];
+    tiles[r] = tiles_of(P, length[r]);
+    mine += (float)tiles[r];
   }
-  long long total = mine;
-#pragma unroll
-  for (int d = 32; d; d >>= 1) total += __shfl_xor(total, d);
-  const long long items = (long long)P.kv_heads * P.head_tiles;
-  p.total = total * items;
-  long long each = (p.total + TARGET - 1) / TARGET;
-  each = (each + WAVES - 1) / WAVES * WAVES;
-  p.each = each < WAVES ? WAVES : (int)each;
-  int sum = 0;
+  const float total = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, scan_add(mine)), 63)) * (float)items;
+  found.once = total * (TILE * 4.0f) * (float)P.dim > CACHED;
+  // tiles of a part, in whole steps of the workgroup; rounded up, so that TARGET parts and one a row suffice whatever the
+  // sums' rounding
+  float most = ceilf(total * (1.00001f / (WAVES * TARGET)));
+  const unsigned each = WAVES * (unsigned)fminf(fmaxf(most, 1.0f), (float)(1 << 24));
+  int sum = 0, parts[4];
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
-    p.before[r] = sum;
-    sum += 4 * lane + r < P.rows ? p.parts(r) : 0;
+    if (r < each_lane) {
+      parts[r] = row0 + r < P.rows ? max(1, (int)((tiles[r] + each - 1) / each)) : 0;   // (an empty row has its zeros written)
+    } else {
+      parts[r] = 0;
+    }
+    before[r] = sum;
+    sum += parts[r];
   }
-  int upto = sum;
+  const int front = scan_add(sum) - sum;
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int o = __shfl_up(upto, d);
-    if (lane >= d) upto += o;
+  for (int r = 0; r < 4; ++r) {
+    if (r >= each_lane) break;
+    const int at = part - front - before[r];
+    const unsigned long long hit = __ballot(at >= 0 && at < parts[r]);
+    if (hit) {
+      const int src = __builtin_ctzll(hit);
+      found.row = src * each_lane + r;
+      found.length = __builtin_amdgcn_readlane(length[r], src);
+      found.nth = __builtin_amdgcn_readlane(at, src);
+      found.nparts = __builtin_amdgcn_readlane(parts[r], src);
+    }
   }
-#pragma unroll
-  for (int r = 0; r < 4; ++r) p.before[r] += upto - sum;
-  return p;
+  return found;
 }
 
 // Keys and values of a call pass through once: loads that keep nothing in the caches read 7.1 TB/s where others read 6.2.
@@ -157,7 +190,7 @@ __device__ __forceinline__ f4_t get4(const float* at) {
 }
 
 template <int KC, bool FULL, bool BF>
-__global__ __launch_bounds__(64 * WAVES, 2) void dz_attention_kernel(const AttnParams P) {
+__global__ __launch_bounds__(64 * WAVES, KC == 8 && !FULL ? 1 : 2) void dz_attention_kernel(const AttnParams P) {
   typedef Type<BF> Ty;
   typedef typename Ty::v8 v8;
   constexpr int NB = (KC + 3) / 4;     // blocks of 128 dims
@@ -169,22 +202,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void dz_attention_kernel(const AttnP
   const int kvh = item / P.head_tiles, head0 = kvh * P.share + item % P.head_tiles * HEADS;
   const int nheads = min(HEADS, (kvh + 1) * P.share - head0);
 
-  // the row whose part this is
-  const Plan plan = make_plan(P, lane);
-  int row = -1, nth = 0, nparts = 0;
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int n = plan.parts(r), at = part - plan.before[r];
-    const unsigned long long hit = __ballot(4 * lane + r < P.rows && at >= 0 && at < n);
-    if (hit) {
-      const int src = __builtin_ctzll(hit);
-      row = 4 * src + r;
-      nth = __builtin_amdgcn_readlane(at, src);
-      nparts = __builtin_amdgcn_readlane(n, src);
-    }
-  }
+  const Part mine = find_part(P, part, items, lane);
+  const int row = mine.row, length = mine.length, nth = mine.nth, nparts = mine.nparts;
   if (row < 0) return;
-  const int length = P.lengths[row];
   int first, end;
   span(P, length, first, end);
   if (length > end && nth == 0 && item == 0 && threadIdx.x == 0) atomicOr(P.status, 4u);
@@ -334,7 +354,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void dz_attention_kernel(const AttnP
         }
     }
   };
-  if (plan.total * (TILE * 4ll * P.dim) > CACHED)
+  if (mine.once)
     walk(std::integral_constant<bool, true>());
   else
     walk(std::integral_constant<bool, false>());
@@ -343,7 +363,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void dz_attention_kernel(const AttnP
 
   // the four wavefronts' sums joined: [wave][head][dim], then maxima and sums
   const int ld = P.dim + 4;
-  float* mine = lds + wave * nheads * ld;
+  float* sums = lds + wave * nheads * ld;
   float* stat = lds + P.stat_at;
   if (col < nheads) {
 #pragma unroll
@@ -352,8 +372,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void dz_attention_kernel(const AttnP
       for (int i = 0; i < 4; ++i) {
         const int d = 128 * b + 8 * (4 * g + i);
         if (d < P.dim) {
-          *(f4_t*)(mine + col * ld + d) = f4_t{acc[8 * b][i], acc[8 * b + 1][i], acc[8 * b + 2][i], acc[8 * b + 3][i]};
-          *(f4_t*)(mine + col * ld + d + 4) = f4_t{acc[8 * b + 4][i], acc[8 * b + 5][i], acc[8 * b + 6][i], acc[8 * b + 7][i]};
+          *(f4_t*)(sums + col * ld + d) = f4_t{acc[8 * b][i], acc[8 * b + 1][i], acc[8 * b + 2][i], acc[8 * b + 3][i]};
+          *(f4_t*)(sums + col * ld + d + 4) = f4_t{acc[8 * b + 4][i], acc[8 * b + 5][i], acc[8 * b + 6][i], acc[8 * b + 7][i]};
         }
       }
     if (g == 0) {
@@ -409,65 +429,65 @@ __global__ __launch_bounds__(64 * WAVES, 2) void dz_attention_kernel(const AttnP
   if (!*flag) return;
   const size_t step = (size_t)items * P.part_floats;
   const float* from = P.parts + ((size_t)(part - nth) * items + item) * P.part_floats;
-  // factors of the parts, [head][part], and behind them the heads' sums
-  float* factor = lds;
-  float* total = stat;
-  for (int h = wave; h < nheads; h += WAVES) {
-    const float* p = from + nheads * P.dim + 2 * h;
-    float m = -INFINITY;
-    for (int s = lane; s < nparts; s += 64) m = fmaxf(m, get(p + s * step)[0]);
-#pragma unroll
-    for (int d = 32; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
-    float l = 0.0f;
-    for (int s = lane; s < nparts; s += 64) {
-      const f2_t ml = get(p + s * step);
-      const float f = ml[0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[0] - m);
-      factor[h * nparts + s] = f;
-      l += ml[0] == -INFINITY ? 0.0f : f * ml[1];
-    }
-#pragma unroll
-    for (int d = 32; d; d >>= 1) l += __shfl_xor(l, d);
-    if (lane == 0) total[h] = l;
-  }
-  __syncthreads();
-  // threads that have no values of their own share the parts of others': slice c of `slices`
+  // a thread takes four values of a head over every `slices`-th part, sixteen on their way at a time; threads that have none
+  // of their own share the parts of others'
   int slices = 1;
   while (2 * slices * spots <= 64 * WAVES) slices *= 2;
-  float* shared = lds + (nheads * nparts + 3) / 4 * 4;   // [slice][spot]
+  float* shared = lds;                                // [slice][spot]: values, maximum and sum
   for (int x = threadIdx.x; x < spots * slices; x += 64 * WAVES) {
-    const int spot = x % spots, c = x / spots, h = spot / quads, d = spot % quads * 4;
-    const float *p = from + h * P.dim + d, *f = factor + h * nparts;
+    const int spot = x % spots, h = spot / quads, d = spot % quads * 4;
+    const float *p = from + h * P.dim + d, *stats = from + nheads * P.dim + 2 * h;
+    float m = -INFINITY, l = 0.0f;
     f4_t o = {0, 0, 0, 0};
-    int s = c;
-    for (; s + 7 * slices < nparts; s += 8 * slices) {
-      f4_t w[8];
+    for (int s = x / spots; s < nparts; s += AT_ONCE * slices) {
+      f4_t w[AT_ONCE];
+      f2_t ml[AT_ONCE];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = get4(p + (s + i * slices) * step);
+      for (int i = 0; i < AT_ONCE; ++i) {
+        const int at = min(s + i * slices, nparts - 1);
+        ml[i] = get(stats + at * step);
+        w[i] = get4(p + at * step);
+      }
+      float up = m;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float fs = f[s + i * slices];
-        o += fs == 0.0f ? f4_t{0, 0, 0, 0} : w[i] * fs;
+      for (int i = 0; i < AT_ONCE; ++i) {
+        if (s + i * slices >= nparts) ml[i][0] = -INFINITY;
+        up = fmaxf(up, ml[i][0]);
+      }
+      const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - up);
+      l *= f, o *= f, m = up;
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i) {
+        const bool none = ml[i][0] == -INFINITY;
+        const float fs = none ? 0.0f : __builtin_amdgcn_exp2f(ml[i][0] - up);
+        l += none ? 0.0f : ml[i][1] * fs;
+        o += none ? f4_t{0, 0, 0, 0} : w[i] * fs;
       }
     }
-    for (; s < nparts; s += slices) {
-      const float fs = f[s];
-      o += fs == 0.0f ? f4_t{0, 0, 0, 0} : get4(p + s * step) * fs;
+    if (slices == 1) {
+      store(h, d, o, l);
+    } else {
+      *(f4_t*)(shared + 8 * x) = o;
+      *(f2_t*)(shared + 8 * x + 4) = f2_t{m, l};
     }
-    if (slices == 1)
-      store(h, d, o, total[h]);
-    else
-      *(f4_t*)(shared + 4 * x) = o;
   }
   if (slices == 1) return;
   __syncthreads();
   for (int spot = threadIdx.x; spot < spots; spot += 64 * WAVES) {
+    float m = -INFINITY, l = 0.0f;
     f4_t o = {0, 0, 0, 0};
-    for (int c = 0; c < slices; ++c) o += *(const f4_t*)(shared + 4 * (c * spots + spot));
-    store(spot / quads, spot % quads * 4, o, total[spot / quads]);
+    for (int c = 0; c < slices; ++c) m = fmaxf(m, shared[8 * (c * spots + spot) + 4]);
+    for (int c = 0; c < slices; ++c) {
+      const float* at = shared + 8 * (c * spots + spot);
+      if (at[4] == -INFINITY) continue;
+      const float f = __builtin_amdgcn_exp2f(at[4] - m);
+      l += at[5] * f;
+      o += *(const f4_t*)at * f;
+    }
+    store(spot / quads, spot % quads * 4, o, l);
   }
 }
 
-// Workgroups that a launch of so many rows can come to.
 // Rows that go in one launch.
 inline int group_rows(int items) { return COUNTERS / items < GROUP_ROWS ? COUNTERS / items : GROUP_ROWS; }
 
@@ -510,6 +530,16 @@ size_t dz_paged_attention_bytes(int rows, int heads, int kv_heads, int dim, int 
   return groups > (long long)together * items ? (size_t)groups * most * (dim + 4) * 4 : 0;   // (no row has parts)
 }
 
+unsigned long long dz_capture_id(void* stream) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (hipStreamGetCaptureInfo((hipStream_t)stream, &status, &id) != hipSuccess) {
+    (void)hipGetLastError();
+    return 0;
+  }
+  return status == hipStreamCaptureStatusActive ? id : 0;
+}
+
 int dz_paged_attention(const dz_attention_args* a, void* stream) {
   if (!a || a->bytes != (int64_t)sizeof(*a)) return DZ_EINVAL;
   if (!shapes_fit(a->rows, a->heads, a->kv_heads, a->dim, a->page_size, a->pages_per_row)) return DZ_EPAGES;
@@ -545,9 +575,9 @@ int dz_paged_attention(const dz_attention_args* a, void* stream) {
   const int most = P.share < HEADS ? P.share : HEADS, items = P.kv_heads * P.head_tiles;
   P.part_floats = most * (a->dim + 4);
   P.scale = a->scale * 1.44269504088896340736f;
-  // the wavefronts' sums; or the factors of all parts that a row can have, and what threads add up for others
-  const size_t sums = (size_t)WAVES * most * (a->dim + 4), joins = (size_t)most * (TARGET / items + 2) + 4 * 64 * WAVES;
-  const size_t lds = ((sums > joins ? sums : joins + 3) / 4 * 4 + 2 * WAVES * HEADS + 4) * 4;
+  // the wavefronts' sums; or what threads add up for others
+  const size_t sums = (size_t)WAVES * most * (a->dim + 4), joins = 8 * 64 * WAVES;
+  const size_t lds = ((sums > joins ? sums : joins) + 2 * WAVES * HEADS + 4) * 4;
   P.stat_at = (int)(lds / 4) - (2 * WAVES * HEADS + 4);
   const kernel_t kern = a->dtype == DZ_BF16 ? kernel_for<true>(a->dim) : kernel_for<false>(a->dim);
   const int kc = chunks_of(a->dim), which = kc * 4 + (a->dim == 32 * kc) * 2 + a->dtype;
@@ -562,6 +592,7 @@ int dz_paged_attention(const dz_attention_args* a, void* stream) {
     P.tables = a->tables + row * P.table_row;
     P.lengths = a->lengths + row;
     const long long groups = most_groups(P.rows, items, (long long)a->pages_per_row * a->page_size);
+    P.single = groups == (long long)P.rows * items;
     hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(64 * WAVES), lds, st, P);
   }
   return hipGetLastError() == hipSuccess ? DZ_OK : DZ_ELAUNCH;

@@ -209,18 +209,30 @@ class _Space(NamedTuple):
 _spaces: Dict[Tuple[int, int], _Space] = {}       # (device, stream)
 
 
+# (device, stream) -> (capture, counters) of the graph that is being captured there
+_captured: Dict[Tuple[int, int], Tuple[int, torch.Tensor]] = {}
+
+
 def _parts_space(device: torch.device, need: int) -> _Space:
-    """Calls on one stream follow each other and share theirs.  A captured call has its own: its graph may be replayed beside
-    anything."""
+    """Calls on one stream follow each other and share theirs.  A graph may be replayed beside anything: it has counters of its
+    own, cleared in it by the first captured call on a stream, and every captured call room of its own."""
     key = device.index, ops._stream()
-    space = None if _capturing() else _spaces.get(key)
-    if space is None or space.work_bytes < need:
+    capture = _lib.lib().dz_capture_id(key[1])
+    if capture:
+        made = _captured.get(key)
+        if made is None or made[0] != capture:
+            made = _captured[key] = capture, torch.zeros(COUNTERS, dtype=torch.int32, device=device)
+        counters, size = made[1], need
+    else:
+        space = _spaces.get(key)
+        if space is not None and space.work_bytes >= need:
+            return space
         counters = torch.zeros(COUNTERS, dtype=torch.int32, device=device) if space is None else space.counters
-        size = need if _capturing() else max(need, 1 << 20)
-        work = torch.empty(size, dtype=torch.uint8, device=device)
-        space = _Space(counters, work, counters.data_ptr(), work.data_ptr(), size)
-        if not _capturing():
-            _spaces[key] = space
+        size = max(need, 1 << 20)
+    work = torch.empty(size, dtype=torch.uint8, device=device)
+    space = _Space(counters, work, counters.data_ptr(), work.data_ptr(), size)
+    if not capture:
+        _spaces[key] = space
     return space
 
 

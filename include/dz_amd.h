@@ -505,6 +505,9 @@ typedef struct dz_attention_args {
 size_t dz_paged_attention_bytes(int rows, int heads, int kv_heads, int dim, int page_size, int pages_per_row);
 int dz_paged_attention(const dz_attention_args* args, void* stream);
 
+/* The capture that is going on on a stream (0: none), as the runtime numbers them. */
+unsigned long long dz_capture_id(void* stream);
+
 /* The first `rot` values of every head of q and k turned to their token's position: pair i is (i, i + rot / 2), or with
  * neighbours != 0 (2 i, 2 i + 1), its angle positions[t] * turns[i] full turns, the turned values times `factor`;
  * the others are copied.  Without slots: k_out [tokens, kv_heads, dim] (strides k_out_token, k_out_head), and
