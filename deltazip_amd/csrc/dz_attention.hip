@@ -21,9 +21,16 @@
 // weight then has 16 (bf16) or 22 (fp16) bits, and the output's error is its own rounding.  Sums are fp32.
 //
 // The work is cut on the device, which alone knows the lengths: every wavefront reads the lengths of the launch's
-// rows (up to 256, up to four a lane), and takes for the tiles of a workgroup as many as make about `target` workgroups.
-// Parts of a row are joined by the workgroup that is done last of them (a counter per row and item says which),
-// in the order of the tokens, so results do not depend on timing.
+// rows (up to 256, up to four a lane) and cuts them into as many equal parts as make 512 or 768 workgroups together.
+// Rows of much work go first: 200 rows of 1 to 4000 tokens 96 -> 78 us.  Parts are joined by the workgroup that is done last
+// of up to 16 of them, and these joined ones again (counters say who is last), in the order of the tokens: results
+// do not depend on timing.
+//
+// Measured (keys and values over the time of the launch): 128 rows of 1025 tokens of 32 key heads of 128 330 us, 6.5 TB/s;
+// 32 of 1024 86 us, 6.2; one of 131071 tokens of 8 97 us, 5.5, of which 76 at the rate of a kernel that only reads (7.1 TB/s with
+// loads that keep nothing in the caches, 6.2 with others; a copy moves 4.9 to 5.4); one of 17 tokens 5 us, of which an empty
+// launch takes 2.5.  A compute unit has some 64 KB on their way at most, which at 2 us is 30 GB/s: what long
+// rows lose is the uneven ends of their parts (63 to 86 us) and the two joins (9 us).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -42,14 +49,15 @@ constexpr int WAVES = 4;               // wavefronts of a workgroup
 constexpr int TILE = 32;               // tokens of a step
 constexpr int HEADS = 16;              // heads taken together: columns of a matrix instruction
 constexpr int GROUP_ROWS = 256;        // rows of a launch: four lengths a lane
-#ifndef TGT
-#define TGT 512
-#endif
-constexpr int TARGET = TGT;           // workgroups that the work is cut into, rows' last parts apart
-constexpr int COUNTERS = DZ_ATTENTION_COUNTERS;   // rows of a launch times their items, at most
+constexpr int TARGET = 768;            // workgroups that the work of a launch is cut into at most, rows' last parts apart
+constexpr int FEW_ROWS = 16;           // below: two workgroups for each of 256 compute units
+constexpr int COUNTERS = DZ_ATTENTION_COUNTERS / 2;   // workgroups of a launch with parts, at most
 constexpr size_t LDS_MOST = 96 << 10;
-constexpr float CACHED = 64 << 20;     // bytes of keys and values
-constexpr int AT_ONCE = 16;            // parts that a join asks for at a time
+constexpr float CACHED = 64 << 20;     // bytes of keys and values up to which they may be in the last cache, of 256 MB (24 rows of 1000
+                                       // tokens, 40 MB, in turn with two others': 20 us, past the caches 25)
+constexpr int GROUP = 16;              // parts joined at once
+constexpr int WHOLE = 12;              // tiles up to which a row has one part: a join takes as long as three steps (300 tokens 9.7 -> 8.7 us)
+constexpr int LONG = 32;               // tiles of a part up to which no row has more than GROUP: joins in two takes cost 3 us more (8000 tokens 18.5 -> 16)
 
 struct AttnParams {
   const char *q, *k, *v;
@@ -61,7 +69,7 @@ struct AttnParams {
   long long q_row, q_head, k_page, k_head, k_token, v_page, v_head, v_token, out_row, out_head, table_row;   // bytes; out, table: elements
   unsigned num_pages;
   int rows, heads, kv_heads, share, head_tiles, dim, shift, pages_per_row, window, part_floats, stat_at, single;
-  float scale;
+  float scale, cut;
 };
 
 template <bool BF>
@@ -138,26 +146,34 @@ __device__ __forceinline__ Part find_part(const AttnParams& P, int part, int ite
   }
   const float total = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, scan_add(mine)), 63)) * (float)items;
   found.once = total * (TILE * 4.0f) * (float)P.dim > CACHED;
-  // tiles of a part, in whole steps of the workgroup; rounded up, so that TARGET parts and one a row suffice whatever the
-  // sums' rounding
-  float most = ceilf(total * (1.00001f / (WAVES * TARGET)));
+  // tiles of a part, in whole steps of the workgroup (sums above 2^24 are rounded, which may come to one part more)
+  const float most = ceilf(total * P.cut);
   const unsigned each = WAVES * (unsigned)fminf(fmaxf(most, 1.0f), (float)(1 << 24));
-  int sum = 0, parts[4];
+  int parts[4], heavy = 0, light = 0;
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
+    parts[r] = 0;
     if (r < each_lane) {
-      parts[r] = row0 + r < P.rows ? max(1, (int)((tiles[r] + each - 1) / each)) : 0;   // (an empty row has its zeros written)
-    } else {
-      parts[r] = 0;
+      parts[r] = tiles[r] <= WHOLE ? 1 : (int)((tiles[r] + each - 1) / each);      // (an empty row has its zeros written)
+      if (parts[r] > GROUP && tiles[r] <= GROUP * LONG) parts[r] = GROUP;
+      if (row0 + r >= P.rows) parts[r] = 0;
     }
-    before[r] = sum;
-    sum += parts[r];
+    const bool is = 2 * tiles[r] > (int)each;
+    before[r] = is ? heavy : light;
+    if (is)
+      heavy += parts[r];
+    else
+      light += parts[r];
   }
-  const int front = scan_add(sum) - sum;
+  // rows of much work first: they are dealt to the compute units evenly, and the others fill up
+  const int upto = scan_add(heavy), front_heavy = upto - heavy;
+  const int front_light = scan_add(light) - light + __builtin_amdgcn_readlane(upto, 63);
+#pragma unroll
+  for (int r = 0; r < 4; ++r) before[r] += 2 * tiles[r] > (int)each ? front_heavy : front_light;
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     if (r >= each_lane) break;
-    const int at = part - front - before[r];
+    const int at = part - before[r];
     const unsigned long long hit = __ballot(at >= 0 && at < parts[r]);
     if (hit) {
       const int src = __builtin_ctzll(hit);
@@ -176,18 +192,24 @@ __device__ __forceinline__ u4_t load16(const char* at) {
   return ONCE ? __builtin_nontemporal_load((const u4_t*)at) : *(const u4_t*)at;
 }
 
-// Sums of parts go from one workgroup to another past the caches of the eight dies (agent scope, relaxed): a fence
-// there writes back and empties a whole cache, which took six times as long as the attention itself.
-__device__ __forceinline__ void put(float* at, f2_t x) {
-  __hip_atomic_store((unsigned long long*)at, __builtin_bit_cast(unsigned long long, x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ f2_t get(const float* at) {
-  return __builtin_bit_cast(f2_t, __hip_atomic_load((const unsigned long long*)at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-}
-__device__ __forceinline__ f4_t get4(const float* at) {
-  const f2_t a = get(at), b = get(at + 2);
-  return f4_t{a[0], a[1], b[0], b[1]};
-}
+// Sums of parts go from one workgroup to another past the caches of the eight dies (sc1: agent scope): a fence there writes
+// back and empties a whole cache, which took six times as long as the attention itself.
+struct Shared {
+  __amdgpu_buffer_rsrc_t at;
+  __device__ __forceinline__ explicit Shared(float* base) : at(__builtin_amdgcn_make_buffer_rsrc(base, 0, 0xffffffff, 0x00027000)) {}
+  __device__ __forceinline__ void put(unsigned offset, f4_t x) const {
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4_t, x), at, offset, 0, 16);
+  }
+  __device__ __forceinline__ void put(unsigned offset, f2_t x) const {
+    __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u2_t, x), at, offset, 0, 16);
+  }
+  __device__ __forceinline__ f4_t get4(unsigned offset) const {
+    return __builtin_bit_cast(f4_t, __builtin_amdgcn_raw_buffer_load_b128(at, offset, 0, 16));
+  }
+  __device__ __forceinline__ f2_t get2(unsigned offset) const {
+    return __builtin_bit_cast(f2_t, __builtin_amdgcn_raw_buffer_load_b64(at, offset, 0, 16));
+  }
+};
 
 template <int KC, bool FULL, bool BF>
 __global__ __launch_bounds__(64 * WAVES, KC == 8 && !FULL ? 1 : 2) void dz_attention_kernel(const AttnParams P) {
@@ -382,14 +404,19 @@ __global__ __launch_bounds__(64 * WAVES, KC == 8 && !FULL ? 1 : 2) void dz_atten
     }
   }
   __syncthreads();
-  float* to = nparts > 1 ? P.parts + (size_t)blockIdx.x * P.part_floats : nullptr;
   const int quads = P.dim / 4, spots = nheads * quads;
+  const Shared parts(P.parts);
+  const unsigned record = P.part_floats * 4u, stats = nheads * P.dim * 4u;      // bytes of a part, of its values
   auto store = [&](int h, int d, f4_t o, float l) {
     const f4_t y = tiles ? o / l : f4_t{0, 0, 0, 0};
     uint16_t* at = P.out + row * P.out_row + (head0 + h) * P.out_head + d;
     const u2_t w = {(unsigned)Ty::round(y[0]) | (unsigned)Ty::round(y[1]) << 16,
                     (unsigned)Ty::round(y[2]) | (unsigned)Ty::round(y[3]) << 16};
     *(u2_t*)at = w;
+  };
+  auto leave = [&](unsigned slot, int h, int d, f4_t o, float m, float l) {
+    parts.put(slot * record + (h * P.dim + d) * 4, o);
+    if (d == 0) parts.put(slot * record + stats + 8 * h, f2_t{m, l});
   };
   for (int x = threadIdx.x; x < spots; x += 64 * WAVES) {
     const int h = x / quads, d = x % quads * 4;
@@ -405,96 +432,111 @@ __global__ __launch_bounds__(64 * WAVES, KC == 8 && !FULL ? 1 : 2) void dz_atten
       l += mw == -INFINITY ? 0.0f : lw * f;
       o += mw == -INFINITY ? f4_t{0, 0, 0, 0} : *(const f4_t*)(lds + (w * nheads + h) * ld + d) * f;
     }
-    if (to) {
-      put(to + h * P.dim + d, f2_t{o[0], o[1]});
-      put(to + h * P.dim + d + 2, f2_t{o[2], o[3]});
-      if (d == 0) put(to + nheads * P.dim + 2 * h, f2_t{m, l});
-    } else {
+    if (nparts > 1)
+      leave(blockIdx.x, h, d, o, m, l);
+    else
       store(h, d, o, l);
-    }
   }
-  if (!to) return;
+  if (nparts <= 1) return;
 
-  // the last of a row's parts to be done joins them
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this wavefront's sums have arrived
-  __syncthreads();
+  // The last to be done of up to GROUP parts joins them; in a row of more it leaves the result behind the parts, and the last to
+  // be done of these joins those.
   int* flag = (int*)(stat + 2 * WAVES * HEADS);
-  if (threadIdx.x == 0) {
-    unsigned* counter = P.counters + row * items + item;
-    const bool last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)nparts - 1;
-    if (last) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // as the next call wants it
-    *flag = last;
-  }
-  __syncthreads();
-  if (!*flag) return;
-  const size_t step = (size_t)items * P.part_floats;
-  const float* from = P.parts + ((size_t)(part - nth) * items + item) * P.part_floats;
-  // a thread takes four values of a head over every `slices`-th part, sixteen on their way at a time; threads that have none
-  // of their own share the parts of others'
+  auto last_of = [&](unsigned* counter, int n) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this wavefront's sums have arrived
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      const bool last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)n - 1;
+      if (last) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // as the next call wants it
+      *flag = last;
+    }
+    __syncthreads();
+    return *flag != 0;
+  };
+  // a thread takes four values of a head over every `slices`-th part; threads that have none of their own share the
+  // parts of others'
   int slices = 1;
   while (2 * slices * spots <= 64 * WAVES) slices *= 2;
-  float* shared = lds;                                // [slice][spot]: values, maximum and sum
-  for (int x = threadIdx.x; x < spots * slices; x += 64 * WAVES) {
-    const int spot = x % spots, h = spot / quads, d = spot % quads * 4;
-    const float *p = from + h * P.dim + d, *stats = from + nheads * P.dim + 2 * h;
-    float m = -INFINITY, l = 0.0f;
-    f4_t o = {0, 0, 0, 0};
-    for (int s = x / spots; s < nparts; s += AT_ONCE * slices) {
-      f4_t w[AT_ONCE];
-      f2_t ml[AT_ONCE];
+  auto join = [&](unsigned slot, unsigned step, int n, auto emit) {
+    auto gather = [&](auto at_once) {
+      constexpr int N = decltype(at_once)::value;      // parts that a thread asks for at a time
+      for (int x = threadIdx.x; x < spots * slices; x += 64 * WAVES) {
+        const int spot = x % spots, h = spot / quads, d = spot % quads * 4;
+        float m = -INFINITY, l = 0.0f;
+        f4_t o = {0, 0, 0, 0};
+        for (int s = x / spots; s < n; s += N * slices) {
+          f4_t w[N];
+          f2_t ml[N];
 #pragma unroll
-      for (int i = 0; i < AT_ONCE; ++i) {
-        const int at = min(s + i * slices, nparts - 1);
-        ml[i] = get(stats + at * step);
-        w[i] = get4(p + at * step);
-      }
-      float up = m;
+          for (int i = 0; i < N; ++i) {
+            const unsigned at = (slot + min(s + i * slices, n - 1) * step) * record;
+            ml[i] = parts.get2(at + stats + 8 * h);
+            w[i] = parts.get4(at + (h * P.dim + d) * 4);
+          }
+          float up = m;
 #pragma unroll
-      for (int i = 0; i < AT_ONCE; ++i) {
-        if (s + i * slices >= nparts) ml[i][0] = -INFINITY;
-        up = fmaxf(up, ml[i][0]);
-      }
-      const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - up);
-      l *= f, o *= f, m = up;
+          for (int i = 0; i < N; ++i) {
+            if (s + i * slices >= n) ml[i][0] = -INFINITY;
+            up = fmaxf(up, ml[i][0]);
+          }
+          const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - up);
+          l *= f, o *= f, m = up;
 #pragma unroll
-      for (int i = 0; i < AT_ONCE; ++i) {
-        const bool none = ml[i][0] == -INFINITY;
-        const float fs = none ? 0.0f : __builtin_amdgcn_exp2f(ml[i][0] - up);
-        l += none ? 0.0f : ml[i][1] * fs;
-        o += none ? f4_t{0, 0, 0, 0} : w[i] * fs;
+          for (int i = 0; i < N; ++i) {
+            const bool none = ml[i][0] == -INFINITY;
+            const float fs = none ? 0.0f : __builtin_amdgcn_exp2f(ml[i][0] - up);
+            l += none ? 0.0f : ml[i][1] * fs;
+            o += none ? f4_t{0, 0, 0, 0} : w[i] * fs;
+          }
+        }
+        if (slices == 1) {
+          emit(h, d, o, m, l);
+        } else {
+          *(f4_t*)(lds + 8 * x) = o;                   // [slice][spot]: values, maximum and sum
+          *(f2_t*)(lds + 8 * x + 4) = f2_t{m, l};
+        }
       }
+    };
+    if (slices >= 4)
+      gather(std::integral_constant<int, GROUP / 4>());
+    else
+      gather(std::integral_constant<int, GROUP>());
+    if (slices == 1) return;
+    __syncthreads();
+    for (int spot = threadIdx.x; spot < spots; spot += 64 * WAVES) {
+      float m = -INFINITY, l = 0.0f;
+      f4_t o = {0, 0, 0, 0};
+      for (int c = 0; c < slices; ++c) m = fmaxf(m, lds[8 * (c * spots + spot) + 4]);
+      for (int c = 0; c < slices; ++c) {
+        const float* at = lds + 8 * (c * spots + spot);
+        if (at[4] == -INFINITY) continue;
+        const float f = __builtin_amdgcn_exp2f(at[4] - m);
+        l += at[5] * f;
+        o += *(const f4_t*)at * f;
+      }
+      emit(spot / quads, spot % quads * 4, o, m, l);
     }
-    if (slices == 1) {
-      store(h, d, o, l);
-    } else {
-      *(f4_t*)(shared + 8 * x) = o;
-      *(f2_t*)(shared + 8 * x + 4) = f2_t{m, l};
-    }
+  };
+  const auto finish = [&](int h, int d, f4_t o, float m, float l) { store(h, d, o, l); };
+  const unsigned slot0 = blockIdx.x - nth * items, mine0 = slot0 + nth / GROUP * GROUP * items;      // of the row's, the group's first part
+  const int members = min(GROUP, nparts - nth / GROUP * GROUP), groups = (nparts + GROUP - 1) / GROUP;
+  if (!last_of(P.counters + mine0, members)) return;
+  if (groups == 1) {
+    join(slot0, items, members, finish);
+    return;
   }
-  if (slices == 1) return;
-  __syncthreads();
-  for (int spot = threadIdx.x; spot < spots; spot += 64 * WAVES) {
-    float m = -INFINITY, l = 0.0f;
-    f4_t o = {0, 0, 0, 0};
-    for (int c = 0; c < slices; ++c) m = fmaxf(m, shared[8 * (c * spots + spot) + 4]);
-    for (int c = 0; c < slices; ++c) {
-      const float* at = shared + 8 * (c * spots + spot);
-      if (at[4] == -INFINITY) continue;
-      const float f = __builtin_amdgcn_exp2f(at[4] - m);
-      l += at[5] * f;
-      o += *(const f4_t*)at * f;
-    }
-    store(spot / quads, spot % quads * 4, o, l);
-  }
+  join(mine0, items, members, [&](int h, int d, f4_t o, float m, float l) { leave(gridDim.x + mine0, h, d, o, m, l); });
+  if (!last_of(P.counters + COUNTERS + slot0, groups)) return;
+  join(gridDim.x + slot0, GROUP * items, groups, finish);
 }
 
 // Rows that go in one launch.
-inline int group_rows(int items) { return COUNTERS / items < GROUP_ROWS ? COUNTERS / items : GROUP_ROWS; }
+inline int group_rows(int items) { return min(GROUP_ROWS, (COUNTERS - TARGET) / items - 1); }
 
 inline long long most_groups(int rows, int items, long long room) {
   const long long whole = (room + TILE - 1) / TILE + 1;          // tiles of the longest row (a window may cut two)
   const long long parts = (whole + WAVES - 1) / WAVES;
-  const long long all = parts * rows * items, cut = TARGET + (long long)rows * items;
+  const long long all = parts * rows * items, cut = TARGET + (rows + 1ll) * items;
   return all < cut ? all : cut;
 }
 
@@ -527,7 +569,7 @@ size_t dz_paged_attention_bytes(int rows, int heads, int kv_heads, int dim, int 
   const int most = share < HEADS ? share : HEADS;
   const int together = group_rows(items) < rows ? group_rows(items) : rows;
   const long long groups = most_groups(together, items, (long long)pages_per_row * page_size);
-  return groups > (long long)together * items ? (size_t)groups * most * (dim + 4) * 4 : 0;   // (no row has parts)
+  return groups > (long long)together * items ? 2 * (size_t)groups * most * (dim + 4) * 4 : 0;   // (no row has parts)
 }
 
 unsigned long long dz_capture_id(void* stream) {
@@ -592,6 +634,7 @@ int dz_paged_attention(const dz_attention_args* a, void* stream) {
     P.tables = a->tables + row * P.table_row;
     P.lengths = a->lengths + row;
     const long long groups = most_groups(P.rows, items, (long long)a->pages_per_row * a->page_size);
+    P.cut = 1.0f / (WAVES * (P.rows < FEW_ROWS ? 512 : TARGET));
     P.single = groups == (long long)P.rows * items;
     hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(64 * WAVES), lds, st, P);
   }

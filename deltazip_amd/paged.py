@@ -30,7 +30,7 @@ _TYPES = {torch.float16: 0, torch.bfloat16: 1}
 _ATTENTION = struct.Struct("=q9Q2q11q8ifi")       # dz_attention_args
 _ROTARY = struct.Struct("=q10Qq14q8ifi")          # dz_rotary_args
 MAX_DIM = 256
-COUNTERS = 16384                  # DZ_ATTENTION_COUNTERS
+COUNTERS = 32768                  # DZ_ATTENTION_COUNTERS
 
 
 class RotaryPositions:

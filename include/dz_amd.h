@@ -59,7 +59,7 @@ extern "C" {
 
 #define DZ_F16  0                 /* element types of the operators on a paged cache */
 #define DZ_BF16 1
-#define DZ_ATTENTION_COUNTERS 16384
+#define DZ_ATTENTION_COUNTERS 32768
 
 /* Library version (major*10000 + minor*100 + patch). */
 int dz_version(void);
