@@ -72,6 +72,8 @@ SIGNATURES = {
     "dz_gemm_f16_select": (_i, [_vp, _vp, _vp, C.c_longlong, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _vp]),
     "dz_paged_attention_bytes": (_sz, [_i] * 6),
     "dz_paged_attention": (_i, [C.c_char_p, _vp]),      # the packed structure
+    "dz_page_status": (_vp, []),
+    "dz_take_page_status": (_i, [_vp, _vp]),
     "dz_capture_id": (C.c_ulonglong, [_vp]),
     "dz_rotary": (_i, [C.c_char_p, _vp]),
     "dz_copy_pages": (_i, [_vp, _i, C.c_longlong, C.c_longlong, _i, _vp, _i, _vp]),

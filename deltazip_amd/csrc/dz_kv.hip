@@ -9,6 +9,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/dz_amd.h"
 #include "dz_device.h"
 
@@ -184,9 +186,33 @@ __global__ __launch_bounds__(256) void dz_copy_pages_kernel(const CopyParams P) 
   __builtin_nontemporal_store(ONCE ? __builtin_nontemporal_load(from) : *from, (u4_t*)(pool + pair.y * P.page_stride) + c);
 }
 
+// What kernels of this process met on this device, for callers that keep no word of their own: it outlives every graph.
+static __device__ unsigned page_status;
+std::atomic<void*> page_status_at[64];
+
+__global__ void dz_take_status_kernel(unsigned* word, unsigned* to) { *to = atomicExch(word, 0u); }
+
 }  // namespace
 
 extern "C" {
+
+uint32_t* dz_page_status(void) {
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return nullptr;
+  void* p = page_status_at[dev].load(std::memory_order_acquire);
+  if (!p) {
+    if (hipGetSymbolAddress(&p, HIP_SYMBOL(page_status)) != hipSuccess || !p) return nullptr;
+    page_status_at[dev].store(p, std::memory_order_release);      // (two racing threads store the same address)
+  }
+  return (uint32_t*)p;
+}
+
+int dz_take_page_status(uint32_t* to, void* stream) {
+  uint32_t* word = dz_page_status();
+  if (!to || !word) return DZ_EINVAL;
+  hipLaunchKernelGGL(dz_take_status_kernel, dim3(1), dim3(1), 0, (hipStream_t)stream, word, to);
+  return hipGetLastError() == hipSuccess ? DZ_OK : DZ_ELAUNCH;
+}
 
 int dz_rotary(const dz_rotary_args* a, void* stream) {
   if (!a || a->bytes != (int64_t)sizeof(*a)) return DZ_EINVAL;
@@ -229,7 +255,10 @@ int dz_rotary(const dz_rotary_args* a, void* stream) {
   units = units < 1 ? 1 : units > 64 ? 64 : units;
   const int each = 256 / units, total = P.heads + (P.k ? P.kv_heads : 0) + (P.v ? P.kv_heads : 0);
   if (total == 0) return DZ_OK;
-  const int slices = (total + each - 1) / each;
+  // a token's heads over as many workgroups as make some 1024 together: with all of them apart each works out the angles again
+  // (8192 tokens of 48 heads 39.8 -> 35.9 us, 4000 of 48 heads of 80 14.8 -> 12.1)
+  const int apart = (total + each - 1) / each, few = (1023 + a->tokens) / a->tokens;
+  const int slices = apart < few ? apart : few;
   typedef void (*kernel_t)(const RotaryParams);
   static const kernel_t kernels[2][8] = {
       {dz_rotary_kernel<false, false, 8, 8>, dz_rotary_kernel<false, false, 2, 8>, dz_rotary_kernel<false, false, 1, 8>, dz_rotary_kernel<false, false, 2, 2>,

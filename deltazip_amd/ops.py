@@ -838,7 +838,7 @@ WS_HEADER_BYTES = 256          # the status word sits in front of the token orde
 
 STATUS_BAD_ID = 1              # a delta id outside [-1, S) was met and treated as -1
 STATUS_SUM_MISSING = 2         # a partial sum of a K-slice did not arrive: that call's output is invalid
-STATUS_BAD_PAGE = 4            # a page, slot or length outside the key/value cache: that call's output is invalid
+STATUS_BAD_PAGE = 4            # a page, slot or length outside the key/value cache: that call's output is invalid (a word of its own)
 
 
 @lru_cache(maxsize=4096)
@@ -864,7 +864,7 @@ def _workspace(device: torch.device, T: int, K: int, N: int) -> torch.Tensor:
 
 def workspace_status(device=None) -> int:
     """Status words of the device's workspaces, OR-ed (bit 0: a delta id outside [-1, S) was seen
-    and treated as -1; bit 1: a partial sum did not arrive; bit 2: a page, slot or length outside the cache).  Synchronises; meant for debugging
+    and treated as -1; bit 1: a partial sum did not arrive).  Synchronises; meant for debugging
     and tests -- the serving path uses `poll_status`."""
     idx = torch.cuda.current_device() if device is None else torch.device(device).index
     status = 0
@@ -913,6 +913,35 @@ def _clear_workspace(ws: torch.Tensor, word: int) -> None:
     ws[:4].zero_()
 
 
+_page_status: Dict[int, int] = {}                  # device -> address of the paged operators' status word, once one has run
+_page_polls: Dict[int, Tuple[torch.Tensor, "torch.cuda.Event"]] = {}
+
+
+def _poll_pages(dev: int, wait: bool) -> int:
+    """The same look at the word of the paged operators, which all streams of a device share: taken and cleared in one
+    step, so that no report is lost.  With `wait` behind everything the device has been given."""
+    if dev not in _page_status:
+        return 0
+    with torch.cuda.device(dev):
+        if wait:
+            torch.cuda.synchronize()
+        pending = _page_polls.pop(dev, None)
+        word = 0
+        if pending is not None:
+            if not pending[1].query():
+                _page_polls[dev] = pending
+                return 0
+            word = int(pending[0][0])
+        host, event = (torch.zeros(1, dtype=torch.int32, pin_memory=True), torch.cuda.Event()) if pending is None else pending
+        _lib.check(_lib.lib().dz_take_page_status(host.data_ptr(), _stream()), "dz_take_page_status")
+        event.record()
+        if wait:
+            event.synchronize()
+            return word | int(host[0])
+        _page_polls[dev] = host, event
+        return word
+
+
 def poll_status(device=None, wait: bool = False) -> None:
     """The serving path's look at the status words, without a synchronisation of its own: every call
     evaluates the copy the previous call started (if it has completed, or after waiting for it when
@@ -920,12 +949,12 @@ def poll_status(device=None, wait: bool = False) -> None:
     workspace's stream.  Raises DeltaKernelError / warns as `raise_for_status` says; a reported
     failure also clears the workspace.  With `wait` the current state is read as well (this
     synchronises with the workspace's stream)."""
-    if not _workspaces:
-        return                                        # no fused call has run yet (or no GPU at all)
+    if not _workspaces and not _page_status:
+        return                                        # no call has run yet (or no GPU at all)
     idx = None if device is None else torch.device(device).index
     if idx is None:
         idx = torch.cuda.current_device()
-    found = 0
+    found = _poll_pages(idx, wait)
     for key, ws in list(_workspaces.items()):
         if key[0] != idx:
             continue

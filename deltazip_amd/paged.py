@@ -10,8 +10,8 @@ serving/csrc/cache_kernels, serving/csrc/attention) and take the place of plain 
 cache.  float16 and bfloat16; arithmetic in 32 bits and more, one rounding per output.  Work is enqueued on the
 current stream of the tensors' device; nothing synchronises, and everything can be captured into a graph.
 
-What only the kernels can see -- a page or slot outside the pool, a length beyond the table -- goes to the status word of
-the stream's workspace (`ops.poll_status`, `DeltaModelManager.check_status`): `ops.DeltaKernelError`.
+What only the kernels can see -- a page or slot outside the pool, a length beyond the table -- goes to a status word that
+`ops.poll_status` (`DeltaModelManager.check_status`) looks at with the others: `ops.DeltaKernelError`.
 """
 from __future__ import annotations
 
@@ -173,15 +173,15 @@ def _pages(name: str, t: torch.Tensor, q: torch.Tensor) -> None:
 _UNPACKED = object()
 
 
-def _place() -> Tuple[int, int, int]:
-    """(current device, current stream, status word of its workspace)."""
-    dev, stream = ops._current_device(), ops._stream()
-    ws = ops._workspaces.get((dev, stream))
-    return dev, stream, (ops._workspace(torch.device("cuda", dev), 1, 256, 32) if ws is None else ws).data_ptr()
-
-
-def _status(device: torch.device) -> int:
-    return ops._workspace(device, 1, 256, 32).data_ptr()
+def _status(dev: int) -> int:
+    """Address of the device's status word for the paged cache; the current device's."""
+    at = ops._page_status.get(dev)
+    if at is None:
+        at = _lib.lib().dz_page_status()
+        if not at:
+            raise RuntimeError("the library has no memory on the current device")
+        ops._page_status[dev] = at
+    return at
 
 
 def _elsewhere(t: torch.Tensor) -> bool:
@@ -254,9 +254,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     status word.  The order of a row's sums follows the lengths of all rows of the call (the work is cut by them,
     256 rows at a time): the same lengths give the same bits."""
     if out is None and q.is_cuda:
-        dev, stream, status = _place()
+        dev, stream = ops._current_device(), ops._stream()
         space = None if _capturing() else _spaces.get((dev, stream))
-        out = _lib.host().attend(q, k_pages, v_pages, block_tables, lengths, scale, window, dev, stream, status,
+        out = _lib.host().attend(q, k_pages, v_pages, block_tables, lengths, scale, window, dev, stream, _status(dev),
                                  *((0, 0, 0) if space is None else space[2:]))
         if out is not None:
             return out
@@ -298,7 +298,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     ks, vs = k_pages.stride(), v_pages.stride()
     args = _ATTENTION.pack(
         _ATTENTION.size, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), block_tables.data_ptr(), lengths.data_ptr(),
-        out.data_ptr(), space.work_at if need else 0, space.counters_at if need else 0, _status(q.device), need, pages, _stride(q, 0), _stride(q, 1),
+        out.data_ptr(), space.work_at if need else 0, space.counters_at if need else 0, _status(q.get_device()), need, pages, _stride(q, 0), _stride(q, 1),
         ks[0] if pages > 1 else 0, ks[1] if kv_heads > 1 else 0, ks[2], vs[0] if pages > 1 else 0, vs[1] if kv_heads > 1 else 0,
         vs[2], _stride(out, 0), _stride(out, 1), block_tables.stride(0) if rows > 1 else 0, rows, heads, kv_heads, dim, page_size,
         width, min(int(window), (1 << 31) - 1), _TYPES[q.dtype], dim ** -0.5 if scale is None else scale, 0)
@@ -313,7 +313,7 @@ def _rotate(q, k, v, positions, slots, rope, q_out, k_out, v_out, page_size, num
     args = _ROTARY.pack(
         _ROTARY.size, q.data_ptr(), 0 if k is None else k.data_ptr(), 0 if v is None else v.data_ptr(), q_out.data_ptr(),
         0 if k is None else k_out.data_ptr(), 0 if v is None else v_out.data_ptr(), positions.data_ptr(),
-        slots.data_ptr() if paged else 0, 0 if rope is None else rope.on(q.device).data_ptr(), _status(q.device) if paged else 0,
+        slots.data_ptr() if paged else 0, 0 if rope is None else rope.on(q.device).data_ptr(), _status(q.get_device()) if paged else 0,
         num_pages, _stride(q, 0), _stride(q, 1), *((0, 0) if k is None else (_stride(k, 0), _stride(k, 1))),
         *((0, 0) if v is None else (_stride(v, 0), _stride(v, 1))), _stride(q_out, 0), _stride(q_out, 1),
         *((0, 0, 0) if k is None else strides(k_out)), *((0, 0, 0) if v is None else strides(v_out)),
@@ -377,9 +377,10 @@ def append_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torc
     returned as it is.  No two tokens may have one slot: what is there afterwards may be parts of either.  Strides as
     for `rotary`."""
     if q.is_cuda and (out is None or out is q):
-        dev, stream, status = _place()
+        dev = ops._current_device()
         turns = None if rope is None else rope._packed.get(dev, _UNPACKED)
-        made = _lib.host().rotate(q, k, v, positions, slots, turns, k_pages, v_pages, out is q or rope is None, dev, stream, status)
+        made = _lib.host().rotate(q, k, v, positions, slots, turns, k_pages, v_pages, out is q or rope is None, dev, ops._stream(),
+                                  _status(dev))
         if made is not None:
             return made
     ops._need_cuda(q, k, v, positions, slots, k_pages, v_pages, out)

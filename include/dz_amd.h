@@ -505,6 +505,12 @@ typedef struct dz_attention_args {
 size_t dz_paged_attention_bytes(int rows, int heads, int kv_heads, int dim, int page_size, int pages_per_row);
 int dz_paged_attention(const dz_attention_args* args, void* stream);
 
+/* A status word for the operators on a paged cache, on the current device: memory of the library's, for the life of the process
+ * (NULL: no device).  dz_take_page_status writes what is there to `to` (memory that the device can write, pinned host memory for
+ * one) and clears it, in the order of the stream. */
+uint32_t* dz_page_status(void);
+int dz_take_page_status(uint32_t* to, void* stream);
+
 /* The capture that is going on on a stream (0: none), as the runtime numbers them. */
 unsigned long long dz_capture_id(void* stream);
 

@@ -872,3 +872,60 @@ def test_llama_steps_over_the_paged_cache(dev):
     step = torch.cat((tokens[:B - 1], tokens[:1]))
     got = model.paged_step(step, cache, cache.batch(names), sample_rows=torch.tensor([0, B - 1], device=dev))
     assert got.shape == (2, V) and torch.equal(got[0], got[1]) and torch.isfinite(got).all()
+
+
+@pytest.mark.gpu
+def test_a_graph_replayed_before_others_and_after_eager_calls(dev):
+    """Graphs share nothing: the second is replayed first, with rows that are split, and the first behind it; the number of a
+    capture is its own."""
+    from deltazip_amd import _lib, ops, paged_attention
+    p = _problem(dev, torch.float16, [5000, 40, 9000], 8, 2, 128, 16, 77)
+    want = paged_attention(*p)
+    torch.cuda.synchronize()
+    graphs, seen = [], []
+    for _ in range(3):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            seen.append(_lib.lib().dz_capture_id(ops._stream()))
+            made = [paged_attention(*p) for _ in range(3)]
+        graphs.append((g, made))
+    assert 0 not in seen and len(set(seen)) == 3 and _lib.lib().dz_capture_id(ops._stream()) == 0
+    for n in (1, 0, 2, 0, 1, 1):
+        g, made = graphs[n]
+        for t in made:
+            t.zero_()
+        g.replay()
+        assert torch.equal(paged_attention(*p), want)
+        torch.cuda.synchronize()
+        for t in made:
+            assert torch.equal(t, want)
+
+
+@pytest.mark.gpu
+def test_a_bad_page_of_a_replay_is_reported_once(dev):
+    from deltazip_amd import ops, paged_attention
+    q, k, v, tables, ln = _problem(dev, torch.float16, [40, 20], 2, 2, 64, 16, 41)
+    fixed = tables.clone()
+    paged_attention(q, k, v, fixed, ln)
+    ops.poll_status(dev, wait=True)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        paged_attention(q, k, v, fixed, ln)
+    for bad in (False, True, False, True):
+        fixed.copy_(tables)
+        if bad:
+            fixed[1, 0] = len(k) + 5
+        g.replay()
+        if bad:
+            with pytest.raises(ops.DeltaKernelError, match="paged"):
+                ops.poll_status(dev, wait=True)
+        else:
+            ops.poll_status(dev, wait=True)
+    fixed[1, 0] = -9
+    g.replay()
+    torch.cuda.synchronize()
+    ops.poll_status(dev)                       # starts the look,
+    torch.cuda.synchronize()
+    with pytest.raises(ops.DeltaKernelError, match="paged"):
+        ops.poll_status(dev)                   # which the next call takes in
+    ops.poll_status(dev, wait=True)
