@@ -68,7 +68,7 @@ struct AttnParams {
   unsigned* status;
   long long q_row, q_head, k_page, k_head, k_token, v_page, v_head, v_token, out_row, out_head, table_row;   // bytes; out, table: elements
   unsigned num_pages;
-  int rows, heads, kv_heads, share, head_tiles, dim, shift, pages_per_row, window, part_floats, stat_at, single;
+  int rows, heads, kv_heads, share, head_tiles, dim, shift, pages_per_row, window, part_floats, stat_at, single, once;
   float scale, cut;
 };
 
@@ -131,6 +131,7 @@ __device__ __forceinline__ Part find_part(const AttnParams& P, int part, int ite
   if (P.single) {                      // (no row can have a second part)
     found.row = part;
     found.length = P.lengths[part];
+    found.once = P.once;
     return found;
   }
   // lane l has rows l * each_lane .. ; their tiles, and the parts in front of them
@@ -534,8 +535,8 @@ __global__ __launch_bounds__(64 * WAVES, KC == 8 && !FULL ? 1 : 2) void dz_atten
 inline int group_rows(int items) { return min(GROUP_ROWS, (COUNTERS - TARGET) / items - 1); }
 
 inline long long most_groups(int rows, int items, long long room) {
-  const long long whole = (room + TILE - 1) / TILE + 1;          // tiles of the longest row (a window may cut two)
-  const long long parts = (whole + WAVES - 1) / WAVES;
+  const long long whole = (room + TILE - 1) / TILE;              // tiles of the longest row
+  const long long parts = whole <= WHOLE ? 1 : (whole + WAVES - 1) / WAVES;
   const long long all = parts * rows * items, cut = TARGET + (rows + 1ll) * items;
   return all < cut ? all : cut;
 }
@@ -633,7 +634,10 @@ int dz_paged_attention(const dz_attention_args* a, void* stream) {
     P.out = (uint16_t*)a->out + row * P.out_row;
     P.tables = a->tables + row * P.table_row;
     P.lengths = a->lengths + row;
-    const long long groups = most_groups(P.rows, items, (long long)a->pages_per_row * a->page_size);
+    long long seen = (long long)a->pages_per_row * a->page_size;
+    if (a->window && a->window + 2ll * TILE < seen) seen = a->window + 2ll * TILE;             // (it may begin and end inside a tile)
+    const long long groups = most_groups(P.rows, items, seen);
+    P.once = (float)P.rows * items * seen * 4.0f * a->dim > CACHED;
     P.cut = 1.0f / (WAVES * (P.rows < FEW_ROWS ? 512 : TARGET));
     P.single = groups == (long long)P.rows * items;
     hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(64 * WAVES), lds, st, P);

@@ -8,7 +8,8 @@
 They stand where the reference's serving engine has its own kernels for these (serving/csrc/pos_encoding,
 serving/csrc/cache_kernels, serving/csrc/attention) and take the place of plain tensor operations over a padded
 cache.  float16 and bfloat16; arithmetic in 32 bits and more, one rounding per output.  Work is enqueued on the
-current stream of the tensors' device; nothing synchronises, and everything can be captured into a graph.
+current stream of the tensors' device; nothing synchronises, and everything can be captured into a graph.  They serve
+inference: no gradients are recorded.
 
 What only the kernels can see -- a page or slot outside the pool, a length beyond the table -- goes to a status word that
 `ops.poll_status` (`DeltaModelManager.check_status`) looks at with the others: `ops.DeltaKernelError`.
@@ -217,7 +218,7 @@ def _parts_space(device: torch.device, need: int) -> _Space:
     """Calls on one stream follow each other and share theirs.  A graph may be replayed beside anything: it has counters of its
     own, cleared in it by the first captured call on a stream, and every captured call room of its own."""
     key = device.index, ops._stream()
-    capture = _lib.lib().dz_capture_id(key[1])
+    capture = _lib.lib().dz_capture_id(key[1]) if _capturing() else 0
     if capture:
         made = _captured.get(key)
         if made is None or made[0] != capture:
@@ -249,7 +250,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     side and on multiples of 8 values (dim too, up to 256); pages of 8 to 1024 tokens, a power of two.
 
     A row of length 0 gives zeros.  Nothing behind a row's length is read, in the tables or in the pages, whatever
-    is there.  Several rows may share pages, and several rows of one sequence at lengths of their own are a prompt's
+    is there; what it sees counts, and values there that are not finite give values that are not, in their row and head.  Several
+    rows may share pages, and several rows of one sequence at lengths of their own are a prompt's
     tokens.  A length beyond its table is cut; a page number outside the pool is read as page 0; either is reported through the
     status word.  The order of a row's sums follows the lengths of all rows of the call (the work is cut by them,
     256 rows at a time): the same lengths give the same bits."""
