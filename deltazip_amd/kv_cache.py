@@ -234,6 +234,9 @@ class PagedKVCache:
         is a padded row: it stores nothing and its attention is zero.  width: pages of a table's row (default: as many
         as the longest needs).  out: a batch of as many rows to write over (a captured step reads it; width is its tables')."""
         rows = len(seqs)
+        named = [x for x in seqs if x is not None]
+        if len(set(named)) < len(named):
+            raise ValueError("a sequence is named twice: its new token has one slot")
         found = [None if x is None else self._get(x) for x in seqs]
         if any(s is not None and not s.length for s in found):
             raise ValueError("a sequence without tokens has no newest one")

@@ -240,7 +240,7 @@ def _parts_space(device: torch.device, need: int) -> _Space:
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_tables: torch.Tensor,
                     lengths: torch.Tensor, scale: Optional[float] = None, window: int = 0,
                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """Attention of one new token per row (serving/csrc/attention, paged_attention_v1 / _v2):
+    """Attention of one new token per row (serving/csrc/attention):
 
         out[r, h] = softmax(scale q[r, h] . K)  V    over tokens max(0, n - window) .. n - 1 of row r, n = lengths[r]
 
@@ -373,7 +373,7 @@ def append_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torc
               out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """A step's tokens stored in the cache, in one launch: k, turned, and v [tokens, kv_heads, dim] go to place
     slots[t] % page_size of page slots[t] // page_size of k_pages and v_pages [pages, kv_heads, page_size, dim]
-    (serving/csrc/cache_kernels, reshape_and_cache), and q [tokens, heads, dim], turned, is returned (or written to `out`, which
+    (serving/csrc/cache_kernels), and q [tokens, heads, dim], turned, is returned (or written to `out`, which
     may be q itself).  positions and slots int64 [tokens]; a negative slot stores nothing (a padded row: its q is turned all the
     same); one beyond the pages neither, and is reported through the status word.  rope None: nothing is turned, and q is
     returned as it is.  No two tokens may have one slot: what is there afterwards may be parts of either.  Strides as
@@ -425,7 +425,7 @@ def append_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torc
 
 def copy_pages(pools: Union[torch.Tensor, Sequence[torch.Tensor]], pairs) -> None:
     """Page `a` copied over page `b` for every (a, b) of `pairs`, in every pool: in place, in one launch for up to 320 pairs
-    and 128 pools (serving/csrc/cache_kernels, copy_blocks).  pools: one tensor [pools, pages, ...], or a sequence of
+    and 128 pools (serving/csrc/cache_kernels).  pools: one tensor [pools, pages, ...], or a sequence of
     [pages, ...] of one shape, type and stride, pages contiguous and of a multiple of 16 bytes.  pairs: host integers [n, 2],
     a tensor or a sequence; they are read before the call returns (a graph that captures the call copies the same
     pages at every replay).  All copies run side by side: no page may be written twice, or be both read and written."""

@@ -223,6 +223,8 @@ def test_calls_that_do_not_fit_change_nothing(monkeypatch):
         cache.slots("a", 3, 10)
     with pytest.raises(ValueError):
         cache.batch(["a"], width=1)
+    with pytest.raises(ValueError, match="twice"):
+        cache.batch(["a", None, "a"])
     cache.add("empty")
     with pytest.raises(ValueError):
         cache.batch(["empty"])
@@ -929,3 +931,60 @@ def test_a_bad_page_of_a_replay_is_reported_once(dev):
     with pytest.raises(ops.DeltaKernelError, match="paged"):
         ops.poll_status(dev)                   # which the next call takes in
     ops.poll_status(dev, wait=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 2, 15, 16, 17, 63, 64, 65, 128, 129, 192, 193, 255, 256, 257, 300])
+def test_attention_of_any_number_of_rows(dev, rows):
+    """Lengths that are cut into one part, several, and more than are joined at once, in any order of the rows."""
+    from deltazip_amd import paged_attention
+    rng = random.Random(rows)
+    lengths = [rng.choice([0, 1, 5, 30, 64, 100, 383, 384, 385, 400, 600]) for _ in range(rows)]
+    lengths[rng.randrange(rows)] = 7000 + 2000 * (rows % 3)
+    if rows > 3:
+        lengths[rng.randrange(rows)] = 17000
+    p = _problem(dev, torch.float16, lengths, 2, 1, 32, 32, rows)
+    got = paged_attention(*p)
+    _hold(got, *p, 32 ** -0.5)
+    assert torch.equal(got, paged_attention(*p))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seed", range(60))
+def test_attention_over_drawn_sizes(dev, seed):
+    from deltazip_amd import paged_attention
+    rng = random.Random(1000 + seed)
+    kv = rng.choice([1, 1, 2, 3, 5, 8])
+    heads = kv * rng.choice([1, 1, 2, 3, 4, 7, 8, 16, 17, 24])
+    dim, ps, rows = 8 * rng.randrange(1, 33), 8 << rng.randrange(0, 8), rng.choice([1, 2, 3, 7, 20, 40])
+    most = max(2, 60000 // (rows * heads))
+    lengths = [rng.choice([0, 1, rng.randrange(1, 40), rng.randrange(1, most), most]) for _ in range(rows)]
+    q, k, v, tables, ln = _problem(dev, rng.choice(TYPES), lengths, heads, kv, dim, ps, seed)
+    window = rng.choice([0, 0, 1, 7, 64, rng.randrange(1, most + 1), 2 * most])
+    if rng.random() < 0.5:                              # tokens in front of heads, and both pools in one
+        both = torch.stack((k.transpose(1, 2), v.transpose(1, 2)), 1).contiguous()
+        k, v = both[:, 0].transpose(1, 2), both[:, 1].transpose(1, 2)
+    scale = rng.choice([dim ** -0.5, 1.0, -0.1, 0.0])
+    _hold(paged_attention(q, k, v, tables, ln, scale=scale, window=window), q, k, v, tables, ln, scale, window)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seed", range(30))
+def test_append_over_drawn_sizes(dev, seed):
+    """Against the restatement: turned queries, and every slot of the pools, those that nothing was stored at included."""
+    from deltazip_amd import RotaryPositions, append_kv
+    rng = random.Random(2000 + seed)
+    heads, kv, dim = rng.randrange(1, 30), rng.randrange(1, 9), 2 * rng.randrange(1, 129)
+    rot, ps, tokens, dtype = 2 * rng.randrange(1, dim // 2 + 1), 8 << rng.randrange(0, 6), rng.choice([1, 2, 9, 64, 333]), rng.choice(TYPES)
+    rope = RotaryPositions(dim, rotary_dim=rot, interleaved=rng.random() < 0.5, base=rng.choice([100.0, 10000.0, 1e6]))
+    q, k, v = _qkv(dev, dtype, tokens, heads, kv, dim, seed)
+    pages = -(-tokens // ps) + 2
+    kp, vp = (torch.randn(pages, kv, ps, dim, device=dev).to(dtype) for _ in range(2))
+    slots, pos = torch.randperm(pages * ps, device=dev)[:tokens], torch.randint(-50, 1 << 22, (tokens,), device=dev)
+    wk, wv = kp.clone(), vp.clone()
+    _turned(append_kv(q, k, v, pos, slots, rope, kp, vp), q, pos, rope)
+    page, place = slots // ps, slots % ps
+    _turned(kp[page, :, place], k, pos, rope)
+    assert torch.equal(vp[page, :, place], v)
+    wk[page, :, place], wv[page, :, place] = kp[page, :, place], v
+    assert torch.equal(kp, wk) and torch.equal(vp, wv)
