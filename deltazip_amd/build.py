@@ -74,10 +74,11 @@ def host_command():
     """The compiler's line for the Python extension (plain C++ over torch's headers, linked with libdz_amd.so)."""
     import torch
     from torch.utils.cpp_extension import include_paths, library_paths
-    libs = [f"-L{d}" for d in library_paths()] + ["-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10"]
+    libs = [f"-L{d}" for d in library_paths()] + ["-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_hip"]
     return [shutil.which("g++") or "c++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{d}" for d in include_paths()),
-            f"-I{sysconfig.get_paths()['include']}", os.path.join(CSRC, "dz_host.cpp"), LIB, *libs, "-Wl,-rpath,$ORIGIN", "-o", HOST]
+            f"-I{sysconfig.get_paths()['include']}", "-I/opt/rocm/include", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
+            os.path.join(CSRC, "dz_host.cpp"), LIB, *libs, "-Wl,-rpath,$ORIGIN", "-o", HOST]
 
 
 if __name__ == "__main__":

@@ -7,8 +7,13 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ops/empty.h>
+#include <ATen/ops/zeros.h>
+#include <c10/hip/HIPFunctions.h>
+#include <c10/hip/HIPStream.h>
 
 #include <cmath>
+#include <map>
+#include <utility>
 #include <vector>
 
 #include "../../include/dz_amd.h"
@@ -34,13 +39,49 @@ bool index_on(const at::Tensor& t, int64_t n, at::ScalarType type, int dev) {
 }
 bool floats(at::ScalarType t) { return t == at::kHalf || t == at::kBFloat16; }
 
-// attend(q, k_pages, v_pages, tables, lengths, scale or None, window, device, stream, status, counters, work, work_bytes)
+// Where a call goes: the current device and stream, and the device's status word once Python has taken note of it.
+uint32_t* status_at[64];
+struct Place {
+  int dev;
+  void* stream;
+  uint32_t* status;
+  Place() : dev(c10::hip::current_device()), stream(c10::hip::getCurrentHIPStream((c10::DeviceIndex)dev).stream()),
+            status(dev >= 0 && dev < 64 ? status_at[dev] : nullptr) {}
+};
+
+// Counters, all zero between calls, and room for the sums of parts, of a stream: calls on it follow each other.  (Never freed: it
+// may outlive the runtime's own end.)
+struct Space {
+  at::Tensor counters, work;
+};
+Space& space_of(const Place& p, size_t need, const at::Tensor& like) {
+  static auto* spaces = new std::map<std::pair<int, void*>, Space>;
+  Space& s = (*spaces)[{p.dev, p.stream}];
+  if (!s.counters.defined()) s.counters = at::zeros({DZ_ATTENTION_COUNTERS}, like.options().dtype(at::kInt));
+  if (!s.work.defined() || (size_t)s.work.numel() < need)
+    s.work = at::empty({(int64_t)(need > (1 << 20) ? need : 1 << 20)}, like.options().dtype(at::kByte));
+  return s;
+}
+
+// arm(device, address of its status word)
+PyObject* arm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  const long dev = n == 2 ? PyLong_AsLong(a[0]) : -1;
+  void* at = n == 2 ? PyLong_AsVoidPtr(a[1]) : nullptr;
+  if (PyErr_Occurred()) return nullptr;
+  if (dev >= 0 && dev < 64) status_at[dev] = (uint32_t*)at;
+  Py_RETURN_NONE;
+}
+
+// attend(q, k_pages, v_pages, tables, lengths, scale or None, window)
 PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (n != 13) Py_RETURN_NONE;
+  if (n != 7) Py_RETURN_NONE;
   const at::Tensor *q = tensor(a[0]), *k = tensor(a[1]), *v = tensor(a[2]), *tables = tensor(a[3]), *lengths = tensor(a[4]);
   if (!q || !k || !v || !tables || !lengths || !PyLong_CheckExact(a[6]) || !(a[5] == Py_None || PyFloat_CheckExact(a[5]))) Py_RETURN_NONE;
-  const int dev = (int)PyLong_AsLong(a[7]);
+  if (!q->is_cuda()) Py_RETURN_NONE;
+  const Place here;
+  const int dev = here.dev;
+  if (!here.status) Py_RETURN_NONE;
   int overflow = 0;
   const long window = PyLong_AsLongAndOverflow(a[6], &overflow);
   if (overflow || window < 0 || window > 0x7fffffff) Py_RETURN_NONE;
@@ -53,16 +94,20 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!index_on(*lengths, rows, at::kInt, dev)) Py_RETURN_NONE;
   const int width = (int)tables->size(1);
   const size_t need = dz_paged_attention_bytes((int)rows, (int)heads, (int)kv_heads, (int)dim, (int)ps, width);
-  const size_t room = PyLong_AsSize_t(a[12]);
-  if (need > room) Py_RETURN_NONE;
+  void *work = nullptr, *counters = nullptr;
+  if (need) {
+    if (dz_capture_id(here.stream)) Py_RETURN_NONE;    // (a graph has its own)
+    Space& space = space_of(here, need, *q);
+    work = space.work.data_ptr(), counters = space.counters.data_ptr();
+  }
   at::Tensor out = at::empty({rows, heads, dim}, q->options());
   dz_attention_args c{};
   c.bytes = sizeof(c);
   c.q = q->data_ptr(), c.k_pages = k->data_ptr(), c.v_pages = v->data_ptr();
   c.tables = (const int32_t*)tables->data_ptr(), c.lengths = (const int32_t*)lengths->data_ptr();
   c.out = out.data_ptr();
-  c.work = (void*)pointer(a[11]), c.counters = (uint32_t*)pointer(a[10]), c.status = (uint32_t*)pointer(a[9]);
-  c.work_bytes = (int64_t)room, c.num_pages = k->size(0);
+  c.work = work, c.counters = (uint32_t*)counters, c.status = here.status;
+  c.work_bytes = (int64_t)need, c.num_pages = k->size(0);
   c.q_row = step(*q, 0), c.q_head = step(*q, 1);
   c.k_page = step(*k, 0), c.k_head = step(*k, 1), c.k_token = k->stride(2);
   c.v_page = step(*v, 0), c.v_head = step(*v, 1), c.v_token = v->stride(2);
@@ -70,26 +115,27 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   c.rows = (int)rows, c.heads = (int)heads, c.kv_heads = (int)kv_heads, c.dim = (int)dim, c.page_size = (int)ps;
   c.pages_per_row = width, c.window = (int)window, c.dtype = q->scalar_type() == at::kBFloat16 ? DZ_BF16 : DZ_F16;
   c.scale = a[5] == Py_None ? (float)(1.0 / std::sqrt((double)dim)) : (float)PyFloat_AS_DOUBLE(a[5]);
-  void* stream = (void*)pointer(a[8]);
   if (PyErr_Occurred()) return nullptr;
   int rc;
   Py_BEGIN_ALLOW_THREADS
-  rc = dz_paged_attention(&c, stream);
+  rc = dz_paged_attention(&c, here.stream);
   Py_END_ALLOW_THREADS
   if (rc) Py_RETURN_NONE;
   return THPVariable_Wrap(std::move(out));
   END_HANDLE_TH_ERRORS
 }
 
-// rotate(q, k, v, positions, slots, (turns, rot, neighbours, factor, head_dim) or None, k_pages, v_pages, q in place, device, stream, status):
+// rotate(q, k, v, positions, slots, (turns, rot, neighbours, factor, head_dim) or None, k_pages, v_pages, q in place):
 // q turned (append_kv); without pages, v and slots None: (q turned, k turned or None) (rotary)
 PyObject* rotate(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (n != 12) Py_RETURN_NONE;
+  if (n != 9) Py_RETURN_NONE;
   const bool paged = a[4] != Py_None;
   const at::Tensor *q = tensor(a[0]), *k = tensor(a[1]), *positions = tensor(a[3]);
-  const int dev = (int)PyLong_AsLong(a[9]);
-  if (!q || !positions || (!k && (paged || a[1] != Py_None))) Py_RETURN_NONE;
+  if (!q || !q->is_cuda()) Py_RETURN_NONE;
+  const Place here;
+  const int dev = here.dev;
+  if (!positions || (paged && !here.status) || (!k && (paged || a[1] != Py_None))) Py_RETURN_NONE;
   const at::ScalarType type = q->scalar_type();
   if (!floats(type) || !heads_on(*q, type, dev) || q->size(0) < 1 || q->size(0) > 0x7fffffff || q->size(1) < 1 || q->size(1) > 4096) Py_RETURN_NONE;
   const int64_t tokens = q->size(0), dim = q->size(2);
@@ -117,7 +163,7 @@ PyObject* rotate(PyObject*, PyObject* const* a, Py_ssize_t n) {
         kp->data_ptr() == vp->data_ptr() || !kp->is_contiguous() || !vp->is_contiguous())
       Py_RETURN_NONE;
     c.v = v->data_ptr(), c.v_row = step(*v, 0), c.v_head = step(*v, 1);
-    c.slots = (const int64_t*)slots->data_ptr(), c.status = (uint32_t*)pointer(a[11]);
+    c.slots = (const int64_t*)slots->data_ptr(), c.status = here.status;
     c.num_pages = kp->size(0), c.page_size = (int)kp->size(2);
     c.k_out = kp->data_ptr(), c.k_out_page = step(*kp, 0), c.k_out_head = step(*kp, 1), c.k_out_token = kp->stride(2);
     c.v_out = vp->data_ptr(), c.v_out_page = step(*vp, 0), c.v_out_head = step(*vp, 1), c.v_out_token = vp->stride(2);
@@ -141,11 +187,10 @@ PyObject* rotate(PyObject*, PyObject* const* a, Py_ssize_t n) {
   }
   c.positions = (const int64_t*)positions->data_ptr();
   c.tokens = (int)tokens, c.heads = in_place && !c.rot ? 0 : (int)q->size(1), c.dim = (int)dim, c.dtype = type == at::kBFloat16 ? DZ_BF16 : DZ_F16;
-  void* stream = (void*)pointer(a[10]);
   if (PyErr_Occurred()) return nullptr;
   int rc;
   Py_BEGIN_ALLOW_THREADS
-  rc = dz_rotary(&c, stream);
+  rc = dz_rotary(&c, here.stream);
   Py_END_ALLOW_THREADS
   if (rc) Py_RETURN_NONE;
   if (in_place) {
@@ -166,13 +211,15 @@ PyObject* rotate(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// copy(pools [n, pages, ...], pairs [m, 2] on the host, device, stream): True where the copies were launched
+// copy(pools [n, pages, ...], pairs [m, 2] on the host): True where the copies were launched
 PyObject* copy(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (n != 4) Py_RETURN_NONE;
+  if (n != 2) Py_RETURN_NONE;
   const at::Tensor *pools = tensor(a[0]), *pairs = tensor(a[1]);
-  const int dev = (int)PyLong_AsLong(a[2]);
-  if (!pools || !pairs || !pools->is_cuda() || pools->get_device() != dev || pools->dim() < 2 || !pools->is_contiguous() || pools->numel() == 0 ||
+  if (!pools || !pairs || !pools->is_cuda()) Py_RETURN_NONE;
+  const Place here;
+  const int dev = here.dev;
+  if (pools->get_device() != dev || pools->dim() < 2 || !pools->is_contiguous() || pools->numel() == 0 ||
       pools->size(1) >= (1ll << 31) || pools->size(0) > (1 << 20))
     Py_RETURN_NONE;
   if (!pairs->is_cpu() || pairs->scalar_type() != at::kLong || pairs->dim() != 2 || pairs->size(1) != 2 || !pairs->is_contiguous() ||
@@ -201,18 +248,18 @@ PyObject* copy(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!fits) Py_RETURN_NONE;
   std::vector<void*> at(npools);
   for (int64_t i = 0; i < npools; ++i) at[i] = (char*)pools->data_ptr() + i * pages * bytes;
-  void* stream = (void*)pointer(a[3]);
   if (PyErr_Occurred()) return nullptr;
   int rc;
   Py_BEGIN_ALLOW_THREADS
-  rc = dz_copy_pages(at.data(), (int)npools, bytes, bytes, (int)pages, list.data(), (int)m, stream);
+  rc = dz_copy_pages(at.data(), (int)npools, bytes, bytes, (int)pages, list.data(), (int)m, here.stream);
   Py_END_ALLOW_THREADS
   if (rc) Py_RETURN_NONE;
   Py_RETURN_TRUE;
   END_HANDLE_TH_ERRORS
 }
 
-PyMethodDef methods[] = {{"attend", (PyCFunction)(void (*)(void))attend, METH_FASTCALL, nullptr},
+PyMethodDef methods[] = {{"arm", (PyCFunction)(void (*)(void))arm, METH_FASTCALL, nullptr},
+                         {"attend", (PyCFunction)(void (*)(void))attend, METH_FASTCALL, nullptr},
                          {"rotate", (PyCFunction)(void (*)(void))rotate, METH_FASTCALL, nullptr},
                          {"copy", (PyCFunction)(void (*)(void))copy, METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};

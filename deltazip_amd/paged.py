@@ -182,6 +182,7 @@ def _status(dev: int) -> int:
         if not at:
             raise RuntimeError("the library has no memory on the current device")
         ops._page_status[dev] = at
+        _lib.host().arm(dev, at)
     return at
 
 
@@ -255,11 +256,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     tokens.  A length beyond its table is cut; a page number outside the pool is read as page 0; either is reported through the
     status word.  The order of a row's sums follows the lengths of all rows of the call (the work is cut by them,
     256 rows at a time): the same lengths give the same bits."""
-    if out is None and q.is_cuda:
-        dev, stream = ops._current_device(), ops._stream()
-        space = None if _capturing() else _spaces.get((dev, stream))
-        out = _lib.host().attend(q, k_pages, v_pages, block_tables, lengths, scale, window, dev, stream, _status(dev),
-                                 *((0, 0, 0) if space is None else space[2:]))
+    if out is None:
+        out = _lib.host().attend(q, k_pages, v_pages, block_tables, lengths, scale, window)
         if out is not None:
             return out
     ops._need_cuda(q, k_pages, v_pages, block_tables, lengths, out)
@@ -330,9 +328,8 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     value); returns new tensors, or writes `out` = (q, k): the inputs themselves (in place, as
     serving/csrc/pos_encoding does) or memory of their own.  Rows and heads may have any stride of an even number of values;
     with strides, sizes and half of rotary_dim multiples of eight, requests are four times as wide."""
-    if out is None and q.is_cuda:
-        dev, stream = ops._current_device(), ops._stream()
-        made = _lib.host().rotate(q, k, None, positions, None, rope._packed.get(dev), None, None, False, dev, stream, 0)
+    if out is None:
+        made = _lib.host().rotate(q, k, None, positions, None, rope._packed.get(q.get_device()), None, None, False)
         if made is not None:
             return made
     ops._need_cuda(q, k, positions)
@@ -378,11 +375,9 @@ def append_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torc
     same); one beyond the pages neither, and is reported through the status word.  rope None: nothing is turned, and q is
     returned as it is.  No two tokens may have one slot: what is there afterwards may be parts of either.  Strides as
     for `rotary`."""
-    if q.is_cuda and (out is None or out is q):
-        dev = ops._current_device()
-        turns = None if rope is None else rope._packed.get(dev, _UNPACKED)
-        made = _lib.host().rotate(q, k, v, positions, slots, turns, k_pages, v_pages, out is q or rope is None, dev, ops._stream(),
-                                  _status(dev))
+    if out is None or out is q:
+        turns = None if rope is None else rope._packed.get(q.get_device(), _UNPACKED)
+        made = _lib.host().rotate(q, k, v, positions, slots, turns, k_pages, v_pages, out is q or rope is None)
         if made is not None:
             return made
     ops._need_cuda(q, k, v, positions, slots, k_pages, v_pages, out)
@@ -434,7 +429,7 @@ def copy_pages(pools: Union[torch.Tensor, Sequence[torch.Tensor]], pairs) -> Non
     if isinstance(pairs, np.ndarray) and pairs.dtype == np.int64:
         pairs = torch.from_numpy(pairs)
     stacked = isinstance(pools, torch.Tensor)
-    if stacked and pools.is_cuda and _lib.host().copy(pools, pairs, ops._current_device(), ops._stream()):
+    if stacked and _lib.host().copy(pools, pairs):
         return
     if stacked:
         if pools.dim() < 2:
