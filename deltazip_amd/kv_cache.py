@@ -2,9 +2,8 @@
 
 The pages of all layers are held in one tensor, [2 layers, pages, kv_heads, page_size, head_dim]; a page number
 means the same page in each.  Sequences that were forked share pages: a page is copied when a sequence is
-about to write to one that others still read.  What the reference's serving engine keeps in its block manager and
-cache engine (serving/vllm/core/block_manager.py, serving/vllm/worker/cache_engine.py) is here one class; the
-scheduler stays the caller's.
+about to write to one that others still read.  What the reference's serving engine (serving/vllm) divides between its scheduler
+and its workers is here one class; the scheduling itself stays the caller's.
 
 All bookkeeping is on the host and known when a call returns; what the device does follows in the order of the
 current stream.  A cache serves one stream at a time: a page that was freed may be given away while kernels in

@@ -39,7 +39,7 @@ class RotaryPositions:
     pairs -- (i, i + rotary_dim / 2), or neighbours with `interleaved` -- by position * base^(-2 i / rotary_dim).
 
     `scaling` is the entry of a model's configuration that stretches the positions beyond the trained ones
-    (`max_position`), as the reference reads it (serving/vllm/model_executor/layers/rotary_embedding.py):
+    (`max_position`), as the reference's model layers read it (serving/vllm/model_executor):
       {"type": "linear", "factor": s}    positions divided by s
       {"type": "dynamic", "factor": s}   the base raised for s times the trained length
       {"type": "yarn", "factor": s, "original_max_position_embeddings": m, "extrapolation_factor": 1, "attn_factor": 1,
