@@ -251,16 +251,16 @@ class PagedKVCache:
         place, slot = (host[8 * rows * i:8 * rows * (i + 1)].view(np.int64) for i in range(2))
         lengths = host[16 * rows:20 * rows].view(np.int32)
         tables = host[20 * rows:].view(np.int32).reshape(rows, width)
-        slot[:] = -1
-        for i, s in enumerate(found):
-            if s is not None:
-                last = s.length - 1
-                page = s.pages[last // self.page_size]
-                if self._users[page] > 1:
-                    raise ValueError("a row's newest token lies in a page that other sequences hold too: extend makes it its own")
-                place[i], lengths[i] = last, s.length
-                slot[i] = page * self.page_size + last % self.page_size
-                tables[i, :len(s.pages)] = self._rows[s.row, :len(s.pages)]
+        at = np.fromiter((0 if s is None else s.row for s in found), np.int64, rows)
+        length = np.fromiter((0 if s is None else s.length for s in found), np.int64, rows)
+        real, last = length > 0, np.maximum(length - 1, 0)
+        page = self._rows[at, last // self.page_size]
+        if any(self._users[p] > 1 for p in page[real].tolist()):
+            raise ValueError("a row's newest token lies in a page that other sequences hold too: extend makes it its own")
+        place[:], lengths[:] = last, length
+        slot[:] = np.where(real, page.astype(np.int64) * self.page_size + last % self.page_size, -1)
+        columns = np.arange(min(width, self.max_pages))
+        tables[:, :len(columns)] = np.where(columns < -(-length // self.page_size)[:, None], self._rows[at, :len(columns)], 0)
         dev = torch.from_numpy(host).to(self.pool.device)
         made = PagedBatch(dev[:8 * rows].view(torch.int64), dev[8 * rows:16 * rows].view(torch.int64),
                           dev[20 * rows:].view(torch.int32).view(rows, width), dev[16 * rows:20 * rows].view(torch.int32))
