@@ -628,8 +628,8 @@ int dz_paged_attention(const dz_attention_args* a, void* stream) {
   if (lds > 65536 && !dz_lds_limit_once(attr_done[which], (const void*)kern, (int)LDS_MOST)) return DZ_ELAUNCH;
   const hipStream_t st = (hipStream_t)stream;
   const int together = group_rows(items);
-  for (int row = 0; row < a->rows; row += together) {
-    P.rows = a->rows - row < together ? a->rows - row : together;
+  for (long long row = 0; row < a->rows; row += together) {
+    P.rows = a->rows - row < together ? (int)(a->rows - row) : together;
     P.q = (const char*)a->q + row * P.q_row;
     P.out = (uint16_t*)a->out + row * P.out_row;
     P.tables = a->tables + row * P.table_row;

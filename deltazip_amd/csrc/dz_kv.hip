@@ -258,7 +258,7 @@ int dz_rotary(const dz_rotary_args* a, void* stream) {
   if (total == 0) return DZ_OK;
   // a token's heads over as many workgroups as make some 1024 together: with all of them apart each works out the angles again
   // (8192 tokens of 48 heads 39.8 -> 35.9 us, 4000 of 48 heads of 80 14.8 -> 12.1)
-  const int apart = (total + each - 1) / each, few = (1023 + a->tokens) / a->tokens;
+  const int apart = (total + each - 1) / each, few = a->tokens < 1024 ? (1023 + a->tokens) / a->tokens : 1;
   const int slices = apart < few ? apart : few;
   typedef void (*kernel_t)(const RotaryParams);
   static const kernel_t kernels[2][8] = {
@@ -280,14 +280,14 @@ int dz_copy_pages(void* const* pools, int npools, long long page_stride, long lo
   if (page_bytes % 16 || page_stride % 16 || page_stride < page_bytes || page_bytes / 16 > 0x7fffffff - 256) return DZ_EPAGES;
   for (int i = 0; i < npools; ++i)
     if (!pools[i] || ((uintptr_t)pools[i] & 15)) return DZ_EALIGN;
-  for (int i = 0; i < 2 * npairs; ++i)
+  for (long long i = 0; i < 2ll * npairs; ++i)
     if (pairs[i] < 0 || pairs[i] >= num_pages) return DZ_EINVAL;
   const bool once = (double)page_bytes * npools * npairs > (double)(256 << 20);     // (more than the last cache holds)
   CopyParams P;
   P.page_stride = page_stride;
   P.chunks = (int)(page_bytes / 16);
-  for (int p0 = 0; p0 < npairs; p0 += COPY_PAIRS) {
-    const int np = npairs - p0 < COPY_PAIRS ? npairs - p0 : COPY_PAIRS;
+  for (long long p0 = 0; p0 < npairs; p0 += COPY_PAIRS) {
+    const int np = npairs - p0 < COPY_PAIRS ? (int)(npairs - p0) : COPY_PAIRS;
     for (int i = 0; i < np; ++i) P.pairs[i] = int2{pairs[2 * (p0 + i)], pairs[2 * (p0 + i) + 1]};
     for (int l0 = 0; l0 < npools; l0 += COPY_POOLS) {
       const int nl = npools - l0 < COPY_POOLS ? npools - l0 : COPY_POOLS;

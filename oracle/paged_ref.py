@@ -2,7 +2,7 @@
 
 Written from the formulas: rotary positions as products of complex numbers, attention row by row over the tokens
 that a row sees.  Inputs of any floating type are taken at their values; results are float64.  Checked by
-tests/test_paged.py against closed forms before it is used as the checker.
+tests/test_paged.py against closed forms before the kernels are held to it.
 """
 from __future__ import annotations
 
