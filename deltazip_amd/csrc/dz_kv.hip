@@ -5,7 +5,7 @@
 // for pair i of the first `rot` values of a head: (i, i + rot / 2), or (2 i, 2 i + 1) where neighbours are paired.  turns
 // is in 64 bits and so is position * turns up to its fraction, so that angles of far positions lose nothing; sine and
 // cosine of the fraction are taken in 32 bits, once per token and pair, and serve all heads from LDS.
-// Everything here is bound by reading its inputs and writing its outputs once: 8192 tokens of 48 heads of 128 stored in 34 us, 5.9 TB/s;
+// Everything here is bound by reading its inputs and writing its outputs once: 8192 tokens of 48 heads of 128 stored in 35 us, 5.7 TB/s;
 // 700 pages of 64 pools of 32 KiB copied in 541, 5.4; 128 tokens of 96 heads 3.3, of which an empty launch takes 2.5.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -22,13 +22,13 @@ struct RotaryParams {
   char *q_out, *k_out;                 // k_out: rows, or the cache's pages where there are slots
   char* v_out;
   const long long *positions, *slots;
-  const double* turns;
   unsigned* status;
   long long q_row, q_head, k_row, k_head, v_row, v_head;                     // bytes
   long long qo_row, qo_head, ko_page, ko_head, ko_token, vo_page, vo_head, vo_token;
   long long capacity;                  // tokens that the pages hold
   int heads, kv_heads, dim, rot, shift;
   float factor;
+  double turns[128];                   // by value: no memory that a call in flight, or a graph, depends on
 };
 
 template <bool BF>
@@ -231,7 +231,7 @@ int dz_rotary(const dz_rotary_args* a, void* stream) {
   P.q = (const char*)a->q, P.k = (const char*)a->k, P.v = (const char*)a->v;
   P.q_out = (char*)a->q_out, P.k_out = (char*)a->k_out, P.v_out = (char*)a->v_out;
   P.positions = (const long long*)a->positions, P.slots = (const long long*)a->slots;
-  P.turns = a->turns, P.status = a->status;
+  P.status = a->status;
   P.q_row = 2 * a->q_row, P.q_head = 2 * a->q_head, P.k_row = 2 * a->k_row, P.k_head = 2 * a->k_head, P.v_row = 2 * a->v_row,
   P.v_head = 2 * a->v_head, P.qo_row = 2 * a->q_out_row, P.qo_head = 2 * a->q_out_head;
   P.ko_page = 2 * a->k_out_page, P.ko_head = 2 * a->k_out_head, P.ko_token = 2 * a->k_out_token;
@@ -268,6 +268,7 @@ int dz_rotary(const dz_rotary_args* a, void* stream) {
        dz_rotary_kernel<true, false, 1, 2>, dz_rotary_kernel<true, true, 8, 8>, dz_rotary_kernel<true, true, 2, 8>, dz_rotary_kernel<true, true, 2, 2>}};
   const int which = a->neighbours ? (turn == 8 ? 5 : copy ? 6 : 7) : turn == 8 ? 0 : copy ? (turn == 2 ? 1 : 2) : turn == 2 ? 3 : 4;
   const kernel_t kern = kernels[a->dtype == DZ_BF16][which];
+  for (int i = 0; i < a->rot / 2; ++i) P.turns[i] = a->turns[i];
   hipLaunchKernelGGL(kern, dim3(a->tokens, slices), dim3(units, each), 0, (hipStream_t)stream, P);
   return hipGetLastError() == hipSuccess ? DZ_OK : DZ_ELAUNCH;
 }

@@ -45,10 +45,10 @@ class RotaryPositions:
       {"type": "yarn", "factor": s, "original_max_position_embeddings": m, "extrapolation_factor": 1, "attn_factor": 1,
        "beta_fast": 32, "beta_slow": 1}  pairs that turn less than beta_slow times within m positions stretched, those that turn
                                          more than beta_fast kept, a ramp between; turned values times attn_factor (0.1 ln s + 1)
-    Angles are held in 64 bits, as turns per position.  Made once per model; call `on(device)` before a capture."""
+    Angles are held in 64 bits, as turns per position, on the host: a call takes them along."""
 
     def __init__(self, head_dim: int, rotary_dim: Optional[int] = None, base: float = 10000.0, max_position: int = 4096,
-                 interleaved: bool = False, scaling: Optional[Mapping] = None, device=None) -> None:
+                 interleaved: bool = False, scaling: Optional[Mapping] = None) -> None:
         r = head_dim if rotary_dim is None else rotary_dim
         if head_dim < 2 or head_dim > MAX_DIM or head_dim % 2:
             raise ValueError(f"head_dim must be even, up to {MAX_DIM}")
@@ -87,23 +87,9 @@ class RotaryPositions:
         if scaling:
             raise ValueError(f"entries of the scaling that {kind!r} has no use for: {sorted(scaling)}")
         self.frequencies = torch.from_numpy(freq)                         # radians per position, float64
-        self._turns: Dict[torch.device, torch.Tensor] = {}
-        self._packed: Dict[int, tuple] = {}                               # device index -> what the host's half takes
-        if device is not None:
-            self.on(device)
-
-    def on(self, device) -> torch.Tensor:
-        """Turns per position of every pair, float64 on the device."""
-        device = torch.device(device)
-        if device.index is None:
-            device = torch.device(device.type, torch.cuda.current_device())
-        t = self._turns.get(device)
-        if t is None:
-            if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("RotaryPositions.on(device) has to be called before the capture")
-            t = self._turns[device] = (self.frequencies / (2 * math.pi)).to(device)
-            self._packed[device.index] = (t.data_ptr(), self.rotary_dim, int(self.interleaved), self.attention_factor, self.head_dim)
-        return t
+        self._turns = freq / (2 * math.pi)
+        # what the host's half of a call takes: address of the turns, pairs' values, layout, factor, head size
+        self._packed = (self._turns.ctypes.data, r, int(self.interleaved), self.attention_factor, head_dim)
 
 
 def _stride(t: torch.Tensor, d: int) -> int:
@@ -169,9 +155,6 @@ def _pages(name: str, t: torch.Tensor, q: torch.Tensor) -> None:
         raise ValueError("a page must hold a power of two of tokens, from 8 to 1024")
     if not 1 <= t.shape[0] < 1 << 31 or not t.shape[1]:
         raise ValueError(f"{name} holds no pages")
-
-
-_UNPACKED = object()
 
 
 def _status(dev: int) -> int:
@@ -313,7 +296,7 @@ def _rotate(q, k, v, positions, slots, rope, q_out, k_out, v_out, page_size, num
     args = _ROTARY.pack(
         _ROTARY.size, q.data_ptr(), 0 if k is None else k.data_ptr(), 0 if v is None else v.data_ptr(), q_out.data_ptr(),
         0 if k is None else k_out.data_ptr(), 0 if v is None else v_out.data_ptr(), positions.data_ptr(),
-        slots.data_ptr() if paged else 0, 0 if rope is None else rope.on(q.device).data_ptr(), _status(q.get_device()) if paged else 0,
+        slots.data_ptr() if paged else 0, 0 if rope is None else rope._packed[0], _status(q.get_device()) if paged else 0,
         num_pages, _stride(q, 0), _stride(q, 1), *((0, 0) if k is None else (_stride(k, 0), _stride(k, 1))),
         *((0, 0) if v is None else (_stride(v, 0), _stride(v, 1))), _stride(q_out, 0), _stride(q_out, 1),
         *((0, 0, 0) if k is None else strides(k_out)), *((0, 0, 0) if v is None else strides(v_out)),
@@ -329,7 +312,7 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     serving/csrc/pos_encoding does) or memory of their own.  Rows and heads may have any stride of an even number of values;
     with strides, sizes and half of rotary_dim multiples of eight, requests are four times as wide."""
     if out is None:
-        made = _lib.host().rotate(q, k, None, positions, None, rope._packed.get(q.get_device()), None, None, False)
+        made = _lib.host().rotate(q, k, None, positions, None, rope._packed, None, None, False)
         if made is not None:
             return made
     ops._need_cuda(q, k, positions)
@@ -376,8 +359,7 @@ def append_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torc
     returned as it is.  No two tokens may have one slot: what is there afterwards may be parts of either.  Strides as
     for `rotary`."""
     if out is None or out is q:
-        turns = None if rope is None else rope._packed.get(q.get_device(), _UNPACKED)
-        made = _lib.host().rotate(q, k, v, positions, slots, turns, k_pages, v_pages, out is q or rope is None)
+        made = _lib.host().rotate(q, k, v, positions, slots, None if rope is None else rope._packed, k_pages, v_pages, out is q or rope is None)
         if made is not None:
             return made
     ops._need_cuda(q, k, v, positions, slots, k_pages, v_pages, out)

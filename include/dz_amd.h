@@ -527,7 +527,7 @@ typedef struct dz_rotary_args {
   const void *q, *k, *v;                  /* [tokens, heads or kv_heads, dim] */
   void *q_out, *k_out, *v_out;
   const int64_t *positions, *slots;       /* [tokens]; slots or NULL */
-  const double *turns;                    /* [rot / 2] */
+  const double *turns;                    /* [rot / 2], host memory: read before the call returns */
   uint32_t *status;
   int64_t num_pages;
   int64_t q_row, q_head, k_row, k_head, v_row, v_head, q_out_row, q_out_head;

@@ -768,7 +768,7 @@ def test_captured_steps_follow_the_tables_of_the_replay(dev):
     heads, kv, dim, rows = 4, 2, 128, 5
     cache = PagedKVCache(1, 400, 16, kv, dim, max_tokens=4096, device=dev)
     cache.pool.normal_()
-    rope = RotaryPositions(dim, device=dev)
+    rope = RotaryPositions(dim)
     names = list(range(rows))
     for s, n in zip(names, (3, 700, 64, 15, 2000)):
         cache.add(s, n)
