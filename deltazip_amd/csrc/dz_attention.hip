@@ -68,7 +68,7 @@ struct AttnParams {
   unsigned* status;
   long long q_row, q_head, k_page, k_head, k_token, v_page, v_head, v_token, out_row, out_head, table_row;   // bytes; out, table: elements
   unsigned num_pages;
-  int rows, heads, kv_heads, share, head_tiles, dim, shift, pages_per_row, window, part_floats, stat_at, single, once;
+  int rows, heads, kv_heads, share, head_tiles, dim, shift, pages_per_row, window, part_floats, stat_at, single, once, shared;
   float scale, cut;
 };
 
@@ -146,7 +146,7 @@ __device__ __forceinline__ Part find_part(const AttnParams& P, int part, int ite
     mine += (float)tiles[r];
   }
   const float total = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, scan_add(mine)), 63)) * (float)items;
-  found.once = total * (TILE * 4.0f) * (float)P.dim > CACHED;
+  found.once = !P.shared && total * (TILE * 4.0f) * (float)P.dim > CACHED;
   // tiles of a part, in whole steps of the workgroup (sums above 2^24 are rounded, which may come to one part more)
   const float most = ceilf(total * P.cut);
   const unsigned each = WAVES * (unsigned)fminf(fmaxf(most, 1.0f), (float)(1 << 24));
@@ -187,7 +187,8 @@ __device__ __forceinline__ Part find_part(const AttnParams& P, int part, int ite
   return found;
 }
 
-// Keys and values of a call pass through once: loads that keep nothing in the caches read 7.1 TB/s where others read 6.2.
+// Keys and values of a call pass through once: loads that keep nothing in the caches read 7.1 TB/s where others read 6.2.  Not so
+// where rows share pages: 16 rows of one sequence's 4096 tokens of 32 key heads 119 -> 82 us with the others.
 template <bool ONCE>
 __device__ __forceinline__ u4_t load16(const char* at) {
   return ONCE ? __builtin_nontemporal_load((const u4_t*)at) : *(const u4_t*)at;
@@ -615,6 +616,7 @@ int dz_paged_attention(const dz_attention_args* a, void* stream) {
   P.heads = a->heads, P.kv_heads = a->kv_heads, P.share = a->heads / a->kv_heads;
   P.head_tiles = (P.share + HEADS - 1) / HEADS;
   P.dim = a->dim, P.shift = __builtin_ctz(a->page_size), P.pages_per_row = a->pages_per_row, P.window = a->window;
+  P.shared = a->shared != 0;
   const int most = P.share < HEADS ? P.share : HEADS, items = P.kv_heads * P.head_tiles;
   P.part_floats = most * (a->dim + 4);
   P.scale = a->scale * 1.44269504088896340736f;
@@ -637,7 +639,7 @@ int dz_paged_attention(const dz_attention_args* a, void* stream) {
     long long seen = (long long)a->pages_per_row * a->page_size;
     if (a->window && a->window + 2ll * TILE < seen) seen = a->window + 2ll * TILE;             // (it may begin and end inside a tile)
     const long long groups = most_groups(P.rows, items, seen);
-    P.once = (float)P.rows * items * seen * 4.0f * a->dim > CACHED;
+    P.once = !P.shared && (float)P.rows * items * seen * 4.0f * a->dim > CACHED;
     P.cut = 1.0f / (WAVES * (P.rows < FEW_ROWS ? 512 : TARGET));
     P.single = groups == (long long)P.rows * items;
     hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(64 * WAVES), lds, st, P);

@@ -72,10 +72,10 @@ PyObject* arm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Py_RETURN_NONE;
 }
 
-// attend(q, k_pages, v_pages, tables, lengths, scale or None, window)
+// attend(q, k_pages, v_pages, tables, lengths, scale or None, window, shared)
 PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (n != 7) Py_RETURN_NONE;
+  if (n != 8) Py_RETURN_NONE;
   const at::Tensor *q = tensor(a[0]), *k = tensor(a[1]), *v = tensor(a[2]), *tables = tensor(a[3]), *lengths = tensor(a[4]);
   if (!q || !k || !v || !tables || !lengths || !PyLong_CheckExact(a[6]) || !(a[5] == Py_None || PyFloat_CheckExact(a[5]))) Py_RETURN_NONE;
   if (!q->is_cuda()) Py_RETURN_NONE;
@@ -113,7 +113,7 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   c.v_page = step(*v, 0), c.v_head = step(*v, 1), c.v_token = v->stride(2);
   c.out_row = heads * dim, c.out_head = dim, c.table_row = step(*tables, 0);
   c.rows = (int)rows, c.heads = (int)heads, c.kv_heads = (int)kv_heads, c.dim = (int)dim, c.page_size = (int)ps;
-  c.pages_per_row = width, c.window = (int)window, c.dtype = q->scalar_type() == at::kBFloat16 ? DZ_BF16 : DZ_F16;
+  c.pages_per_row = width, c.window = (int)window, c.shared = PyObject_IsTrue(a[7]) == 1, c.dtype = q->scalar_type() == at::kBFloat16 ? DZ_BF16 : DZ_F16;
   c.scale = a[5] == Py_None ? (float)(1.0 / std::sqrt((double)dim)) : (float)PyFloat_AS_DOUBLE(a[5]);
   if (PyErr_Occurred()) return nullptr;
   int rc;

@@ -27,11 +27,13 @@ class OutOfPages(RuntimeError):
 
 class PagedBatch(NamedTuple):
     """What a step of one new token per row needs of the cache, on the device: the newest token's position and slot
-    (int64 [rows]), the tables (int32 [rows, pages]) and lengths (int32 [rows], the new token counted)."""
+    (int64 [rows]), the tables (int32 [rows, pages]) and lengths (int32 [rows], the new token counted); and, on the host, whether
+    rows share most of their pages (for `paged_attention`)."""
     positions: torch.Tensor
     slots: torch.Tensor
     block_tables: torch.Tensor
     lengths: torch.Tensor
+    shared: bool = False
 
 
 class _Sequence:
@@ -60,6 +62,7 @@ class PagedKVCache:
         self.values: Sequence[torch.Tensor] = self.pool[num_layers:].unbind(0)
         self._free = list(range(num_pages))         # a heap: low pages first
         self._users = [0] * num_pages               # sequences that hold a page
+        self._spared = 0                            # pages that sharing has spared: holders beyond the first
         self._seqs: Dict[Hashable, _Sequence] = {}
         self._rows = np.zeros((8, self.max_pages), dtype=np.int32)                 # tables, a row per sequence
         self._free_rows = list(range(8))[::-1]
@@ -150,6 +153,7 @@ class PagedKVCache:
                 at = s.length // self.page_size
                 old, new = s.pages[at], self._take()
                 self._users[old] -= 1
+                self._spared -= 1
                 s.pages[at] = self._rows[s.row, at] = new
                 pairs.append((old, new))
             for at in range(len(s.pages), self._pages_for(s.length + tokens)):
@@ -167,6 +171,7 @@ class PagedKVCache:
             raise ValueError(f"sequence {child!r} is in the cache")
         for page in p.pages:
             self._users[page] += 1
+        self._spared += len(p.pages)
         s = self._seqs[child] = _Sequence(self._new_row(), p.length, list(p.pages))
         self._rows[s.row, :len(p.pages)] = p.pages
 
@@ -180,7 +185,9 @@ class PagedKVCache:
 
     def _release(self, page: int) -> None:
         self._users[page] -= 1
-        if not self._users[page]:
+        if self._users[page]:
+            self._spared -= 1
+        else:
             heapq.heappush(self._free, page)
 
     def truncate(self, seq: Hashable, length: int) -> None:
@@ -263,9 +270,10 @@ class PagedKVCache:
         tables[:, :len(columns)] = np.where(columns < -(-length // self.page_size)[:, None], self._rows[at, :len(columns)], 0)
         dev = torch.from_numpy(host).to(self.pool.device)
         made = PagedBatch(dev[:8 * rows].view(torch.int64), dev[8 * rows:16 * rows].view(torch.int64),
-                          dev[20 * rows:].view(torch.int32).view(rows, width), dev[16 * rows:20 * rows].view(torch.int32))
+                          dev[20 * rows:].view(torch.int32).view(rows, width), dev[16 * rows:20 * rows].view(torch.int32),
+                          2 * self._spared > sum([len(s.pages) for s in found if s is not None]))
         if out is None:
             return made
-        for to, t in zip(out, made):
+        for to, t in zip(out[:4], made):
             to.copy_(t)
-        return out
+        return out._replace(shared=made.shared)

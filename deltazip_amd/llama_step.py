@@ -88,7 +88,7 @@ class LlamaAttention(nn.Module):
         qkv, _ = self.qkv_proj(hidden)
         q, k, v = (t.unflatten(1, (self.num_heads, self.head_dim)) for t in qkv.chunk(3, dim=-1))
         q = append_kv(q, k, v, batch.positions, batch.slots, rope, keys, values)
-        out = paged_attention(q, keys, values, batch.block_tables, batch.lengths)
+        out = paged_attention(q, keys, values, batch.block_tables, batch.lengths, shared=batch.shared)
         out, _ = self.o_proj(out.flatten(1))
         return out
 

@@ -113,6 +113,7 @@ def _check(cache, model):
         assert cache.length(seq) == len(tokens) and len(cache.pages(seq)) == -(-len(tokens) // cache.page_size)
         for p in cache.pages(seq):
             users[p] += 1
+    assert cache._spared == sum(u - 1 for u in users if u)
     assert cache._users == users and sorted(cache._free) == [p for p in range(cache.num_pages) if not users[p]]
     assert len(cache) == len(model) and cache.free_pages == users.count(0)
 
@@ -181,9 +182,14 @@ def test_pages_are_shared_until_written(monkeypatch):
     cache.fork("a", "b")
     cache.fork("a", "c")
     assert cache.pages("a") == cache.pages("b") == cache.pages("c") and cache.free_pages == 38
+    cache.add("alone", 160)
+    cache.extend(["alone"])
+    assert not cache.batch(["alone"]).shared
+    cache.free("alone")
     cache.extend(["a", "b", "c"])              # two of three are given copies of the last page, the last keeps it
     assert cache.free_pages == 36 and len({cache.pages(s)[1] for s in "abc"}) == 3 and len({cache.pages(s)[0] for s in "abc"}) == 1
     _store(cache, ["a", "b", "c"], [1.0, 2.0, 3.0])
+    assert cache.batch(["a"]).shared and not cache.batch(["a", "b", "c"]).shared      # (two spared of two seen, of six)
     for s, value in zip("abc", (1.0, 2.0, 3.0)):
         assert _seen(cache, s)[0].tolist() == [5.0] * 11 + [value]
     with pytest.raises(ValueError, match="other sequences"):
@@ -233,7 +239,7 @@ def test_calls_that_do_not_fit_change_nothing(monkeypatch):
     assert b.positions.tolist() == [8, 0, 7] and b.lengths.tolist() == [9, 0, 8] and b.slots[1] == -1
     assert b.block_tables.shape == (3, 5) and b.block_tables[0, :2].tolist() == list(cache.pages("a"))
     again = cache.batch([None, "b", "a"], out=b)
-    assert again is b and b.lengths.tolist() == [0, 8, 9]
+    assert all(x is y for x, y in zip(again[:4], b)) and b.lengths.tolist() == [0, 8, 9]
     for bad in (dict(page_size=12), dict(page_size=4), dict(pages=0), dict(dtype=torch.float32)):
         with pytest.raises(ValueError):
             _cache_on("cpu", **bad)
@@ -249,7 +255,7 @@ def test_c_entry_points_check_their_arguments(dzlib):
     from deltazip_amd import paged
     P = 0x1000
     names = ("bytes q k v tables lengths out work counters status work_bytes num_pages q_row q_head k_page k_head k_token v_page v_head v_token "
-             "out_row out_head table_row rows heads kv_heads dim page_size pages_per_row window dtype scale reserved").split()
+             "out_row out_head table_row rows heads kv_heads dim page_size pages_per_row window dtype scale shared").split()
     ok = dict(zip(names, [paged._ATTENTION.size] + [P] * 9 + [1 << 30, 10] + [4096, 128, 65536, 2048, 128, 65536, 2048, 128, 4096, 128, 4]
                   + [2, 32, 32, 128, 16, 40, 0, 0, 0.1, 0]))
     attend = lambda **kw: dzlib.dz_paged_attention(paged._ATTENTION.pack(*{**ok, **kw}.values()), None)
@@ -445,6 +451,9 @@ def test_attention_of_many_rows(dev, dtype):
     q = torch.randn(90, 2, 64, device=dev).to(dtype)
     shared = q, k, v, tables.expand(90, -1), torch.arange(1, 91, dtype=torch.int32, device=dev)
     _hold(paged_attention(*shared), *shared, 0.125)
+    assert torch.equal(paged_attention(*shared, shared=True), paged_attention(*shared))
+    p = _problem(dev, dtype, [900] * 24, 16, 8, 128, 16, 13)                 # (past the caches, unless it is said to be shared)
+    assert torch.equal(paged_attention(*p, shared=True), paged_attention(*p))
 
 
 @pytest.mark.gpu
