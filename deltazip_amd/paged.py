@@ -54,8 +54,8 @@ class RotaryPositions:
             raise ValueError(f"head_dim must be even, up to {MAX_DIM}")
         if r < 2 or r > head_dim or r % 2:
             raise ValueError("rotary_dim must be even and at most head_dim")
-        if not base > 0 or max_position < 1:
-            raise ValueError("base and max_position must be positive")
+        if not base > 1 or max_position < 1:
+            raise ValueError("base must be above 1 and max_position positive")
         self.head_dim, self.rotary_dim, self.interleaved = head_dim, r, bool(interleaved)
         self.attention_factor = 1.0
         scaling = dict(scaling or {})
@@ -88,8 +88,18 @@ class RotaryPositions:
             raise ValueError(f"entries of the scaling that {kind!r} has no use for: {sorted(scaling)}")
         self.frequencies = torch.from_numpy(freq)                         # radians per position, float64
         self._turns = freq / (2 * math.pi)
+        self._pack()
+
+    def _pack(self) -> None:
         # what the host's half of a call takes: address of the turns, pairs' values, layout, factor, head size
-        self._packed = (self._turns.ctypes.data, r, int(self.interleaved), self.attention_factor, head_dim)
+        self._packed = (self._turns.ctypes.data, self.rotary_dim, int(self.interleaved), self.attention_factor, self.head_dim)
+
+    def __getstate__(self):
+        return {k: v for k, v in self.__dict__.items() if k != "_packed"}
+
+    def __setstate__(self, state) -> None:
+        self.__dict__.update(state)
+        self._pack()                                                      # (a copy's turns lie elsewhere)
 
 
 def _stride(t: torch.Tensor, d: int) -> int:
@@ -125,7 +135,6 @@ def _writable(name: str, t: torch.Tensor) -> None:
         if stride < upto:
             raise ValueError(f"elements of {name} overlap")
         upto = stride * size
-    return
 
 
 def _extent(t: torch.Tensor) -> Tuple[int, int]:

@@ -75,6 +75,21 @@ def test_frequencies_of_the_scalings():
         RotaryPositions(64, scaling={"type": "other", "factor": 2.0})
 
 
+@pytest.mark.parametrize("how", ["copy", "deepcopy", "pickle"])
+def test_positions_that_were_copied_are_their_own(how):
+    """What a call is handed points into the copy, not into what it was copied from."""
+    import copy
+    import pickle
+    from deltazip_amd import RotaryPositions
+    first = RotaryPositions(64, rotary_dim=20, interleaved=True, scaling={"type": "yarn", "factor": 4.0})
+    made = {"copy": copy.copy, "deepcopy": copy.deepcopy, "pickle": lambda x: pickle.loads(pickle.dumps(x))}[how](first)
+    assert made._packed[0] == made._turns.ctypes.data and made._packed[1:] == first._packed[1:]
+    got = np.ctypeslib.as_array(C.cast(made._packed[0], C.POINTER(C.c_double)), (10,))
+    assert np.array_equal(got, first.frequencies.numpy() / (2 * math.pi)) and torch.equal(made.frequencies, first.frequencies)
+    if how != "copy":
+        assert made._packed[0] != first._packed[0]
+
+
 # ---------------------------------------------------------------------------------------------
 # the host's bookkeeping
 # ---------------------------------------------------------------------------------------------
