@@ -187,6 +187,10 @@ __device__ __forceinline__ Part find_part(const AttnParams& P, int part, int ite
   return found;
 }
 
+// What the sums of a piece of a row with the maximum `top` count for in sums with the maximum `up`.  A piece without a maximum
+// has sums of zero, or of NaN (a score that is NaN raises no maximum), and these have to stay.
+__device__ __forceinline__ float weight_of(float top, float up) { return top == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - up); }
+
 // Keys and values of a call pass through once: loads that keep nothing in the caches read 7.1 TB/s where others read 6.2.  Not so
 // where rows share pages: 16 rows of one sequence's 4096 tokens of 32 key heads 119 -> 82 us with the others.
 template <bool ONCE>
@@ -430,9 +434,9 @@ __global__ __launch_bounds__(64 * WAVES, KC == 8 && !FULL ? 1 : 2) void dz_atten
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) {
       const float lw = stat[(w * HEADS + h) * 2 + 1], mw = stat[(w * HEADS + h) * 2];
-      const float f = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw - m);
-      l += mw == -INFINITY ? 0.0f : lw * f;
-      o += mw == -INFINITY ? f4_t{0, 0, 0, 0} : *(const f4_t*)(lds + (w * nheads + h) * ld + d) * f;
+      const float f = weight_of(mw, m);
+      l += lw * f;
+      o += *(const f4_t*)(lds + (w * nheads + h) * ld + d) * f;
     }
     if (nparts > 1)
       leave(blockIdx.x, h, d, o, m, l);
@@ -481,12 +485,12 @@ __global__ __launch_bounds__(64 * WAVES, KC == 8 && !FULL ? 1 : 2) void dz_atten
             if (s + i * slices >= n) ml[i][0] = -INFINITY;
             up = fmaxf(up, ml[i][0]);
           }
-          const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - up);
+          const float f = weight_of(m, up);
           l *= f, o *= f, m = up;
 #pragma unroll
           for (int i = 0; i < N; ++i) {
-            const bool none = ml[i][0] == -INFINITY;
-            const float fs = none ? 0.0f : __builtin_amdgcn_exp2f(ml[i][0] - up);
+            const bool none = s + i * slices >= n;       // (the last part a second time)
+            const float fs = weight_of(ml[i][0], up);
             l += none ? 0.0f : ml[i][1] * fs;
             o += none ? f4_t{0, 0, 0, 0} : w[i] * fs;
           }
@@ -511,8 +515,7 @@ __global__ __launch_bounds__(64 * WAVES, KC == 8 && !FULL ? 1 : 2) void dz_atten
       for (int c = 0; c < slices; ++c) m = fmaxf(m, lds[8 * (c * spots + spot) + 4]);
       for (int c = 0; c < slices; ++c) {
         const float* at = lds + 8 * (c * spots + spot);
-        if (at[4] == -INFINITY) continue;
-        const float f = __builtin_amdgcn_exp2f(at[4] - m);
+        const float f = weight_of(at[4], m);
         l += at[5] * f;
         o += *(const f4_t*)at * f;
       }

@@ -517,6 +517,25 @@ def test_attention_of_values_that_are_not_finite(dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv,dim", [(4, 2, 64), (2, 2, 8), (6, 3, 256), (20, 2, 128)])
+@pytest.mark.parametrize("n,first,last", [(7, 0, 7), (33, 32, 33), (65, 64, 65), (97, 96, 97), (100, 32, 64), (128, 96, 128), (2048, 512, 640),
+                                          (2048, 1920, 2048), (5000, 4999, 5000), (20480, 4096, 6144), (40000, 39999, 40000)])
+def test_attention_keeps_nan_of_pieces_without_a_maximum(dev, dtype, heads, kv, dim, n, first, last):
+    """Keys that are NaN in all that a wavefront, or a part of a split row, sees: the newest token alone in its tile, whole tiles,
+    whole parts (of 4 tiles), all 16 parts that are joined first.  Their heads are NaN; the other heads and rows have the bits that they had."""
+    from deltazip_amd import paged_attention
+    q, k, v, tables, ln = p = _problem(dev, dtype, [40, n, 300], heads, kv, dim, 16, 90)
+    clean = paged_attention(*p)
+    t = torch.arange(first, last, device=dev)
+    k[tables[1].long()[t // 16], 0, t % 16] = float("nan")
+    got = paged_attention(*p)
+    share = heads // kv
+    assert torch.isnan(got[1, :share]).all()
+    assert torch.equal(got[1, share:], clean[1, share:]) and torch.equal(got[[0, 2]], clean[[0, 2]])
+
+
+@pytest.mark.gpu
 def test_attention_strides_and_orders(dev):
     """Queries as slices of a wider projection, pages with tokens in front of heads, keys and values in one tensor, out in
     a wider one: the same bits as the plain layouts."""
