@@ -49,12 +49,14 @@ struct Place {
             status(dev >= 0 && dev < 64 ? status_at[dev] : nullptr) {}
 };
 
-// Counters, all zero between calls, and room for the sums of parts, of a stream: calls on it follow each other.  (Never freed: it
-// may outlive the runtime's own end.)
+// Counters, all zero between calls, and room for the sums of parts, of a stream: calls on it follow each other.  A call holds
+// what it is given until it has launched: meanwhile a call of another thread may put larger room in its place, and room that
+// nothing holds is given to that thread's next tensor, whose kernels may be ahead of the first call's.  (The map is never freed: it may
+// outlive the runtime's own end.)
 struct Space {
   at::Tensor counters, work;
 };
-Space& space_of(const Place& p, size_t need, const at::Tensor& like) {
+Space space_of(const Place& p, size_t need, const at::Tensor& like) {
   static auto* spaces = new std::map<std::pair<int, void*>, Space>;
   Space& s = (*spaces)[{p.dev, p.stream}];
   if (!s.counters.defined()) s.counters = at::zeros({DZ_ATTENTION_COUNTERS}, like.options().dtype(at::kInt));
@@ -94,11 +96,10 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!index_on(*lengths, rows, at::kInt, dev)) Py_RETURN_NONE;
   const int width = (int)tables->size(1);
   const size_t need = dz_paged_attention_bytes((int)rows, (int)heads, (int)kv_heads, (int)dim, (int)ps, width);
-  void *work = nullptr, *counters = nullptr;
+  Space space;
   if (need) {
     if (dz_capture_id(here.stream)) Py_RETURN_NONE;    // (a graph has its own)
-    Space& space = space_of(here, need, *q);
-    work = space.work.data_ptr(), counters = space.counters.data_ptr();
+    space = space_of(here, need, *q);
   }
   at::Tensor out = at::empty({rows, heads, dim}, q->options());
   dz_attention_args c{};
@@ -106,7 +107,8 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   c.q = q->data_ptr(), c.k_pages = k->data_ptr(), c.v_pages = v->data_ptr();
   c.tables = (const int32_t*)tables->data_ptr(), c.lengths = (const int32_t*)lengths->data_ptr();
   c.out = out.data_ptr();
-  c.work = work, c.counters = (uint32_t*)counters, c.status = here.status;
+  if (need) c.work = space.work.data_ptr(), c.counters = (uint32_t*)space.counters.data_ptr();
+  c.status = here.status;
   c.work_bytes = (int64_t)need, c.num_pages = k->size(0);
   c.q_row = step(*q, 0), c.q_head = step(*q, 1);
   c.k_page = step(*k, 0), c.k_head = step(*k, 1), c.k_token = k->stride(2);

@@ -4,6 +4,7 @@ import ctypes as C
 import math
 import random
 import struct
+import threading
 
 import numpy as np
 import pytest
@@ -868,6 +869,47 @@ def test_calls_on_two_streams_do_not_meet(dev):
         torch.cuda.synchronize()
         for a, b in zip(got, want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_room_for_parts_outlives_a_larger_call_of_another_thread(dev):
+    """Two host threads on one stream: while a call of many launches is under way, another thread's call puts larger room in the
+    place of its own, and tensors made then may lie where the first call's parts are."""
+    from deltazip_amd import paged_attention
+    rows, n = 1 << 17, 1000
+    q = torch.randn(256, 1, 8, dtype=torch.float16, device=dev).repeat(rows // 256, 1, 1)
+    k, v = (torch.randn(256, 1, 1024, 8, dtype=torch.float16, device=dev) for _ in range(2))
+    tables = torch.arange(256, dtype=torch.int32, device=dev).repeat(rows // 256)[:, None].contiguous()
+    ln = torch.full((rows,), n, dtype=torch.int32, device=dev)
+    want = paged_attention(q[:256].contiguous(), k, v, tables[:256], ln[:256])
+    wide = torch.zeros(256, 512, 256, dtype=torch.float16, device=dev)
+    pages = torch.zeros(1, 32, 1024, 256, dtype=torch.float16, device=dev)
+    none = torch.zeros(256, dtype=torch.int32, device=dev)
+    torch.cuda.synchronize()
+    for _ in range(4):
+        stream, under_way, got, after = torch.cuda.Stream(), threading.Event(), [], []
+
+        def many():
+            with torch.cuda.stream(stream):
+                paged_attention(q[:512], k, v, tables[:512], ln[:512])     # (the stream has room for this size)
+                under_way.set()
+                got.append(paged_attention(q, k, v, tables, ln))
+
+        def larger():
+            with torch.cuda.stream(stream):
+                under_way.wait()
+                after.append(paged_attention(wide, pages, pages, none[:, None], none))
+                for _ in range(8):
+                    after.append(torch.full((1 << 20,), 7, dtype=torch.uint8, device=dev))
+
+        threads = [threading.Thread(target=f) for f in (many, larger)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        torch.cuda.synchronize()
+        assert torch.equal(got[0].view(-1, 256, 1, 8), want.expand(rows // 256, -1, -1, -1)) and (after[0] == 0).all()
+        assert all((t == 7).all() for t in after[1:])
 
 
 @pytest.mark.gpu
