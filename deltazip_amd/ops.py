@@ -883,22 +883,25 @@ _warned_bad_id = False
 
 def raise_for_status(word: int, where: str = "multi-delta linear") -> None:
     """What a status word means to the caller.  Bits 1 and 2 -> DeltaKernelError (a RuntimeError, as every
-    failure of the reference's ops is a Python exception); bit 0 -> one warning per process."""
+    failure of the reference's ops is a Python exception) that names every bit; bit 0 alone -> one warning per process."""
     global _warned_bad_id
+    wrong = []
     if word & STATUS_SUM_MISSING:
-        raise DeltaKernelError(
+        wrong.append(
             f"{where}: a partial sum of a K dimension split over workgroups did not arrive within the kernel's "
             "bounded wait; the outputs of the calls since the last check are invalid (status bit 1). The "
             "workspace has been cleared; repeat the step.")
     if word & STATUS_BAD_PAGE:
-        raise DeltaKernelError(
+        wrong.append(
             "paged cache: a page number or slot outside the pool, or a length beyond its table, was met; the outputs of "
             "the calls since the last check are invalid (status bit 2).")
+    bad_id = f"{where}: a delta id outside [-1, S) was met and served as -1 (base weight only; status bit 0)"
+    if wrong:                                         # all that there is to say: the words have been cleared
+        raise DeltaKernelError("\n".join(wrong + [bad_id] if word & STATUS_BAD_ID else wrong))
     if word & STATUS_BAD_ID and not _warned_bad_id:
         _warned_bad_id = True
         import warnings
-        warnings.warn(f"{where}: a delta id outside [-1, S) was met and served as -1 (base weight only; status bit 0)",
-                      RuntimeWarning, stacklevel=3)
+        warnings.warn(bad_id, RuntimeWarning, stacklevel=3)
 
 
 # (device, stream) -> (pinned int32[1], event of the copy that fills it)

@@ -27,6 +27,17 @@ def test_status_word_meaning():
     ops._warned_bad_id = False
 
 
+@pytest.mark.parametrize("bits", range(2, 8))
+def test_an_error_names_every_bit_of_the_word(bits):
+    """The words are cleared as they are looked at: what an error leaves out is never said."""
+    before = ops._warned_bad_id
+    with pytest.raises(ops.DeltaKernelError) as e:
+        ops.raise_for_status(bits)
+    for bit, text in ((ops.STATUS_BAD_ID, "delta id outside"), (ops.STATUS_SUM_MISSING, "did not arrive"), (ops.STATUS_BAD_PAGE, "paged cache")):
+        assert (text in str(e.value)) == bool(bits & bit)
+    assert ops._warned_bad_id == before
+
+
 @pytest.mark.gpu
 def test_poll_status_raises_and_clears(dev):
     ops._warned_bad_id = False
