@@ -58,11 +58,18 @@ class RotaryPositions:
             raise ValueError("base must be above 1 and max_position positive")
         self.head_dim, self.rotary_dim, self.interleaved = head_dim, r, bool(interleaved)
         self.attention_factor = 1.0
-        scaling = dict(scaling or {})
-        kind, s = scaling.pop("type", scaling.pop("rope_type", None)), float(scaling.pop("factor", 1.0))
+        kind, s = None, 1.0
+        if scaling:
+            scaling = dict(scaling)
+            kind, s = scaling.pop("type", scaling.pop("rope_type", None)), scaling.pop("factor", None)
+            if kind is None:
+                raise ValueError("a scaling must name its type")
+            if kind not in ("linear", "dynamic", "yarn"):
+                raise NotImplementedError(f"positions scaled by {kind!r}: linear, dynamic and yarn are known")
+            if s is None or not 1.0 <= float(s) < math.inf:
+                raise ValueError("a scaling must have a factor of at least 1")
+            s = float(s)
         i = np.arange(r // 2, dtype=np.float64)
-        if kind is not None and not s >= 1.0:
-            raise ValueError("the factor of a scaling must be at least 1")
         if kind == "dynamic":
             if r == 2:
                 raise ValueError("dynamic scaling needs more than one pair")
@@ -82,8 +89,6 @@ class RotaryPositions:
             keep = (1.0 - ramp) * kept
             freq = freq / s * (1.0 - keep) + freq * keep
             self.attention_factor = float(scaling.pop("attn_factor", 1.0)) * (0.1 * math.log(s) + 1.0)
-        elif kind not in (None, "linear", "dynamic"):
-            raise NotImplementedError(f"positions scaled by {kind!r}: linear, dynamic and yarn are known")
         if scaling:
             raise ValueError(f"entries of the scaling that {kind!r} has no use for: {sorted(scaling)}")
         self.frequencies = torch.from_numpy(freq)                         # radians per position, float64

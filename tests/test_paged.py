@@ -76,6 +76,17 @@ def test_frequencies_of_the_scalings():
         RotaryPositions(64, scaling={"type": "other", "factor": 2.0})
 
 
+@pytest.mark.parametrize("scaling", [{"factor": 4.0}, {"type": None, "factor": 4.0}, {"type": "linear"}, {"type": "dynamic"}, {"rope_type": "yarn"},
+                                     {"original_max_position_embeddings": 4096}, {"type": "linear", "factor": math.inf},
+                                     {"type": "yarn", "factor": math.nan}, {"type": "linear", "factor": None}])
+def test_scalings_that_say_too_little_are_refused(scaling):
+    """An entry without a type or a factor would leave positions as they are, and no one would know."""
+    from deltazip_amd import RotaryPositions
+    with pytest.raises(ValueError, match="scaling must"):
+        RotaryPositions(64, scaling=scaling)
+    assert torch.equal(RotaryPositions(64, scaling={}).frequencies, RotaryPositions(64).frequencies)
+
+
 @pytest.mark.parametrize("how", ["copy", "deepcopy", "pickle"])
 def test_positions_that_were_copied_are_their_own(how):
     """What a call is handed points into the copy, not into what it was copied from."""
