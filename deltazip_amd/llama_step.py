@@ -185,7 +185,15 @@ class LlamaForDecodeStep(nn.Module):
         hd = cfg.hidden_size // cfg.num_attention_heads
         inv = 1.0 / (cfg.rope_theta ** (torch.arange(0, hd, 2, device=device).float() / hd))
         self.register_buffer("inv_freq", inv, persistent=False)
-        self.rope = RotaryPositions(hd, base=cfg.rope_theta, max_position=cfg.max_position_embeddings)
+        self._rope: Optional[RotaryPositions] = None
+
+    @property
+    def rope(self) -> RotaryPositions:
+        """The positions of `paged_step`, made when it first asks: `decode_step` takes sizes that they do not."""
+        if self._rope is None:
+            cfg = self.config
+            self._rope = RotaryPositions(cfg.hidden_size // cfg.num_attention_heads, base=cfg.rope_theta, max_position=cfg.max_position_embeddings)
+        return self._rope
 
     def projections(self) -> List[Tuple[str, nn.Module]]:
         """(name, module) of every projection, in execution order."""

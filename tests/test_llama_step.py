@@ -158,3 +158,28 @@ def test_decode_step_matches_the_oracle_layer_by_layer(dev, B):
     base_h, _ = ref.decoder_layer(hid, res, w, none, np.full(B, -1), kv_before[0][0], kv_before[0][1], CTX, HEADS,
                                   cfg.rms_norm_eps, cfg.rope_theta)
     assert not _close(out_h.float().numpy(), base_h.float().numpy())
+
+
+@pytest.mark.parametrize("hidden,heads,theta", [(1024, 2, 10000.0), (64, 4, 1.0)])
+def test_models_that_the_paged_cache_does_not_take_step_over_the_padded_one(hidden, heads, theta):
+    """Heads of 512, positions of base 1: the padded cache's step works in plain operators and asks nothing of the paged one's."""
+    from deltazip_amd.llama_step import LlamaForDecodeStep, LlamaStepConfig
+    cfg = LlamaStepConfig(hidden_size=hidden, intermediate_size=64, num_attention_heads=heads, num_hidden_layers=1, vocab_size=32, rope_theta=theta)
+    model = LlamaForDecodeStep(cfg, generator=torch.Generator().manual_seed(3))
+
+    class WithBias(torch.nn.Module):                      # what a delta layer returns
+        def __init__(self, linear):
+            super().__init__()
+            self.linear = linear
+
+        def forward(self, x):
+            return self.linear(x), None
+
+    for layer in model.model.layers:
+        for block, names in ((layer.self_attn, ("qkv_proj", "o_proj")), (layer.mlp, ("gate_up_proj", "down_proj"))):
+            for name in names:
+                setattr(block, name, WithBias(getattr(block, name)))
+    got = model.decode_step(torch.tensor([1, 2, 3]), model.make_kv_cache(3, 5, "cpu"), 5)
+    assert got.shape == (3, 32) and torch.isfinite(got).all()
+    with pytest.raises(ValueError):
+        model.rope
