@@ -39,6 +39,26 @@ bool index_on(const at::Tensor& t, int64_t n, at::ScalarType type, int dev) {
 }
 bool floats(at::ScalarType t) { return t == at::kHalf || t == at::kBFloat16; }
 
+// Whether [n, heads, dim] tensors of one type share nothing: by their ends, or, with rows of one stride (slices of a
+// projection), by those of a row.
+int64_t reach(const at::Tensor& t, int from) {
+  int64_t n = 1;
+  for (int d = from; d < t.dim(); ++d) n += (t.size(d) - 1) * t.stride(d);
+  return n;
+}
+bool ends_apart(const at::Tensor& a, const at::Tensor& b) {
+  const int64_t at = ((const char*)b.data_ptr() - (const char*)a.data_ptr()) / (int64_t)a.element_size();
+  return at >= reach(a, 0) || -at >= reach(b, 0);
+}
+bool rows_apart(const at::Tensor& a, const at::Tensor& b) {
+  if (ends_apart(a, b)) return true;
+  const int64_t row = a.stride(0);
+  if (a.size(0) < 2 || b.stride(0) != row || row < 1) return false;
+  int64_t at = ((const char*)b.data_ptr() - (const char*)a.data_ptr()) / (int64_t)a.element_size() % row;
+  if (at < 0) at += row;
+  return at >= reach(a, 1) && at + reach(b, 1) <= row;
+}
+
 // Where a call goes: the current device and stream, and the device's status word once Python has taken note of it.
 uint32_t* status_at[64];
 struct Place {
@@ -162,8 +182,10 @@ PyObject* rotate(PyObject*, PyObject* const* a, Py_ssize_t n) {
     v = tensor(a[2]), slots = tensor(a[4]), kp = tensor(a[6]), vp = tensor(a[7]);
     if (!v || !slots || !kp || !vp || !heads_on(*v, type, dev) || v->sizes() != k->sizes() || !index_on(*slots, tokens, at::kLong, dev) ||
         !pages_on(*kp, *q, dev) || !pages_on(*vp, *q, dev) || kp->sizes() != vp->sizes() || kp->size(1) != k->size(1) ||
-        kp->data_ptr() == vp->data_ptr() || !kp->is_contiguous() || !vp->is_contiguous())
+        !kp->is_contiguous() || !vp->is_contiguous())
       Py_RETURN_NONE;
+    if (!ends_apart(*kp, *vp) || !ends_apart(*kp, *k) || !ends_apart(*kp, *v) || !ends_apart(*vp, *k) || !ends_apart(*vp, *v)) Py_RETURN_NONE;
+    if (c.rot && (!ends_apart(*kp, *q) || !ends_apart(*vp, *q))) Py_RETURN_NONE;
     c.v = v->data_ptr(), c.v_row = step(*v, 0), c.v_head = step(*v, 1);
     c.slots = (const int64_t*)slots->data_ptr(), c.status = here.status;
     c.num_pages = kp->size(0), c.page_size = (int)kp->size(2);
@@ -175,6 +197,7 @@ PyObject* rotate(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (in_place) {
     c.q_out = q->data_ptr(), c.q_out_row = step(*q, 0), c.q_out_head = step(*q, 1);
     if ((tokens > 1 && q->stride(0) < q->size(1) * q->stride(1)) || (q->size(1) > 1 && q->stride(1) < dim)) Py_RETURN_NONE;
+    if (c.rot && (!rows_apart(*q, *k) || !rows_apart(*q, *v))) Py_RETURN_NONE;
   } else {
     q_out = at::empty(q->sizes(), q->options());
     c.q_out = q_out.data_ptr(), c.q_out_row = q->size(1) * dim, c.q_out_head = dim;

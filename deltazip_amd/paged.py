@@ -142,19 +142,43 @@ def _writable(name: str, t: torch.Tensor) -> None:
         upto = stride * size
 
 
-def _extent(t: torch.Tensor) -> Tuple[int, int]:
-    upto = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1 if t.numel() else 0
-    return t.data_ptr(), t.data_ptr() + upto * t.element_size()
+def _meet(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether an element of one may lie where one of the other does: exact where the larger strides step over what the
+    smaller ones reach (slices of one projection, pools in one tensor), and else wherever the two's memory overlaps."""
+    if not a.numel() or not b.numel():
+        return False
+    size, at = a.element_size(), b.data_ptr() - a.data_ptr()
+    reach = [sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1 for t in (a, b)]
+    if at >= reach[0] * size or -at >= reach[1] * b.element_size():
+        return False
+    if b.element_size() != size or at % size:
+        return True
+    steps: Dict[int, list] = {}                       # stride -> steps of a and of b
+    for which, t in enumerate((a, b)):
+        for n, s in zip(t.shape, t.stride()):
+            if n > 1 and s:
+                both = steps.setdefault(s, [0, 0])
+                if both[which]:
+                    return True
+                both[which] = n - 1
+    apart = {at // size}                              # from a row of a to one of b, by the strides so far; none: they do not meet
+    for s in sorted(steps, reverse=True):
+        na, nb = steps[s]
+        reach = [reach[0] - na * s, reach[1] - nb * s]
+        if s < max(reach):
+            return True
+        apart = {d - k * s for d in apart for k in (d // s, d // s + 1) if -nb <= k <= na}
+        apart = {d for d in apart if -reach[1] < d < reach[0]}
+        if not apart:
+            return False
+    return 0 in apart
 
 
 def _apart(name: str, out: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
-    """An output given by the caller lies apart from what is read."""
-    lo, hi = _extent(out)
+    """What is written lies apart from what is read, and from what else is written."""
     for t in others:
-        if t is not None:
-            a, b = _extent(t)
-            if lo < b and a < hi:
-                raise ValueError(f"{name} must be memory of its own")
+        if t is not None and _meet(out, t):
+            raise ValueError(f"{name} must be memory of its own")
 
 
 def _itself(out: torch.Tensor, t: torch.Tensor) -> bool:
@@ -288,7 +312,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         if out.shape != q.shape:
             raise ValueError("out must have q's shape")
         _writable("out", out)
-        _apart("out", out, q, k_pages, v_pages)
+        _apart("out", out, q, k_pages, v_pages, block_tables, lengths)
     if rows == 0:
         return out
     need = _attention_bytes(rows, heads, kv_heads, dim, page_size, width)
@@ -355,8 +379,7 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
                 if o.shape != t.shape:
                     raise ValueError(f"out[{n}] must have its input's shape")
                 _writable(f"out[{n}]", o)
-                if not _itself(o, t):
-                    _apart(f"out[{n}]", o, q, k, out[1 - n])
+                _apart(f"out[{n}]", o, None if _itself(o, t) else t, (k, q)[n], out[1 - n], positions)
         out = out[0], out[1]
     if q.shape[0] and (q.shape[1] or k is not None):
         _rotate(q, k, None, positions, None, rope, out[0], out[1], None, 8, 0)
@@ -371,8 +394,8 @@ def append_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torc
     (serving/csrc/cache_kernels), and q [tokens, heads, dim], turned, is returned (or written to `out`, which
     may be q itself).  positions and slots int64 [tokens]; a negative slot stores nothing (a padded row: its q is turned all the
     same); one beyond the pages neither, and is reported through the status word.  rope None: nothing is turned, and q is
-    returned as it is.  No two tokens may have one slot: what is there afterwards may be parts of either.  Strides as
-    for `rotary`."""
+    returned as it is.  No two tokens may have one slot: what is there afterwards may be parts of either.  q, k and v lie
+    outside the pages, and a q that is written lies apart from k and v.  Strides as for `rotary`."""
     if out is None or out is q:
         made = _lib.host().rotate(q, k, v, positions, slots, None if rope is None else rope._packed, k_pages, v_pages, out is q or rope is None)
         if made is not None:
@@ -393,10 +416,13 @@ def append_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torc
     _pages("v_pages", v_pages, q)
     if k_pages.shape != v_pages.shape or k_pages.shape[1] != k.shape[1]:
         raise ValueError("k_pages and v_pages must have one shape, with k's heads")
-    if k_pages.data_ptr() == v_pages.data_ptr():
+    if _meet(k_pages, v_pages):
         raise ValueError("keys and values need pages of their own")
     _writable("k_pages", k_pages)
     _writable("v_pages", v_pages)
+    turned = rope is not None or (out is not None and out is not q)          # whether q is read
+    for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
+        _apart(name, t, q if turned else None, k, v)
     _index("positions", positions, q.shape[0], torch.int64)
     _index("slots", slots, q.shape[0], torch.int64)
     if out is not None:
@@ -404,8 +430,8 @@ def append_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torc
         if out.shape != q.shape:
             raise ValueError("out must have q's shape")
         _writable("out", out)
-        if not _itself(out, q):
-            _apart("out", out, q, k, v, k_pages, v_pages)
+        if turned:
+            _apart("out", out, None if _itself(out, q) else q, k, v, k_pages, v_pages, positions, slots)
     elif rope is None:
         out = q
     else:

@@ -336,6 +336,37 @@ def test_host_tensors_are_refused(dzlib):
             call()
 
 
+@pytest.mark.parametrize("seed", range(8))
+def test_tensors_that_share_elements_are_told_from_those_that_do_not(seed):
+    """Against the elements themselves: no two that share one are taken for apart, and where strides step over what is inside them, none
+    that are apart are taken for sharing."""
+    from deltazip_amd.paged import _meet
+    rng, store = random.Random(seed), torch.arange(4000, dtype=torch.int16)
+    met = apart = 0
+    for _ in range(600):
+        inner = rng.choice([1, 2, 3, 8])
+        head = inner * rng.randrange(1, 4)
+        heads = rng.randrange(1, 6)
+        row = head * heads * rng.randrange(1, 3) + rng.randrange(0, 9)
+        views = []
+        for _ in range(2):
+            n, h, d = rng.randrange(1, 6), rng.randrange(1, heads + 1), rng.randrange(1, inner + 1)
+            at = rng.randrange(0, 2 * row) + 500
+            shape, strides = (n, h, d), (row, head, 1)
+            order = rng.choice([(0, 1, 2), (1, 0, 2), (2, 0, 1)])
+            views.append(store.as_strided([shape[i] for i in order], [strides[i] for i in order], at))
+        a, b = views
+        share = bool(set(a.flatten().tolist()) & set(b.flatten().tolist()))
+        assert _meet(a, b) == _meet(b, a) == share
+        met, apart = met + share, apart + (not share)
+        # any strides at all: never taken for apart wrongly
+        c, d = (store.as_strided([rng.randrange(1, 5) for _ in range(3)], [rng.randrange(0, 30) for _ in range(3)], rng.randrange(0, 60)) for _ in range(2))
+        if set(c.flatten().tolist()) & set(d.flatten().tolist()):
+            assert _meet(c, d)
+    assert met > 50 and apart > 50
+    assert not _meet(store[:0], store) and not _meet(store[:10], store[10:]) and _meet(store[:10], store.view(torch.int32)[4:])
+
+
 def test_status_word_of_a_bad_page():
     from deltazip_amd import ops
     with pytest.raises(ops.DeltaKernelError, match="paged"):
@@ -380,6 +411,51 @@ def test_arguments_that_do_not_fit_are_refused(dev):
                          (h(2, 1, 64).expand(2, 6, 64), [(0, 1)])):
         with pytest.raises(ValueError):
             copy_pages(pools, pairs)
+
+
+@pytest.mark.gpu
+def test_outputs_that_share_memory_with_what_is_read_are_refused(dev):
+    """Kernels read and write side by side: a key that is turned in place must not be a query's memory, and the like."""
+    from deltazip_amd import RotaryPositions, append_kv, paged_attention, rotary
+    h = lambda *s: torch.randn(s, device=dev).half()
+    rope, pos, slots = RotaryPositions(16), torch.arange(3, device=dev), torch.tensor([0, 9, 17], device=dev)
+    x, wide = h(3, 4, 16), h(3, 8, 16)
+    for q, k, out in ((x, x, (x, x)), (x, x, (x, h(3, 4, 16))), (x, x, (h(3, 4, 16), x)), (x, x[:, 1:3], (x, x[:, 1:3])),
+                      (wide[:, :4], wide[:, 3:6], (wide[:, :4], wide[:, 3:6])), (x, h(3, 2, 16), (wide[:, :4], wide[:, 3:5]))):
+        with pytest.raises(ValueError, match="own"):
+            rotary(q, k, pos, rope, out=out)
+    pool = h(2, 4, 2, 8, 16)
+    kp, vp = pool.unbind(0)
+    k, v = h(3, 2, 16), h(3, 2, 16)
+    for q, kk, vv, kpages, vpages, out in (
+            (x, x[:, :2], v, kp, vp, x), (x, k, x[:, 1:3], kp, vp, x), (wide[:, :4], wide[:, 3:5], v, kp, vp, wide[:, :4]),
+            (x, kp[:3, :, 2], v, kp, vp, None), (x, k, kp[:3, :, 2], kp, vp, None), (x, k, vp[1:4, :, 7], kp, vp, None),
+            (kp[:3, :, :2].reshape(3, 4, 16), k, v, pool.view(8, 2, 8, 16)[:4], pool.view(8, 2, 8, 16)[3:7], None),
+            (pool[0].view(-1, 4, 16)[:3], k, v, kp, vp, None), (x, k, v, kp, vp, pool[1].view(-1, 4, 16)[5:8])):
+        with pytest.raises(ValueError, match="own"):
+            append_kv(q, kk, vv, pos, slots, rope, kpages, vpages, out=out)
+    table = torch.zeros(2, 3, dtype=torch.int32, device=dev)
+    words = torch.zeros(2, 4, 8, dtype=torch.int32, device=dev)
+    for tables, ln in ((table, words.view(-1)[:2]), (words.view(2, 32)[:, :3], table[:, 0].contiguous())):
+        with pytest.raises(ValueError, match="own"):
+            paged_attention(h(2, 4, 16), kp, vp, tables, ln, out=words.view(torch.float16))
+    # slices of one projection, pages of one pool, an output between inputs: apart
+    want_q, want_k = rotary(wide[:, :4], wide[:, 4:6], pos, rope)
+    both = pool.clone().transpose(0, 1).contiguous()
+    for pages in ((pool[0], pool[1]), (both[:, 0], both[:, 1])):
+        for into in ("q", "apart", "late"):
+            w = torch.cat((wide, h(3, 4, 16)), 1)
+            q, kk, vv = w[:, :4], w[:, 4:6], w[:, 6:8]
+            out = {"q": q, "apart": w[:, 8:], "late": None}[into]
+            rest = w.clone()
+            got = append_kv(q, kk, vv, pos, slots, rope, *pages, out=out)
+            assert torch.equal(got, want_q) and torch.equal(w[:, 4:8], rest[:, 4:8])
+            for p, want in zip(pages, (want_k, wide[:, 6:8])):
+                assert torch.equal(p[slots // 8, :, slots % 8], want)
+    w = wide.clone()
+    rotary(w[:, :4], w[:, 4:6], pos, rope, out=(w[:, :4], w[:, 4:6]))
+    assert torch.equal(w[:, :4], want_q) and torch.equal(w[:, 4:6], want_k) and torch.equal(w[:, 6:], wide[:, 6:])
+    assert append_kv(x, k, x[:, :2], pos, slots, None, kp, vp) is x               # (a query that nothing turns is not touched)
 
 
 # ---------------------------------------------------------------------------------------------
