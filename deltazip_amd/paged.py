@@ -441,10 +441,26 @@ def append_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torc
     return out
 
 
+def _pools_meet(at: Sequence[int], pages: int, stride: int, size: int) -> bool:
+    """Whether pools that begin at these addresses share memory: they follow each other, or those that do not take turns within
+    a page's stride."""
+    at = sorted(at)
+    run = at[:1]
+    for a, b in zip(at, at[1:] + [at[-1] + pages * stride]):
+        if b - a < (pages - 1) * stride + size:
+            run.append(b)
+            continue
+        places = sorted((x - run[0]) % stride for x in run)
+        if any(y - x < size for x, y in zip(places, places[1:] + [stride])):
+            return True
+        run = [b]
+    return False
+
+
 def copy_pages(pools: Union[torch.Tensor, Sequence[torch.Tensor]], pairs) -> None:
     """Page `a` copied over page `b` for every (a, b) of `pairs`, in every pool: in place, in one launch for up to 320 pairs
     and 128 pools (serving/csrc/cache_kernels).  pools: one tensor [pools, pages, ...], or a sequence of
-    [pages, ...] of one shape, type and stride, pages contiguous and of a multiple of 16 bytes.  pairs: host integers [n, 2],
+    [pages, ...] of one shape, type and stride that share no memory, pages contiguous and of a multiple of 16 bytes.  pairs: host integers [n, 2],
     a tensor or a sequence; they are read before the call returns (a graph that captures the call copies the same
     pages at every replay).  All copies run side by side: no page may be written twice, or be both read and written."""
     if isinstance(pairs, list):
@@ -496,7 +512,7 @@ def copy_pages(pools: Union[torch.Tensor, Sequence[torch.Tensor]], pairs) -> Non
     if len(written) < len(pairs) or not written.isdisjoint(pairs[:, 0].tolist()):
         raise ValueError("a page is written twice, or both read and written")
     at = [first.data_ptr() + i * step for i in range(n)] if stacked else [t.data_ptr() for t in pools]
-    if len(set(at)) < n:
-        raise ValueError("a pool is named twice")
+    if _pools_meet(at, pages, stride, size):
+        raise ValueError("pools share memory")
     _lib.check(_lib.lib().dz_copy_pages((C.c_void_p * n)(*at), n, stride, size, pages, pairs.ctypes.data, len(pairs), ops._stream()),
                "dz_copy_pages")

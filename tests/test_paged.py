@@ -367,6 +367,24 @@ def test_tensors_that_share_elements_are_told_from_those_that_do_not(seed):
     assert not _meet(store[:0], store) and not _meet(store[:10], store[10:]) and _meet(store[:10], store.view(torch.int32)[4:])
 
 
+def test_pools_that_share_memory_are_told_from_those_that_do_not():
+    from deltazip_amd.paged import _pools_meet
+    rng = random.Random(5)
+    for _ in range(3000):
+        pages, size = rng.randrange(1, 6), rng.randrange(1, 5)
+        stride = size + rng.choice([0, 0, 3, 2 * size, 3 * size])
+        at = [rng.randrange(0, 60) for _ in range(rng.randrange(1, 4))]
+        cells = [{a + p * stride + i for p in range(pages) for i in range(size)} for a in at]
+        share = len(set().union(*cells)) < sum(len(c) for c in cells)
+        if share:
+            assert _pools_meet(at, pages, stride, size)
+        elif len(at) == 1 or pages == 1 or all(abs(a - b) >= pages * stride for i, a in enumerate(at) for b in at[:i]):
+            assert not _pools_meet(at, pages, stride, size)
+    # layers that take turns within a page, keys and values in tensors of their own at any distance
+    layers = [base + 16 * i for base in (1000, 1000 + 5 * 64 + 16) for i in range(4)]
+    assert not _pools_meet(layers, 5, 64, 16) and _pools_meet(layers + [1008], 5, 64, 16) and _pools_meet(layers + [1064], 5, 64, 16)
+
+
 def test_status_word_of_a_bad_page():
     from deltazip_amd import ops
     with pytest.raises(ops.DeltaKernelError, match="paged"):
@@ -832,6 +850,23 @@ def test_copy_pages(dev, pools, pages, shape, pairs):
     copy_pages(got, [])
     copy_pages([], order)
     assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+def test_pools_that_share_memory_are_refused(dev):
+    """Every pool's copies run beside the others': a page of one that lies in another's would be read as it is written."""
+    from deltazip_amd import copy_pages
+    flat = torch.randn(12, 64, device=dev).half()
+    for pools in ([flat[:6], flat[1:7]], [flat[:6], flat[:6]], [flat[6:], flat[:8][2:]], flat.as_strided((2, 6, 64), (64, 64, 1))):
+        with pytest.raises(ValueError, match="share memory"):
+            copy_pages(pools, [(0, 1)])
+    # keys and values of layers that take turns within a page
+    keys, values = (torch.randn(6, 4, 64, device=dev).half() for _ in range(2))
+    want = [t.clone() for t in (keys, values)]
+    for w in want:
+        w[[1, 3]] = w[[0, 5]]
+    copy_pages(list(keys.unbind(1)) + list(values.unbind(1)), [(0, 1), (5, 3)])
+    assert torch.equal(keys, want[0]) and torch.equal(values, want[1])
 
 
 # ---------------------------------------------------------------------------------------------
