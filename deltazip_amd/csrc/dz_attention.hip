@@ -619,7 +619,7 @@ int dz_paged_attention(const dz_attention_args* a, void* stream) {
   P.heads = a->heads, P.kv_heads = a->kv_heads, P.share = a->heads / a->kv_heads;
   P.head_tiles = (P.share + HEADS - 1) / HEADS;
   P.dim = a->dim, P.shift = __builtin_ctz(a->page_size), P.pages_per_row = a->pages_per_row, P.window = a->window;
-  P.shared = a->shared != 0;
+  P.shared = a->shared && a->rows > 1;                             // (one row reads its pages once)
   const int most = P.share < HEADS ? P.share : HEADS, items = P.kv_heads * P.head_tiles;
   P.part_floats = most * (a->dim + 4);
   P.scale = a->scale * 1.44269504088896340736f;

@@ -28,7 +28,8 @@ class OutOfPages(RuntimeError):
 class PagedBatch(NamedTuple):
     """What a step of one new token per row needs of the cache, on the device: the newest token's position and slot
     (int64 [rows]), the tables (int32 [rows, pages]) and lengths (int32 [rows], the new token counted); and, on the host, whether
-    rows share most of their pages (for `paged_attention`)."""
+    most of its rows' pages are another of its rows', too (for `paged_attention`, which takes no notice of it for one row; of
+    one row: whether sharing spares the cache most of as many pages).  A captured step keeps what it was captured with."""
     positions: torch.Tensor
     slots: torch.Tensor
     block_tables: torch.Tensor
@@ -238,7 +239,8 @@ class PagedKVCache:
     def batch(self, seqs: Sequence[Optional[Hashable]], width: Optional[int] = None, out: Optional[PagedBatch] = None) -> PagedBatch:
         """The step's tensors for these sequences, one row each, whose newest token is the one `extend` made room for.  None
         is a padded row: it stores nothing and its attention is zero.  width: pages of a table's row (default: as many
-        as the longest needs).  out: a batch of as many rows to write over (a captured step reads it; width is its tables')."""
+        as the longest needs).  out: a batch of as many rows to write over (a captured step reads it; width is its tables');
+        what is returned has the tensors of `out` and `shared` of these rows."""
         rows = len(seqs)
         named = [x for x in seqs if x is not None]
         if len(set(named)) < len(named):
@@ -267,11 +269,18 @@ class PagedKVCache:
         place[:], lengths[:] = last, length
         slot[:] = np.where(real, page.astype(np.int64) * self.page_size + last % self.page_size, -1)
         columns = np.arange(min(width, self.max_pages))
-        tables[:, :len(columns)] = np.where(columns < -(-length // self.page_size)[:, None], self._rows[at, :len(columns)], 0)
+        inside = columns < -(-length // self.page_size)[:, None]
+        tables[:, :len(columns)] = np.where(inside, self._rows[at, :len(columns)], 0)
+        held = sum([len(s.pages) for s in found if s is not None])
+        shared = 2 * self._spared > held             # (no more than the whole cache's can be this batch's)
+        if shared and rows > 1:
+            distinct = np.zeros(self.num_pages, dtype=bool)
+            distinct[tables[:, :len(columns)][inside]] = True
+            shared = 2 * (held - int(distinct.sum())) > held
         dev = torch.from_numpy(host).to(self.pool.device)
         made = PagedBatch(dev[:8 * rows].view(torch.int64), dev[8 * rows:16 * rows].view(torch.int64),
                           dev[20 * rows:].view(torch.int32).view(rows, width), dev[16 * rows:20 * rows].view(torch.int32),
-                          2 * self._spared > sum([len(s.pages) for s in found if s is not None]))
+                          shared)
         if out is None:
             return made
         for to, t in zip(out[:4], made):

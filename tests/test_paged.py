@@ -228,6 +228,24 @@ def test_pages_are_shared_until_written(monkeypatch):
     assert cache.free_pages == 40 and len(cache) == 0
 
 
+def test_rows_are_shared_among_those_of_the_batch(monkeypatch):
+    """What sequences outside the batch share has no part in it."""
+    cache = _cache_on("cpu", monkeypatch, pages=200)
+    for parent in ("a", "b"):
+        cache.add(parent, 83)
+        for i in range(5):
+            cache.fork(parent, f"{parent}{i}")
+    cache.add("x", 9)
+    cache.add("y", 20)
+    cache.extend(["a", "b", "x", "y", *(f"{p}{i}" for p in "ab" for i in range(5))])
+    shared = lambda *seqs: cache.batch(list(seqs)).shared
+    assert not shared("x", "y") and not shared("x", None) and not shared("a", None, None) and not shared("a", "b")
+    assert not shared("a", "b", "x", "y") and not shared("a", "a0")          # (ten pages of 22 are met twice)
+    assert shared("a", "a0", "a1") and shared(*(f"b{i}" for i in range(5)), "x", None) and shared("a", "a0", "a1", "b", "b0", "b1", "y")
+    out = cache.batch(["a", "a0", "a1"])
+    assert out.shared and not cache.batch(["a", "b", "x"], out=out).shared
+
+
 def test_calls_that_do_not_fit_change_nothing(monkeypatch):
     from deltazip_amd.kv_cache import OutOfPages
     cache = _cache_on("cpu", monkeypatch, pages=4)
