@@ -148,22 +148,29 @@ class PagedKVCache:
             copied.append(not own)
         if need > len(self._free):
             raise OutOfPages(f"{need} pages wanted, {len(self._free)} free")
-        pairs = []
+        # copies first: where they fail nothing has changed
+        pairs = [(s.pages[s.length // self.page_size], self._take()) for s, copy in zip(found, copied) if copy]
+        if pairs:
+            try:
+                copy_pages(self.pool, pairs)
+            except BaseException:
+                for _, page in pairs:
+                    self._users[page] = 0
+                    heapq.heappush(self._free, page)
+                raise
+        made = iter(pairs)
         for s, copy in zip(found, copied):
             if copy:
                 at = s.length // self.page_size
-                old, new = s.pages[at], self._take()
+                old, new = next(made)
                 self._users[old] -= 1
                 self._spared -= 1
                 s.pages[at] = self._rows[s.row, at] = new
-                pairs.append((old, new))
             for at in range(len(s.pages), self._pages_for(s.length + tokens)):
                 page = self._take()
                 s.pages.append(page)
                 self._rows[s.row, at] = page
             s.length += tokens
-        if pairs:
-            copy_pages(self.pool, pairs)
 
     def fork(self, parent: Hashable, child: Hashable) -> None:
         """`child` begins as `parent` is now and shares its pages."""
@@ -210,6 +217,7 @@ class PagedKVCache:
         holes = [p for p in range(n) if not self._users[p]]
         moves = dict(zip([p for p in used if p >= n], holes))
         if moves:
+            copy_pages(self.pool, list(moves.items()))
             for s in self._seqs.values():
                 if any(p in moves for p in s.pages):
                     s.pages[:] = [moves.get(p, p) for p in s.pages]
@@ -217,7 +225,6 @@ class PagedKVCache:
             for old, new in moves.items():
                 self._users[new], self._users[old] = self._users[old], 0
             self._free = list(range(n, self.num_pages))
-            copy_pages(self.pool, list(moves.items()))
         return n
 
     # -- what the operators are given --------------------------------------------------------

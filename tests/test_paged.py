@@ -246,6 +246,35 @@ def test_rows_are_shared_among_those_of_the_batch(monkeypatch):
     assert out.shared and not cache.batch(["a", "b", "x"], out=out).shared
 
 
+def test_a_copy_that_fails_changes_nothing(monkeypatch):
+    """extend and compact of a pool that copy_pages refuses (it is on the host): every sequence has the pages it had."""
+    from deltazip_amd import kv_cache
+    cache = _cache_on("cpu")
+    model = {}
+    for s, n in (("gone", 20), ("a", 11), ("c", 8)):
+        cache.add(s, n)
+        model[s] = [0] * n
+    for s in ("b", "d"):
+        cache.fork("a", s)
+        model[s] = [0] * 11
+    cache.free("gone")
+    del model["gone"]
+    state = lambda: ({s: (cache.pages(s), cache.length(s)) for s in model}, sorted(cache._free), list(cache._users), cache._spared)
+    before = state()
+    for call in (lambda: cache.extend(["a", "c", "b", "d"], 9), cache.compact):
+        with pytest.raises(ValueError, match="GPU"):
+            call()
+        assert state() == before
+        _check(cache, model)
+    monkeypatch.setattr(kv_cache, "copy_pages", _plain_copy)
+    cache.extend(["a", "c", "b", "d"], 9)
+    for s in model:
+        model[s] = model[s] + [0] * 9
+    _check(cache, model)
+    assert cache.compact() == 10 and len({cache.pages(s)[1] for s in "abd"}) == 3
+    _check(cache, model)
+
+
 def test_calls_that_do_not_fit_change_nothing(monkeypatch):
     from deltazip_amd.kv_cache import OutOfPages
     cache = _cache_on("cpu", monkeypatch, pages=4)
