@@ -116,7 +116,7 @@ def host():
         try:
             from . import _host as made
         except ImportError as e:
-            raise RuntimeError("deltazip_amd/_host.so is missing or does not fit: build it with `python -m deltazip_amd.build`") from e
+            raise RuntimeError("the Python extension deltazip_amd/_host is missing or does not fit: build it with `python -m deltazip_amd.build`") from e
         _host = made
     return _host
 
