@@ -189,11 +189,15 @@ class LlamaForDecodeStep(nn.Module):
 
     @property
     def rope(self) -> RotaryPositions:
-        """The positions of `paged_step`, made when it first asks: `decode_step` takes sizes that they do not."""
+        """The positions of `paged_step`, made when it first asks (`decode_step` takes sizes that they do not), or the caller's own."""
         if self._rope is None:
             cfg = self.config
             self._rope = RotaryPositions(cfg.hidden_size // cfg.num_attention_heads, base=cfg.rope_theta, max_position=cfg.max_position_embeddings)
         return self._rope
+
+    @rope.setter
+    def rope(self, made: RotaryPositions) -> None:
+        self._rope = made
 
     def projections(self) -> List[Tuple[str, nn.Module]]:
         """(name, module) of every projection, in execution order."""

@@ -183,3 +183,15 @@ def test_models_that_the_paged_cache_does_not_take_step_over_the_padded_one(hidd
     assert got.shape == (3, 32) and torch.isfinite(got).all()
     with pytest.raises(ValueError):
         model.rope
+
+
+def test_positions_of_the_paged_step_can_be_the_callers():
+    import copy
+    from deltazip_amd import RotaryPositions
+    from deltazip_amd.llama_step import LlamaForDecodeStep, LlamaStepConfig
+    cfg = LlamaStepConfig(hidden_size=64, intermediate_size=64, num_attention_heads=4, num_hidden_layers=1, vocab_size=32, max_position_embeddings=128)
+    model = LlamaForDecodeStep(cfg, generator=torch.Generator().manual_seed(3))
+    first = model.rope
+    assert first is model.rope and first.head_dim == 16 and torch.equal(first.frequencies, RotaryPositions(16, max_position=128).frequencies)
+    model.rope = scaled = RotaryPositions(16, scaling={"type": "linear", "factor": 2.0})
+    assert model.rope is scaled and torch.equal(copy.deepcopy(model).rope.frequencies, scaled.frequencies)
