@@ -76,7 +76,7 @@ def build_host(verbose: bool = False) -> str:
     """Builds the Python extension over libdz_amd.so, which must be there."""
     _run(host_command(), verbose)
     untagged = os.path.join(HERE, "_host.so")                  # any interpreter would import it
-    if os.path.exists(untagged):
+    if untagged != HOST and os.path.exists(untagged):
         os.remove(untagged)
     return HOST
 
