@@ -26,10 +26,11 @@
 // of up to 16 of them, and these joined ones again (counters say who is last), in the order of the tokens: results
 // do not depend on timing.
 //
-// Measured (keys and values over the time of the launch): 128 rows of 1025 tokens of 32 key heads of 128 330 us, 6.5 TB/s;
-// 32 of 1024 86 us, 6.2; one of 131071 tokens of 8 97 us, 5.5, of which 76 at the rate of a kernel that only reads (7.1 TB/s with
+// Measured (keys and values over the time of a call among others): 128 rows of 1025 tokens of 32 key heads of 128 325 us, 6.6 TB/s;
+// 32 of 1024 84 us, 6.4; one of 131071 tokens of 8 94 us, 5.7, of which 76 at the rate of a kernel that only reads (7.1 TB/s with
 // loads that keep nothing in the caches, 6.2 with others; a copy moves 4.9 to 5.4); one of 17 tokens 5 us, of which an empty
-// launch takes 2.5.  A compute unit has some 64 KB on their way at most, which at 2 us is 30 GB/s: what long
+// launch takes 2.5.  32 rows of 1024 tokens of 16 key heads of 256 93 us, 5.8 TB/s; of 200 205 us, 2.0: the form of heads of 200 to 248 takes
+// more than half of the registers, so one wavefront a SIMD asks for keys no step ahead.  A compute unit has some 64 KB on their way at most, which at 2 us is 30 GB/s: what long
 // rows lose is the uneven ends of their parts (63 to 86 us) and the two joins (9 us).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -192,7 +193,7 @@ __device__ __forceinline__ Part find_part(const AttnParams& P, int part, int ite
 __device__ __forceinline__ float weight_of(float top, float up) { return top == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - up); }
 
 // Keys and values of a call pass through once: loads that keep nothing in the caches read 7.1 TB/s where others read 6.2.  Not so
-// where rows share pages: 16 rows of one sequence's 4096 tokens of 32 key heads 119 -> 82 us with the others.
+// where rows share pages: 16 rows of one sequence's 4096 tokens of 32 key heads 130 -> 81 us with the others.
 template <bool ONCE>
 __device__ __forceinline__ u4_t load16(const char* at) {
   return ONCE ? __builtin_nontemporal_load((const u4_t*)at) : *(const u4_t*)at;

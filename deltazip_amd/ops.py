@@ -951,7 +951,7 @@ def poll_status(device=None, wait: bool = False) -> None:
     `wait` is set) and starts the next one, a 4-byte device-to-host copy into pinned memory on the
     workspace's stream.  Raises DeltaKernelError / warns as `raise_for_status` says; a reported
     failure also clears the workspace.  With `wait` the current state is read as well (this
-    synchronises with the workspace's stream)."""
+    synchronises with the workspace's stream and, once an operator on a paged cache has run there, with the whole device)."""
     if not _workspaces and not _page_status:
         return                                        # no call has run yet (or no GPU at all)
     idx = None if device is None else torch.device(device).index

@@ -273,7 +273,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 
     A row of length 0 gives zeros.  Nothing behind a row's length is read, in the tables or in the pages, whatever
     is there; what it sees counts, and values there that are not finite give values that are not, in their row and head.  Several
-    rows may share pages (`shared` says that most of what they see is: the same bits, up to 1.5 times as fast then, a
+    rows may share pages (`shared` says that most of what they see is: the same bits, up to 1.6 times as fast then, a
     tenth slower if it is not so; of one row nothing is), and several rows of one sequence at lengths of their own are a prompt's
     tokens.  A length beyond its table is cut; a page number outside the pool is read as page 0; either is reported through the
     status word.  The order of a row's sums follows the lengths of all rows of the call (the work is cut by them,

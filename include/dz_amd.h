@@ -499,7 +499,7 @@ typedef struct dz_attention_args {
   int64_t q_row, q_head, k_page, k_head, k_token, v_page, v_head, v_token, out_row, out_head, table_row;
   int32_t rows, heads, kv_heads, dim, page_size, pages_per_row, window, dtype;
   float scale;
-  int32_t shared;                         /* rows see the same pages: worth keeping in the caches (results are the same) */
+  int32_t shared;                         /* rows see the same pages: worth keeping in the caches (results are the same; of one row nothing is) */
 } dz_attention_args;
 
 size_t dz_paged_attention_bytes(int rows, int heads, int kv_heads, int dim, int page_size, int pages_per_row);
