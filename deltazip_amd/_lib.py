@@ -72,6 +72,9 @@ SIGNATURES = {
     "dz_gemm_f16_select": (_i, [_vp, _vp, _vp, C.c_longlong, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _vp]),
     "dz_paged_attention_bytes": (_sz, [_i] * 6),
     "dz_paged_attention": (_i, [C.c_char_p, _vp]),      # the packed structure
+    "dz_prefix_attention_bytes": (_sz, [_i] * 6),
+    "dz_prefix_attention": (_i, [C.c_char_p, _vp]),
+    "dz_extend_tables": (_i, [C.c_char_p, _vp]),
     "dz_page_status": (_vp, []),
     "dz_take_page_status": (_i, [_vp, _vp]),
     "dz_capture_id": (C.c_ulonglong, [_vp]),

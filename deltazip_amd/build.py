@@ -19,7 +19,8 @@ LIB = os.path.join(HERE, "libdz_amd.so")
 HOST = os.path.join(HERE, "_host" + sysconfig.get_config_var("EXT_SUFFIX"))     # (of this interpreter: no other imports it)
 
 SOURCES = ["dz_repack.cpp", "dz_kernels.hip", "dz_mdl32.hip", "dz_gemm.hip", "dz_gemm24.hip", "dz_gemm24_rows.hip",
-           "dz_gemm24_mixed.hip", "dz_obs.hip", "dz_probe.hip", "dz_attention.hip", "dz_kv.hip"]
+           "dz_gemm24_mixed.hip", "dz_obs.hip", "dz_probe.hip", "dz_attention.hip", "dz_kv.hip",
+           "dz_prefix.hip", "dz_grow.hip"]
 
 # packed fp32 VALU instructions are switched off for every device compilation in this project
 HIPCC_FLAGS = [

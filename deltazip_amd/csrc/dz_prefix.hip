@@ -1,0 +1,611 @@
+// Attention of the new tokens of a batch over a paged key/value cache, where groups of rows share their first tokens.
+//
+//   o_i = sum_t 2^(s_t - m) v_t / sum_t 2^(s_t - m),   s_t = scale log2(e) q_i.k_t,   t < n - (c - 1 - i)
+//
+// for token i of the c new ones of a row with n tokens, and every head.  A group's rows see the same first tokens: the sums over
+// these are taken for all of the group's tokens and heads at once, so that its keys and values are read once (per 128 queries)
+// and not once per row, and joined with the sums over what is each row's own:
+//   m = max m_p,  l = sum l_p 2^(m_p - m),  o = sum o_p 2^(m_p - m) / l
+//
+// The work is units (a group's prefix; a row's own tokens) of tiles of 128 queries (a token and one of the heads that share a key)
+// times pieces of the tokens that these see.  dz_prefix_plan_kernel, one workgroup, makes the list of them from the lengths, which only
+// the device knows; a workgroup of dz_prefix_kernel takes one of them for one key head; dz_prefix_join_kernel joins.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <atomic>
+
+#include "../../include/dz_amd.h"
+#include "dz_attend.h"
+
+namespace {
+
+typedef short s4_t __attribute__((ext_vector_type(4)));
+typedef short s8_t __attribute__((ext_vector_type(8)));
+
+constexpr int TILE = 128;              // queries of a workgroup
+constexpr int STEP = 64;               // tokens of a step
+constexpr int TARGET = 512;            // pieces that the work is cut into at most, units' last ones apart
+constexpr int LEAST = 256;             // tokens of a piece
+constexpr int GROUPS = DZ_PREFIX_GROUPS;
+constexpr int PLAN = 1024;             // threads of the plan
+
+struct Unit {
+  int tok0, ntok;                      // its queries' tokens
+  int k0, n;                           // tokens seen: k0 .. n - 1 (by the last of its queries)
+  int np, tiles;                       // pieces, tiles
+  int row, pref;                       // whose table; of a row: its group's unit, or -1
+  long long part;                      // records of its sums, or -1: it has one piece, and nothing else to join
+  int causal, pad;
+};
+struct Item {
+  int unit, tile, piece, pad;
+};
+
+struct PrefixParams {
+  const char *q, *k, *v;
+  const int *tables, *lengths, *starts, *groups, *prefixes;
+  uint16_t* out;
+  unsigned* status;
+  int* head;                           // [0]: how many items there are
+  Unit* units;                         // the groups', the rows'
+  Item* items;
+  int* row_of;                         // of every token, where starts say
+  float* parts;                        // records of dim + 4 floats: values, maximum, sum
+  long long q_row, q_head, k_page, k_head, k_token, v_page, v_head, v_token, out_row, out_head, table_row;   // bytes; out, table: elements
+  long long room_parts;
+  unsigned num_pages;
+  int tokens, rows, ngroups, heads, kv_heads, share, dim, shift, pages_per_row, room_items;
+  float scale;
+};
+
+__device__ __forceinline__ int tiles_for(const PrefixParams& P, int tokens) { return (int)(((long long)tokens * P.share + TILE - 1) / TILE); }
+
+// The last i in [0, n) with at[i] <= x, or -1.
+template <typename T>
+__device__ __forceinline__ int last_upto(const T* at, int n, T x) {
+  int lo = 0, hi = n;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (at[mid] <= x)
+      lo = mid + 1;
+    else
+      hi = mid;
+  }
+  return lo - 1;
+}
+
+__global__ __launch_bounds__(PLAN) void dz_prefix_plan_kernel(const PrefixParams P) {
+  __shared__ int first[GROUPS + 1], cut[GROUPS], leader[GROUPS], alone[GROUPS];      // of groups: rows, prefix, row whose table, tiles apart
+  __shared__ int items_to[PLAN];
+  __shared__ long long wave_parts[PLAN / 64];
+  __shared__ int wave_items[PLAN / 64];
+  __shared__ float wave_work[PLAN / 64];
+  __shared__ int2 made[PLAN];            // of a round's units: tiles, pieces
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int room = P.pages_per_row << P.shift;
+  int bad = 0, bad_groups = 0;
+  for (int r = tid; r < P.rows; r += PLAN) {
+    if (P.starts) {
+      const int a = P.starts[r], b = P.starts[r + 1];
+      bad |= a < 0 || b < a || b > P.tokens;
+    }
+    if (P.lengths[r] > room) atomicOr(P.status, 4u);
+  }
+  for (int g = tid; g < P.ngroups; g += PLAN) {
+    const int a = P.groups[g], b = P.groups[g + 1];
+    bad_groups |= a < 0 || b < a || b > P.rows;
+    first[g] = a, first[g + 1] = b;                       // (neighbours write the same)
+    cut[g] = min(P.prefixes[g], room);
+    leader[g] = P.rows;
+    alone[g] = 0;
+  }
+  bad = __syncthreads_or(bad);
+  bad_groups = __syncthreads_or(bad_groups);
+  if ((bad || bad_groups) && tid == 0) atomicOr(P.status, 4u);
+  const int rows = bad ? 0 : P.rows, groups = bad || bad_groups ? 0 : P.ngroups;
+  auto count_of = [&](int r) { return P.starts ? P.starts[r + 1] - P.starts[r] : 1; };
+  auto length_of = [&](int r) { return max(0, min(P.lengths[r], room)); };
+  auto start_of = [&](int r) { return P.starts ? P.starts[r] : r; };
+  auto group_of = [&](int r) {
+    const int g = groups ? last_upto(first, groups, r) : -1;
+    return g >= 0 && r < first[g + 1] ? g : -1;
+  };
+  // a prefix ends where the first of its rows' new tokens sees no more of it
+  for (int r = tid; r < rows; r += PLAN) {
+    const int g = group_of(r), n = length_of(r), c = count_of(r);
+    if (g >= 0 && n > 0 && c > 0) {
+      atomicMin(&cut[g], max(0, n - c + 1));
+      atomicMin(&leader[g], r);
+      atomicAdd(&alone[g], tiles_for(P, c));
+    }
+  }
+  __syncthreads();
+  // and is taken apart from the rows only where that spares tiles
+  for (int g = tid; g < groups; g += PLAN) {
+    const int tokens = start_of(first[g + 1]) - start_of(first[g]);
+    if (cut[g] <= 0 || leader[g] >= rows || tiles_for(P, tokens) >= alone[g]) cut[g] = 0;
+  }
+  __syncthreads();
+  auto unit_of = [&](int u) {
+    Unit x = {0, 0, 0, 0, 0, 0, 0, -1, -1, 0, 0};
+    if (u < groups) {
+      if (cut[u]) {
+        x.tok0 = start_of(first[u]);
+        x.ntok = start_of(first[u + 1]) - x.tok0;
+        x.n = cut[u];
+        x.row = leader[u];
+      }
+    } else {
+      const int r = u - groups, g = group_of(r);
+      x.tok0 = start_of(r);
+      x.ntok = count_of(r);
+      x.n = length_of(r);
+      x.row = r;
+      x.causal = 1;
+      if (g >= 0 && cut[g] && x.n > 0 && x.ntok > 0) {
+        x.k0 = cut[g];
+        x.pref = g;
+      }
+    }
+    x.tiles = tiles_for(P, x.ntok);
+    return x;
+  };
+  const int units = groups + rows;
+  float work = 0.0f;
+  for (int u = tid; u < units; u += PLAN) {
+    const Unit x = unit_of(u);
+    work += (float)x.tiles * (float)(x.n - x.k0);
+  }
+  work = scan_add(work);
+  if (lane == 63) wave_work[wave] = work;
+  __syncthreads();
+  work = 0.0f;
+  for (int w = 0; w < PLAN / 64; ++w) work += wave_work[w];
+  // tokens of a piece, in whole steps (sums above 2^24 are rounded: a piece is a little longer)
+  const float want = ceilf(work * 1.0001f * (float)P.kv_heads * (1.0f / TARGET) * (1.0f / STEP));
+  const int each = STEP * (int)fminf(fmaxf(want, (float)(LEAST / STEP)), (float)(1 << 24));
+
+  int items0 = 0;                      // in front of this round of units
+  long long parts0 = 0;
+  for (int u0 = 0; u0 < units; u0 += PLAN) {
+    const int u = u0 + tid;
+    Unit x = {0, 0, 0, 0, 0, 0, 0, -1, -1, 0, 0};
+    int items = 0;
+    long long parts = 0;
+    if (u < units) {
+      x = unit_of(u);
+      x.np = (x.n - x.k0 + each - 1) / each;
+      if (x.tiles == 0) x.np = 0;
+      items = x.tiles * x.np;
+      if (x.np > 1 || x.k0 > 0 || !x.causal) parts = (long long)x.np * x.ntok * P.heads;
+    }
+    const int items_upto = scan_add(items);
+    // (a sum of 64 bits over a wavefront: two of 32)
+    long long parts_upto = parts;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const long long y = __shfl_up(parts_upto, d);
+      if (lane >= d) parts_upto += y;
+    }
+    if (lane == 63) wave_items[wave] = items_upto, wave_parts[wave] = parts_upto;
+    __syncthreads();
+    const int begin = items0;
+    int before = items0;
+    long long parts_before = parts0;
+    for (int w = 0; w < PLAN / 64; ++w) {
+      if (w < wave) before += wave_items[w], parts_before += wave_parts[w];
+      items0 += wave_items[w], parts0 += wave_parts[w];
+    }
+    items_to[tid] = before + items_upto;
+    if (parts) x.part = parts_before + parts_upto - parts;
+    made[tid] = make_int2(x.tiles, x.np);
+    if (u < units) P.units[u < groups ? u : P.ngroups + u - groups] = x;
+    __syncthreads();
+    for (int i = begin + tid; i < items0; i += PLAN) {
+      const int at = last_upto(items_to, PLAN, i) + 1;                     // the first unit that ends behind i
+      const int tiles = made[at].x, rest = i - (items_to[at] - tiles * made[at].y);
+      // tiles that share keys and values next to each other; of a row's, those that see most first
+      if (i < P.room_items) P.items[i] = Item{u0 + at < groups ? u0 + at : P.ngroups + u0 + at - groups, tiles - 1 - rest % tiles, rest / tiles, 0};
+    }
+    __syncthreads();
+  }
+  if (P.starts)
+    for (int t = tid; t < P.tokens; t += PLAN) {
+      int r = rows ? last_upto(P.starts, rows, t) : -1;
+      if (r >= 0 && t >= P.starts[r + 1]) r = -1;
+      P.row_of[t] = r;
+    }
+  if (tid == 0) {
+    const bool fits = items0 <= P.room_items && parts0 <= P.room_parts;
+    if (!fits) atomicOr(P.status, 4u);
+    P.head[0] = fits ? items0 : 0;
+  }
+}
+
+// Requests of 16 bytes of a token's row lie in LDS in the order c ^ swizzled(token): 8 tokens' one request, which a key's operand reads at
+// a time, and 4 tokens' two, which a transposing read of values does, are then in banks of their own.
+template <int KC>
+__device__ __forceinline__ int swizzled(int token) {
+  return KC % 4 == 0 ? 2 * (token & 7) : KC % 2 == 0 ? 2 * (token >> 1 & 3) : 2 * (token >> 2 & 1);
+}
+
+template <int KC, bool FULL, bool BF>
+__global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void dz_prefix_kernel(const PrefixParams P) {
+  typedef Type<BF> Ty;
+  typedef typename Ty::v8 v8;
+  constexpr int ROW = KC * 64;                         // bytes of a token in LDS
+  constexpr int HALF = STEP * ROW, STAGE = 2 * HALF;   // keys, values
+  constexpr unsigned BAD = BF ? 0x7f80u : 0x7c00u;     // exponent of what is not finite
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
+  const int nth = blockIdx.x / P.kv_heads, kvh = blockIdx.x % P.kv_heads;
+  if (nth >= P.head[0]) return;
+  const Item item = P.items[nth];
+  const Unit U = P.units[item.unit];
+  const int queries = U.ntok * P.share, x0 = item.tile * TILE, in_tile = min(TILE, queries - x0);
+  auto limit_of = [&](int x) { return U.causal ? max(U.n - (U.ntok - 1 - x / P.share), 0) : U.n; };      // tokens that query x sees
+  const int end = max(limit_of(x0 + in_tile - 1), U.k0);
+  const long long len = end - U.k0;
+  // pieces meet between steps, and steps lie in whole pages or hold whole pages
+  auto bound = [&](int p) { return p == U.np ? end : max(U.k0, (U.k0 + (int)(len * p / U.np)) & ~(STEP - 1)); };
+  const int lo = bound(item.piece), hi = bound(item.piece + 1), begin = lo < hi ? lo & ~(STEP - 1) : hi;
+
+  const int last_page = (hi - 1) >> P.shift, in_page = (1 << P.shift) - 1;
+  const int* table = P.tables + U.row * P.table_row;
+  int page0 = begin >> P.shift;        // of the 64 page numbers that the lanes hold
+  auto fetch = [&](int base) {
+    const int at = base + lane;
+    unsigned id = at <= last_page && begin < hi ? (unsigned)table[at] : 0u;
+    if (id >= P.num_pages) {
+      atomicOr(P.status, 4u);
+      id = 0;
+    }
+    return id;
+  };
+  unsigned ids = fetch(page0), next_ids = fetch(page0 + 64);
+
+  const int per_row = P.dim / 8;       // requests of a token's row
+  if (!FULL) {                         // behind the head's end: zeros, which meet the queries' zeros
+    for (int i = threadIdx.x; i < 2 * STAGE / 16; i += 256) *(u4_t*)(lds + 16 * i) = u4_t{0, 0, 0, 0};
+    __syncthreads();
+  }
+  // a wavefront brings in 16 tokens of each step; request i of a lane is for token 16 wave + (64 i + lane) / (4 KC)
+  int req_token[KC], req_at[KC];
+#pragma unroll
+  for (int i = 0; i < KC; ++i) {
+    const int at = 64 * i + lane;
+    req_token[i] = at / (4 * KC);
+    const int c = at % (4 * KC) ^ swizzled<KC>(req_token[i]);
+    req_at[i] = FULL || c < per_row ? 16 * c : -1;
+  }
+  auto issue = [&](int s, int buf) {
+    if (((min(s + STEP, hi) - 1) >> P.shift) >= page0 + 64) {
+      ids = next_ids;
+      page0 += 64;
+      next_ids = fetch(page0 + 64);
+    }
+    char* to = lds + buf * STAGE + wave * 16 * ROW;
+    const int t0 = s + 16 * wave;
+#pragma unroll
+    for (int i = 0; i < KC; ++i) {
+      const int t = min(t0 + req_token[i], hi - 1);        // (behind the end: the last one again)
+      const unsigned id = __shfl(ids, (t >> P.shift) - page0);
+      const char* k = P.k + id * P.k_page + kvh * P.k_head + (t & in_page) * P.k_token + req_at[i];
+      const char* v = P.v + id * P.v_page + kvh * P.v_head + (t & in_page) * P.v_token + req_at[i];
+      if (FULL || req_at[i] >= 0) {
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)k, (__attribute__((address_space(3))) void*)(to + i * 1024), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)v, (__attribute__((address_space(3))) void*)(to + HALF + i * 1024), 16, 0, 0);
+      }
+    }
+  };
+  if (begin < hi) issue(begin, 0);
+
+  auto work = [&](auto cols) __attribute__((always_inline)) {
+    constexpr int NC = decltype(cols)::value;          // tiles of 16 queries of a wavefront
+    const int mine = wave * 16 * NC;                   // its first query in the tile
+    const bool active = mine < in_tile;
+    v8 q[NC][KC];
+    int lim[NC];
+    f4_t acc[NC][2 * KC];
+    float top[NC], sum[NC];
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      const int x = mine + 16 * n + col, xx = x0 + min(x, in_tile - 1);
+      const int token = U.tok0 + xx / P.share, head = kvh * P.share + xx % P.share;
+#pragma unroll
+      for (int c = 0; c < KC; ++c) {
+        u4_t w = {0, 0, 0, 0};
+        if (x < in_tile && (FULL || 32 * c + 8 * g < P.dim)) w = *(const u4_t*)(P.q + token * P.q_row + head * P.q_head + (32 * c + 8 * g) * 2);
+        q[n][c] = __builtin_bit_cast(v8, w);
+      }
+      lim[n] = min(limit_of(xx), hi);
+      top[n] = -INFINITY, sum[n] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 2 * KC; ++j) acc[n][j] = f4_t{0, 0, 0, 0};
+    }
+    const int seen_by_all = min(limit_of(x0 + min(mine, in_tile - 1)), hi), seen_by_last = min(limit_of(x0 + min(mine + 16 * NC, in_tile) - 1), hi);
+
+    auto step = [&](int s, const char* at) __attribute__((always_inline)) {
+      const bool edge = s + STEP > seen_by_all || s < lo;
+      const char* keys = at + col * ROW;
+      const int turn_k = swizzled<KC>(col);
+      f4_t sc[NC][4];
+#pragma unroll
+      for (int a = 0; a < 4; ++a) {
+        v8 kw[KC];
+#pragma unroll
+        for (int c = 0; c < KC; ++c) kw[c] = *(const v8*)(keys + a * 16 * ROW + ((4 * c + g) ^ turn_k) * 16);
+#pragma unroll
+        for (int n = 0; n < NC; ++n) {
+          f4_t c4 = {0, 0, 0, 0};
+#pragma unroll
+          for (int c = 0; c < KC; ++c) c4 = Ty::mma(kw[c], q[n][c], c4);
+          sc[n][a] = c4 * P.scale;
+        }
+      }
+      bool spoilt = false;             // values that are not finite, where some queries do not see all tokens
+      if (edge) {
+#pragma unroll
+        for (int n = 0; n < NC; ++n)
+#pragma unroll
+          for (int a = 0; a < 4; ++a)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (s + 16 * a + 4 * g + i >= lim[n] || s + 16 * a + 4 * g + i < lo) sc[n][a][i] = -INFINITY;
+        unsigned found = 0;
+#pragma unroll 4
+        for (int i = lane; i < HALF / 16; i += 64) {
+          const u4_t w = *(const u4_t*)(at + HALF + 16 * i);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) found |= (w[e] & (BAD | BAD << 16)) + ((0x8000u - BAD) | (0x8000u - BAD) << 16);
+        }
+        spoilt = __any(found & 0x80008000u);
+      }
+      v8 p[NC][2];
+#pragma unroll
+      for (int n = 0; n < NC; ++n) {
+        float most = sc[n][0][0];
+#pragma unroll
+        for (int e = 1; e < 16; ++e) most = fmaxf(most, sc[n][e >> 2][e & 3]);
+        // the reference moves only where a score is more than twice above it
+        if (__any(most > top[n] + 1.0f)) {
+          most = fmaxf(most, __shfl_xor(most, 16));
+          most = fmaxf(most, __shfl_xor(most, 32));
+          const float up = fmaxf(most, top[n]);
+          const float f = top[n] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top[n] - up);
+          top[n] = up;
+          sum[n] *= f;
+#pragma unroll
+          for (int j = 0; j < 2 * KC; ++j) acc[n][j] *= f;
+        }
+        const float ref = top[n] == -INFINITY ? 0.0f : top[n] - Ty::BIAS;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float x = __builtin_amdgcn_exp2f(sc[n][e >> 2][e & 3] - ref);
+          sum[n] += x;
+          p[n][e >> 3][e & 7] = Ty::one(x);
+        }
+      }
+      // a transposing read: lanes of a row of 16 name 4 tokens' 16 dims, and each gets one dim of the four
+      const char* values = at + HALF + (4 * g + (col >> 2)) * ROW + (col & 1) * 8;
+      const int turn_v = swizzled<KC>(4 * g + (col >> 2));
+      auto product = [&](auto is_spoilt) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < 2 * KC; ++j)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const char* from = values + 2 * h * 16 * ROW + ((2 * j + (col >> 1 & 1)) ^ turn_v) * 16;
+            const s4_t a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4_t*)from);
+            const s4_t a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4_t*)(from + 16 * ROW));
+            s8_t w = {a0[0], a0[1], a0[2], a0[3], a1[0], a1[1], a1[2], a1[3]};
+            if (decltype(is_spoilt)::value) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                if (((unsigned)w[e] & BAD) == BAD) w[e] = 0;
+            }
+#pragma unroll
+            for (int n = 0; n < NC; ++n) acc[n][j] = Ty::mma(__builtin_bit_cast(v8, w), p[n][h], acc[n][j]);
+          }
+      };
+      if (__builtin_expect(!spoilt, 1)) {
+        product(std::integral_constant<bool, false>());
+      } else {
+        // a weight of 0 would take them to queries that do not see them: left out of the product, and added where they are seen
+        product(std::integral_constant<bool, true>());
+        int quad = 4 * g;
+        asm volatile("" : "+v"(quad));   // (addresses of this rare path are not worth registers all along)
+#pragma unroll 1
+        for (int t = 0; t < STEP; ++t)
+#pragma unroll
+          for (int j = 0; j < 2 * KC; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint16_t w = *(const uint16_t*)(at + HALF + t * ROW + ((2 * j + (quad >> 3)) ^ swizzled<KC>(t)) * 16 + ((quad & 7) + i) * 2);
+              const float y = BF ? __builtin_bit_cast(float, (unsigned)w << 16) : (float)__builtin_bit_cast(_Float16, w);
+#pragma unroll
+              for (int n = 0; n < NC; ++n)
+                if ((w & BAD) == BAD && s + t < lim[n] && s + t >= lo) acc[n][j][i] += y;
+            }
+      }
+    };
+
+    int buf = 0;
+    for (int s = begin; s < hi; s += STEP, buf ^= 1) {
+      __builtin_amdgcn_s_waitcnt(0x0070);              // vmcnt(0) lgkmcnt(0): this wavefront's share of the step is in,
+      __syncthreads();                                 // and the others'; no one reads the other buffer any more
+      if (s + STEP < hi) issue(s + STEP, buf ^ 1);
+      if (!active || s >= seen_by_last) continue;
+      step(s, lds + buf * STAGE);
+    }
+    if (!active) return;
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      const int x = mine + 16 * n + col;
+      sum[n] += __shfl_xor(sum[n], 16);
+      sum[n] += __shfl_xor(sum[n], 32);
+      if (x >= in_tile) continue;
+      const int xx = x0 + x;
+      if (U.part >= 0) {
+        float* record = P.parts + (U.part + ((long long)item.piece * P.kv_heads + kvh) * queries + xx) * (P.dim + 4);
+#pragma unroll
+        for (int j = 0; j < 2 * KC; ++j)
+          if (FULL || 16 * j + 4 * g < P.dim) *(f4_t*)(record + 16 * j + 4 * g) = acc[n][j];
+        if (g == 0) *(f2_t*)(record + P.dim) = f2_t{top[n], sum[n]};
+      } else {
+        uint16_t* to = P.out + (U.tok0 + xx / P.share) * P.out_row + (kvh * P.share + xx % P.share) * P.out_head;
+        const bool sees = limit_of(xx) > 0;
+#pragma unroll
+        for (int j = 0; j < 2 * KC; ++j) {
+          const f4_t y = sees ? acc[n][j] / sum[n] : f4_t{0, 0, 0, 0};
+          const u2_t w = {(unsigned)Ty::round(y[0]) | (unsigned)Ty::round(y[1]) << 16, (unsigned)Ty::round(y[2]) | (unsigned)Ty::round(y[3]) << 16};
+          if (FULL || 16 * j + 4 * g < P.dim) *(u2_t*)(to + 16 * j + 4 * g) = w;
+        }
+      }
+    }
+  };
+  if (in_tile > 64)
+    work(std::integral_constant<int, 2>());
+  else
+    work(std::integral_constant<int, 1>());
+}
+
+// A workgroup a token: the pieces of its row's sums and of its group's, or zeros.
+template <bool BF>
+__global__ __launch_bounds__(256) void dz_prefix_join_kernel(const PrefixParams P) {
+  typedef Type<BF> Ty;
+  const int t = blockIdx.x, row = P.starts ? P.row_of[t] : t;
+  Unit own = {0, 0, 0, 0, 0, 0, 0, -1, -1, 0, 0}, pre = own;
+  bool sees = false;
+  if (row >= 0) {
+    own = P.units[P.ngroups + row];
+    sees = own.n - (own.ntok - 1 - (t - own.tok0)) > 0;
+    if (own.pref >= 0) pre = P.units[own.pref];
+  }
+  if (sees && own.np == 1 && own.part < 0) return;      // (stored already)
+  const int quads = P.dim / 4, stride = P.dim + 4;
+  for (int x = threadIdx.x; x < P.heads * quads; x += 256) {
+    const int h = x / quads, d = x % quads * 4, kvh = h / P.share;
+    float m = -INFINITY, l = 0.0f;
+    f4_t o = {0, 0, 0, 0};
+    auto gather = [&](const Unit& u) {
+      const long long queries = (long long)u.ntok * P.share, at = kvh * queries + (long long)(t - u.tok0) * P.share + h % P.share;
+      const float* record = P.parts + (u.part + at) * stride;
+      for (int p = 0; p < u.np; ++p, record += P.kv_heads * queries * stride) {
+        const f4_t w = *(const f4_t*)(record + d);
+        const f2_t ml = *(const f2_t*)(record + P.dim);
+        const float up = fmaxf(m, ml[0]), f = weight_of(m, up), fs = weight_of(ml[0], up);
+        l = l * f + ml[1] * fs;
+        o = o * f + w * fs;
+        m = up;
+      }
+    };
+    if (sees) {
+      if (pre.part >= 0) gather(pre);
+      if (own.part >= 0) gather(own);
+    }
+    const f4_t y = sees ? o / l : f4_t{0, 0, 0, 0};
+    const u2_t w = {(unsigned)Ty::round(y[0]) | (unsigned)Ty::round(y[1]) << 16, (unsigned)Ty::round(y[2]) | (unsigned)Ty::round(y[3]) << 16};
+    *(u2_t*)(P.out + t * P.out_row + h * P.out_head + d) = w;
+  }
+}
+
+typedef void (*kernel_t)(const PrefixParams);
+inline int chunks_of(int dim) { return dim <= 64 ? 2 : dim <= 96 ? 3 : dim <= 128 ? 4 : dim <= 192 ? 6 : 8; }
+template <int KC, bool BF>
+kernel_t kernel_of(int dim) {
+  return dim == 32 * KC ? dz_prefix_kernel<KC, true, BF> : dz_prefix_kernel<KC, false, BF>;
+}
+template <bool BF>
+kernel_t kernel_for(int dim) {
+  const int kc = chunks_of(dim);
+  return kc == 2 ? kernel_of<2, BF>(dim) : kc == 3 ? kernel_of<3, BF>(dim) : kc == 4 ? kernel_of<4, BF>(dim)
+         : kc == 6 ? kernel_of<6, BF>(dim) : kernel_of<8, BF>(dim);
+}
+
+inline bool shapes_fit(int tokens, int rows, int groups, int heads, int kv_heads, int dim, int page_size, int pages_per_row) {
+  return tokens >= 0 && rows >= 0 && rows <= (1 << 20) && groups >= 0 && groups <= GROUPS && heads >= 1 && kv_heads >= 1 && heads <= 4096 &&
+         heads % kv_heads == 0 && (long long)tokens * heads < (1ll << 31) && dim >= 8 && dim <= 256 && dim % 8 == 0 && page_size >= 8 &&
+         page_size <= 1024 && (page_size & (page_size - 1)) == 0 && pages_per_row >= 0 && (long long)pages_per_row * page_size <= (1ll << 30);
+}
+
+// What a call's plan comes to at most.
+struct Room {
+  long long items, parts;              // items of one key head; records
+  size_t units_at, items_at, rows_at, parts_at, bytes;
+};
+inline Room room_of(int tokens, int rows, int groups, int heads, int kv_heads, int dim) {
+  Room m;
+  const long long queries = (long long)tokens * (heads / kv_heads), whole = (queries + TILE - 1) / TILE;
+  const long long some = rows < tokens ? rows : tokens, both = groups ? 2 : 1;
+  // a unit's tiles: the last one is not full; pieces: of TARGET in all one more of each tile
+  m.items = both * whole + some + (groups < tokens ? groups : tokens) + TARGET / kv_heads + 1;
+  m.parts = both * tokens * heads + (long long)TILE * (TARGET + kv_heads);
+  auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+  m.units_at = 256;
+  m.items_at = up(m.units_at + sizeof(Unit) * (size_t)(rows + groups));
+  m.rows_at = up(m.items_at + sizeof(Item) * (size_t)m.items);
+  m.parts_at = up(m.rows_at + 4 * (size_t)tokens);
+  m.bytes = m.parts_at + (size_t)m.parts * (dim + 4) * 4;
+  return m;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t dz_prefix_attention_bytes(int tokens, int rows, int groups, int heads, int kv_heads, int dim) {
+  if (!shapes_fit(tokens, rows, groups, heads, kv_heads, dim, 8, 0)) return 0;
+  return room_of(tokens, rows, groups, heads, kv_heads, dim).bytes;
+}
+
+int dz_prefix_attention(const dz_prefix_args* a, void* stream) {
+  if (!a || a->bytes != (int64_t)sizeof(*a)) return DZ_EINVAL;
+  if (!shapes_fit(a->tokens, a->rows, a->groups_n, a->heads, a->kv_heads, a->dim, a->page_size, a->pages_per_row)) return DZ_EPAGES;
+  if (a->dtype != DZ_F16 && a->dtype != DZ_BF16) return DZ_EINVAL;
+  if (!a->starts && a->tokens != a->rows) return DZ_EINVAL;
+  if (a->tokens == 0) return DZ_OK;
+  if (!a->q || !a->k_pages || !a->v_pages || (!a->tables && a->pages_per_row && a->rows) || (!a->lengths && a->rows) || !a->out || !a->status) return DZ_EINVAL;
+  if (a->groups_n && (!a->groups || !a->prefixes)) return DZ_EINVAL;
+  if (a->num_pages < 1 || a->num_pages > 0x7fffffffll) return DZ_EPAGES;
+  const int64_t strides[] = {a->q_row, a->q_head, a->k_page, a->k_head, a->k_token, a->v_page, a->v_head, a->v_token, a->out_row, a->out_head};
+  for (int64_t s : strides)
+    if (s < 0 || s % 8) return DZ_EALIGN;
+  if (((uintptr_t)a->q | (uintptr_t)a->k_pages | (uintptr_t)a->v_pages | (uintptr_t)a->out) & 15) return DZ_EALIGN;
+  if (((uintptr_t)a->tables | (uintptr_t)a->lengths | (uintptr_t)a->starts | (uintptr_t)a->groups | (uintptr_t)a->prefixes | (uintptr_t)a->status) & 3)
+    return DZ_EALIGN;
+  if (a->table_row < 0) return DZ_EPAGES;
+  const Room m = room_of(a->tokens, a->rows, a->groups_n, a->heads, a->kv_heads, a->dim);
+  if (!a->work || (size_t)a->work_bytes < m.bytes || ((uintptr_t)a->work & 15)) return DZ_EWORKSPACE;
+  const long long grid = m.items * a->kv_heads;
+  if (grid > 0x7fffffffll) return DZ_EPAGES;
+
+  PrefixParams P;
+  char* work = (char*)a->work;
+  P.q = (const char*)a->q, P.k = (const char*)a->k_pages, P.v = (const char*)a->v_pages;
+  P.tables = a->tables, P.lengths = a->lengths, P.starts = a->starts, P.groups = a->groups, P.prefixes = a->prefixes;
+  P.out = (uint16_t*)a->out, P.status = a->status;
+  P.head = (int*)work, P.units = (Unit*)(work + m.units_at), P.items = (Item*)(work + m.items_at), P.row_of = (int*)(work + m.rows_at);
+  P.parts = (float*)(work + m.parts_at);
+  P.q_row = 2 * a->q_row, P.q_head = 2 * a->q_head;
+  P.k_page = 2 * a->k_page, P.k_head = 2 * a->k_head, P.k_token = 2 * a->k_token;
+  P.v_page = 2 * a->v_page, P.v_head = 2 * a->v_head, P.v_token = 2 * a->v_token;
+  P.out_row = a->out_row, P.out_head = a->out_head, P.table_row = a->table_row;
+  P.room_parts = m.parts, P.room_items = (int)m.items;
+  P.num_pages = (unsigned)a->num_pages;
+  P.tokens = a->tokens, P.rows = a->rows, P.ngroups = a->groups_n, P.heads = a->heads, P.kv_heads = a->kv_heads, P.share = a->heads / a->kv_heads;
+  P.dim = a->dim, P.shift = __builtin_ctz(a->page_size), P.pages_per_row = a->pages_per_row;
+  P.scale = a->scale * 1.44269504088896340736f;
+  const int kc = chunks_of(a->dim), which = kc * 4 + (a->dim == 32 * kc) * 2 + a->dtype;
+  const size_t lds = 2 * (size_t)(8 * kc) * 1024;
+  const kernel_t kern = a->dtype == DZ_BF16 ? kernel_for<true>(a->dim) : kernel_for<false>(a->dim);
+  static std::atomic<unsigned long long> attr_done[36];        // one per kernel
+  if (lds > 65536 && !dz_lds_limit_once(attr_done[which], (const void*)kern, (int)lds)) return DZ_ELAUNCH;
+  const hipStream_t st = (hipStream_t)stream;
+  hipLaunchKernelGGL(dz_prefix_plan_kernel, dim3(1), dim3(PLAN), 0, st, P);
+  hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(256), lds, st, P);
+  hipLaunchKernelGGL(a->dtype == DZ_BF16 ? dz_prefix_join_kernel<true> : dz_prefix_join_kernel<false>, dim3(a->tokens), dim3(256), 0, st, P);
+  return hipGetLastError() == hipSuccess ? DZ_OK : DZ_ELAUNCH;
+}
+
+}  // extern "C"

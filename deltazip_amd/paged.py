@@ -3,6 +3,8 @@
   rotary            queries and keys turned to their positions
   append_kv         the same for the tokens of a step, their keys and values stored in the cache
   paged_attention   one new token per row over the pages of its table
+  prefix_attention  new tokens of every row, one or many, over prefixes that rows share and what is each row's own
+  extend_tables     tables, positions and slots of the tokens that rows get next, on the device
   copy_pages        pages copied within every pool (forks, compaction)
 
 They stand where the reference's serving engine has its own kernels for these (serving/csrc/pos_encoding,
@@ -30,8 +32,11 @@ from . import _lib, ops
 _TYPES = {torch.float16: 0, torch.bfloat16: 1}
 _ATTENTION = struct.Struct("=q9Q2q11q8ifi")       # dz_attention_args
 _ROTARY = struct.Struct("=q10Qq14q8ifi")          # dz_rotary_args
+_PREFIX = struct.Struct("=q11Q2q11q9if")          # dz_prefix_args
+_EXTEND = struct.Struct("=q11Qq6i")               # dz_extend_args
 MAX_DIM = 256
 COUNTERS = 32768                  # DZ_ATTENTION_COUNTERS
+MAX_GROUPS = 2048                 # DZ_PREFIX_GROUPS
 
 
 class RotaryPositions:
@@ -217,6 +222,11 @@ def _attention_bytes(rows: int, heads: int, kv_heads: int, dim: int, page_size: 
     return _lib.lib().dz_paged_attention_bytes(rows, heads, kv_heads, dim, page_size, pages_per_row)
 
 
+@lru_cache(maxsize=1024)
+def _prefix_bytes(tokens: int, rows: int, groups: int, heads: int, kv_heads: int, dim: int) -> int:
+    return _lib.lib().dz_prefix_attention_bytes(tokens, rows, groups, heads, kv_heads, dim)
+
+
 _capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
 
 
@@ -325,6 +335,158 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         vs[2], _stride(out, 0), _stride(out, 1), block_tables.stride(0) if rows > 1 else 0, rows, heads, kv_heads, dim, page_size,
         width, min(int(window), (1 << 31) - 1), _TYPES[q.dtype], dim ** -0.5 if scale is None else scale, int(bool(shared)))
     _lib.check(_lib.lib().dz_paged_attention(args, ops._stream()), "dz_paged_attention")
+    return out
+
+
+def prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_tables: torch.Tensor, lengths: torch.Tensor,
+                     starts: Optional[torch.Tensor] = None, groups: Optional[torch.Tensor] = None, prefixes: Optional[torch.Tensor] = None,
+                     scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of the new tokens of every row, one or many, where groups of rows share their first tokens, which are read
+    once for all of a group:
+
+        out[t, h] = softmax(scale q[t, h] . K)  V    over tokens 0 .. n - c + i of row r, n = lengths[r]
+
+    for token t = starts[r] + i of the c = starts[r + 1] - starts[r] new ones of row r, the last of its n (drafted tokens, a prompt or a
+    piece of one).  starts int32 [rows + 1], rising; None: q has one token of each row.  q [tokens, heads, dim]; pages,
+    block_tables [rows, n], lengths [rows], scale and strides as for `paged_attention`.
+
+    Rows groups[g] .. groups[g + 1] - 1 (int32 [n + 1], rising, up to 2048 groups) have their first prefixes[g] (int32 [n]) tokens in common: samples of
+    one prompt, chats with one system prompt, questions about one document.  They are read through the table of the
+    first of these rows that has tokens; what is longer than the first new token of any of them sees is each row's own.  None: nothing
+    is shared.
+
+    Tokens of no row (in front of starts[0], behind starts[rows]) and those of rows of length 0 give zeros; nothing that a token
+    does not see reaches its output, whatever is there.  Starts that do not rise within q leave all rows without tokens, groups
+    that do not rise within the rows share nothing; these, lengths beyond the tables and page numbers outside the pool are reported through the
+    status word.  The weights of 17 and more queries a key (tokens times heads that share one) are rounded to q's type, as their products with the values take
+    them.  The same call gives the same bits; they depend on the lengths of all of its rows."""
+    ops._need_cuda(q, k_pages, v_pages, block_tables, lengths, starts, groups, prefixes, out)
+    if _elsewhere(q):
+        with torch.cuda.device(q.device):
+            return prefix_attention(q, k_pages, v_pages, block_tables, lengths, starts, groups, prefixes, scale, out)
+    _same_place(q, k_pages, v_pages, block_tables, lengths, starts, groups, prefixes, out)
+    _heads("q", q)
+    _pages("k_pages", k_pages, q)
+    _pages("v_pages", v_pages, q)
+    tokens, heads, dim = q.shape
+    pages, kv_heads, page_size, _ = k_pages.shape
+    if v_pages.shape != k_pages.shape:
+        raise ValueError("k_pages and v_pages must have one shape")
+    if heads % kv_heads or not heads or heads > 4096 or dim % 8 or dim > MAX_DIM:
+        raise ValueError(f"heads must be a multiple of kv_heads, up to 4096, and dim one of 8, up to {MAX_DIM}")
+    if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or (block_tables.shape[1] > 1 and block_tables.stride(1) != 1):
+        raise ValueError("block_tables must be an int32 tensor [rows, n] with contiguous rows")
+    rows, width = block_tables.shape
+    if rows > 1 << 20 or tokens * heads >= 1 << 31:
+        raise ValueError("more than 2^20 rows, or 2^31 heads of all tokens")
+    if width * page_size > 1 << 30:
+        raise ValueError("block_tables of more than 2^30 tokens a row")
+    _index("lengths", lengths, rows, torch.int32)
+    if starts is not None:
+        _index("starts", starts, rows + 1, torch.int32)
+    elif tokens != rows:
+        raise ValueError(f"q holds {tokens} tokens of {rows} rows: starts says whose they are")
+    if (groups is None) != (prefixes is None):
+        raise ValueError("groups and prefixes come together")
+    ngroups = 0 if prefixes is None else prefixes.numel()
+    if ngroups > MAX_GROUPS:
+        raise ValueError(f"more than {MAX_GROUPS} groups")
+    if prefixes is not None:
+        _index("prefixes", prefixes, ngroups, torch.int32)
+        _index("groups", groups, ngroups + 1, torch.int32)
+    if out is None:
+        out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=q.device)
+    else:
+        _heads("out", out, q)
+        if out.shape != q.shape:
+            raise ValueError("out must have q's shape")
+        _writable("out", out)
+        _apart("out", out, q, k_pages, v_pages, block_tables, lengths, starts, groups, prefixes)
+    if tokens == 0:
+        return out
+    need = _prefix_bytes(tokens, rows, ngroups, heads, kv_heads, dim)
+    space = _parts_space(q.device, need)
+    ks, vs = k_pages.stride(), v_pages.stride()
+    at = lambda t: 0 if t is None else t.data_ptr()
+    args = _PREFIX.pack(
+        _PREFIX.size, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), block_tables.data_ptr(), lengths.data_ptr(), at(starts), at(groups),
+        at(prefixes), out.data_ptr(), space.work_at, _status(q.get_device()), need, pages, _stride(q, 0), _stride(q, 1),
+        ks[0] if pages > 1 else 0, ks[1] if kv_heads > 1 else 0, ks[2], vs[0] if pages > 1 else 0, vs[1] if kv_heads > 1 else 0, vs[2],
+        _stride(out, 0), _stride(out, 1), block_tables.stride(0) if rows > 1 else 0, tokens, rows, ngroups, heads, kv_heads, dim, page_size, width,
+        _TYPES[q.dtype], dim ** -0.5 if scale is None else scale)
+    _lib.check(_lib.lib().dz_prefix_attention(args, ops._stream()), "dz_prefix_attention")
+    return out
+
+
+class TableStep(NamedTuple):
+    """What `extend_tables` makes: rows' lengths (int32 [rows]) and the pages taken (int32 [1]) after it, where each row's new tokens
+    begin (int32 [rows + 1]), and every new token's position and slot (int64)."""
+    lengths: torch.Tensor
+    taken: torch.Tensor
+    starts: torch.Tensor
+    positions: torch.Tensor
+    slots: torch.Tensor
+
+
+def extend_tables(block_tables: torch.Tensor, lengths: torch.Tensor, counts: torch.Tensor, free_pages: torch.Tensor, taken: torch.Tensor,
+                  page_size: int, tokens: Optional[int] = None, out: Optional[TableStep] = None) -> TableStep:
+    """Room for the tokens that rows get next, made on the device: what `PagedKVCache.extend` and `batch` do on the host.
+
+    Row r has lengths[r] tokens and gets counts[r] more (int32 [rows]); the pages that it needs for them are the next of
+    free_pages (int32 [n]) behind the first taken[0] (int32 [1]), in the order of the rows, and are written into its row of block_tables
+    (int32 [rows, n], in place; a page that is partly filled is filled up first).  Returns the new lengths and pages taken, and for
+    every new token its position and its slot, as `append_kv` takes them.
+
+    tokens: the call's places (up to 2^24); the rows' new tokens follow each other, row r's from starts[r] on, as `prefix_attention`
+    takes them, and what is left over has position 0 and slot -1.  None: a place a row, counts are 0 or 1, and row r's
+    token is token r (position 0 and slot -1 where it has none).
+
+    All or nothing: where the pages, a row's table or the places are too few, or a length or count is negative, nothing is changed,
+    starts are 0 and all slots -1, and the status word says so.  out: a result to write over; its lengths and taken may be the inputs (a captured call then goes
+    one step on with every replay)."""
+    ops._need_cuda(block_tables, lengths, counts, free_pages, taken, *(out or ()))
+    if _elsewhere(block_tables):
+        with torch.cuda.device(block_tables.device):
+            return extend_tables(block_tables, lengths, counts, free_pages, taken, page_size, tokens, out)
+    _same_place(block_tables, lengths, counts, free_pages, taken, *(out or ()))
+    if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or (block_tables.shape[1] > 1 and block_tables.stride(1) != 1):
+        raise ValueError("block_tables must be an int32 tensor [rows, n] with contiguous rows")
+    rows, width = block_tables.shape
+    _writable("block_tables", block_tables)
+    if rows > 1 << 20:
+        raise ValueError("more than 2^20 rows")
+    if page_size < 8 or page_size > 1024 or page_size & (page_size - 1):
+        raise ValueError("a page must hold a power of two of tokens, from 8 to 1024")
+    if width * page_size > 1 << 30:
+        raise ValueError("block_tables of more than 2^30 tokens a row")
+    _index("lengths", lengths, rows, torch.int32)
+    _index("counts", counts, rows, torch.int32)
+    _index("free_pages", free_pages, free_pages.numel(), torch.int32)
+    _index("taken", taken, 1, torch.int32)
+    if free_pages.numel() >= 1 << 31:
+        raise ValueError("free_pages of 2^31 pages or more")
+    packed = tokens is not None
+    tokens = rows if tokens is None else int(tokens)
+    if not 0 <= tokens <= 1 << 24:
+        raise ValueError("tokens must be 0 to 2^24")
+    read = (counts, free_pages, block_tables)
+    if out is None:
+        dev = block_tables.device
+        both = torch.empty((2, tokens), dtype=torch.int64, device=dev)
+        rest = torch.empty(2 * rows + 2, dtype=torch.int32, device=dev)
+        out = TableStep(rest[:rows], rest[rows:rows + 1], rest[rows + 1:], both[0], both[1])
+    else:
+        for name, t, n, dtype in zip(TableStep._fields, out, (rows, 1, rows + 1, tokens, tokens), (torch.int32,) * 3 + (torch.int64,) * 2):
+            _index(f"out.{name}", t, n, dtype)
+        for i, t in enumerate(out):
+            _apart(f"out.{TableStep._fields[i]}", t, *read, *out[:i], None if i == 0 and _itself(t, lengths) else lengths,
+                   None if i == 1 and _itself(t, taken) else taken)
+    _apart("block_tables", block_tables, lengths, counts, free_pages, taken)
+    args = _EXTEND.pack(
+        _EXTEND.size, block_tables.data_ptr(), lengths.data_ptr(), counts.data_ptr(), free_pages.data_ptr(), taken.data_ptr(), out.lengths.data_ptr(),
+        out.taken.data_ptr(), out.starts.data_ptr(), out.positions.data_ptr(), out.slots.data_ptr(), _status(block_tables.get_device()),
+        block_tables.stride(0) if rows > 1 else 0, rows, width, page_size, free_pages.numel(), tokens, int(packed))
+    _lib.check(_lib.lib().dz_extend_tables(args, ops._stream()), "dz_extend_tables")
     return out
 
 

@@ -60,6 +60,7 @@ extern "C" {
 #define DZ_F16  0                 /* element types of the operators on a paged cache */
 #define DZ_BF16 1
 #define DZ_ATTENTION_COUNTERS 32768
+#define DZ_PREFIX_GROUPS 2048     /* most groups of rows that dz_prefix_attention takes */
 
 /* Library version (major*10000 + minor*100 + patch). */
 int dz_version(void);
@@ -504,6 +505,56 @@ typedef struct dz_attention_args {
 
 size_t dz_paged_attention_bytes(int rows, int heads, int kv_heads, int dim, int page_size, int pages_per_row);
 int dz_paged_attention(const dz_attention_args* args, void* stream);
+
+/* The new tokens of every row over the tokens up to each, several of a row and prefixes that rows share taken at once:
+ *   out[t, h] = softmax_u(scale q[t, h] . k[u, h / (heads / kv_heads)]) v[u, ...],  u < n - (c - 1 - i)
+ * for token t = starts[r] + i of the c = starts[r + 1] - starts[r] new ones of row r with n = lengths[r] tokens; starts NULL: one
+ * of each row (tokens = rows).  Rows groups[g] .. groups[g + 1] - 1 have their first prefixes[g] tokens in common (cut to what
+ * the first new token of each sees), which are read through the table of the first of them that has tokens.  groups_n 0: nothing is shared.
+ * Tokens of no row, and those that see nothing, give zeros; lengths, tables and pages as in dz_paged_attention.  Starts that do
+ * not rise from 0 or more to `tokens` or less leave no row any token, groups that do not rise within the rows share nothing; either
+ * sets bit 2 of *status.  work: dz_prefix_attention_bytes() bytes, any contents, that no call overlapping in time uses.  rows <= 2^20,
+ * groups_n <= DZ_PREFIX_GROUPS, tokens * heads < 2^31. */
+typedef struct dz_prefix_args {
+  int64_t bytes;
+  const void *q, *k_pages, *v_pages;      /* q [tokens, heads, dim]; pages [num_pages, kv_heads, page_size, dim] */
+  const int32_t *tables, *lengths;        /* [rows, pages_per_row], [rows] */
+  const int32_t *starts;                  /* [rows + 1] or NULL */
+  const int32_t *groups, *prefixes;       /* [groups_n + 1], [groups_n] */
+  void *out;                              /* [tokens, heads, dim] */
+  void *work;
+  uint32_t *status;
+  int64_t work_bytes, num_pages;
+  int64_t q_row, q_head, k_page, k_head, k_token, v_page, v_head, v_token, out_row, out_head, table_row;
+  int32_t tokens, rows, groups_n, heads, kv_heads, dim, page_size, pages_per_row, dtype;
+  float scale;
+} dz_prefix_args;
+
+size_t dz_prefix_attention_bytes(int tokens, int rows, int groups_n, int heads, int kv_heads, int dim);
+int dz_prefix_attention(const dz_prefix_args* args, void* stream);
+
+/* Room for the tokens that rows get next.  Row r has lengths[r] tokens and gets counts[r] more: the pages that it needs for them are
+ * free_pages[*taken], free_pages[*taken + 1], ... in the order of the rows, written into its table (what it had, the last page
+ * partly filled, stays).  lengths_out = lengths + counts, *taken_out = *taken + the pages given (either may be its input), and for token i of
+ * row r's new ones, positions[t] = lengths[r] + i and slots[t] = its place in the pages, page * page_size + place.  packed != 0: the
+ * tokens follow each other, t = starts[r] + i with starts [rows + 1] the sums of counts in front of each row; else t = r,
+ * starts[r] = r, tokens = rows and counts are 0 or 1.  Places of no token have position 0 and slot -1.
+ * All or nothing: where a length or count is below 0, a row outgrows its table, the counts are more than `tokens` (<= 2^24) or the
+ * pages more than free_n, all places are of no token, starts are 0, lengths, *taken and tables what they were, and bit 2 of
+ * *status is set.  A page below 0 gives the slot -1 and sets it, too. */
+typedef struct dz_extend_args {
+  int64_t bytes;
+  int32_t *tables;                        /* [rows, pages_per_row], rows every table_row */
+  const int32_t *lengths, *counts;        /* [rows] */
+  const int32_t *free_pages, *taken;      /* [free_n], [1] */
+  int32_t *lengths_out, *taken_out, *starts;
+  int64_t *positions, *slots;             /* [tokens] */
+  uint32_t *status;
+  int64_t table_row;
+  int32_t rows, pages_per_row, page_size, free_n, tokens, packed;
+} dz_extend_args;
+
+int dz_extend_tables(const dz_extend_args* args, void* stream);
 
 /* A status word for the operators on a paged cache, on the current device: memory of the library's, for the life of the process
  * (NULL: no device).  dz_take_page_status writes what is there to `to` (memory that the device can write, pinned host memory for

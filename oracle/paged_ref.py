@@ -58,3 +58,61 @@ def attention_bound(want, size, most, dtype, dim, tokens):
     half = torch.finfo(dtype).eps / 2
     weight = 2 * ((dim + 4) * 2.0 ** -24 * most + 2.0 ** -21 + tokens * 2.0 ** -24) + half ** 2
     return half * want.abs() + size * weight[..., None] * (1 + half) + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+
+
+def tokens_as_rows(starts, lengths, tables, groups=None, prefixes=None, page_size=None):
+    """(rows, lengths, tables) of the new tokens of a batch as rows of one token each: what `attention` above takes.  A row with a prefix reads it through
+    the table of the first row of its group that has tokens."""
+    starts, lengths, tables = [int(x) for x in starts], [int(n) for n in lengths], tables.cpu().clone()
+    if groups is not None:
+        for g, prefix in enumerate(prefixes.tolist()):
+            rows = [r for r in range(int(groups[g]), int(groups[g + 1])) if lengths[r] > 0 and starts[r + 1] > starts[r]]
+            for r in rows:
+                # as far as the first new token of each sees; a page that the prefix ends in is shared as a whole only where it is the same page
+                cut = max(0, min([prefix] + [lengths[x] - (starts[x + 1] - starts[x]) + 1 for x in rows]))
+                tables[r, :cut // page_size] = tables[rows[0], :cut // page_size]
+    row, length = [], []
+    for r, n in enumerate(lengths):
+        c = starts[r + 1] - starts[r]
+        for i in range(c):
+            row.append(r)
+            length.append(max(0, n - (c - 1 - i)) if n > 0 else 0)
+    return row, torch.tensor(length, dtype=torch.int64), tables[row] if row else tables[:0]
+
+
+def prefix_bound(want, size, most, dtype, dim, tokens, largest):
+    """attention_bound for weights that are rounded to the type, as 2^(s - m + 14) in float16, which keeps those above 2^-28 of the
+    largest to half a step and of the others all but 2^-39 each."""
+    half = torch.finfo(dtype).eps / 2
+    lost = tokens * 2.0 ** -39 * largest if dtype == torch.float16 else 0.0
+    return attention_bound(want, size, most, dtype, dim, tokens) + half * (1 + half) * size + lost
+
+
+def extend_tables(tables, lengths, counts, free, taken, page_size, tokens=None):
+    """Token by token; None where something does not fit.  (tables, lengths, taken, starts, positions, slots) as lists."""
+    tables = [list(map(int, row)) for row in tables]
+    width = len(tables[0]) if tables else 0
+    packed = tokens is not None
+    if any(n < 0 or c < 0 or n + c > width * page_size or (not packed and c > 1) for n, c in zip(lengths, counts)):
+        return None
+    if taken < 0 or (packed and sum(counts) > tokens):
+        return None
+    starts, positions, slots = [], [], []
+    for r, (n, c) in enumerate(zip(lengths, counts)):
+        starts.append(len(positions))
+        for t in range(n, n + c):
+            if t % page_size == 0:
+                if taken >= len(free):
+                    return None
+                tables[r][t // page_size] = int(free[taken])
+                taken += 1
+            positions.append(t)
+            slots.append(tables[r][t // page_size] * page_size + t % page_size)
+        if not packed and c == 0:
+            positions.append(0)
+            slots.append(-1)
+    starts.append(len(positions))
+    if packed:
+        positions += [0] * (tokens - len(positions))
+        slots += [-1] * (tokens - len(slots))
+    return tables, [n + c for n, c in zip(lengths, counts)], taken, starts, positions, slots
