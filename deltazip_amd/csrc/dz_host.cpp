@@ -37,6 +37,11 @@ bool pages_on(const at::Tensor& t, const at::Tensor& q, int dev) {
 bool index_on(const at::Tensor& t, int64_t n, at::ScalarType type, int dev) {
   return t.dim() == 1 && t.size(0) == n && t.scalar_type() == type && t.is_cuda() && t.get_device() == dev && (n < 2 || t.stride(0) == 1);
 }
+// int32 [rows, pages], pages of a row side by side
+bool tables_on(const at::Tensor& t, int dev) {
+  return t.dim() == 2 && t.scalar_type() == at::kInt && t.is_cuda() && t.get_device() == dev && t.size(0) >= 1 && t.size(0) <= (1 << 20) && t.size(1) >= 1 &&
+         t.size(1) <= (1 << 27) && (t.size(1) == 1 || t.stride(1) == 1);
+}
 bool floats(at::ScalarType t) { return t == at::kHalf || t == at::kBFloat16; }
 
 // Whether [n, heads, dim] tensors of one type share nothing: by their ends, or, with rows of one stride (slices of a
@@ -110,9 +115,7 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!floats(q->scalar_type()) || !heads_on(*q, q->scalar_type(), dev) || !pages_on(*k, *q, dev) || !pages_on(*v, *q, dev)) Py_RETURN_NONE;
   const int64_t rows = q->size(0), heads = q->size(1), dim = q->size(2), kv_heads = k->size(1), ps = k->size(2);
   if (rows < 1 || rows > (1 << 20) || heads < 1 || heads > 4096 || heads % kv_heads || dim % 8 || dim > 256 || v->sizes() != k->sizes()) Py_RETURN_NONE;
-  if (tables->dim() != 2 || tables->scalar_type() != at::kInt || !tables->is_cuda() || tables->get_device() != dev || tables->size(0) != rows ||
-      tables->size(1) < 1 || tables->size(1) > (1 << 27) || tables->size(1) * ps > (1ll << 30) || (tables->size(1) > 1 && tables->stride(1) != 1))
-    Py_RETURN_NONE;
+  if (!tables_on(*tables, dev) || tables->size(0) != rows || tables->size(1) * ps > (1ll << 30)) Py_RETURN_NONE;
   if (!index_on(*lengths, rows, at::kInt, dev)) Py_RETURN_NONE;
   const int width = (int)tables->size(1);
   const size_t need = dz_paged_attention_bytes((int)rows, (int)heads, (int)kv_heads, (int)dim, (int)ps, width);
@@ -144,6 +147,107 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Py_END_ALLOW_THREADS
   if (rc) Py_RETURN_NONE;
   return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// prefix(q, k_pages, v_pages, tables, lengths, starts, groups, prefixes (None: there are none), scale or None)
+PyObject* prefix(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 9) Py_RETURN_NONE;
+  const at::Tensor *q = tensor(a[0]), *k = tensor(a[1]), *v = tensor(a[2]), *tables = tensor(a[3]), *lengths = tensor(a[4]);
+  if (!q || !k || !v || !tables || !lengths || !(a[8] == Py_None || PyFloat_CheckExact(a[8])) || !q->is_cuda()) Py_RETURN_NONE;
+  const at::Tensor *starts = tensor(a[5]), *groups = tensor(a[6]), *prefixes = tensor(a[7]);
+  if ((!starts && a[5] != Py_None) || (!groups && a[6] != Py_None) || (!prefixes && a[7] != Py_None) || !groups != !prefixes) Py_RETURN_NONE;
+  const Place here;
+  const int dev = here.dev;
+  if (!here.status) Py_RETURN_NONE;
+  if (!floats(q->scalar_type()) || !heads_on(*q, q->scalar_type(), dev) || !pages_on(*k, *q, dev) || !pages_on(*v, *q, dev) || v->sizes() != k->sizes()) Py_RETURN_NONE;
+  const int64_t tokens = q->size(0), heads = q->size(1), dim = q->size(2), kv_heads = k->size(1), ps = k->size(2);
+  if (!tables_on(*tables, dev)) Py_RETURN_NONE;
+  const int64_t rows = tables->size(0), width = tables->size(1), ngroups = prefixes ? prefixes->numel() : 0;
+  if (tokens < 1 || heads < 1 || heads > 4096 || heads % kv_heads || tokens * heads >= (1ll << 31) || dim % 8 || dim > 256 || width * ps > (1ll << 30) ||
+      (!starts && tokens != rows) || ngroups > DZ_PREFIX_GROUPS)
+    Py_RETURN_NONE;
+  if (!index_on(*lengths, rows, at::kInt, dev) || (starts && !index_on(*starts, rows + 1, at::kInt, dev)) ||
+      (prefixes && (!index_on(*prefixes, ngroups, at::kInt, dev) || !index_on(*groups, ngroups + 1, at::kInt, dev))))
+    Py_RETURN_NONE;
+  const size_t need = dz_prefix_attention_bytes((int)tokens, (int)rows, (int)ngroups, (int)heads, (int)kv_heads, (int)dim);
+  if (!need || dz_capture_id(here.stream)) Py_RETURN_NONE;       // (a graph has its own room)
+  const Space space = space_of(here, need, *q);
+  at::Tensor out = at::empty({tokens, heads, dim}, q->options());
+  dz_prefix_args c{};
+  c.bytes = sizeof(c);
+  c.q = q->data_ptr(), c.k_pages = k->data_ptr(), c.v_pages = v->data_ptr();
+  c.tables = (const int32_t*)tables->data_ptr(), c.lengths = (const int32_t*)lengths->data_ptr();
+  c.starts = starts ? (const int32_t*)starts->data_ptr() : nullptr;
+  if (ngroups) c.groups = (const int32_t*)groups->data_ptr(), c.prefixes = (const int32_t*)prefixes->data_ptr();
+  c.out = out.data_ptr(), c.work = space.work.data_ptr(), c.status = here.status;
+  c.work_bytes = (int64_t)need, c.num_pages = k->size(0);
+  c.q_row = step(*q, 0), c.q_head = step(*q, 1);
+  c.k_page = step(*k, 0), c.k_head = step(*k, 1), c.k_token = k->stride(2);
+  c.v_page = step(*v, 0), c.v_head = step(*v, 1), c.v_token = v->stride(2);
+  c.out_row = heads * dim, c.out_head = dim, c.table_row = step(*tables, 0);
+  c.tokens = (int)tokens, c.rows = (int)rows, c.groups_n = (int)ngroups, c.heads = (int)heads, c.kv_heads = (int)kv_heads, c.dim = (int)dim;
+  c.page_size = (int)ps, c.pages_per_row = (int)width, c.dtype = q->scalar_type() == at::kBFloat16 ? DZ_BF16 : DZ_F16;
+  c.scale = a[8] == Py_None ? (float)(1.0 / std::sqrt((double)dim)) : (float)PyFloat_AS_DOUBLE(a[8]);
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = dz_prefix_attention(&c, here.stream);
+  Py_END_ALLOW_THREADS
+  if (rc) Py_RETURN_NONE;
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// A piece of a tensor's memory as a tensor.
+at::Tensor piece_of(const at::Tensor& t, int64_t from, int64_t n) {
+  at::Tensor y = at::detail::make_tensor<c10::TensorImpl>(c10::TensorImpl::VIEW, c10::Storage(t.storage()), t.key_set(), t.dtype());
+  y.unsafeGetTensorImpl()->set_storage_offset(from);
+  y.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+  return y;
+}
+
+// extend(tables, lengths, counts, free_pages, taken, page_size, tokens or None): (lengths, taken, starts, positions, slots)
+PyObject* extend(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 7) Py_RETURN_NONE;
+  const at::Tensor *tables = tensor(a[0]), *lengths = tensor(a[1]), *counts = tensor(a[2]), *free = tensor(a[3]), *taken = tensor(a[4]);
+  if (!tables || !lengths || !counts || !free || !taken || !PyLong_CheckExact(a[5]) || !(a[6] == Py_None || PyLong_CheckExact(a[6])) || !tables->is_cuda()) Py_RETURN_NONE;
+  const Place here;
+  const int dev = here.dev;
+  if (!here.status || !tables_on(*tables, dev)) Py_RETURN_NONE;
+  int overflow = 0;
+  const long ps = PyLong_AsLongAndOverflow(a[5], &overflow);
+  if (overflow || ps < 8 || ps > 1024 || (ps & (ps - 1))) Py_RETURN_NONE;
+  const int64_t rows = tables->size(0), width = tables->size(1), pages = free->numel();
+  const long tokens = a[6] == Py_None ? rows : PyLong_AsLongAndOverflow(a[6], &overflow);
+  if (overflow || tokens < 0 || tokens > (1 << 24) || width * ps > (1ll << 30) || (rows > 1 && tables->stride(0) < width)) Py_RETURN_NONE;
+  if (!index_on(*lengths, rows, at::kInt, dev) || !index_on(*counts, rows, at::kInt, dev) || pages > 0x7fffffff || !index_on(*free, pages, at::kInt, dev) ||
+      !index_on(*taken, 1, at::kInt, dev))
+    Py_RETURN_NONE;
+  if (!ends_apart(*tables, *lengths) || !ends_apart(*tables, *counts) || !ends_apart(*tables, *free) || !ends_apart(*tables, *taken)) Py_RETURN_NONE;
+  const at::Tensor both = at::empty({2 * tokens}, tables->options().dtype(at::kLong)), rest = at::empty({2 * rows + 2}, tables->options());
+  dz_extend_args c{};
+  c.bytes = sizeof(c);
+  c.tables = (int32_t*)tables->data_ptr(), c.lengths = (const int32_t*)lengths->data_ptr(), c.counts = (const int32_t*)counts->data_ptr();
+  c.free_pages = (const int32_t*)free->data_ptr(), c.taken = (const int32_t*)taken->data_ptr();
+  c.lengths_out = (int32_t*)rest.data_ptr(), c.taken_out = c.lengths_out + rows, c.starts = c.taken_out + 1;
+  c.positions = (int64_t*)both.data_ptr(), c.slots = c.positions + tokens, c.status = here.status;
+  c.table_row = step(*tables, 0);
+  c.rows = (int)rows, c.pages_per_row = (int)width, c.page_size = (int)ps, c.free_n = (int)pages, c.tokens = (int)tokens, c.packed = a[6] != Py_None;
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = dz_extend_tables(&c, here.stream);
+  Py_END_ALLOW_THREADS
+  if (rc) Py_RETURN_NONE;
+  PyObject* made = PyTuple_New(5);
+  if (!made) return nullptr;
+  PyTuple_SET_ITEM(made, 0, THPVariable_Wrap(piece_of(rest, 0, rows)));
+  PyTuple_SET_ITEM(made, 1, THPVariable_Wrap(piece_of(rest, rows, 1)));
+  PyTuple_SET_ITEM(made, 2, THPVariable_Wrap(piece_of(rest, rows + 1, rows + 1)));
+  PyTuple_SET_ITEM(made, 3, THPVariable_Wrap(piece_of(both, 0, tokens)));
+  PyTuple_SET_ITEM(made, 4, THPVariable_Wrap(piece_of(both, tokens, tokens)));
+  return made;
   END_HANDLE_TH_ERRORS
 }
 
@@ -285,6 +389,8 @@ PyObject* copy(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 PyMethodDef methods[] = {{"arm", (PyCFunction)(void (*)(void))arm, METH_FASTCALL, nullptr},
                          {"attend", (PyCFunction)(void (*)(void))attend, METH_FASTCALL, nullptr},
+                         {"prefix", (PyCFunction)(void (*)(void))prefix, METH_FASTCALL, nullptr},
+                         {"extend", (PyCFunction)(void (*)(void))extend, METH_FASTCALL, nullptr},
                          {"rotate", (PyCFunction)(void (*)(void))rotate, METH_FASTCALL, nullptr},
                          {"copy", (PyCFunction)(void (*)(void))copy, METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};

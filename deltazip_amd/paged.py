@@ -360,6 +360,10 @@ def prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     that do not rise within the rows share nothing; these, lengths beyond the tables and page numbers outside the pool are reported through the
     status word.  The weights of 17 and more queries a key (tokens times heads that share one) are rounded to q's type, as their products with the values take
     them.  The same call gives the same bits; they depend on the lengths of all of its rows."""
+    if out is None:
+        made = _lib.host().prefix(q, k_pages, v_pages, block_tables, lengths, starts, groups, prefixes, scale)
+        if made is not None:
+            return made
     ops._need_cuda(q, k_pages, v_pages, block_tables, lengths, starts, groups, prefixes, out)
     if _elsewhere(q):
         with torch.cuda.device(q.device):
@@ -444,6 +448,10 @@ def extend_tables(block_tables: torch.Tensor, lengths: torch.Tensor, counts: tor
     All or nothing: where the pages, a row's table or the places are too few, or a length or count is negative, nothing is changed,
     starts are 0 and all slots -1, and the status word says so.  out: a result to write over; its lengths and taken may be the inputs (a captured call then goes
     one step on with every replay)."""
+    if out is None:
+        made = _lib.host().extend(block_tables, lengths, counts, free_pages, taken, page_size, tokens)
+        if made is not None:
+            return TableStep(*made)
     ops._need_cuda(block_tables, lengths, counts, free_pages, taken, *(out or ()))
     if _elsewhere(block_tables):
         with torch.cuda.device(block_tables.device):
