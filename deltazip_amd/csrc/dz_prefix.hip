@@ -55,7 +55,7 @@ struct PrefixParams {
   long long q_row, q_head, k_page, k_head, k_token, v_page, v_head, v_token, out_row, out_head, table_row;   // bytes; out, table: elements
   long long room_parts;
   unsigned num_pages;
-  int tokens, rows, ngroups, heads, kv_heads, share, dim, shift, pages_per_row, room_items;
+  int tokens, rows, ngroups, heads, kv_heads, share, dim, shift, pages_per_row, room_items, near;
   float scale;
 };
 
@@ -270,16 +270,22 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void dz_prefix_kernel(const P
     for (int i = threadIdx.x; i < 2 * STAGE / 16; i += 256) *(u4_t*)(lds + 16 * i) = u4_t{0, 0, 0, 0};
     __syncthreads();
   }
-  // a wavefront brings in 16 tokens of each step; request i of a lane is for token 16 wave + (64 i + lane) / (4 KC)
+  // a wavefront brings in 16 tokens of each step; request i of a lane is for token (64 i + lane) / (4 KC) of them
   int req_token[KC], req_at[KC];
+  unsigned req_k[KC], req_v[KC];       // bytes from the first of the 16 in their page
 #pragma unroll
   for (int i = 0; i < KC; ++i) {
     const int at = 64 * i + lane;
     req_token[i] = at / (4 * KC);
     const int c = at % (4 * KC) ^ swizzled<KC>(req_token[i]);
     req_at[i] = FULL || c < per_row ? 16 * c : -1;
+    req_k[i] = req_token[i] * (unsigned)P.k_token + 16 * c;
+    req_v[i] = req_token[i] * (unsigned)P.v_token + 16 * c;
   }
-  auto issue = [&](int s, int buf) {
+  auto bring = [&](const char* from, char* to) __attribute__((always_inline)) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+  };
+  auto issue = [&](int s, int buf) __attribute__((always_inline)) {
     if (((min(s + STEP, hi) - 1) >> P.shift) >= page0 + 64) {
       ids = next_ids;
       page0 += 64;
@@ -287,15 +293,25 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void dz_prefix_kernel(const P
     }
     char* to = lds + buf * STAGE + wave * 16 * ROW;
     const int t0 = s + 16 * wave;
+    if (P.near && t0 + 16 <= hi) {     // all of one page: its place is the wavefront's
+      const long long id = __builtin_amdgcn_readlane(ids, (t0 >> P.shift) - page0);
+      const char* k = P.k + id * P.k_page + kvh * P.k_head + (t0 & in_page) * P.k_token;
+      const char* v = P.v + id * P.v_page + kvh * P.v_head + (t0 & in_page) * P.v_token;
 #pragma unroll
-    for (int i = 0; i < KC; ++i) {
-      const int t = min(t0 + req_token[i], hi - 1);        // (behind the end: the last one again)
-      const unsigned id = __shfl(ids, (t >> P.shift) - page0);
-      const char* k = P.k + id * P.k_page + kvh * P.k_head + (t & in_page) * P.k_token + req_at[i];
-      const char* v = P.v + id * P.v_page + kvh * P.v_head + (t & in_page) * P.v_token + req_at[i];
-      if (FULL || req_at[i] >= 0) {
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)k, (__attribute__((address_space(3))) void*)(to + i * 1024), 16, 0, 0);
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)v, (__attribute__((address_space(3))) void*)(to + HALF + i * 1024), 16, 0, 0);
+      for (int i = 0; i < KC; ++i)
+        if (FULL || req_at[i] >= 0) {
+          bring(k + req_k[i], to + i * 1024);
+          bring(v + req_v[i], to + HALF + i * 1024);
+        }
+    } else {
+#pragma unroll
+      for (int i = 0; i < KC; ++i) {
+        const int t = min(t0 + req_token[i], hi - 1);      // (behind the end: the last one again)
+        const unsigned id = __shfl(ids, (t >> P.shift) - page0);
+        if (FULL || req_at[i] >= 0) {
+          bring(P.k + id * P.k_page + kvh * P.k_head + (t & in_page) * P.k_token + req_at[i], to + i * 1024);
+          bring(P.v + id * P.v_page + kvh * P.v_head + (t & in_page) * P.v_token + req_at[i], to + HALF + i * 1024);
+        }
       }
     }
   };
@@ -309,6 +325,7 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void dz_prefix_kernel(const P
     int lim[NC];
     f4_t acc[NC][2 * KC];
     float top[NC], sum[NC];
+    const float scale = fabsf(P.scale);
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
       const int x = mine + 16 * n + col, xx = x0 + min(x, in_tile - 1);
@@ -318,6 +335,10 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void dz_prefix_kernel(const P
         u4_t w = {0, 0, 0, 0};
         if (x < in_tile && (FULL || 32 * c + 8 * g < P.dim)) w = *(const u4_t*)(P.q + token * P.q_row + head * P.q_head + (32 * c + 8 * g) * 2);
         q[n][c] = __builtin_bit_cast(v8, w);
+      }
+      if (P.scale < 0.0f) {            // (the largest score is that of the largest product)
+#pragma unroll
+        for (int c = 0; c < KC; ++c) q[n][c] = -q[n][c];
       }
       lim[n] = min(limit_of(xx), hi);
       top[n] = -INFINITY, sum[n] = 0.0f;
@@ -331,28 +352,40 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void dz_prefix_kernel(const P
       const char* keys = at + col * ROW;
       const int turn_k = swizzled<KC>(col);
       f4_t sc[NC][4];
+      v8 kw[2][KC];
+      auto load_keys = [&](int a) __attribute__((always_inline)) {
+#pragma unroll
+        for (int c = 0; c < KC; ++c) kw[a & 1][c] = *(const v8*)(keys + a * 16 * ROW + ((4 * c + g) ^ turn_k) * 16);
+      };
+      load_keys(0);
 #pragma unroll
       for (int a = 0; a < 4; ++a) {
-        v8 kw[KC];
+        if (a < 3) load_keys(a + 1);
 #pragma unroll
-        for (int c = 0; c < KC; ++c) kw[c] = *(const v8*)(keys + a * 16 * ROW + ((4 * c + g) ^ turn_k) * 16);
+        for (int n = 0; n < NC; ++n) sc[n][a] = f4_t{0, 0, 0, 0};
 #pragma unroll
-        for (int n = 0; n < NC; ++n) {
-          f4_t c4 = {0, 0, 0, 0};
+        for (int c = 0; c < KC; ++c)
 #pragma unroll
-          for (int c = 0; c < KC; ++c) c4 = Ty::mma(kw[c], q[n][c], c4);
-          sc[n][a] = c4 * P.scale;
-        }
+          for (int n = 0; n < NC; ++n) sc[n][a] = Ty::mma(kw[a & 1][c], q[n][c], sc[n][a]);
+        __builtin_amdgcn_sched_barrier(0);
       }
+      // a transposing read: lanes of a row of 16 name 4 tokens' 16 dims, and each gets one dim of the four
+      const char* values = at + HALF + (4 * g + (col >> 2)) * ROW + (col & 1) * 8;
+      const int turn_v = swizzled<KC>(4 * g + (col >> 2));
+      s8_t vw[2][4];                   // of two groups of 32 dims, for 2 x 32 tokens each
+      auto load_values = [&](int jj) __attribute__((always_inline)) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int j = 2 * jj + (x >> 1), h = x & 1;
+          const char* from = values + 2 * h * 16 * ROW + ((2 * j + (col >> 1 & 1)) ^ turn_v) * 16;
+          const s4_t a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4_t*)from);
+          const s4_t a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4_t*)(from + 16 * ROW));
+          vw[jj & 1][x] = s8_t{a0[0], a0[1], a0[2], a0[3], a1[0], a1[1], a1[2], a1[3]};
+        }
+      };
       bool spoilt = false;             // values that are not finite, where some queries do not see all tokens
+      auto hidden = [&](int n, int e) { return s + 16 * (e >> 2) + 4 * g + (e & 3) >= lim[n] || s + 16 * (e >> 2) + 4 * g + (e & 3) < lo; };
       if (edge) {
-#pragma unroll
-        for (int n = 0; n < NC; ++n)
-#pragma unroll
-          for (int a = 0; a < 4; ++a)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (s + 16 * a + 4 * g + i >= lim[n] || s + 16 * a + 4 * g + i < lo) sc[n][a][i] = -INFINITY;
         unsigned found = 0;
 #pragma unroll 4
         for (int i = lane; i < HALF / 16; i += 64) {
@@ -361,13 +394,20 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void dz_prefix_kernel(const P
           for (int e = 0; e < 4; ++e) found |= (w[e] & (BAD | BAD << 16)) + ((0x8000u - BAD) | (0x8000u - BAD) << 16);
         }
         spoilt = __any(found & 0x80008000u);
+#pragma unroll
+        for (int n = 0; n < NC; ++n)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (hidden(n, e)) sc[n][e >> 2][e & 3] = -INFINITY;
       }
+      load_values(0);
       v8 p[NC][2];
 #pragma unroll
       for (int n = 0; n < NC; ++n) {
         float most = sc[n][0][0];
 #pragma unroll
         for (int e = 1; e < 16; ++e) most = fmaxf(most, sc[n][e >> 2][e & 3]);
+        most *= scale;
         // the reference moves only where a score is more than twice above it
         if (__any(most > top[n] + 1.0f)) {
           most = fmaxf(most, __shfl_xor(most, 16));
@@ -379,42 +419,18 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void dz_prefix_kernel(const P
 #pragma unroll
           for (int j = 0; j < 2 * KC; ++j) acc[n][j] *= f;
         }
-        const float ref = top[n] == -INFINITY ? 0.0f : top[n] - Ty::BIAS;
+        const float ref = top[n] == -INFINITY ? 0.0f : Ty::BIAS - top[n];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const float x = __builtin_amdgcn_exp2f(sc[n][e >> 2][e & 3] - ref);
+          const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][e >> 2][e & 3], scale, ref));
           sum[n] += x;
           p[n][e >> 3][e & 7] = Ty::one(x);
         }
       }
-      // a transposing read: lanes of a row of 16 name 4 tokens' 16 dims, and each gets one dim of the four
-      const char* values = at + HALF + (4 * g + (col >> 2)) * ROW + (col & 1) * 8;
-      const int turn_v = swizzled<KC>(4 * g + (col >> 2));
-      auto product = [&](auto is_spoilt) __attribute__((always_inline)) {
-#pragma unroll
-        for (int j = 0; j < 2 * KC; ++j)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const char* from = values + 2 * h * 16 * ROW + ((2 * j + (col >> 1 & 1)) ^ turn_v) * 16;
-            const s4_t a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4_t*)from);
-            const s4_t a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4_t*)(from + 16 * ROW));
-            s8_t w = {a0[0], a0[1], a0[2], a0[3], a1[0], a1[1], a1[2], a1[3]};
-            if (decltype(is_spoilt)::value) {
-#pragma unroll
-              for (int e = 0; e < 8; ++e)
-                if (((unsigned)w[e] & BAD) == BAD) w[e] = 0;
-            }
-#pragma unroll
-            for (int n = 0; n < NC; ++n) acc[n][j] = Ty::mma(__builtin_bit_cast(v8, w), p[n][h], acc[n][j]);
-          }
-      };
-      if (__builtin_expect(!spoilt, 1)) {
-        product(std::integral_constant<bool, false>());
-      } else {
-        // a weight of 0 would take them to queries that do not see them: left out of the product, and added where they are seen
-        product(std::integral_constant<bool, true>());
+      if (__builtin_expect(spoilt, 0)) {
+        // a weight of 0 would take what is not finite to queries that do not see it: left out of the products, and added where it is seen
         int quad = 4 * g;
-        asm volatile("" : "+v"(quad));   // (addresses of this rare path are not worth registers all along)
+        asm volatile("" : "+v"(quad));                     // (addresses of this rare path are not worth registers all along)
 #pragma unroll 1
         for (int t = 0; t < STEP; ++t)
 #pragma unroll
@@ -424,9 +440,25 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void dz_prefix_kernel(const P
               const uint16_t w = *(const uint16_t*)(at + HALF + t * ROW + ((2 * j + (quad >> 3)) ^ swizzled<KC>(t)) * 16 + ((quad & 7) + i) * 2);
               const float y = BF ? __builtin_bit_cast(float, (unsigned)w << 16) : (float)__builtin_bit_cast(_Float16, w);
 #pragma unroll
-              for (int n = 0; n < NC; ++n)
-                if ((w & BAD) == BAD && s + t < lim[n] && s + t >= lo) acc[n][j][i] += y;
+              for (int n = 0; n < NC; ++n) acc[n][j][i] += (w & BAD) == BAD && s + t < lim[n] && s + t >= lo ? y : 0.0f;
             }
+      }
+#pragma unroll
+      for (int jj = 0; jj < KC; ++jj) {
+        if (jj + 1 < KC) load_values(jj + 1);
+        if (__builtin_expect(spoilt, 0)) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (((unsigned)vw[jj & 1][x][e] & BAD) == BAD) vw[jj & 1][x][e] = 0;
+        }
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+          for (int n = 0; n < NC; ++n)
+            acc[n][2 * jj + (x >> 1)] = Ty::mma(__builtin_bit_cast(v8, vw[jj & 1][x]), p[n][x & 1], acc[n][2 * jj + (x >> 1)]);
+        __builtin_amdgcn_sched_barrier(0);
       }
     };
 
@@ -455,9 +487,10 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void dz_prefix_kernel(const P
       } else {
         uint16_t* to = P.out + (U.tok0 + xx / P.share) * P.out_row + (kvh * P.share + xx % P.share) * P.out_head;
         const bool sees = limit_of(xx) > 0;
+        const float part = 1.0f / sum[n];
 #pragma unroll
         for (int j = 0; j < 2 * KC; ++j) {
-          const f4_t y = sees ? acc[n][j] / sum[n] : f4_t{0, 0, 0, 0};
+          const f4_t y = sees ? acc[n][j] * part : f4_t{0, 0, 0, 0};
           const u2_t w = {(unsigned)Ty::round(y[0]) | (unsigned)Ty::round(y[1]) << 16, (unsigned)Ty::round(y[2]) | (unsigned)Ty::round(y[3]) << 16};
           if (FULL || 16 * j + 4 * g < P.dim) *(u2_t*)(to + 16 * j + 4 * g) = w;
         }
@@ -504,7 +537,7 @@ __global__ __launch_bounds__(256) void dz_prefix_join_kernel(const PrefixParams 
       if (pre.part >= 0) gather(pre);
       if (own.part >= 0) gather(own);
     }
-    const f4_t y = sees ? o / l : f4_t{0, 0, 0, 0};
+    const f4_t y = sees ? o * (1.0f / l) : f4_t{0, 0, 0, 0};
     const u2_t w = {(unsigned)Ty::round(y[0]) | (unsigned)Ty::round(y[1]) << 16, (unsigned)Ty::round(y[2]) | (unsigned)Ty::round(y[3]) << 16};
     *(u2_t*)(P.out + t * P.out_row + h * P.out_head + d) = w;
   }
@@ -595,7 +628,10 @@ int dz_prefix_attention(const dz_prefix_args* a, void* stream) {
   P.num_pages = (unsigned)a->num_pages;
   P.tokens = a->tokens, P.rows = a->rows, P.ngroups = a->groups_n, P.heads = a->heads, P.kv_heads = a->kv_heads, P.share = a->heads / a->kv_heads;
   P.dim = a->dim, P.shift = __builtin_ctz(a->page_size), P.pages_per_row = a->pages_per_row;
-  P.scale = a->scale * 1.44269504088896340736f;
+  // (of nothing: so little that finite products make no difference, and those at minus infinity stay there)
+  P.scale = a->scale == 0.0f ? 1.4e-45f : a->scale * 1.44269504088896340736f;
+  // 16 tokens that a wavefront asks for lie in one page, within 32 bits
+  P.near = a->page_size >= 16 && P.k_token < (1 << 27) && P.v_token < (1 << 27);
   const int kc = chunks_of(a->dim), which = kc * 4 + (a->dim == 32 * kc) * 2 + a->dtype;
   const size_t lds = 2 * (size_t)(8 * kc) * 1024;
   const kernel_t kern = a->dtype == DZ_BF16 ? kernel_for<true>(a->dim) : kernel_for<false>(a->dim);
