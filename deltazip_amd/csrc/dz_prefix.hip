@@ -28,7 +28,6 @@ constexpr int STEP = 64;               // tokens of a step
 constexpr int TARGET = 512;            // pieces that the work is cut into at most, units' last ones apart
 constexpr int LEAST = 256;             // tokens of a piece
 constexpr int GROUPS = DZ_PREFIX_GROUPS;
-constexpr int PLAN = 1024;             // threads of the plan
 
 struct Unit {
   int tok0, ntok;                      // its queries' tokens
@@ -75,8 +74,12 @@ __device__ __forceinline__ int last_upto(const T* at, int n, T x) {
   return lo - 1;
 }
 
+// One workgroup.  KEPT: rows and groups are no more than its threads, and what is known of them stays in LDS: 6.0 -> 3.x us.
+template <int PLAN, bool KEPT>
 __global__ __launch_bounds__(PLAN) void dz_prefix_plan_kernel(const PrefixParams P) {
-  __shared__ int first[GROUPS + 1], cut[GROUPS], leader[GROUPS], alone[GROUPS];      // of groups: rows, prefix, row whose table, tiles apart
+  constexpr int G = KEPT ? PLAN : GROUPS;
+  __shared__ int first[G + 1], cut[G], leader[G], alone[G];      // of groups: rows, prefix, row whose table, tiles apart
+  __shared__ int kept_length[KEPT ? PLAN : 1], kept_start[KEPT ? PLAN + 1 : 1];
   __shared__ int items_to[PLAN];
   __shared__ long long wave_parts[PLAN / 64];
   __shared__ int wave_items[PLAN / 64];
@@ -86,16 +89,15 @@ __global__ __launch_bounds__(PLAN) void dz_prefix_plan_kernel(const PrefixParams
   const int room = P.pages_per_row << P.shift;
   int bad = 0, bad_groups = 0;
   for (int r = tid; r < P.rows; r += PLAN) {
-    if (P.starts) {
-      const int a = P.starts[r], b = P.starts[r + 1];
-      bad |= a < 0 || b < a || b > P.tokens;
-    }
-    if (P.lengths[r] > room) atomicOr(P.status, 4u);
+    const int n = P.lengths[r], a = P.starts ? P.starts[r] : r, b = P.starts ? P.starts[r + 1] : r + 1;
+    bad |= a < 0 || b < a || b > P.tokens;
+    if (n > room) atomicOr(P.status, 4u);
+    if (KEPT) kept_length[r] = max(0, min(n, room)), kept_start[r] = a, kept_start[r + 1] = b;      // (neighbours write the same)
   }
   for (int g = tid; g < P.ngroups; g += PLAN) {
     const int a = P.groups[g], b = P.groups[g + 1];
     bad_groups |= a < 0 || b < a || b > P.rows;
-    first[g] = a, first[g + 1] = b;                       // (neighbours write the same)
+    first[g] = a, first[g + 1] = b;
     cut[g] = min(P.prefixes[g], room);
     leader[g] = P.rows;
     alone[g] = 0;
@@ -104,9 +106,9 @@ __global__ __launch_bounds__(PLAN) void dz_prefix_plan_kernel(const PrefixParams
   bad_groups = __syncthreads_or(bad_groups);
   if ((bad || bad_groups) && tid == 0) atomicOr(P.status, 4u);
   const int rows = bad ? 0 : P.rows, groups = bad || bad_groups ? 0 : P.ngroups;
-  auto count_of = [&](int r) { return P.starts ? P.starts[r + 1] - P.starts[r] : 1; };
-  auto length_of = [&](int r) { return max(0, min(P.lengths[r], room)); };
-  auto start_of = [&](int r) { return P.starts ? P.starts[r] : r; };
+  auto length_of = [&](int r) { return KEPT ? kept_length[r] : max(0, min(P.lengths[r], room)); };
+  auto start_of = [&](int r) { return KEPT ? (P.rows ? kept_start[r] : 0) : P.starts ? P.starts[r] : r; };
+  auto count_of = [&](int r) { return start_of(r + 1) - start_of(r); };
   auto group_of = [&](int r) {
     const int g = groups ? last_upto(first, groups, r) : -1;
     return g >= 0 && r < first[g + 1] ? g : -1;
@@ -212,8 +214,8 @@ __global__ __launch_bounds__(PLAN) void dz_prefix_plan_kernel(const PrefixParams
   }
   if (P.starts)
     for (int t = tid; t < P.tokens; t += PLAN) {
-      int r = rows ? last_upto(P.starts, rows, t) : -1;
-      if (r >= 0 && t >= P.starts[r + 1]) r = -1;
+      int r = rows ? last_upto(KEPT ? (const int*)kept_start : P.starts, rows, t) : -1;
+      if (r >= 0 && t >= start_of(r + 1)) r = -1;
       P.row_of[t] = r;
     }
   if (tid == 0) {
@@ -503,43 +505,79 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void dz_prefix_kernel(const P
     work(std::integral_constant<int, 1>());
 }
 
-// A workgroup a token: the pieces of its row's sums and of its group's, or zeros.
-template <bool BF>
+// The pieces of a token's row's sums and of its group's joined, or zeros.  A thread takes four values of a head over every SLICES-th
+// piece, four at once on their way; a workgroup takes 256 / SLICES such places, and every gridDim.y-th set of them.
+template <int SLICES, bool BF>
 __global__ __launch_bounds__(256) void dz_prefix_join_kernel(const PrefixParams P) {
   typedef Type<BF> Ty;
+  constexpr int SPOTS = 256 / SLICES, AT_ONCE = 4;
+  __shared__ float shared[SLICES > 1 ? 256 * 8 : 1];
   const int t = blockIdx.x, row = P.starts ? P.row_of[t] : t;
   Unit own = {0, 0, 0, 0, 0, 0, 0, -1, -1, 0, 0}, pre = own;
   bool sees = false;
   if (row >= 0) {
     own = P.units[P.ngroups + row];
     sees = own.n - (own.ntok - 1 - (t - own.tok0)) > 0;
-    if (own.pref >= 0) pre = P.units[own.pref];
+    if (sees && own.pref >= 0) pre = P.units[own.pref];
   }
   if (sees && own.np == 1 && own.part < 0) return;      // (stored already)
-  const int quads = P.dim / 4, stride = P.dim + 4;
-  for (int x = threadIdx.x; x < P.heads * quads; x += 256) {
-    const int h = x / quads, d = x % quads * 4, kvh = h / P.share;
+  const int quads = P.dim / 4, places = P.heads * quads;
+  const long long stride = P.dim + 4, pre_queries = (long long)pre.ntok * P.share, own_queries = (long long)own.ntok * P.share;
+  const int pieces = sees ? pre.np + own.np : 0;
+  const int slice = threadIdx.x / SPOTS;
+  for (int x0 = blockIdx.y * SPOTS; x0 < places; x0 += gridDim.y * SPOTS) {
+    const int x = x0 + threadIdx.x % SPOTS, h = min(x, places - 1) / quads, d = x % quads * 4, kvh = h / P.share, hs = h % P.share;
+    const float* from_pre = P.parts + (pre.part + kvh * pre_queries + (long long)(t - pre.tok0) * P.share + hs) * stride;
+    const float* from_own = P.parts + (own.part + kvh * own_queries + (long long)(t - own.tok0) * P.share + hs) * stride;
     float m = -INFINITY, l = 0.0f;
     f4_t o = {0, 0, 0, 0};
-    auto gather = [&](const Unit& u) {
-      const long long queries = (long long)u.ntok * P.share, at = kvh * queries + (long long)(t - u.tok0) * P.share + h % P.share;
-      const float* record = P.parts + (u.part + at) * stride;
-      for (int p = 0; p < u.np; ++p, record += P.kv_heads * queries * stride) {
-        const f4_t w = *(const f4_t*)(record + d);
-        const f2_t ml = *(const f2_t*)(record + P.dim);
-        const float up = fmaxf(m, ml[0]), f = weight_of(m, up), fs = weight_of(ml[0], up);
-        l = l * f + ml[1] * fs;
-        o = o * f + w * fs;
-        m = up;
+    for (int p0 = slice; p0 < pieces; p0 += SLICES * AT_ONCE) {
+      f4_t w[AT_ONCE];
+      f2_t ml[AT_ONCE];
+      float up = m;
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i) {
+        const int p = min(p0 + i * SLICES, pieces - 1);
+        const float* record = p < pre.np ? from_pre + p * (P.kv_heads * pre_queries * stride) : from_own + (p - pre.np) * (P.kv_heads * own_queries * stride);
+        w[i] = *(const f4_t*)(record + d);
+        ml[i] = *(const f2_t*)(record + P.dim);
       }
-    };
-    if (sees) {
-      if (pre.part >= 0) gather(pre);
-      if (own.part >= 0) gather(own);
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i) {
+        if (p0 + i * SLICES >= pieces) ml[i] = f2_t{-INFINITY, 0.0f}, w[i] = f4_t{0, 0, 0, 0};       // (the last one a second time)
+        up = fmaxf(up, ml[i][0]);
+      }
+      const float f = weight_of(m, up);
+      l *= f, o *= f, m = up;
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i) {
+        const float fs = weight_of(ml[i][0], up);
+        l += ml[i][1] * fs;
+        o += w[i] * fs;
+      }
     }
-    const f4_t y = sees ? o * (1.0f / l) : f4_t{0, 0, 0, 0};
-    const u2_t w = {(unsigned)Ty::round(y[0]) | (unsigned)Ty::round(y[1]) << 16, (unsigned)Ty::round(y[2]) | (unsigned)Ty::round(y[3]) << 16};
-    *(u2_t*)(P.out + t * P.out_row + h * P.out_head + d) = w;
+    if constexpr (SLICES > 1) {
+      float* mine = shared + threadIdx.x * 8;
+      *(f4_t*)mine = o;
+      *(f2_t*)(mine + 4) = f2_t{m, l};
+      __syncthreads();
+      if (slice == 0) {
+        const float* all = shared + threadIdx.x * 8;
+        for (int c = 1; c < SLICES; ++c) m = fmaxf(m, all[c * SPOTS * 8 + 4]);
+        l = 0.0f, o = f4_t{0, 0, 0, 0};
+        for (int c = 0; c < SLICES; ++c) {
+          const float f = weight_of(all[c * SPOTS * 8 + 4], m);
+          l += all[c * SPOTS * 8 + 5] * f;
+          o += *(const f4_t*)(all + c * SPOTS * 8) * f;
+        }
+      }
+      __syncthreads();
+    }
+    if (slice == 0 && x < places) {
+      const f4_t y = sees ? o * (1.0f / l) : f4_t{0, 0, 0, 0};
+      const u2_t w = {(unsigned)Ty::round(y[0]) | (unsigned)Ty::round(y[1]) << 16, (unsigned)Ty::round(y[2]) | (unsigned)Ty::round(y[3]) << 16};
+      *(u2_t*)(P.out + t * P.out_row + h * P.out_head + d) = w;
+    }
   }
 }
 
@@ -638,9 +676,21 @@ int dz_prefix_attention(const dz_prefix_args* a, void* stream) {
   static std::atomic<unsigned long long> attr_done[36];        // one per kernel
   if (lds > 65536 && !dz_lds_limit_once(attr_done[which], (const void*)kern, (int)lds)) return DZ_ELAUNCH;
   const hipStream_t st = (hipStream_t)stream;
-  hipLaunchKernelGGL(dz_prefix_plan_kernel, dim3(1), dim3(PLAN), 0, st, P);
+  const int most_units = a->rows > a->groups_n ? a->rows : a->groups_n;
+  if (most_units <= 256)
+    hipLaunchKernelGGL((dz_prefix_plan_kernel<256, true>), dim3(1), dim3(256), 0, st, P);
+  else if (most_units <= 1024)
+    hipLaunchKernelGGL((dz_prefix_plan_kernel<1024, true>), dim3(1), dim3(1024), 0, st, P);
+  else
+    hipLaunchKernelGGL((dz_prefix_plan_kernel<1024, false>), dim3(1), dim3(1024), 0, st, P);
   hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(256), lds, st, P);
-  hipLaunchKernelGGL(a->dtype == DZ_BF16 ? dz_prefix_join_kernel<true> : dz_prefix_join_kernel<false>, dim3(a->tokens), dim3(256), 0, st, P);
+  // of few outputs the pieces, too, are shared out; of many tokens, most of which are stored already, a workgroup takes all heads
+  const long long values = (long long)a->tokens * a->heads * (a->dim / 4);
+  const bool few = values <= (1 << 17);
+  const long long sets = ((long long)a->heads * (a->dim / 4) * (few ? 8 : 1) + 255) / 256, most = 1 + 8192 / a->tokens;
+  const kernel_t join = few ? (a->dtype == DZ_BF16 ? dz_prefix_join_kernel<8, true> : dz_prefix_join_kernel<8, false>)
+                            : (a->dtype == DZ_BF16 ? dz_prefix_join_kernel<1, true> : dz_prefix_join_kernel<1, false>);
+  hipLaunchKernelGGL(join, dim3(a->tokens, (unsigned)(sets < most ? sets : most)), dim3(256), 0, st, P);
   return hipGetLastError() == hipSuccess ? DZ_OK : DZ_ELAUNCH;
 }
 
