@@ -6,19 +6,7 @@
 // share a key head are taken together, up to 16 at once, so that every key and value is read once.  What bounds it
 // is the reading of keys and values: 4 flops per byte and head against the 300 that the card has.
 //
-// A wavefront walks 32 tokens at a time and holds all of it in registers:
-//   scores   C[token, head] = K[token, dim] Q[dim, head] on v_mfma_f32_16x16x32, two tiles of 16 tokens: lane l has
-//            head l % 16 and tokens 4 (l / 16) + i of each tile
-//   weights  those 8 values are just what the second product's operand wants of lane l if its k index 8 (l / 16) + e
-//            stands for token 4 (l / 16) + e % 4 of tile e / 4: nothing crosses lanes but the maximum
-//   values   C[dim, head] += V^T[dim, token] P[token, head]: a lane loads 8 dims (16 bytes) of its 8 tokens and
-//            turns the 8 x 8 block with 32 byte permutes; row r of product j stands for dim 8 r + j, so rows are
-//            read whole
-// The unused columns of the matrix instructions cost nothing: they are under a tenth of the time at one head per key.
-//
-// The running maximum moves only where a score is more than twice above it (in 2^s): weights are held times 2^14
-// (fp16) so that they use the type's range, at most 2^15, and are split in two values of the type, high and low: a
-// weight then has 16 (bf16) or 22 (fp16) bits, and the output's error is its own rounding.  Sums are fp32.
+// A wavefront walks 32 tokens at a time and holds all of it in registers (dz_attend.h).
 //
 // The work is cut on the device, which alone knows the lengths: every wavefront reads the lengths of the launch's
 // rows (up to 256, up to four a lane) and cuts them into as many equal parts as make 512 or 768 workgroups together.
@@ -43,7 +31,6 @@
 namespace {
 
 constexpr int WAVES = 4;               // wavefronts of a workgroup
-constexpr int TILE = 32;               // tokens of a step
 constexpr int HEADS = 16;              // heads taken together: columns of a matrix instruction
 constexpr int GROUP_ROWS = 256;        // rows of a launch: four lengths a lane
 constexpr int TARGET = 768;            // workgroups that the work of a launch is cut into at most, rows' last parts apart
@@ -149,13 +136,6 @@ __device__ __forceinline__ Part find_part(const AttnParams& P, int part, int ite
   return found;
 }
 
-// Keys and values of a call pass through once: loads that keep nothing in the caches read 7.1 TB/s where others read 6.2.  Not so
-// where rows share pages: 16 rows of one sequence's 4096 tokens of 32 key heads 130 -> 81 us with the others.
-template <bool ONCE>
-__device__ __forceinline__ u4_t load16(const char* at) {
-  return ONCE ? __builtin_nontemporal_load((const u4_t*)at) : *(const u4_t*)at;
-}
-
 // Sums of parts go from one workgroup to another past the caches of the eight dies (sc1: agent scope): a fence there writes
 // back and empties a whole cache, which took six times as long as the attention itself.
 struct Shared {
@@ -180,7 +160,6 @@ __global__ __launch_bounds__(64 * WAVES, KC == 8 && !FULL ? 1 : 2) void dz_atten
   typedef Type<BF> Ty;
   typedef typename Ty::v8 v8;
   constexpr int NB = (KC + 3) / 4;     // blocks of 128 dims
-  constexpr bool AHEAD = KC <= 6;      // (heads of 256: no registers for it)
   extern __shared__ float lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
   const int items = P.kv_heads * P.head_tiles;
@@ -201,149 +180,22 @@ __global__ __launch_bounds__(64 * WAVES, KC == 8 && !FULL ? 1 : 2) void dz_atten
   const int t1 = tile0 + lo + (hi - lo) * (wave + 1) / WAVES;
 
   // queries: lane holds dims 32 c + 8 g .. + 7 of head `col`
-  v8 q[KC];
+  Walk<KC, FULL, BF> walk;
 #pragma unroll
   for (int c = 0; c < KC; ++c) {
     u4_t w = {0, 0, 0, 0};
     if (col < nheads && 32 * c + 8 * g < P.dim)
       w = *(const u4_t*)(P.q + row * P.q_row + (head0 + col) * P.q_head + (32 * c + 8 * g) * 2);
-    q[c] = __builtin_bit_cast(v8, w);
+    walk.q[c] = __builtin_bit_cast(v8, w);
   }
-
-  f4_t acc[8 * NB];
-#pragma unroll
-  for (int j = 0; j < 8 * NB; ++j) acc[j] = f4_t{0, 0, 0, 0};
-  float top = -INFINITY, sum = 0.0f;   // of head `col`: the reference maximum, this lane's share of the sum
-
   const int* table = P.tables + row * P.table_row;
-  const int last_page = (end - 1) >> P.shift;
-  int page0 = t0 * TILE >> P.shift;    // of the 64 page numbers that the lanes hold
-  auto fetch = [&](int base) {
-    const int at = base + lane;
-    unsigned id = at <= last_page && at >= first >> P.shift ? (unsigned)table[at] : 0u;
-    if (id >= P.num_pages) {
-      atomicOr(P.status, 4u);
-      id = 0;
-    }
-    return id;
-  };
-  unsigned ids = 0, next_ids = 0;
-  if (t0 < t1) {
-    ids = fetch(page0);
-    next_ids = fetch(page0 + 64);
-  }
-  const int in_page = (1 << P.shift) - 1;
-
-  auto walk = [&](auto once) __attribute__((always_inline)) {
-    constexpr bool ONCE = decltype(once)::value;
-    u4_t kw[2][KC], vw[NB][8];
-    // a token's page number, of those that the lanes hold; behind the ends: the nearest token that the row sees
-    auto place = [&](const char* pages, long long page, long long head, long long token, int t, bool edge) {
-      if (edge) t = max(first, min(t, end - 1));
-      const unsigned id = __shfl(ids, (t >> P.shift) - page0);
-      return pages + id * page + kvh * head + (t & in_page) * token;
-    };
-    auto load_keys = [&](int tok, bool edge) {
-#pragma unroll
-      for (int a = 0; a < 2; ++a) {
-        const char* at = place(P.k, P.k_page, P.k_head, P.k_token, tok + 16 * a + col, edge);
-#pragma unroll
-        for (int c = 0; c < KC; ++c) {
-          const bool in = FULL || 32 * c + 8 * g < P.dim;
-          kw[a][c] = load16<ONCE>(at + (in ? 64 * c + 16 * g : 0));
-          if (!in) kw[a][c] = u4_t{0, 0, 0, 0};
-        }
-      }
-    };
-    auto at_edge = [&](int tok) { return tok < first || tok + TILE > end; };
-    auto turn_page = [&](int tok) {
-      if (((tok + TILE - 1) >> P.shift) >= page0 + 64) {       // (a tile has 4 pages at most)
-        ids = next_ids;
-        page0 += 64;
-        next_ids = fetch(page0 + 64);
-      }
-    };
-    if (AHEAD && t0 < t1) load_keys(t0 * TILE, at_edge(t0 * TILE));
-    for (; t0 < t1; ++t0) {
-      const int tok = t0 * TILE;
-      const bool edge = at_edge(tok);
-      if (!AHEAD) {
-        turn_page(tok);
-        load_keys(tok, edge);
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const char* at = place(P.v, P.v_page, P.v_head, P.v_token, tok + 16 * (e >> 2) + 4 * g + (e & 3), edge);
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-          const int d = 128 * b + 8 * col;             // (a lane behind the head's end makes values that no one stores)
-          vw[b][e] = load16<ONCE>(at + (FULL && KC % 4 == 0 || d < P.dim ? 2 * d : 0));
-        }
-      }
-      float s[8];
-#pragma unroll
-      for (int a = 0; a < 2; ++a) {
-        f4_t c4 = {0, 0, 0, 0};
-#pragma unroll
-        for (int c = 0; c < KC; ++c) c4 = Ty::mma(__builtin_bit_cast(v8, kw[a][c]), q[c], c4);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[4 * a + i] = c4[i] * P.scale;
-      }
-      // the next step's keys are on their way while this one's values come in
-      if (AHEAD && t0 + 1 < t1) {
-        turn_page(tok + TILE);
-        load_keys(tok + TILE, at_edge(tok + TILE));
-      }
-      if (edge) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int t = tok + 16 * (e >> 2) + 4 * g + (e & 3);
-          if (t < first || t >= end) {
-            s[e] = -INFINITY;
-#pragma unroll
-            for (int b = 0; b < NB; ++b) vw[b][e] = u4_t{0, 0, 0, 0};   // (what is masked has no part in the product)
-          }
-        }
-      }
-      float most = s[0];
-#pragma unroll
-      for (int e = 1; e < 8; ++e) most = fmaxf(most, s[e]);
-      most = fmaxf(most, __shfl_xor(most, 16));
-      most = fmaxf(most, __shfl_xor(most, 32));
-      if (__any(most > top + 1.0f)) {
-        const float up = fmaxf(most, top);
-        const float f = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - up);
-        top = up;
-        sum *= f;
-#pragma unroll
-        for (int j = 0; j < 8 * NB; ++j) acc[j] *= f;
-      }
-      const float ref = top == -INFINITY ? 0.0f : top - Ty::BIAS;
-      v8 ph, pl;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float p = __builtin_amdgcn_exp2f(s[e] - ref);
-        sum += p;
-        ph[e] = Ty::one(p);
-        pl[e] = Ty::one(p - (float)ph[e]);
-      }
-#pragma unroll
-      for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const unsigned sel = j & 1 ? 0x07060302u : 0x05040100u;
-          u4_t w;
-#pragma unroll
-          for (int x = 0; x < 4; ++x) w[x] = __builtin_amdgcn_perm(vw[b][2 * x + 1][j >> 1], vw[b][2 * x][j >> 1], sel);
-          const v8 vt = __builtin_bit_cast(v8, w);
-          acc[8 * b + j] = Ty::mma(vt, pl, Ty::mma(vt, ph, acc[8 * b + j]));
-        }
-    }
-  };
   if (mine.once)
-    walk(std::integral_constant<bool, true>());
+    walk.template run<true, false>(P, table, kvh, first, end, t0, t1, end, end);
   else
-    walk(std::integral_constant<bool, false>());
+    walk.template run<false, false>(P, table, kvh, first, end, t0, t1, end, end);
+  const auto& acc = walk.acc;
+  const float top = walk.top;
+  float sum = walk.sum;
   sum += __shfl_xor(sum, 16);
   sum += __shfl_xor(sum, 32);
 

@@ -23,7 +23,9 @@ namespace {
 typedef short s4_t __attribute__((ext_vector_type(4)));
 typedef short s8_t __attribute__((ext_vector_type(8)));
 
-constexpr int TILE = 128;              // queries of a workgroup
+constexpr int ROWS = 128;              // queries of a workgroup
+constexpr int FEW = 16;                // queries of a unit up to which wavefronts share out its tokens and not its queries
+constexpr float CACHED = 64 << 20;     // bytes of keys and values up to which they may be in the last cache
 constexpr int STEP = 64;               // tokens of a step
 constexpr int TARGET = 512;            // pieces that the work is cut into at most, units' last ones apart
 constexpr int LEAST = 256;             // tokens of a piece
@@ -46,7 +48,7 @@ struct PrefixParams {
   const int *tables, *lengths, *starts, *groups, *prefixes;
   uint16_t* out;
   unsigned* status;
-  int* head;                           // [0]: how many items there are
+  int* head;                           // [0]: how many items there are, of them the groups' [2]; [1]: whether keys and values are more than the caches keep
   Unit* units;                         // the groups', the rows'
   Item* items;
   int* row_of;                         // of every token, where starts say
@@ -58,7 +60,7 @@ struct PrefixParams {
   float scale;
 };
 
-__device__ __forceinline__ int tiles_for(const PrefixParams& P, int tokens) { return (int)(((long long)tokens * P.share + TILE - 1) / TILE); }
+__device__ __forceinline__ int tiles_for(const PrefixParams& P, int tokens) { return (int)(((long long)tokens * P.share + ROWS - 1) / ROWS); }
 
 // The last i in [0, n) with at[i] <= x, or -1.
 template <typename T>
@@ -200,6 +202,7 @@ __global__ __launch_bounds__(PLAN) void dz_prefix_plan_kernel(const PrefixParams
       items0 += wave_items[w], parts0 += wave_parts[w];
     }
     items_to[tid] = before + items_upto;
+    if (u == groups - 1) P.head[2] = before + items_upto;
     if (parts) x.part = parts_before + parts_upto - parts;
     made[tid] = make_int2(x.tiles, x.np);
     if (u < units) P.units[u < groups ? u : P.ngroups + u - groups] = x;
@@ -219,9 +222,11 @@ __global__ __launch_bounds__(PLAN) void dz_prefix_plan_kernel(const PrefixParams
       P.row_of[t] = r;
     }
   if (tid == 0) {
+    if (!groups) P.head[2] = 0;
     const bool fits = items0 <= P.room_items && parts0 <= P.room_parts;
     if (!fits) atomicOr(P.status, 4u);
     P.head[0] = fits ? items0 : 0;
+    P.head[1] = work * (float)P.kv_heads * (4.0f * (float)P.dim) > CACHED;
   }
 }
 
@@ -230,6 +235,77 @@ __global__ __launch_bounds__(PLAN) void dz_prefix_plan_kernel(const PrefixParams
 template <int KC>
 __device__ __forceinline__ int swizzled(int token) {
   return KC % 4 == 0 ? 2 * (token & 7) : KC % 2 == 0 ? 2 * (token >> 1 & 3) : 2 * (token >> 2 & 1);
+}
+
+// A piece of a unit of up to FEW queries: the four wavefronts walk a quarter of its tokens each, with keys and values in registers, and
+// join their sums.
+template <int KC, bool FULL, bool BF>
+__device__ __forceinline__ void few_queries(const PrefixParams& P, const Unit& U, int piece, int kvh, int lo, int hi, bool once, float* lds) {
+  typedef Type<BF> Ty;
+  typedef typename Ty::v8 v8;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
+  const int queries = U.ntok * P.share;
+  auto limit_of = [&](int x) { return U.causal ? max(U.n - (U.ntok - 1 - x / P.share), 0) : U.n; };
+  Walk<KC, FULL, BF> walk;
+  const int mine = min(col, queries - 1);
+  const char* from = P.q + (U.tok0 + mine / P.share) * P.q_row + (kvh * P.share + mine % P.share) * P.q_head;
+#pragma unroll
+  for (int c = 0; c < KC; ++c) {
+    u4_t w = {0, 0, 0, 0};
+    if (col < queries && 32 * c + 8 * g < P.dim) w = *(const u4_t*)(from + (32 * c + 8 * g) * 2);
+    walk.q[c] = __builtin_bit_cast(v8, w);
+  }
+  const int* table = P.tables + U.row * P.table_row;
+  const int tile0 = lo / TILE, tiles = lo < hi ? (hi + TILE - 1) / TILE - tile0 : 0;
+  const int t0 = tile0 + tiles * wave / 4, t1 = tile0 + tiles * (wave + 1) / 4, limit = min(limit_of(mine), hi), seen_by_all = min(limit_of(0), hi);
+  if (seen_by_all < hi)
+    walk.template run<false, true>(P, table, kvh, lo, hi, t0, t1, limit, seen_by_all);
+  else if (once)
+    walk.template run<true, false>(P, table, kvh, lo, hi, t0, t1, hi, hi);
+  else
+    walk.template run<false, false>(P, table, kvh, lo, hi, t0, t1, hi, hi);
+  float sum = walk.sum;
+  sum += __shfl_xor(sum, 16);
+  sum += __shfl_xor(sum, 32);
+  const int ld = P.dim + 4;
+  float *sums = lds + wave * queries * ld, *stat = lds + 4 * FEW * ld;       // [wave][query][dim], then maxima and sums
+  if (col < queries) {
+#pragma unroll
+    for (int b = 0; b < walk.NB; ++b)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int d = 128 * b + 8 * (4 * g + i);
+        if (d < P.dim) {
+          *(f4_t*)(sums + col * ld + d) = f4_t{walk.acc[8 * b][i], walk.acc[8 * b + 1][i], walk.acc[8 * b + 2][i], walk.acc[8 * b + 3][i]};
+          *(f4_t*)(sums + col * ld + d + 4) = f4_t{walk.acc[8 * b + 4][i], walk.acc[8 * b + 5][i], walk.acc[8 * b + 6][i], walk.acc[8 * b + 7][i]};
+        }
+      }
+    if (g == 0) *(f2_t*)(stat + (wave * FEW + col) * 2) = f2_t{walk.top, sum};
+  }
+  __syncthreads();
+  const int quads = P.dim / 4;
+  for (int x = threadIdx.x; x < queries * quads; x += 256) {
+    const int y = x / quads, d = x % quads * 4;
+    float m = -INFINITY, l = 0.0f;
+    f4_t o = {0, 0, 0, 0};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) m = fmaxf(m, stat[(w * FEW + y) * 2]);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = weight_of(stat[(w * FEW + y) * 2], m);
+      l += stat[(w * FEW + y) * 2 + 1] * f;
+      o += *(const f4_t*)(lds + (w * queries + y) * ld + d) * f;
+    }
+    if (U.part >= 0) {
+      float* record = P.parts + (U.part + ((long long)piece * P.kv_heads + kvh) * queries + y) * ld;
+      *(f4_t*)(record + d) = o;
+      if (d == 0) *(f2_t*)(record + P.dim) = f2_t{m, l};
+    } else {
+      o = limit_of(y) > 0 ? o * (1.0f / l) : f4_t{0, 0, 0, 0};
+      const u2_t w = {(unsigned)Ty::round(o[0]) | (unsigned)Ty::round(o[1]) << 16, (unsigned)Ty::round(o[2]) | (unsigned)Ty::round(o[3]) << 16};
+      *(u2_t*)(P.out + (U.tok0 + y / P.share) * P.out_row + (kvh * P.share + y % P.share) * P.out_head + d) = w;
+    }
+  }
 }
 
 template <int KC, bool FULL, bool BF>
@@ -241,11 +317,15 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void dz_prefix_kernel(const P
   constexpr unsigned BAD = BF ? 0x7f80u : 0x7c00u;     // exponent of what is not finite
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
-  const int nth = blockIdx.x / P.kv_heads, kvh = blockIdx.x % P.kv_heads;
-  if (nth >= P.head[0]) return;
-  const Item item = P.items[nth];
+  const int turn = blockIdx.x / P.kv_heads, kvh = blockIdx.x % P.kv_heads, all = P.head[0], shared = P.head[2];
+  if (turn >= all) return;
+  // prefixes' pieces, which keep the matrix cores busy, and rows' own, which wait for memory: a compute unit each of both, then the others
+  const int round = max(1, 256 / P.kv_heads), pairs = min(shared, all - shared) / round, at = turn % (2 * round);
+  const int nth = turn >= pairs * 2 * round ? turn - pairs * round : turn / (2 * round) * round + (at < round ? at : at - round);
+  const bool of_prefix = turn >= pairs * 2 * round ? nth < shared : at < round;
+  const Item item = P.items[turn >= pairs * 2 * round ? (of_prefix ? nth : turn) : of_prefix ? nth : shared + nth];
   const Unit U = P.units[item.unit];
-  const int queries = U.ntok * P.share, x0 = item.tile * TILE, in_tile = min(TILE, queries - x0);
+  const int queries = U.ntok * P.share, x0 = item.tile * ROWS, in_tile = min(ROWS, queries - x0);
   auto limit_of = [&](int x) { return U.causal ? max(U.n - (U.ntok - 1 - x / P.share), 0) : U.n; };      // tokens that query x sees
   const int end = max(limit_of(x0 + in_tile - 1), U.k0);
   const long long len = end - U.k0;
@@ -253,6 +333,10 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void dz_prefix_kernel(const P
   auto bound = [&](int p) { return p == U.np ? end : max(U.k0, (U.k0 + (int)(len * p / U.np)) & ~(STEP - 1)); };
   const int lo = bound(item.piece), hi = bound(item.piece + 1), begin = lo < hi ? lo & ~(STEP - 1) : hi;
 
+  if (queries <= FEW) {
+    few_queries<KC, FULL, BF>(P, U, item.piece, kvh, lo, hi, P.head[1] != 0, (float*)lds);
+    return;
+  }
   const int last_page = (hi - 1) >> P.shift, in_page = (1 << P.shift) - 1;
   const int* table = P.tables + U.row * P.table_row;
   int page0 = begin >> P.shift;        // of the 64 page numbers that the lanes hold
@@ -607,11 +691,11 @@ struct Room {
 };
 inline Room room_of(int tokens, int rows, int groups, int heads, int kv_heads, int dim) {
   Room m;
-  const long long queries = (long long)tokens * (heads / kv_heads), whole = (queries + TILE - 1) / TILE;
+  const long long queries = (long long)tokens * (heads / kv_heads), whole = (queries + ROWS - 1) / ROWS;
   const long long some = rows < tokens ? rows : tokens, both = groups ? 2 : 1;
   // a unit's tiles: the last one is not full; pieces: of TARGET in all one more of each tile
   m.items = both * whole + some + (groups < tokens ? groups : tokens) + TARGET / kv_heads + 1;
-  m.parts = both * tokens * heads + (long long)TILE * (TARGET + kv_heads);
+  m.parts = both * tokens * heads + (long long)ROWS * (TARGET + kv_heads);
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
   m.units_at = 256;
   m.items_at = up(m.units_at + sizeof(Unit) * (size_t)(rows + groups));
@@ -671,7 +755,8 @@ int dz_prefix_attention(const dz_prefix_args* a, void* stream) {
   // 16 tokens that a wavefront asks for lie in one page, within 32 bits
   P.near = a->page_size >= 16 && P.k_token < (1 << 27) && P.v_token < (1 << 27);
   const int kc = chunks_of(a->dim), which = kc * 4 + (a->dim == 32 * kc) * 2 + a->dtype;
-  const size_t lds = 2 * (size_t)(8 * kc) * 1024;
+  // two steps' keys and values; or the sums of four wavefronts and their maxima
+  const size_t steps = 2 * (size_t)(8 * kc) * 1024, sums = (4 * FEW * (size_t)(a->dim + 4) + 8 * FEW) * 4, lds = steps > sums ? steps : sums;
   const kernel_t kern = a->dtype == DZ_BF16 ? kernel_for<true>(a->dim) : kernel_for<false>(a->dim);
   static std::atomic<unsigned long long> attr_done[36];        // one per kernel
   if (lds > 65536 && !dz_lds_limit_once(attr_done[which], (const void*)kern, (int)lds)) return DZ_ELAUNCH;
