@@ -28,6 +28,7 @@ constexpr int FEW = 16;                // queries of a unit up to which wavefron
 constexpr float CACHED = 64 << 20;     // bytes of keys and values up to which they may be in the last cache
 constexpr int STEP = 64;               // tokens of a step
 constexpr int TARGET = 512;            // pieces that the work is cut into at most, units' last ones apart
+constexpr int TARGET_FEW = 2048;       // and those of units of few queries, whose sums take little room
 constexpr int LEAST = 256;             // tokens of a piece
 constexpr int GROUPS = DZ_PREFIX_GROUPS;
 
@@ -40,7 +41,8 @@ struct Unit {
   int causal, pad;
 };
 struct Item {
-  int unit, tile, piece, pad;
+  Unit unit;
+  int tile, piece, pad[2];
 };
 
 struct PrefixParams {
@@ -48,10 +50,10 @@ struct PrefixParams {
   const int *tables, *lengths, *starts, *groups, *prefixes;
   uint16_t* out;
   unsigned* status;
-  int* head;                           // [0]: how many items there are, of them the groups' [2]; [1]: whether keys and values are more than the caches keep
+  int* head;                           // [0]: how many items there are, of them the groups' [2]; [1]: whether keys and values are more than
+                                       // the caches keep; [3]: whether no row has any tokens, as what says so does not fit
   Unit* units;                         // the groups', the rows'
   Item* items;
-  int* row_of;                         // of every token, where starts say
   float* parts;                        // records of dim + 4 floats: values, maximum, sum
   long long q_row, q_head, k_page, k_head, k_token, v_page, v_head, v_token, out_row, out_head, table_row;   // bytes; out, table: elements
   long long room_parts;
@@ -76,157 +78,209 @@ __device__ __forceinline__ int last_upto(const T* at, int n, T x) {
   return lo - 1;
 }
 
-// One workgroup.  KEPT: rows and groups are no more than its threads, and what is known of them stays in LDS: 6.0 -> 3.x us.
-template <int PLAN, bool KEPT>
-__global__ __launch_bounds__(PLAN) void dz_prefix_plan_kernel(const PrefixParams P) {
-  constexpr int G = KEPT ? PLAN : GROUPS;
-  __shared__ int first[G + 1], cut[G], leader[G], alone[G];      // of groups: rows, prefix, row whose table, tiles apart
-  __shared__ int kept_length[KEPT ? PLAN : 1], kept_start[KEPT ? PLAN + 1 : 1];
-  __shared__ int items_to[PLAN];
-  __shared__ long long wave_parts[PLAN / 64];
-  __shared__ int wave_items[PLAN / 64];
-  __shared__ float wave_work[PLAN / 64];
-  __shared__ int2 made[PLAN];            // of a round's units: tiles, pieces
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int room = P.pages_per_row << P.shift;
-  int bad = 0, bad_groups = 0;
-  for (int r = tid; r < P.rows; r += PLAN) {
-    const int n = P.lengths[r], a = P.starts ? P.starts[r] : r, b = P.starts ? P.starts[r + 1] : r + 1;
-    bad |= a < 0 || b < a || b > P.tokens;
-    if (n > room) atomicOr(P.status, 4u);
-    if (KEPT) kept_length[r] = max(0, min(n, room)), kept_start[r] = a, kept_start[r + 1] = b;      // (neighbours write the same)
+// The plan, as N threads of a workgroup make it together.  KEPT: rows, and groups and rows together, are no more than these, and what is known of
+// them stays in LDS.
+template <int N, bool KEPT>
+struct PlanRoom {
+  static constexpr int G = KEPT ? N : GROUPS;
+  int first[G + 1], cut[G], leader[G], alone[G];       // of groups: rows, prefix, row whose table, tiles apart
+  int length[KEPT ? N : 1], start[KEPT ? N + 1 : 1];
+  long long wave_parts[N / 64];
+  int wave_items[N / 64];
+  float wave_work[N / 64], wave_few[N / 64];
+};
+
+template <int N, bool KEPT>
+struct Planner {
+  const PrefixParams& P;
+  PlanRoom<N, KEPT>& S;
+  const int tid, lane, wave, room;
+  int rows, groups;                    // that count
+  int each, each_few;                  // tokens of a piece
+  bool once;                           // keys and values are more than the caches keep
+  int items;                           // in front of the round of units that `place` is at
+  long long parts;
+
+  __device__ __forceinline__ Planner(const PrefixParams& p, PlanRoom<N, KEPT>& s)
+      : P(p), S(s), tid(threadIdx.x), lane(tid & 63), wave(tid >> 6), room(p.pages_per_row << p.shift), items(0), parts(0) {}
+
+  __device__ __forceinline__ int length_of(int r) const { return KEPT ? S.length[r] : max(0, min(P.lengths[r], room)); }
+  __device__ __forceinline__ int start_of(int r) const { return KEPT ? (P.rows ? S.start[r] : 0) : P.starts ? P.starts[r] : r; }
+  __device__ __forceinline__ int count_of(int r) const { return start_of(r + 1) - start_of(r); }
+  __device__ __forceinline__ int group_of(int r) const {
+    const int g = groups ? last_upto(S.first, groups, r) : -1;
+    return g >= 0 && r < S.first[g + 1] ? g : -1;
   }
-  for (int g = tid; g < P.ngroups; g += PLAN) {
-    const int a = P.groups[g], b = P.groups[g + 1];
-    bad_groups |= a < 0 || b < a || b > P.rows;
-    first[g] = a, first[g + 1] = b;
-    cut[g] = min(P.prefixes[g], room);
-    leader[g] = P.rows;
-    alone[g] = 0;
-  }
-  bad = __syncthreads_or(bad);
-  bad_groups = __syncthreads_or(bad_groups);
-  if ((bad || bad_groups) && tid == 0) atomicOr(P.status, 4u);
-  const int rows = bad ? 0 : P.rows, groups = bad || bad_groups ? 0 : P.ngroups;
-  auto length_of = [&](int r) { return KEPT ? kept_length[r] : max(0, min(P.lengths[r], room)); };
-  auto start_of = [&](int r) { return KEPT ? (P.rows ? kept_start[r] : 0) : P.starts ? P.starts[r] : r; };
-  auto count_of = [&](int r) { return start_of(r + 1) - start_of(r); };
-  auto group_of = [&](int r) {
-    const int g = groups ? last_upto(first, groups, r) : -1;
-    return g >= 0 && r < first[g + 1] ? g : -1;
-  };
-  // a prefix ends where the first of its rows' new tokens sees no more of it
-  for (int r = tid; r < rows; r += PLAN) {
-    const int g = group_of(r), n = length_of(r), c = count_of(r);
-    if (g >= 0 && n > 0 && c > 0) {
-      atomicMin(&cut[g], max(0, n - c + 1));
-      atomicMin(&leader[g], r);
-      atomicAdd(&alone[g], tiles_for(P, c));
+
+  // Checks what the device alone knows and finds the prefixes that are taken apart from their rows; tell: reports it.
+  __device__ __forceinline__ void begin(bool tell) {
+    int bad = 0, bad_groups = 0, beyond = 0;
+    for (int r = tid; r < P.rows; r += N) {
+      const int n = P.lengths[r], a = P.starts ? P.starts[r] : r, b = P.starts ? P.starts[r + 1] : r + 1;
+      bad |= a < 0 || b < a || b > P.tokens;
+      beyond |= n > room;
+      if (KEPT) S.length[r] = max(0, min(n, room)), S.start[r] = a, S.start[r + 1] = b;      // (neighbours write the same)
     }
+    for (int g = tid; g < P.ngroups; g += N) {
+      const int a = P.groups[g], b = P.groups[g + 1];
+      bad_groups |= a < 0 || b < a || b > P.rows;
+      S.first[g] = a, S.first[g + 1] = b;
+      S.cut[g] = min(P.prefixes[g], room);
+      S.leader[g] = P.rows;
+      S.alone[g] = 0;
+    }
+    if (tell && beyond) atomicOr(P.status, 4u);
+    bad = __syncthreads_or(bad);
+    if (P.ngroups) bad_groups = __syncthreads_or(bad_groups);
+    if (tell && (bad || bad_groups) && tid == 0) atomicOr(P.status, 4u);
+    rows = bad ? 0 : P.rows, groups = bad || bad_groups ? 0 : P.ngroups;
+    if (!groups) return;
+    // a prefix ends where the first of its rows' new tokens sees no more of it
+    for (int r = tid; r < rows; r += N) {
+      const int g = group_of(r), n = length_of(r), c = count_of(r);
+      if (g >= 0 && n > 0 && c > 0) {
+        atomicMin(&S.cut[g], max(0, n - c + 1));
+        atomicMin(&S.leader[g], r);
+        atomicAdd(&S.alone[g], tiles_for(P, c));
+      }
+    }
+    __syncthreads();
+    // and is taken apart from the rows only where that spares tiles
+    for (int g = tid; g < groups; g += N) {
+      const int tokens = start_of(S.first[g + 1]) - start_of(S.first[g]);
+      if (S.cut[g] <= 0 || S.leader[g] >= rows || tiles_for(P, tokens) >= S.alone[g]) S.cut[g] = 0;
+    }
+    __syncthreads();
   }
-  __syncthreads();
-  // and is taken apart from the rows only where that spares tiles
-  for (int g = tid; g < groups; g += PLAN) {
-    const int tokens = start_of(first[g + 1]) - start_of(first[g]);
-    if (cut[g] <= 0 || leader[g] >= rows || tiles_for(P, tokens) >= alone[g]) cut[g] = 0;
-  }
-  __syncthreads();
-  auto unit_of = [&](int u) {
+
+  __device__ __forceinline__ int units() const { return groups + rows; }
+
+  __device__ __forceinline__ Unit unit_of(int u) const {
     Unit x = {0, 0, 0, 0, 0, 0, 0, -1, -1, 0, 0};
     if (u < groups) {
-      if (cut[u]) {
-        x.tok0 = start_of(first[u]);
-        x.ntok = start_of(first[u + 1]) - x.tok0;
-        x.n = cut[u];
-        x.row = leader[u];
+      if (S.cut[u]) {
+        x.tok0 = start_of(S.first[u]);
+        x.ntok = start_of(S.first[u + 1]) - x.tok0;
+        x.n = S.cut[u];
+        x.row = S.leader[u];
       }
-    } else {
+    } else if (u < units()) {
       const int r = u - groups, g = group_of(r);
       x.tok0 = start_of(r);
       x.ntok = count_of(r);
       x.n = length_of(r);
       x.row = r;
       x.causal = 1;
-      if (g >= 0 && cut[g] && x.n > 0 && x.ntok > 0) {
-        x.k0 = cut[g];
+      if (g >= 0 && S.cut[g] && x.n > 0 && x.ntok > 0) {
+        x.k0 = S.cut[g];
         x.pref = g;
       }
     }
     x.tiles = tiles_for(P, x.ntok);
     return x;
-  };
-  const int units = groups + rows;
-  float work = 0.0f;
-  for (int u = tid; u < units; u += PLAN) {
-    const Unit x = unit_of(u);
-    work += (float)x.tiles * (float)(x.n - x.k0);
   }
-  work = scan_add(work);
-  if (lane == 63) wave_work[wave] = work;
-  __syncthreads();
-  work = 0.0f;
-  for (int w = 0; w < PLAN / 64; ++w) work += wave_work[w];
-  // tokens of a piece, in whole steps (sums above 2^24 are rounded: a piece is a little longer)
-  const float want = ceilf(work * 1.0001f * (float)P.kv_heads * (1.0f / TARGET) * (1.0f / STEP));
-  const int each = STEP * (int)fminf(fmaxf(want, (float)(LEAST / STEP)), (float)(1 << 24));
 
-  int items0 = 0;                      // in front of this round of units
-  long long parts0 = 0;
-  for (int u0 = 0; u0 < units; u0 += PLAN) {
-    const int u = u0 + tid;
-    Unit x = {0, 0, 0, 0, 0, 0, 0, -1, -1, 0, 0};
-    int items = 0;
-    long long parts = 0;
-    if (u < units) {
-      x = unit_of(u);
-      x.np = (x.n - x.k0 + each - 1) / each;
-      if (x.tiles == 0) x.np = 0;
-      items = x.tiles * x.np;
-      if (x.np > 1 || x.k0 > 0 || !x.causal) parts = (long long)x.np * x.ntok * P.heads;
+  __device__ __forceinline__ bool few(const Unit& x) const { return (long long)x.ntok * P.share <= FEW; }
+
+  // How long pieces are: tokens times tiles, over the pieces aimed at.
+  __device__ __forceinline__ void lengths_of_pieces() {
+    float all = 0.0f, of_few = 0.0f;
+    for (int u = tid; u < units(); u += N) {
+      const Unit x = unit_of(u);
+      const float w = (float)x.tiles * (float)(x.n - x.k0);
+      all += w;
+      of_few += few(x) ? w : 0.0f;
     }
-    const int items_upto = scan_add(items);
-    // (a sum of 64 bits over a wavefront: two of 32)
-    long long parts_upto = parts;
+    all = scan_add(all), of_few = scan_add(of_few);
+    if (lane == 63) S.wave_work[wave] = all, S.wave_few[wave] = of_few;
+    __syncthreads();
+    all = of_few = 0.0f;
+#pragma unroll
+    for (int w = 0; w < N / 64; ++w) all += S.wave_work[w], of_few += S.wave_few[w];
+    // in whole steps (sums above 2^24 are rounded: a piece is a little longer)
+    auto each_of = [&](float work, int target) {
+      const float want = ceilf(work * 1.0001f * (float)P.kv_heads * (1.0f / (float)target) * (1.0f / STEP));
+      return STEP * (int)fminf(fmaxf(want, (float)(LEAST / STEP)), (float)(1 << 24));
+    };
+    each = each_of(all, TARGET);
+    each_few = min(each, each_of(of_few, TARGET_FEW));
+    once = all * (float)P.kv_heads * (4.0f * (float)P.dim) > CACHED;
+  }
+
+  __device__ __forceinline__ int pieces_of(const Unit& x) const {
+    const int most = few(x) ? each_few : each;
+    return x.tiles ? (x.n - x.k0 + most - 1) / most : 0;
+  }
+
+  // The pieces of this thread's unit, of the next N of them: its items end at what is returned, its records begin at x.part.
+  __device__ __forceinline__ int place(Unit& x) {
+    x.np = pieces_of(x);
+    const int mine = x.tiles * x.np;
+    const long long records = x.np > 1 || x.k0 > 0 || !x.causal ? (long long)x.np * x.ntok * P.heads : 0;
+    const int upto = scan_add(mine);
+    long long records_upto = records;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
-      const long long y = __shfl_up(parts_upto, d);
-      if (lane >= d) parts_upto += y;
+      const long long y = __shfl_up(records_upto, d);
+      if (lane >= d) records_upto += y;
     }
-    if (lane == 63) wave_items[wave] = items_upto, wave_parts[wave] = parts_upto;
+    if (lane == 63) S.wave_items[wave] = upto, S.wave_parts[wave] = records_upto;
     __syncthreads();
-    const int begin = items0;
-    int before = items0;
-    long long parts_before = parts0;
-    for (int w = 0; w < PLAN / 64; ++w) {
-      if (w < wave) before += wave_items[w], parts_before += wave_parts[w];
-      items0 += wave_items[w], parts0 += wave_parts[w];
+    int before = items;
+    long long parts_before = parts;
+#pragma unroll
+    for (int w = 0; w < N / 64; ++w) {
+      if (w < wave) before += S.wave_items[w], parts_before += S.wave_parts[w];
+      items += S.wave_items[w], parts += S.wave_parts[w];
     }
-    items_to[tid] = before + items_upto;
-    if (u == groups - 1) P.head[2] = before + items_upto;
-    if (parts) x.part = parts_before + parts_upto - parts;
-    made[tid] = make_int2(x.tiles, x.np);
-    if (u < units) P.units[u < groups ? u : P.ngroups + u - groups] = x;
+    if (records) x.part = parts_before + records_upto - records;
+    return before + upto;
+  }
+
+  __device__ __forceinline__ bool fits() const { return items <= P.room_items && parts <= P.room_parts; }
+
+  // What others need to know of all of it.
+  __device__ __forceinline__ void tell() const {
+    if (!fits()) atomicOr(P.status, 4u);
+    P.head[0] = fits() ? items : 0;
+    P.head[1] = once;
+    P.head[3] = rows < P.rows || !fits();
+  }
+
+  // Where unit u's entry is: the groups', then the rows'.
+  __device__ __forceinline__ int entry_of(int u) const { return u < groups ? u : P.ngroups + u - groups; }
+};
+
+// One workgroup.
+template <int N, bool KEPT>
+__global__ __launch_bounds__(N) void dz_prefix_plan_kernel(const PrefixParams P) {
+  __shared__ PlanRoom<N, KEPT> room;
+  __shared__ int upto[N];
+  __shared__ __attribute__((aligned(16))) Unit made[N];        // a round's units
+  Planner<N, KEPT> plan(P, room);
+  const int tid = threadIdx.x;
+  plan.begin(true);
+  plan.lengths_of_pieces();
+  for (int u0 = 0; u0 < plan.units(); u0 += N) {
+    const int u = u0 + tid, begin = plan.items;
+    Unit x = plan.unit_of(u);
+    upto[tid] = plan.place(x);
+    made[tid] = x;
+    if (u < plan.units()) P.units[plan.entry_of(u)] = x;
+    if (u == plan.groups - 1) P.head[2] = upto[tid];
     __syncthreads();
-    for (int i = begin + tid; i < items0; i += PLAN) {
-      const int at = last_upto(items_to, PLAN, i) + 1;                     // the first unit that ends behind i
-      const int tiles = made[at].x, rest = i - (items_to[at] - tiles * made[at].y);
+    for (int i = begin + tid; i < plan.items; i += N) {
+      const int at = last_upto(upto, N, i) + 1;                // the first unit that ends behind i
+      const Unit& y = made[at];
+      const int tiles = y.tiles, rest = i - (upto[at] - tiles * y.np);
       // tiles that share keys and values next to each other; of a row's, those that see most first
-      if (i < P.room_items) P.items[i] = Item{u0 + at < groups ? u0 + at : P.ngroups + u0 + at - groups, tiles - 1 - rest % tiles, rest / tiles, 0};
+      if (i < P.room_items) P.items[i] = Item{y, tiles - 1 - rest % tiles, rest / tiles, {0, 0}};
     }
     __syncthreads();
   }
-  if (P.starts)
-    for (int t = tid; t < P.tokens; t += PLAN) {
-      int r = rows ? last_upto(KEPT ? (const int*)kept_start : P.starts, rows, t) : -1;
-      if (r >= 0 && t >= start_of(r + 1)) r = -1;
-      P.row_of[t] = r;
-    }
   if (tid == 0) {
-    if (!groups) P.head[2] = 0;
-    const bool fits = items0 <= P.room_items && parts0 <= P.room_parts;
-    if (!fits) atomicOr(P.status, 4u);
-    P.head[0] = fits ? items0 : 0;
-    P.head[1] = work * (float)P.kv_heads * (4.0f * (float)P.dim) > CACHED;
+    plan.tell();
+    if (!plan.groups) P.head[2] = 0;
   }
 }
 
@@ -321,22 +375,26 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void dz_prefix_kernel(const P
   if (turn >= all) return;
   // prefixes' pieces, which keep the matrix cores busy, and rows' own, which wait for memory: a compute unit each of both, then the others
   const int round = max(1, 256 / P.kv_heads), pairs = min(shared, all - shared) / round, at = turn % (2 * round);
-  const int nth = turn >= pairs * 2 * round ? turn - pairs * round : turn / (2 * round) * round + (at < round ? at : at - round);
-  const bool of_prefix = turn >= pairs * 2 * round ? nth < shared : at < round;
-  const Item item = P.items[turn >= pairs * 2 * round ? (of_prefix ? nth : turn) : of_prefix ? nth : shared + nth];
-  const Unit U = P.units[item.unit];
-  const int queries = U.ntok * P.share, x0 = item.tile * ROWS, in_tile = min(ROWS, queries - x0);
+  int nth = turn;
+  if (turn < pairs * 2 * round)
+    nth = turn / (2 * round) * round + (at < round ? at : shared + at - round);
+  else if (turn - pairs * round < shared)
+    nth = turn - pairs * round;
+  const Item item = P.items[nth];
+  const Unit U = item.unit;
+  const int tile = item.tile, piece = item.piece;
+  const bool once = P.head[1] != 0;
+  const int queries = U.ntok * P.share, x0 = tile * ROWS, in_tile = min(ROWS, queries - x0);
   auto limit_of = [&](int x) { return U.causal ? max(U.n - (U.ntok - 1 - x / P.share), 0) : U.n; };      // tokens that query x sees
   const int end = max(limit_of(x0 + in_tile - 1), U.k0);
   const long long len = end - U.k0;
   // pieces meet between steps, and steps lie in whole pages or hold whole pages
   auto bound = [&](int p) { return p == U.np ? end : max(U.k0, (U.k0 + (int)(len * p / U.np)) & ~(STEP - 1)); };
-  const int lo = bound(item.piece), hi = bound(item.piece + 1), begin = lo < hi ? lo & ~(STEP - 1) : hi;
+  const int lo = bound(piece), hi = bound(piece + 1), begin = lo < hi ? lo & ~(STEP - 1) : hi;
 
   if (queries <= FEW) {
-    few_queries<KC, FULL, BF>(P, U, item.piece, kvh, lo, hi, P.head[1] != 0, (float*)lds);
-    return;
-  }
+    few_queries<KC, FULL, BF>(P, U, piece, kvh, lo, hi, once, (float*)lds);
+  } else {
   const int last_page = (hi - 1) >> P.shift, in_page = (1 << P.shift) - 1;
   const int* table = P.tables + U.row * P.table_row;
   int page0 = begin >> P.shift;        // of the 64 page numbers that the lanes hold
@@ -565,7 +623,7 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void dz_prefix_kernel(const P
       if (x >= in_tile) continue;
       const int xx = x0 + x;
       if (U.part >= 0) {
-        float* record = P.parts + (U.part + ((long long)item.piece * P.kv_heads + kvh) * queries + xx) * (P.dim + 4);
+        float* record = P.parts + (U.part + ((long long)piece * P.kv_heads + kvh) * queries + xx) * (P.dim + 4);
 #pragma unroll
         for (int j = 0; j < 2 * KC; ++j)
           if (FULL || 16 * j + 4 * g < P.dim) *(f4_t*)(record + 16 * j + 4 * g) = acc[n][j];
@@ -587,6 +645,7 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void dz_prefix_kernel(const P
     work(std::integral_constant<int, 2>());
   else
     work(std::integral_constant<int, 1>());
+  }
 }
 
 // The pieces of a token's row's sums and of its group's joined, or zeros.  A thread takes four values of a head over every SLICES-th
@@ -596,7 +655,23 @@ __global__ __launch_bounds__(256) void dz_prefix_join_kernel(const PrefixParams 
   typedef Type<BF> Ty;
   constexpr int SPOTS = 256 / SLICES, AT_ONCE = 4;
   __shared__ float shared[SLICES > 1 ? 256 * 8 : 1];
-  const int t = blockIdx.x, row = P.starts ? P.row_of[t] : t;
+  const int t = blockIdx.x;
+  int row = t;
+  if (P.starts) {
+    __shared__ int found;
+    if (P.rows <= 1024) {
+      if (threadIdx.x == 0) found = -1;
+      __syncthreads();
+      for (int r = threadIdx.x; r < P.rows; r += 256)
+        if (P.starts[r] <= t && t < P.starts[r + 1]) found = r;
+      __syncthreads();
+      row = found;
+    } else {
+      row = last_upto(P.starts, P.rows, t);
+      if (row >= 0 && t >= P.starts[row + 1]) row = -1;
+    }
+  }
+  if (P.head[3]) row = -1;
   Unit own = {0, 0, 0, 0, 0, 0, 0, -1, -1, 0, 0}, pre = own;
   bool sees = false;
   if (row >= 0) {
@@ -687,20 +762,19 @@ inline bool shapes_fit(int tokens, int rows, int groups, int heads, int kv_heads
 // What a call's plan comes to at most.
 struct Room {
   long long items, parts;              // items of one key head; records
-  size_t units_at, items_at, rows_at, parts_at, bytes;
+  size_t units_at, items_at, parts_at, bytes;
 };
 inline Room room_of(int tokens, int rows, int groups, int heads, int kv_heads, int dim) {
   Room m;
   const long long queries = (long long)tokens * (heads / kv_heads), whole = (queries + ROWS - 1) / ROWS;
   const long long some = rows < tokens ? rows : tokens, both = groups ? 2 : 1;
-  // a unit's tiles: the last one is not full; pieces: of TARGET in all one more of each tile
-  m.items = both * whole + some + (groups < tokens ? groups : tokens) + TARGET / kv_heads + 1;
-  m.parts = both * tokens * heads + (long long)ROWS * (TARGET + kv_heads);
+  // a unit's tiles: the last one is not full; pieces: of those aimed at one more of each tile
+  m.items = both * whole + some + (groups < tokens ? groups : tokens) + (TARGET + TARGET_FEW) / kv_heads + 2;
+  m.parts = both * tokens * heads + (long long)ROWS * (TARGET + kv_heads) + (long long)FEW * (TARGET_FEW + kv_heads);
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
   m.units_at = 256;
   m.items_at = up(m.units_at + sizeof(Unit) * (size_t)(rows + groups));
-  m.rows_at = up(m.items_at + sizeof(Item) * (size_t)m.items);
-  m.parts_at = up(m.rows_at + 4 * (size_t)tokens);
+  m.parts_at = up(m.items_at + sizeof(Item) * (size_t)m.items);
   m.bytes = m.parts_at + (size_t)m.parts * (dim + 4) * 4;
   return m;
 }
@@ -740,7 +814,7 @@ int dz_prefix_attention(const dz_prefix_args* a, void* stream) {
   P.q = (const char*)a->q, P.k = (const char*)a->k_pages, P.v = (const char*)a->v_pages;
   P.tables = a->tables, P.lengths = a->lengths, P.starts = a->starts, P.groups = a->groups, P.prefixes = a->prefixes;
   P.out = (uint16_t*)a->out, P.status = a->status;
-  P.head = (int*)work, P.units = (Unit*)(work + m.units_at), P.items = (Item*)(work + m.items_at), P.row_of = (int*)(work + m.rows_at);
+  P.head = (int*)work, P.units = (Unit*)(work + m.units_at), P.items = (Item*)(work + m.items_at),
   P.parts = (float*)(work + m.parts_at);
   P.q_row = 2 * a->q_row, P.q_head = 2 * a->q_head;
   P.k_page = 2 * a->k_page, P.k_head = 2 * a->k_head, P.k_token = 2 * a->k_token;
@@ -755,6 +829,7 @@ int dz_prefix_attention(const dz_prefix_args* a, void* stream) {
   // 16 tokens that a wavefront asks for lie in one page, within 32 bits
   P.near = a->page_size >= 16 && P.k_token < (1 << 27) && P.v_token < (1 << 27);
   const int kc = chunks_of(a->dim), which = kc * 4 + (a->dim == 32 * kc) * 2 + a->dtype;
+  // two steps' keys and values; or the sums of four wavefronts and their maxima
   // two steps' keys and values; or the sums of four wavefronts and their maxima
   const size_t steps = 2 * (size_t)(8 * kc) * 1024, sums = (4 * FEW * (size_t)(a->dim + 4) + 8 * FEW) * 4, lds = steps > sums ? steps : sums;
   const kernel_t kern = a->dtype == DZ_BF16 ? kernel_for<true>(a->dim) : kernel_for<false>(a->dim);
