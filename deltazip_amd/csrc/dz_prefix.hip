@@ -25,11 +25,12 @@ typedef short s8_t __attribute__((ext_vector_type(8)));
 
 constexpr int ROWS = 128;              // queries of a workgroup
 constexpr int FEW = 16;                // queries of a unit up to which wavefronts share out its tokens and not its queries
+constexpr int SHORT = 256;             // tokens of such a unit up to which a wavefront may take it alone
 constexpr float CACHED = 64 << 20;     // bytes of keys and values up to which they may be in the last cache
 constexpr int STEP = 64;               // tokens of a step
 constexpr int TARGET = 512;            // pieces that the work is cut into at most, units' last ones apart
 constexpr int TARGET_FEW = 2048;       // and those of units of few queries, whose sums take little room
-constexpr int LEAST = 256;             // tokens of a piece
+constexpr int LEAST = 256, ENOUGH = 1024;   // tokens of a piece; where there are enough tiles without them
 constexpr int GROUPS = DZ_PREFIX_GROUPS;
 
 struct Unit {
@@ -51,7 +52,9 @@ struct PrefixParams {
   uint16_t* out;
   unsigned* status;
   int* head;                           // [0]: how many items there are, of them the groups' [2]; [1]: whether keys and values are more than
-                                       // the caches keep; [3]: whether no row has any tokens, as what says so does not fit
+                                       // the caches keep; [3]: whether no row has any tokens, as what says so does not fit; [4]: items of short
+                                       // units, in a list from the end, and [5] how many of them a workgroup takes; [6]: whether outputs are
+                                       // left to the join
   Unit* units;                         // the groups', the rows'
   Item* items;
   float* parts;                        // records of dim + 4 floats: values, maximum, sum
@@ -86,8 +89,8 @@ struct PlanRoom {
   int first[G + 1], cut[G], leader[G], alone[G];       // of groups: rows, prefix, row whose table, tiles apart
   int length[KEPT ? N : 1], start[KEPT ? N + 1 : 1];
   long long wave_parts[N / 64];
-  int wave_items[N / 64];
-  float wave_work[N / 64], wave_few[N / 64];
+  int wave_items[N / 64], wave_shorts[N / 64];
+  float wave_work[N / 64], wave_few[N / 64], wave_tiles[N / 64];
 };
 
 template <int N, bool KEPT>
@@ -98,11 +101,11 @@ struct Planner {
   int rows, groups;                    // that count
   int each, each_few;                  // tokens of a piece
   bool once;                           // keys and values are more than the caches keep
-  int items;                           // in front of the round of units that `place` is at
+  int items, shorts;                   // in front of the round of units that `place` is at
   long long parts;
 
   __device__ __forceinline__ Planner(const PrefixParams& p, PlanRoom<N, KEPT>& s)
-      : P(p), S(s), tid(threadIdx.x), lane(tid & 63), wave(tid >> 6), room(p.pages_per_row << p.shift), items(0), parts(0) {}
+      : P(p), S(s), tid(threadIdx.x), lane(tid & 63), wave(tid >> 6), room(p.pages_per_row << p.shift), items(0), shorts(0), parts(0) {}
 
   __device__ __forceinline__ int length_of(int r) const { return KEPT ? S.length[r] : max(0, min(P.lengths[r], room)); }
   __device__ __forceinline__ int start_of(int r) const { return KEPT ? (P.rows ? S.start[r] : 0) : P.starts ? P.starts[r] : r; }
@@ -184,26 +187,30 @@ struct Planner {
 
   // How long pieces are: tokens times tiles, over the pieces aimed at.
   __device__ __forceinline__ void lengths_of_pieces() {
-    float all = 0.0f, of_few = 0.0f;
+    float all = 0.0f, of_few = 0.0f, tiles = 0.0f;
     for (int u = tid; u < units(); u += N) {
       const Unit x = unit_of(u);
       const float w = (float)x.tiles * (float)(x.n - x.k0);
       all += w;
-      of_few += few(x) ? w : 0.0f;
+      if (few(x))
+        of_few += w;
+      else if (x.n > x.k0)
+        tiles += (float)x.tiles;
     }
-    all = scan_add(all), of_few = scan_add(of_few);
-    if (lane == 63) S.wave_work[wave] = all, S.wave_few[wave] = of_few;
+    all = scan_add(all), of_few = scan_add(of_few), tiles = scan_add(tiles);
+    if (lane == 63) S.wave_work[wave] = all, S.wave_few[wave] = of_few, S.wave_tiles[wave] = tiles;
     __syncthreads();
-    all = of_few = 0.0f;
+    all = of_few = tiles = 0.0f;
 #pragma unroll
-    for (int w = 0; w < N / 64; ++w) all += S.wave_work[w], of_few += S.wave_few[w];
+    for (int w = 0; w < N / 64; ++w) all += S.wave_work[w], of_few += S.wave_few[w], tiles += S.wave_tiles[w];
     // in whole steps (sums above 2^24 are rounded: a piece is a little longer)
-    auto each_of = [&](float work, int target) {
+    auto each_of = [&](float work, int target, int least) {
       const float want = ceilf(work * 1.0001f * (float)P.kv_heads * (1.0f / (float)target) * (1.0f / STEP));
-      return STEP * (int)fminf(fmaxf(want, (float)(LEAST / STEP)), (float)(1 << 24));
+      return STEP * (int)fminf(fmaxf(want, (float)(least / STEP)), (float)(1 << 24));
     };
-    each = each_of(all, TARGET);
-    each_few = min(each, each_of(of_few, TARGET_FEW));
+    // (whole tiles that are enough by themselves are spared the join)
+    each = each_of(all, TARGET, tiles * (float)P.kv_heads >= TARGET ? ENOUGH : LEAST);
+    each_few = min(each, each_of(of_few, TARGET_FEW, LEAST));
     once = all * (float)P.kv_heads * (4.0f * (float)P.dim) > CACHED;
   }
 
@@ -212,32 +219,39 @@ struct Planner {
     return x.tiles ? (x.n - x.k0 + most - 1) / most : 0;
   }
 
-  // The pieces of this thread's unit, of the next N of them: its items end at what is returned, its records begin at x.part.
+  // (queries that see as much as each other: 32 rows of up to 200 tokens of their own 34 -> 32 us; 48 of several new ones 34 -> 42)
+  __device__ __forceinline__ bool is_short(const Unit& x) const { return few(x) && x.np == 1 && x.n - x.k0 <= SHORT && (x.ntok == 1 || !x.causal); }
+
+  // The pieces of this thread's unit, of the next N of them: its items (those of short units in a list of their own) end at what is returned, its
+  // records begin at x.part.
   __device__ __forceinline__ int place(Unit& x) {
     x.np = pieces_of(x);
-    const int mine = x.tiles * x.np;
+    const bool apart = is_short(x);
+    const int mine = apart ? 0 : x.tiles * x.np, mine_short = apart;
     const long long records = x.np > 1 || x.k0 > 0 || !x.causal ? (long long)x.np * x.ntok * P.heads : 0;
-    const int upto = scan_add(mine);
+    const int upto = scan_add(mine), shorts_upto = scan_add(mine_short);
     long long records_upto = records;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
       const long long y = __shfl_up(records_upto, d);
       if (lane >= d) records_upto += y;
     }
-    if (lane == 63) S.wave_items[wave] = upto, S.wave_parts[wave] = records_upto;
+    if (lane == 63) S.wave_items[wave] = upto, S.wave_shorts[wave] = shorts_upto, S.wave_parts[wave] = records_upto;
     __syncthreads();
-    int before = items;
+    int before = items, shorts_before = shorts;
     long long parts_before = parts;
 #pragma unroll
     for (int w = 0; w < N / 64; ++w) {
-      if (w < wave) before += S.wave_items[w], parts_before += S.wave_parts[w];
-      items += S.wave_items[w], parts += S.wave_parts[w];
+      if (w < wave) before += S.wave_items[w], shorts_before += S.wave_shorts[w], parts_before += S.wave_parts[w];
+      items += S.wave_items[w], shorts += S.wave_shorts[w], parts += S.wave_parts[w];
     }
     if (records) x.part = parts_before + records_upto - records;
+    const int at = P.room_items - shorts_before - shorts_upto;
+    if (apart && at >= 0) P.items[at] = Item{x, 0, 0, {0, 0}};             // (from the list's end)
     return before + upto;
   }
 
-  __device__ __forceinline__ bool fits() const { return items <= P.room_items && parts <= P.room_parts; }
+  __device__ __forceinline__ bool fits() const { return items + shorts <= P.room_items && parts <= P.room_parts; }
 
   // What others need to know of all of it.
   __device__ __forceinline__ void tell() const {
@@ -245,6 +259,8 @@ struct Planner {
     P.head[0] = fits() ? items : 0;
     P.head[1] = once;
     P.head[3] = rows < P.rows || !fits();
+    P.head[4] = fits() ? shorts : 0;
+    P.head[5] = (long long)shorts * P.kv_heads > TARGET ? 4 : 1;
   }
 
   // Where unit u's entry is: the groups', then the rows'.
@@ -259,6 +275,7 @@ __global__ __launch_bounds__(N) void dz_prefix_plan_kernel(const PrefixParams P)
   __shared__ __attribute__((aligned(16))) Unit made[N];        // a round's units
   Planner<N, KEPT> plan(P, room);
   const int tid = threadIdx.x;
+  int unfinished = 0;                    // whether anything is left to the join
   plan.begin(true);
   plan.lengths_of_pieces();
   for (int u0 = 0; u0 < plan.units(); u0 += N) {
@@ -266,7 +283,10 @@ __global__ __launch_bounds__(N) void dz_prefix_plan_kernel(const PrefixParams P)
     Unit x = plan.unit_of(u);
     upto[tid] = plan.place(x);
     made[tid] = x;
-    if (u < plan.units()) P.units[plan.entry_of(u)] = x;
+    if (u < plan.units()) {
+      P.units[plan.entry_of(u)] = x;
+      unfinished |= u >= plan.groups && x.ntok > 0 && (x.np != 1 || x.part >= 0);
+    }
     if (u == plan.groups - 1) P.head[2] = upto[tid];
     __syncthreads();
     for (int i = begin + tid; i < plan.items; i += N) {
@@ -278,9 +298,11 @@ __global__ __launch_bounds__(N) void dz_prefix_plan_kernel(const PrefixParams P)
     }
     __syncthreads();
   }
+  unfinished = __syncthreads_or(unfinished);
   if (tid == 0) {
     plan.tell();
     if (!plan.groups) P.head[2] = 0;
+    P.head[6] = unfinished || !plan.fits() || plan.rows < P.rows || !P.rows || plan.start_of(0) > 0 || plan.start_of(P.rows) < P.tokens;
   }
 }
 
@@ -291,10 +313,10 @@ __device__ __forceinline__ int swizzled(int token) {
   return KC % 4 == 0 ? 2 * (token & 7) : KC % 2 == 0 ? 2 * (token >> 1 & 3) : 2 * (token >> 2 & 1);
 }
 
-// A piece of a unit of up to FEW queries: the four wavefronts walk a quarter of its tokens each, with keys and values in registers, and
+// A piece of a unit of up to FEW queries, with keys and values in registers: a wavefront walks it alone, or four a quarter of its tokens each, and
 // join their sums.
 template <int KC, bool FULL, bool BF>
-__device__ __forceinline__ void few_queries(const PrefixParams& P, const Unit& U, int piece, int kvh, int lo, int hi, bool once, float* lds) {
+__device__ __forceinline__ void few_queries(const PrefixParams& P, const Unit& U, int piece, int kvh, int lo, int hi, bool once, bool alone, float* lds) {
   typedef Type<BF> Ty;
   typedef typename Ty::v8 v8;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
@@ -311,7 +333,7 @@ __device__ __forceinline__ void few_queries(const PrefixParams& P, const Unit& U
   }
   const int* table = P.tables + U.row * P.table_row;
   const int tile0 = lo / TILE, tiles = lo < hi ? (hi + TILE - 1) / TILE - tile0 : 0;
-  const int t0 = tile0 + tiles * wave / 4, t1 = tile0 + tiles * (wave + 1) / 4, limit = min(limit_of(mine), hi), seen_by_all = min(limit_of(0), hi);
+  const int t0 = alone ? tile0 : tile0 + tiles * wave / 4, t1 = alone ? tile0 + tiles : tile0 + tiles * (wave + 1) / 4, limit = min(limit_of(mine), hi), seen_by_all = min(limit_of(0), hi);
   if (seen_by_all < hi)
     walk.template run<false, true>(P, table, kvh, lo, hi, t0, t1, limit, seen_by_all);
   else if (once)
@@ -322,6 +344,33 @@ __device__ __forceinline__ void few_queries(const PrefixParams& P, const Unit& U
   sum += __shfl_xor(sum, 16);
   sum += __shfl_xor(sum, 32);
   const int ld = P.dim + 4;
+  if (alone) {
+    if (col >= queries) return;
+    float* record = P.parts + (U.part + ((long long)piece * P.kv_heads + kvh) * queries + col) * ld;
+    uint16_t* out = P.out + (U.tok0 + mine / P.share) * P.out_row + (kvh * P.share + mine % P.share) * P.out_head;
+    const float part = limit_of(mine) > 0 ? 1.0f / sum : 0.0f;
+#pragma unroll
+    for (int b = 0; b < walk.NB; ++b)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int d = 128 * b + 8 * (4 * g + i);
+        if (d >= P.dim) continue;
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = walk.acc[8 * b + j][i];
+        if (U.part >= 0) {
+          *(f4_t*)(record + d) = f4_t{x[0], x[1], x[2], x[3]};
+          *(f4_t*)(record + d + 4) = f4_t{x[4], x[5], x[6], x[7]};
+        } else {
+          u4_t w;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) w[j] = (unsigned)Ty::round(x[2 * j] * part) | (unsigned)Ty::round(x[2 * j + 1] * part) << 16;
+          *(u4_t*)(out + d) = w;
+        }
+      }
+    if (U.part >= 0 && g == 0) *(f2_t*)(record + P.dim) = f2_t{walk.top, sum};
+    return;
+  }
   float *sums = lds + wave * queries * ld, *stat = lds + 4 * FEW * ld;       // [wave][query][dim], then maxima and sums
   if (col < queries) {
 #pragma unroll
@@ -371,19 +420,25 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void dz_prefix_kernel(const P
   constexpr unsigned BAD = BF ? 0x7f80u : 0x7c00u;     // exponent of what is not finite
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
-  const int turn = blockIdx.x / P.kv_heads, kvh = blockIdx.x % P.kv_heads, all = P.head[0], shared = P.head[2];
-  if (turn >= all) return;
-  // prefixes' pieces, which keep the matrix cores busy, and rows' own, which wait for memory: a compute unit each of both, then the others
-  const int round = max(1, 256 / P.kv_heads), pairs = min(shared, all - shared) / round, at = turn % (2 * round);
+  const int turn = blockIdx.x / P.kv_heads, kvh = blockIdx.x % P.kv_heads, all = P.head[0], shared = P.head[2], shorts = P.head[4], together = P.head[5];
+  const bool once = P.head[1] != 0, is_short = turn >= all;
   int nth = turn;
-  if (turn < pairs * 2 * round)
-    nth = turn / (2 * round) * round + (at < round ? at : shared + at - round);
-  else if (turn - pairs * round < shared)
-    nth = turn - pairs * round;
+  if (is_short) {
+    // four at once, where there are many of them: each waits by itself for what it asks for
+    const int at = (turn - all) * together + (together > 1 ? wave : 0);
+    if (at >= shorts) return;
+    nth = P.room_items - 1 - at;
+  } else {
+    // prefixes' pieces, which keep the matrix cores busy, and rows' own, which wait for memory: a compute unit each of both, then the others
+    const int round = max(1, 256 / P.kv_heads), pairs = min(shared, all - shared) / round, at = turn % (2 * round);
+    if (turn < pairs * 2 * round)
+      nth = turn / (2 * round) * round + (at < round ? at : shared + at - round);
+    else if (turn - pairs * round < shared)
+      nth = turn - pairs * round;
+  }
   const Item item = P.items[nth];
   const Unit U = item.unit;
   const int tile = item.tile, piece = item.piece;
-  const bool once = P.head[1] != 0;
   const int queries = U.ntok * P.share, x0 = tile * ROWS, in_tile = min(ROWS, queries - x0);
   auto limit_of = [&](int x) { return U.causal ? max(U.n - (U.ntok - 1 - x / P.share), 0) : U.n; };      // tokens that query x sees
   const int end = max(limit_of(x0 + in_tile - 1), U.k0);
@@ -393,7 +448,7 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void dz_prefix_kernel(const P
   const int lo = bound(piece), hi = bound(piece + 1), begin = lo < hi ? lo & ~(STEP - 1) : hi;
 
   if (queries <= FEW) {
-    few_queries<KC, FULL, BF>(P, U, piece, kvh, lo, hi, once, (float*)lds);
+    few_queries<KC, FULL, BF>(P, U, piece, kvh, lo, hi, once, is_short && together > 1, (float*)lds);
   } else {
   const int last_page = (hi - 1) >> P.shift, in_page = (1 << P.shift) - 1;
   const int* table = P.tables + U.row * P.table_row;
@@ -655,87 +710,91 @@ __global__ __launch_bounds__(256) void dz_prefix_join_kernel(const PrefixParams 
   typedef Type<BF> Ty;
   constexpr int SPOTS = 256 / SLICES, AT_ONCE = 4;
   __shared__ float shared[SLICES > 1 ? 256 * 8 : 1];
-  const int t = blockIdx.x;
-  int row = t;
-  if (P.starts) {
-    __shared__ int found;
-    if (P.rows <= 1024) {
-      if (threadIdx.x == 0) found = -1;
-      __syncthreads();
-      for (int r = threadIdx.x; r < P.rows; r += 256)
-        if (P.starts[r] <= t && t < P.starts[r + 1]) found = r;
-      __syncthreads();
-      row = found;
-    } else {
-      row = last_upto(P.starts, P.rows, t);
-      if (row >= 0 && t >= P.starts[row + 1]) row = -1;
-    }
-  }
-  if (P.head[3]) row = -1;
-  Unit own = {0, 0, 0, 0, 0, 0, 0, -1, -1, 0, 0}, pre = own;
-  bool sees = false;
-  if (row >= 0) {
-    own = P.units[P.ngroups + row];
-    sees = own.n - (own.ntok - 1 - (t - own.tok0)) > 0;
-    if (sees && own.pref >= 0) pre = P.units[own.pref];
-  }
-  if (sees && own.np == 1 && own.part < 0) return;      // (stored already)
-  const int quads = P.dim / 4, places = P.heads * quads;
-  const long long stride = P.dim + 4, pre_queries = (long long)pre.ntok * P.share, own_queries = (long long)own.ntok * P.share;
-  const int pieces = sees ? pre.np + own.np : 0;
-  const int slice = threadIdx.x / SPOTS;
-  for (int x0 = blockIdx.y * SPOTS; x0 < places; x0 += gridDim.y * SPOTS) {
-    const int x = x0 + threadIdx.x % SPOTS, h = min(x, places - 1) / quads, d = x % quads * 4, kvh = h / P.share, hs = h % P.share;
-    const float* from_pre = P.parts + (pre.part + kvh * pre_queries + (long long)(t - pre.tok0) * P.share + hs) * stride;
-    const float* from_own = P.parts + (own.part + kvh * own_queries + (long long)(t - own.tok0) * P.share + hs) * stride;
-    float m = -INFINITY, l = 0.0f;
-    f4_t o = {0, 0, 0, 0};
-    for (int p0 = slice; p0 < pieces; p0 += SLICES * AT_ONCE) {
-      f4_t w[AT_ONCE];
-      f2_t ml[AT_ONCE];
-      float up = m;
-#pragma unroll
-      for (int i = 0; i < AT_ONCE; ++i) {
-        const int p = min(p0 + i * SLICES, pieces - 1);
-        const float* record = p < pre.np ? from_pre + p * (P.kv_heads * pre_queries * stride) : from_own + (p - pre.np) * (P.kv_heads * own_queries * stride);
-        w[i] = *(const f4_t*)(record + d);
-        ml[i] = *(const f2_t*)(record + P.dim);
-      }
-#pragma unroll
-      for (int i = 0; i < AT_ONCE; ++i) {
-        if (p0 + i * SLICES >= pieces) ml[i] = f2_t{-INFINITY, 0.0f}, w[i] = f4_t{0, 0, 0, 0};       // (the last one a second time)
-        up = fmaxf(up, ml[i][0]);
-      }
-      const float f = weight_of(m, up);
-      l *= f, o *= f, m = up;
-#pragma unroll
-      for (int i = 0; i < AT_ONCE; ++i) {
-        const float fs = weight_of(ml[i][0], up);
-        l += ml[i][1] * fs;
-        o += w[i] * fs;
+  if (!P.head[6]) return;
+  const bool none = P.head[3] != 0;
+  for (int t = blockIdx.x; t < P.tokens; t += gridDim.x) {
+    int row = t;
+    if (P.starts) {
+      __shared__ int found;
+      if (P.rows <= 1024) {
+        __syncthreads();
+        if (threadIdx.x == 0) found = -1;
+        __syncthreads();
+        for (int r = threadIdx.x; r < P.rows; r += 256)
+          if (P.starts[r] <= t && t < P.starts[r + 1]) found = r;
+        __syncthreads();
+        row = found;
+      } else {
+        row = last_upto(P.starts, P.rows, t);
+        if (row >= 0 && t >= P.starts[row + 1]) row = -1;
       }
     }
-    if constexpr (SLICES > 1) {
-      float* mine = shared + threadIdx.x * 8;
-      *(f4_t*)mine = o;
-      *(f2_t*)(mine + 4) = f2_t{m, l};
-      __syncthreads();
-      if (slice == 0) {
-        const float* all = shared + threadIdx.x * 8;
-        for (int c = 1; c < SLICES; ++c) m = fmaxf(m, all[c * SPOTS * 8 + 4]);
-        l = 0.0f, o = f4_t{0, 0, 0, 0};
-        for (int c = 0; c < SLICES; ++c) {
-          const float f = weight_of(all[c * SPOTS * 8 + 4], m);
-          l += all[c * SPOTS * 8 + 5] * f;
-          o += *(const f4_t*)(all + c * SPOTS * 8) * f;
+    if (none) row = -1;
+    Unit own = {0, 0, 0, 0, 0, 0, 0, -1, -1, 0, 0}, pre = own;
+    bool sees = false;
+    if (row >= 0) {
+      own = P.units[P.ngroups + row];
+      sees = own.n - (own.ntok - 1 - (t - own.tok0)) > 0;
+      if (sees && own.pref >= 0) pre = P.units[own.pref];
+    }
+    if (sees && own.np == 1 && own.part < 0) continue;    // (stored already)
+    const int quads = P.dim / 4, places = P.heads * quads;
+    const long long stride = P.dim + 4, pre_queries = (long long)pre.ntok * P.share, own_queries = (long long)own.ntok * P.share;
+    const int pieces = sees ? pre.np + own.np : 0;
+    const int slice = threadIdx.x / SPOTS;
+    for (int x0 = blockIdx.y * SPOTS; x0 < places; x0 += gridDim.y * SPOTS) {
+      const int x = x0 + threadIdx.x % SPOTS, h = min(x, places - 1) / quads, d = x % quads * 4, kvh = h / P.share, hs = h % P.share;
+      const float* from_pre = P.parts + (pre.part + kvh * pre_queries + (long long)(t - pre.tok0) * P.share + hs) * stride;
+      const float* from_own = P.parts + (own.part + kvh * own_queries + (long long)(t - own.tok0) * P.share + hs) * stride;
+      float m = -INFINITY, l = 0.0f;
+      f4_t o = {0, 0, 0, 0};
+      for (int p0 = slice; p0 < pieces; p0 += SLICES * AT_ONCE) {
+        f4_t w[AT_ONCE];
+        f2_t ml[AT_ONCE];
+        float up = m;
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+          const int p = min(p0 + i * SLICES, pieces - 1);
+          const float* record = p < pre.np ? from_pre + p * (P.kv_heads * pre_queries * stride) : from_own + (p - pre.np) * (P.kv_heads * own_queries * stride);
+          w[i] = *(const f4_t*)(record + d);
+          ml[i] = *(const f2_t*)(record + P.dim);
+        }
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+          if (p0 + i * SLICES >= pieces) ml[i] = f2_t{-INFINITY, 0.0f}, w[i] = f4_t{0, 0, 0, 0};       // (the last one a second time)
+          up = fmaxf(up, ml[i][0]);
+        }
+        const float f = weight_of(m, up);
+        l *= f, o *= f, m = up;
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+          const float fs = weight_of(ml[i][0], up);
+          l += ml[i][1] * fs;
+          o += w[i] * fs;
         }
       }
-      __syncthreads();
-    }
-    if (slice == 0 && x < places) {
-      const f4_t y = sees ? o * (1.0f / l) : f4_t{0, 0, 0, 0};
-      const u2_t w = {(unsigned)Ty::round(y[0]) | (unsigned)Ty::round(y[1]) << 16, (unsigned)Ty::round(y[2]) | (unsigned)Ty::round(y[3]) << 16};
-      *(u2_t*)(P.out + t * P.out_row + h * P.out_head + d) = w;
+      if constexpr (SLICES > 1) {
+        float* mine = shared + threadIdx.x * 8;
+        *(f4_t*)mine = o;
+        *(f2_t*)(mine + 4) = f2_t{m, l};
+        __syncthreads();
+        if (slice == 0) {
+          const float* all = shared + threadIdx.x * 8;
+          for (int c = 1; c < SLICES; ++c) m = fmaxf(m, all[c * SPOTS * 8 + 4]);
+          l = 0.0f, o = f4_t{0, 0, 0, 0};
+          for (int c = 0; c < SLICES; ++c) {
+            const float f = weight_of(all[c * SPOTS * 8 + 4], m);
+            l += all[c * SPOTS * 8 + 5] * f;
+            o += *(const f4_t*)(all + c * SPOTS * 8) * f;
+          }
+        }
+        __syncthreads();
+      }
+      if (slice == 0 && x < places) {
+        const f4_t y = sees ? o * (1.0f / l) : f4_t{0, 0, 0, 0};
+        const u2_t w = {(unsigned)Ty::round(y[0]) | (unsigned)Ty::round(y[1]) << 16, (unsigned)Ty::round(y[2]) | (unsigned)Ty::round(y[3]) << 16};
+        *(u2_t*)(P.out + t * P.out_row + h * P.out_head + d) = w;
+      }
     }
   }
 }
@@ -761,7 +820,7 @@ inline bool shapes_fit(int tokens, int rows, int groups, int heads, int kv_heads
 
 // What a call's plan comes to at most.
 struct Room {
-  long long items, parts;              // items of one key head; records
+  long long items, tiles, parts;       // items of one key head, in so many tiles; records
   size_t units_at, items_at, parts_at, bytes;
 };
 inline Room room_of(int tokens, int rows, int groups, int heads, int kv_heads, int dim) {
@@ -769,7 +828,8 @@ inline Room room_of(int tokens, int rows, int groups, int heads, int kv_heads, i
   const long long queries = (long long)tokens * (heads / kv_heads), whole = (queries + ROWS - 1) / ROWS;
   const long long some = rows < tokens ? rows : tokens, both = groups ? 2 : 1;
   // a unit's tiles: the last one is not full; pieces: of those aimed at one more of each tile
-  m.items = both * whole + some + (groups < tokens ? groups : tokens) + (TARGET + TARGET_FEW) / kv_heads + 2;
+  m.tiles = both * whole + some + (groups < tokens ? groups : tokens);
+  m.items = m.tiles + (TARGET + TARGET_FEW) / kv_heads + 2;
   m.parts = both * tokens * heads + (long long)ROWS * (TARGET + kv_heads) + (long long)FEW * (TARGET_FEW + kv_heads);
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
   m.units_at = 256;
@@ -806,8 +866,10 @@ int dz_prefix_attention(const dz_prefix_args* a, void* stream) {
   if (a->table_row < 0) return DZ_EPAGES;
   const Room m = room_of(a->tokens, a->rows, a->groups_n, a->heads, a->kv_heads, a->dim);
   if (!a->work || (size_t)a->work_bytes < m.bytes || ((uintptr_t)a->work & 15)) return DZ_EWORKSPACE;
-  const long long grid = m.items * a->kv_heads;
-  if (grid > 0x7fffffffll) return DZ_EPAGES;
+  if (m.items * a->kv_heads > 0x7fffffffll) return DZ_EPAGES;
+  // (what tables hold may allow fewer)
+  const long long cuts = ((long long)a->pages_per_row * a->page_size + LEAST - 1) / LEAST, fewer = m.tiles * (cuts < 1 ? 1 : cuts);
+  const long long grid = (m.items < fewer ? m.items : fewer) * a->kv_heads;
 
   PrefixParams P;
   char* work = (char*)a->work;
@@ -837,7 +899,9 @@ int dz_prefix_attention(const dz_prefix_args* a, void* stream) {
   if (lds > 65536 && !dz_lds_limit_once(attr_done[which], (const void*)kern, (int)lds)) return DZ_ELAUNCH;
   const hipStream_t st = (hipStream_t)stream;
   const int most_units = a->rows > a->groups_n ? a->rows : a->groups_n;
-  if (most_units <= 256)
+  if (a->rows + a->groups_n <= 64)
+    hipLaunchKernelGGL((dz_prefix_plan_kernel<64, true>), dim3(1), dim3(64), 0, st, P);
+  else if (most_units <= 256)
     hipLaunchKernelGGL((dz_prefix_plan_kernel<256, true>), dim3(1), dim3(256), 0, st, P);
   else if (most_units <= 1024)
     hipLaunchKernelGGL((dz_prefix_plan_kernel<1024, true>), dim3(1), dim3(1024), 0, st, P);
@@ -850,7 +914,7 @@ int dz_prefix_attention(const dz_prefix_args* a, void* stream) {
   const long long sets = ((long long)a->heads * (a->dim / 4) * (few ? 8 : 1) + 255) / 256, most = 1 + 8192 / a->tokens;
   const kernel_t join = few ? (a->dtype == DZ_BF16 ? dz_prefix_join_kernel<8, true> : dz_prefix_join_kernel<8, false>)
                             : (a->dtype == DZ_BF16 ? dz_prefix_join_kernel<1, true> : dz_prefix_join_kernel<1, false>);
-  hipLaunchKernelGGL(join, dim3(a->tokens, (unsigned)(sets < most ? sets : most)), dim3(256), 0, st, P);
+  hipLaunchKernelGGL(join, dim3(a->tokens < 2048 ? a->tokens : 2048, (unsigned)(sets < most ? sets : most)), dim3(256), 0, st, P);
   return hipGetLastError() == hipSuccess ? DZ_OK : DZ_ELAUNCH;
 }
 
