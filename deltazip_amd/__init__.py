@@ -16,7 +16,7 @@ from .layers import (BaseLayerWithDelta, ColumnParallelLinearWithDelta, DeltaMap
 from .manager import DeltaModelManager, LRUCacheDeltaModelManager, create_delta_manager
 from .ops import (add_delta, add_delta_slice, apply_delta, apply_delta_batch, apply_delta_into, apply_delta_packed_nslice, apply_delta_embed, apply_delta_uncompressed, compress_delta, dequant, merge, multi_delta_linear,
                   native_sizes, repack_gptq_to_native, unrepack_native_to_gptq, segment, stacked_shapes, tile_base, token_order)
-from .kv_cache import PagedBatch, PagedKVCache
+from .kv_cache import PagedBatch, PagedKVCache, PagedRun
 from .paged import RotaryPositions, TableStep, append_kv, copy_pages, extend_tables, paged_attention, prefix_attention, rotary
 from .quant_linear import QuantLinear
 from .sparsegpt import Quantizer, SparseGPT
@@ -32,5 +32,5 @@ __all__ = [
     "from_layer_logits_processor", "apply_delta_embed", "apply_delta_uncompressed", "compress_delta", "apply_delta_batch", "token_order", "apply_delta_into", "apply_delta_packed_nslice",
     "Quantizer", "SparseGPT", "lossy_compress", "tile_base",
     "PagedBatch", "PagedKVCache", "RotaryPositions", "append_kv", "copy_pages", "paged_attention", "rotary",
-    "TableStep", "extend_tables", "prefix_attention",
+    "PagedRun", "TableStep", "extend_tables", "prefix_attention",
 ]

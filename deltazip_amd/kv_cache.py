@@ -18,7 +18,7 @@ import numpy as np
 import torch
 
 
-from .paged import MAX_DIM, copy_pages
+from .paged import MAX_DIM, MAX_GROUPS, TableStep, copy_pages, extend_tables
 
 
 class OutOfPages(RuntimeError):
@@ -29,19 +29,25 @@ class PagedBatch(NamedTuple):
     """What a step of one new token per row needs of the cache, on the device: the newest token's position and slot
     (int64 [rows]), the tables (int32 [rows, pages]) and lengths (int32 [rows], the new token counted); and, on the host, whether
     most of its rows' pages are another of its rows', too (for `paged_attention`, which takes no notice of it for one row; of
-    one row: whether sharing spares the cache most of as many pages).  A captured step keeps what it was captured with."""
+    one row: whether sharing spares the cache most of as many pages).  A captured step keeps what it was captured with.
+
+    With several new tokens of a row, `starts` (int32 [rows + 1]) says where each row's begin among positions and slots; with prefixes that
+    neighbouring rows share, `groups` (int32 [n + 1]) and `prefixes` (int32 [n]) say which: both as `prefix_attention` takes them."""
     positions: torch.Tensor
     slots: torch.Tensor
     block_tables: torch.Tensor
     lengths: torch.Tensor
     shared: bool = False
+    starts: Optional[torch.Tensor] = None
+    groups: Optional[torch.Tensor] = None
+    prefixes: Optional[torch.Tensor] = None
 
 
 class _Sequence:
-    __slots__ = ("row", "length", "pages")
+    __slots__ = ("row", "length", "pages", "running")
 
     def __init__(self, row: int, length: int, pages: List[int]) -> None:
-        self.row, self.length, self.pages = row, length, pages
+        self.row, self.length, self.pages, self.running = row, length, pages, False
 
 
 class PagedKVCache:
@@ -89,6 +95,8 @@ class PagedKVCache:
         s = self._seqs.get(seq)
         if s is None:
             raise ValueError(f"no sequence {seq!r} in the cache")
+        if s.running:
+            raise ValueError(f"sequence {seq!r} is in a run: what it holds is known when that is finished")
         return s
 
     # -- sequences that come, grow, fork and go ----------------------------------------------
@@ -212,6 +220,8 @@ class PagedKVCache:
     def compact(self) -> int:
         """Moves the pages in use to the front of the pool, in all layers, and returns how many there are: every page from
         that number on is free, so pool[:, :n] is all there is to save or swap out."""
+        if any(s.running for s in self._seqs.values()):
+            raise ValueError("a run holds pages of the cache: it has to be finished first")
         used = [p for p in range(self.num_pages) if self._users[p]]
         n = len(used)
         holes = [p for p in range(n) if not self._users[p]]
@@ -243,11 +253,16 @@ class PagedKVCache:
         both = torch.from_numpy(np.stack((t, pages.astype(np.int64) * self.page_size + t % self.page_size))).to(self.pool.device)
         return both[0], both[1]
 
-    def batch(self, seqs: Sequence[Optional[Hashable]], width: Optional[int] = None, out: Optional[PagedBatch] = None) -> PagedBatch:
+    def batch(self, seqs: Sequence[Optional[Hashable]], width: Optional[int] = None, out: Optional[PagedBatch] = None,
+              tokens: Optional[Sequence[int]] = None, prefix: bool = False) -> PagedBatch:
         """The step's tensors for these sequences, one row each, whose newest token is the one `extend` made room for.  None
         is a padded row: it stores nothing and its attention is zero.  width: pages of a table's row (default: as many
         as the longest needs).  out: a batch of as many rows to write over (a captured step reads it; width is its tables');
-        what is returned has the tensors of `out` and `shared` of these rows."""
+        what is returned has the tensors of `out` and `shared` of these rows.
+
+        tokens: how many of each sequence's newest tokens are new (a prompt's, drafted ones; 0 of a padded row), of which the
+        positions and slots follow each other.  prefix: neighbouring rows that hold the same pages at their beginning are told as groups
+        (as many as there are rows, the last ones empty, so that `out` has the same shape)."""
         rows = len(seqs)
         named = [x for x in seqs if x is not None]
         if len(set(named)) < len(named):
@@ -259,22 +274,39 @@ class PagedKVCache:
         if out is not None:
             if out.lengths.shape[0] != rows:
                 raise ValueError(f"out holds {out.lengths.shape[0]} rows, the batch has {rows}")
+            if tokens is not None or out.starts is not None:
+                raise ValueError("out takes one new token of each row")
+            if (out.groups is not None) != bool(prefix):
+                raise ValueError("out must have been made with prefixes, or without, as the batch is")
             width = out.block_tables.shape[1]
         width = max(need, 1) if width is None else width
         if width < need:
             raise ValueError(f"tables of {width} pages for a sequence that has {need}")
-        host = np.zeros(16 * rows + 4 * rows * (width + 1), dtype=np.uint8)          # one transfer for all four
-        place, slot = (host[8 * rows * i:8 * rows * (i + 1)].view(np.int64) for i in range(2))
-        lengths = host[16 * rows:20 * rows].view(np.int32)
-        tables = host[20 * rows:].view(np.int32).reshape(rows, width)
         at = np.fromiter((0 if s is None else s.row for s in found), np.int64, rows)
         length = np.fromiter((0 if s is None else s.length for s in found), np.int64, rows)
-        real, last = length > 0, np.maximum(length - 1, 0)
-        page = self._rows[at, last // self.page_size]
-        if any(self._users[p] > 1 for p in page[real].tolist()):
+        real = length > 0
+        if tokens is None:
+            n, row, position = rows, slice(None), np.maximum(length - 1, 0)
+        else:
+            new = np.asarray(list(tokens), dtype=np.int64)
+            if new.shape != (rows,) or (new < 0).any() or (new > length).any():
+                raise ValueError("tokens must say of every row how many of its tokens are new, at most as many as it has")
+            begin = np.concatenate((np.zeros(1, np.int64), np.cumsum(new)))
+            n, row = int(begin[-1]), np.repeat(np.arange(rows), new)
+            position = (length - new - begin[:-1])[row] + np.arange(n)
+        groups = min(rows, MAX_GROUPS) if prefix else 0
+        parts = [2 * n, 2 * n, rows, rows * width] + ([rows + 1] if tokens is not None else []) + ([groups + 1, groups] if prefix else [])     # words
+        ends = np.cumsum(parts)
+        host = np.zeros(int(ends[-1]), dtype=np.int32)                               # one transfer for all of it
+        pieces = [host[e - p:e] for e, p in zip(ends, parts)]
+        place, slot = pieces[0].view(np.int64), pieces[1].view(np.int64)
+        lengths, tables = pieces[2], pieces[3].reshape(rows, width)
+        page = self._rows[at[row], position // self.page_size]
+        mine = real[row] if tokens is None else np.ones(n, dtype=bool)
+        if any(self._users[p] > 1 for p in set(page[mine].tolist())):
             raise ValueError("a row's newest token lies in a page that other sequences hold too: extend makes it its own")
-        place[:], lengths[:] = last, length
-        slot[:] = np.where(real, page.astype(np.int64) * self.page_size + last % self.page_size, -1)
+        place[:], lengths[:] = position, length
+        slot[:] = np.where(mine, page.astype(np.int64) * self.page_size + position % self.page_size, -1)
         columns = np.arange(min(width, self.max_pages))
         inside = columns < -(-length // self.page_size)[:, None]
         tables[:, :len(columns)] = np.where(inside, self._rows[at, :len(columns)], 0)
@@ -284,12 +316,142 @@ class PagedKVCache:
             distinct = np.zeros(self.num_pages, dtype=bool)
             distinct[tables[:, :len(columns)][inside]] = True
             shared = 2 * (held - int(distinct.sum())) > held
+        if tokens is not None:
+            pieces[4][:] = begin
+        if prefix:
+            bounds, sizes = self._groups_of(tables[:, :len(columns)], inside.sum(1))
+            pieces[-2][:] = rows
+            pieces[-2][:len(bounds[:groups + 1])], pieces[-1][:len(sizes[:groups])] = bounds[:groups + 1], sizes[:groups]
         dev = torch.from_numpy(host).to(self.pool.device)
-        made = PagedBatch(dev[:8 * rows].view(torch.int64), dev[8 * rows:16 * rows].view(torch.int64),
-                          dev[20 * rows:].view(torch.int32).view(rows, width), dev[16 * rows:20 * rows].view(torch.int32),
-                          shared)
+        made = [dev[e - p:e] for e, p in zip(ends.tolist(), parts)]
+        made = PagedBatch(made[0].view(torch.int64), made[1].view(torch.int64), made[3].view(rows, width), made[2], shared,
+                          made[4] if tokens is not None else None, made[-2] if prefix else None, made[-1] if prefix else None)
         if out is None:
             return made
-        for to, t in zip(out[:4], made):
-            to.copy_(t)
+        for to, t in zip(out, made):
+            if isinstance(t, torch.Tensor):
+                to.copy_(t)
         return out._replace(shared=made.shared)
+
+    def _groups_of(self, tables: np.ndarray, used: np.ndarray) -> Tuple[List[int], List[int]]:
+        """(rows where groups of neighbours begin and the last one ends, tokens that each group's rows have in common).  A row joins the group in front of
+        it where that spares as many pages as the group spared without it."""
+        columns = np.arange(tables.shape[1])
+        same = (tables[1:] == tables[:-1]) & (columns < np.minimum(used[1:], used[:-1])[:, None])
+        common = np.where(same.all(1), len(columns), same.argmin(1)).tolist()        # pages, with the row in front
+        bounds, sizes, first = [0], [], 0
+        while first < len(used):
+            last, cut = first + 1, 0
+            while last < len(used):
+                c = min(cut, common[last - 1]) if cut else common[last - 1]
+                if not c or c * (last - first) < cut * (last - first - 1):
+                    break
+                last, cut = last + 1, c
+            if cut == 0 and sizes and sizes[-1] == 0:
+                bounds[-1] = last
+            else:
+                sizes.append(cut * self.page_size)
+                bounds.append(last)
+            first = last
+        return bounds, sizes
+
+    # -- steps that the device goes by itself ---------------------------------------------------
+    def run(self, seqs: Sequence[Optional[Hashable]], steps: int, prefix: bool = False) -> "PagedRun":
+        """Up to `steps` steps of one token per row without the host: the pages that they may need are set aside (`OutOfPages`: too few), and
+        tables, lengths, positions and slots go on on the device.  Until it is finished these sequences are the run's.
+        None is a padded row.  prefix as for `batch`."""
+        if steps < 1:
+            raise ValueError("steps must be positive")
+        named = [x for x in seqs if x is not None]
+        found = [self._get(x) for x in named]
+        before = [s.length for s in found]
+        if len(set(named)) < len(named):
+            raise ValueError("a sequence is named twice")
+        self.extend(named, steps)                       # (pages that others hold too are copied)
+        free: List[int] = []
+        for s, n in zip(found, before):
+            keep = -(-n // self.page_size)
+            free += s.pages[keep:]
+            del s.pages[keep:]
+            s.length = n
+        try:
+            return PagedRun(self, list(seqs), steps, free, prefix)
+        except BaseException:
+            for page in free:
+                self._release(page)
+            raise
+
+
+class PagedRun:
+    """Steps of a batch whose tables, lengths and free pages stay on the device (`PagedKVCache.run`):
+
+        run = cache.run(seqs, steps=64)
+        for _ in range(64):
+            logits = model.paged_step(tokens, cache, run.step())       # or captured once and replayed
+        run.finish()
+
+    `step` makes room for each row's next token and returns the batch of it, the same tensors every time; `counts` (int32 [rows]: 1, or 0
+    of a row that gets no more tokens) may be written between steps.  A step that needs more pages than were set aside stores
+    nothing, of any row, and is reported through the status word.  A captured step is not replayed once the run is finished: the pages that it writes to may be
+    others'."""
+
+    def __init__(self, cache: PagedKVCache, seqs: List[Optional[Hashable]], steps: int, free: List[int], prefix: bool) -> None:
+        self.cache, self._seqs = cache, seqs
+        found = [None if x is None else cache._get(x) for x in seqs]
+        rows = len(seqs)
+        lengths = np.fromiter((0 if s is None else s.length for s in found), np.int32, rows)
+        width = max([-(-int(n) // cache.page_size) for n in lengths + steps * (lengths >= 0)], default=1) if rows else 1
+        width = min(max(width, 1), cache.max_pages)
+        tables = np.zeros((rows, width), dtype=np.int32)
+        for r, s in enumerate(found):
+            if s is not None:
+                tables[r, :len(s.pages)] = s.pages
+        used = -(-lengths.astype(np.int64) // cache.page_size)
+        real = np.fromiter((s is not None for s in found), np.int32, rows)
+        host = np.concatenate((lengths, real, np.zeros(1, np.int32), np.asarray(free, dtype=np.int32), tables.ravel()))
+        dev = torch.from_numpy(host).to(cache.pool.device)
+        self._lengths, self.counts, self._taken = dev[:rows], dev[rows:2 * rows], dev[2 * rows:2 * rows + 1]
+        self._free, self._tables = dev[2 * rows + 1:2 * rows + 1 + len(free)], dev[2 * rows + 1 + len(free):].view(rows, width)
+        self._out = TableStep(self._lengths, self._taken, torch.empty(rows + 1, dtype=torch.int32, device=dev.device),
+                              *torch.empty((2, rows), dtype=torch.int64, device=dev.device))
+        self._pages, self._finished = free, False
+        groups = prefixes = None
+        shared = False
+        if rows:
+            # (the page that a row's tokens go on in is its own: no group has it)
+            bounds, sizes = cache._groups_of(tables, used)
+            shared = 2 * sum(n // cache.page_size * (b - a - 1) for a, b, n in zip(bounds, bounds[1:], sizes)) > int(used.sum())
+            if prefix:
+                n = min(len(sizes), MAX_GROUPS)
+                both = torch.from_numpy(np.asarray(bounds[:n + 1] + sizes[:n], dtype=np.int32)).to(cache.pool.device)
+                groups, prefixes = both[:n + 1], both[n + 1:]
+        self._batch = PagedBatch(self._out.positions, self._out.slots, self._tables, self._lengths, shared, None, groups, prefixes)
+        for s in found:
+            if s is not None:
+                s.running = True
+
+    def step(self) -> PagedBatch:
+        if self._finished:
+            raise ValueError("the run is finished")
+        extend_tables(self._tables, self._lengths, self.counts, self._free, self._taken, self.cache.page_size, out=self._out)
+        return self._batch
+
+    def finish(self) -> None:
+        """Gives the cache its sequences back, as long as they have become, and the pages that were not needed.  Waits for the device."""
+        if self._finished:
+            return
+        lengths, tables = self._lengths.cpu().numpy(), self._tables.cpu().numpy()
+        cache, taken = self.cache, set()
+        for r, x in enumerate(self._seqs):
+            if x is None:
+                continue
+            s = cache._seqs[x]
+            s.length = int(lengths[r])
+            s.pages[:] = tables[r, :-(-s.length // cache.page_size)].tolist()
+            cache._rows[s.row, :len(s.pages)] = s.pages
+            taken.update(s.pages)
+            s.running = False
+        for page in self._pages:
+            if page not in taken:
+                cache._release(page)
+        self._finished = True

@@ -21,7 +21,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .kv_cache import PagedBatch, PagedKVCache
-from .paged import RotaryPositions, append_kv, paged_attention
+from .paged import RotaryPositions, append_kv, paged_attention, prefix_attention
 
 
 @dataclass
@@ -88,7 +88,10 @@ class LlamaAttention(nn.Module):
         qkv, _ = self.qkv_proj(hidden)
         q, k, v = (t.unflatten(1, (self.num_heads, self.head_dim)) for t in qkv.chunk(3, dim=-1))
         q = append_kv(q, k, v, batch.positions, batch.slots, rope, keys, values)
-        out = paged_attention(q, keys, values, batch.block_tables, batch.lengths, shared=batch.shared)
+        if batch.starts is None and batch.groups is None:
+            out = paged_attention(q, keys, values, batch.block_tables, batch.lengths, shared=batch.shared)
+        else:
+            out = prefix_attention(q, keys, values, batch.block_tables, batch.lengths, starts=batch.starts, groups=batch.groups, prefixes=batch.prefixes)
         out, _ = self.o_proj(out.flatten(1))
         return out
 
@@ -245,8 +248,11 @@ class LlamaForDecodeStep(nn.Module):
     @torch.no_grad()
     def paged_step(self, input_ids: torch.Tensor, cache: PagedKVCache, batch: PagedBatch,
                    sample_rows: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """One decode step of sequences that stand where `batch` says (`cache.extend(seqs)`, then `cache.batch(seqs)`): their
-        new tokens' keys and values go into the cache.  Returns the logits [rows, vocab] of `sample_rows` (default: all)."""
+        """One decode step of sequences that stand where `batch` says (`cache.extend(seqs)`, then `cache.batch(seqs)`; or a
+        `cache.run`'s `step()`): their new tokens' keys and values go into the cache.  Returns the logits [rows, vocab] of `sample_rows` (default: all).
+
+        A batch of several new tokens a row (`cache.batch(seqs, tokens=...)`: prompts, drafted tokens) takes them one after the
+        other, and sample_rows counts tokens (`batch.starts[1:] - 1`: each row's last)."""
         emb = self.model.embed_tokens(input_ids.view(-1))
         hidden = emb if not isinstance(emb, tuple) else emb[0]
         residual = None

@@ -78,6 +78,158 @@ def test_host_tensors_are_refused(dzlib):
 
 
 # ---------------------------------------------------------------------------------------------
+# the cache: groups, several new tokens, runs
+# ---------------------------------------------------------------------------------------------
+
+
+def _cache(device="cpu", pages=200, page_size=8, monkeypatch=None, **kw):
+    from deltazip_amd import PagedKVCache, kv_cache
+    if monkeypatch is not None:
+        def copy(pool, pairs):
+            pool[:, [b for _, b in pairs]] = pool[:, [a for a, _ in pairs]]
+
+        def extend(tables, lengths, counts, free, taken, page_size, tokens=None, out=None):
+            made = ref.extend_tables(tables.tolist(), lengths.tolist(), counts.tolist(), free.tolist(), int(taken), page_size, tokens)
+            if made is None:
+                made = tables.tolist(), lengths.tolist(), int(taken), [0] * (len(lengths) + 1), [0] * len(out.slots), [-1] * len(out.slots)
+            tables.copy_(torch.tensor(made[0], dtype=torch.int32).view_as(tables))
+            for t, x in zip(out, (made[1], [made[2]], *made[3:])):
+                t.copy_(torch.tensor(x, dtype=t.dtype))
+            return out
+        monkeypatch.setattr(kv_cache, "copy_pages", copy)
+        monkeypatch.setattr(kv_cache, "extend_tables", extend)
+    return PagedKVCache(1, pages, page_size, 1, 8, max_tokens=400, device=device, **kw)
+
+
+def test_neighbours_that_share_pages_are_groups(monkeypatch):
+    cache = _cache(monkeypatch=monkeypatch)
+    cache.add("a", 40)
+    cache.add("z", 40)
+    for i in range(4):
+        cache.fork("a", i)
+    cache.extend([0, 1, 2, 3], 9)                    # (their sixth pages are their own)
+    cache.fork(3, "late")
+    cache.extend(["late", "z"])
+    b = cache.batch([0, 1, 2, "z", 3, "late", None], prefix=True)
+    assert b.groups.tolist() == [0, 3, 4, 6, 7, 7, 7, 7] and b.prefixes.tolist() == [40, 0, 48, 0, 0, 0, 0] and b.starts is None
+    # a row joins where that spares as many pages as the group without it did
+    b = cache.batch([3, "late", 0, 1], prefix=True)
+    assert b.groups.tolist() == [0, 4, 4, 4, 4] and b.prefixes.tolist() == [40, 0, 0, 0]
+    again = cache.batch([1, None, "z", 2], prefix=True, out=b)
+    assert again.groups is b.groups and b.groups.tolist() == [0, 4, 4, 4, 4] and b.prefixes.tolist() == [0, 0, 0, 0]
+    assert cache.batch([0, 1]).groups is None and cache.batch([], prefix=True).groups.tolist() == [0]
+    for bad in (dict(out=b), dict(out=cache.batch([0, 1, 2, 3]), prefix=True), dict(out=b, prefix=True, tokens=[1] * 4)):
+        with pytest.raises(ValueError):
+            cache.batch([1, None, "z", 2], **bad)
+
+
+@pytest.mark.parametrize("seed", range(10))
+def test_groups_hold_what_their_rows_share(seed):
+    cache, rng = _cache(), random.Random(seed)
+    rows, w = rng.randrange(1, 30), 12
+    import numpy as np
+    used = np.array([rng.choice([0, rng.randrange(1, w + 1)]) for _ in range(rows)])
+    tables = np.zeros((rows, w), dtype=np.int32)
+    for r in range(rows):
+        if used[r]:
+            keep = rng.choice([0, rng.randrange(0, used[r] + 1)]) if r and used[r - 1] else 0
+            tables[r, :used[r]] = [tables[r - 1, i] if i < min(keep, used[r - 1]) else 100 * r + i + 1 for i in range(used[r])]
+    bounds, sizes = cache._groups_of(tables, used)
+    assert bounds[0] == 0 and bounds[-1] == rows and len(sizes) == len(bounds) - 1 and (np.diff(bounds) > 0).all()
+    for a, b, n in zip(bounds, bounds[1:], sizes):
+        assert n % 8 == 0 and (n == 0 or (b - a > 1 and (used[a:b] >= n // 8).all() and (tables[a:b, :n // 8] == tables[a, :n // 8]).all()))
+
+
+def test_batches_of_several_new_tokens(monkeypatch):
+    cache = _cache(monkeypatch=monkeypatch)
+    cache.add("p", 21)
+    cache.add("q", 5)
+    cache.extend(["q"], 4)
+    b = cache.batch(["p", None, "q"], tokens=[21, 0, 4])
+    assert b.starts.tolist() == [0, 21, 21, 25] and b.lengths.tolist() == [21, 0, 9]
+    assert b.positions.tolist() == list(range(21)) + [5, 6, 7, 8]
+    where = {x: cache.slots(x)[1].tolist() for x in "pq"}
+    assert b.slots.tolist() == where["p"] + where["q"][5:]
+    assert cache.batch([None, "q"], tokens=[0, 0]).positions.numel() == 0
+    for bad in ([22, 0, 1], [1, 1, 1], [1, 0], [-1, 0, 1]):
+        with pytest.raises(ValueError):
+            cache.batch(["p", None, "q"], tokens=bad)
+    cache.fork("p", "r")
+    with pytest.raises(ValueError, match="other sequences"):
+        cache.batch(["r"], tokens=[3])
+    cache.extend(["r"], 12)
+    assert cache.batch(["r"], tokens=[12]).positions.tolist() == list(range(21, 33))
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_runs_give_back_what_they_were(monkeypatch, seed):
+    """Against the same steps by the host: the same tokens in the same places of each sequence, and the same number of free pages."""
+    rng = random.Random(seed)
+    cache = _cache(monkeypatch=monkeypatch)
+    for i in range(5):
+        cache.add(i, rng.randrange(0, 30))
+    cache.add("base", 20)
+    for x in "ab":
+        cache.fork("base", x)
+    seqs = ["a", 0, None, 1, "b", 2]
+    before = {x: cache.length(x) for x in seqs if x is not None}
+    steps = rng.randrange(1, 40)
+    kept = {x: cache.pages(x) for x in ("base", 3, 4)}
+    free = cache.free_pages
+    run = cache.run(seqs, steps)
+    lost = rng.randrange(0, steps + 1)
+    for i in range(lost):
+        if i == lost // 2:
+            run.counts[3] = 0
+        b = run.step()
+        assert b.block_tables is run._tables
+        for r, x in enumerate(seqs):
+            n = int(b.lengths[r])
+            if x is None or (r == 3 and i >= lost // 2):
+                assert int(b.slots[r]) == -1
+            else:
+                assert n == before[x] + i + 1 and int(b.positions[r]) == n - 1
+                assert int(b.slots[r]) == int(b.block_tables[r, (n - 1) // 8]) * 8 + (n - 1) % 8
+    for call in (lambda: cache.extend(["a"]), lambda: cache.free(0), lambda: cache.fork(1, "new"), lambda: cache.batch(["b"]), lambda: cache.compact(),
+                 lambda: cache.truncate(2, 0), lambda: cache.run([0], 1), lambda: cache.length("a"), lambda: cache.slots(0)):
+        with pytest.raises(ValueError, match="run"):
+            call()
+    cache.extend([3, 4], 2)                          # others go on
+    cache.truncate(3, cache.length(3) - 2)
+    cache.truncate(4, cache.length(4) - 2)
+    run.finish()
+    run.finish()
+    with pytest.raises(ValueError, match="finished"):
+        run.step()
+    held = [p for x in list(before) + ["base", 3, 4] for p in cache.pages(x)]
+    for x, n in before.items():
+        assert cache.length(x) == n + (lost // 2 if x == 1 else lost)
+        assert len(cache.pages(x)) == -(-cache.length(x) // 8)
+    assert {x: cache.pages(x) for x in kept} == kept
+    assert cache.free_pages == cache.num_pages - len(set(held))
+    for x in list(before) + ["base", 3, 4]:
+        cache.free(x)
+    assert cache.free_pages == cache.num_pages and sorted(cache._free) == list(range(cache.num_pages)) and cache._spared == 0
+
+
+def test_runs_that_do_not_fit_change_nothing(monkeypatch):
+    from deltazip_amd import kv_cache
+    cache = _cache(monkeypatch=monkeypatch, pages=6)
+    cache.add("a", 20)
+    cache.add("b", 3)
+    with pytest.raises(kv_cache.OutOfPages):
+        cache.run(["a", "b"], 30)
+    for call in (lambda: cache.run(["a"], 0), lambda: cache.run(["a", "a"], 1), lambda: cache.run(["x"], 1), lambda: cache.run(["a"], 1000)):
+        with pytest.raises(ValueError):
+            call()
+    monkeypatch.setattr(kv_cache, "TableStep", None)               # (as where the device has no memory left)
+    with pytest.raises(TypeError):
+        cache.run(["a", "b"], 8)
+    assert cache.free_pages == 2 and cache.length("a") == 20 and cache.length("b") == 3
+    cache.extend(["a", "b"])
+
+
+# ---------------------------------------------------------------------------------------------
 # tables
 # ---------------------------------------------------------------------------------------------
 
@@ -591,3 +743,89 @@ def test_prefix_over_drawn_sizes(dev, seed):
     prefixes = [rng.choice([0, 1, ps, int(2 ** rng.uniform(0, 11))]) for _ in range(n)]
     p = _problem(dev, dtype, prefixes, suffixes, news, groups, heads, kv, dim, ps, seed=seed)
     _hold(_run(p, single=not many), *p, most_rows=200)
+
+
+@pytest.mark.gpu
+def test_steps_prompts_and_runs_of_a_model(dev):
+    """Prompts taken in one pass, chats that share a prefix and a captured step of a run, against the same tokens one at a time."""
+    from test_llama_step import BITS, H, HEADS, LAYERS, V, I, _close, _delta_state_dict
+    from deltazip_amd import CompressionConfig, DeltaConfig, DeltaMapping, DeltaModel, create_delta_manager, ops
+    from deltazip_amd.llama_step import LlamaForDecodeStep, LlamaStepConfig
+    cfg = LlamaStepConfig(hidden_size=H, intermediate_size=I, num_attention_heads=HEADS, num_hidden_layers=LAYERS, vocab_size=V, max_position_embeddings=96)
+    model = LlamaForDecodeStep(cfg, device=dev, generator=torch.Generator(device=dev).manual_seed(4))
+    mgr = create_delta_manager(model, max_num_seqs=64, max_num_batched_tokens=64, vocab_size=V, delta_config=DeltaConfig(max_deltas=3, max_bitwidth=BITS))
+    for d in (1, 2):
+        mgr.add_delta(DeltaModel.from_tensors(_delta_state_dict(1000 * d)[0], d, CompressionConfig(bits=BITS, prunen=2, prunem=4, sparsity=0.5), pin_memory=False))
+        mgr.activate_delta(d)
+
+    def ids(deltas):
+        mgr.set_delta_mapping(DeltaMapping(tuple(deltas), tuple(deltas)))
+
+    g = torch.Generator().manual_seed(1)
+    prompts = [torch.randint(0, V, (n,), generator=g).to(dev) for n in (19, 1, 24)]
+    slow, fast = model.make_paged_cache(60, page_size=8, device=dev), model.make_paged_cache(60, page_size=8, device=dev)
+    for c in (slow, fast):
+        c.pool.fill_(float("nan"))
+    want = []
+    for d, p in enumerate(prompts):                  # token by token
+        slow.add(d)
+        ids([d])
+        for t in range(len(p)):
+            slow.extend([d])
+            last = model.paged_step(p[t:t + 1], slow, slow.batch([d]))
+        want.append(last)
+    for d, p in enumerate(prompts):
+        fast.add(d, len(p))
+    ids([d for d, p in enumerate(prompts) for _ in p])
+    b = fast.batch([0, 1, 2], tokens=[len(p) for p in prompts])
+    got = model.paged_step(torch.cat(prompts), fast, b, sample_rows=(b.starts[1:] - 1).long())
+    assert _close(got.float().cpu().numpy(), torch.cat(want).float().cpu().numpy())
+
+    # chats behind the first and the third prompt
+    for c in (slow, fast):
+        for name, parent in (("a", 0), ("b", 0), ("c", 2), ("d", 2), ("e", 2)):
+            c.fork(parent, name)
+    seqs, deltas = ["a", "b", "c", "d", "e", None], [0, 0, 2, 2, 2, 0]
+    ids(deltas)
+    steps = torch.randint(0, V, (12, 6), generator=g).to(dev)
+    want, got = [], []
+    for t in steps[:2]:
+        for c, kept, prefix in ((slow, want, False), (fast, got, True)):
+            c.extend(seqs[:5])
+            kept.append(model.paged_step(t, c, c.batch(seqs, prefix=prefix)))
+    assert fast.batch(seqs, prefix=True).prefixes.tolist()[:2] == [16, 24]
+    run = fast.run(seqs, 10, prefix=True)
+    batch, words = run.step(), torch.empty(6, dtype=torch.long, device=dev)
+    words.copy_(steps[2])
+    got.append(model.paged_step(words, fast, batch))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        logits = model.paged_step(words, fast, run.step())
+    for t in steps[3:]:
+        words.copy_(t)
+        graph.replay()
+        got.append(logits.clone())
+    for t in steps[2:]:
+        slow.extend(seqs[:5])
+        want.append(model.paged_step(t, slow, slow.batch(seqs)))
+    for x, y in zip(got, want):
+        assert _close(x[:5].float().cpu().numpy(), y[:5].float().cpu().numpy())
+    ops.poll_status(wait=True)
+    run.finish()
+    assert [fast.length(x) for x in seqs[:5]] == [slow.length(x) for x in seqs[:5]] and fast.free_pages == slow.free_pages
+    for x in seqs[:5]:
+        (p, s), (_, z) = fast.slots(x, 24), slow.slots(x, 24)
+        for layer in range(LAYERS):
+            for a, c in ((fast.keys[layer], slow.keys[layer]), (fast.values[layer], slow.values[layer])):
+                x1, x2 = a[s // 8, :, s % 8], c[z // 8, :, z % 8]
+                assert torch.isfinite(x1).all() and _close(x1.float().flatten(1).cpu().numpy(), x2.float().flatten(1).cpu().numpy())
+    # more steps than there are pages for: nothing goes on
+    run, n = fast.run(["a"], 1), fast.num_pages
+    assert fast.free_pages == slow.free_pages
+    for _ in range(3):
+        b = run.step()
+    with pytest.raises(ops.DeltaKernelError, match="paged"):
+        ops.poll_status(wait=True)
+    assert b.slots.tolist() == [-1] and b.lengths.tolist() == [32]
+    run.finish()
+    assert fast.length("a") == 32
