@@ -3,7 +3,7 @@
 // Row r has n tokens and gets c more.  With  need = ceil((n + c) / ps) - ceil(n / ps)  and exclusive sums over the rows
 //   page j of its new ones is  free[taken + sum need + j],  and token i of them stands at position n + i, in place (n + i) % ps of
 //   page (n + i) / ps of its table, and at  sum c + i  of the call's tokens (or, a place a row, at r).
-// Every workgroup sums up all rows by itself, 1024 at a time, and so knows alike whether all of the call fits, and none reads
+// Every workgroup sums up all rows by itself, four a thread at a time, and so knows alike whether all of the call fits, and none reads
 // what another writes.  Lengths and the pages taken may be written over the inputs: that is left to a second launch where there is more
 // than one workgroup.
 #include <hip/hip_runtime.h>
@@ -14,8 +14,7 @@
 
 namespace {
 
-constexpr int THREADS = 1024;
-constexpr int EACH = 4096;             // tokens of a workgroup
+constexpr int ROWS = 4;                // rows, and tokens, that a thread takes side by side
 constexpr int MOST = 1 << 24;          // tokens of a call: of 64 rows no more than 2^30
 
 struct ExtendParams {
@@ -27,6 +26,7 @@ struct ExtendParams {
   long long table_row;
   int rows, width, shift, free_n, tokens, packed;
   int tokens_too, rows_too;            // what this launch writes
+  int each;                            // tokens of a workgroup
 };
 
 struct Sums {
@@ -45,98 +45,136 @@ __device__ __forceinline__ bool row_fits(const ExtendParams& P, int r, int& n, i
 }
 
 // Sums over the rows in front of each thread's, and of all.
-__device__ __forceinline__ Sums sums_before(int c, int need, Sums& all, int (*shared)[2]) {
+template <int THREADS>
+__device__ __forceinline__ Sums sums_before(long long c, long long need, Sums& all, long long (*shared)[2]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int tokens = scan_add(c), pages = scan_add(need);
+  long long tokens = c, pages = need;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const long long x = __shfl_up(tokens, d), y = __shfl_up(pages, d);
+    if (lane >= d) tokens += x, pages += y;
+  }
   if (lane == 63) shared[wave][0] = tokens, shared[wave][1] = pages;
   __syncthreads();
   Sums before = {tokens - c, pages - need};
   all = Sums{0, 0};
 #pragma unroll
   for (int w = 0; w < THREADS / 64; ++w) {
-    const int a = shared[w][0], b = shared[w][1];
-    if (w < wave) before.tokens += a, before.pages += b;
-    all.tokens += a, all.pages += b;
+    const long long x = shared[w][0], y = shared[w][1];
+    if (w < wave) before.tokens += x, before.pages += y;
+    all.tokens += x, all.pages += y;
   }
   __syncthreads();
   return before;
 }
 
+template <int THREADS>
 __global__ __launch_bounds__(THREADS) void dz_extend_kernel(const ExtendParams P) {
-  __shared__ int shared[THREADS / 64][2];
-  __shared__ int upto[THREADS], had[THREADS], page_at[THREADS];      // of a round's rows: tokens up to its end, length, its first page in the list
+  constexpr int ROUND = THREADS * ROWS;
+  __shared__ long long shared[THREADS / 64][2];
+  __shared__ int upto[ROUND], had[ROUND], page_at[ROUND];            // of a round's rows: tokens up to its end, length, its first page in the list
   const int tid = threadIdx.x, ps = 1 << P.shift;
   const long long taken = P.taken[0];
-  int n = 0, c = 0, need = 0, bad = 0;
+  int n[ROWS], c[ROWS], need[ROWS], bad = 0;
+  auto load = [&](int r0) __attribute__((always_inline)) {
+    bool fits = true;
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      n[i] = c[i] = need[i] = 0;
+      if (r0 + i < P.rows) fits &= row_fits(P, r0 + i, n[i], c[i], need[i]);
+    }
+    return fits;
+  };
+  auto sums = [&](Sums& all) __attribute__((always_inline)) {
+    long long tokens = 0, pages = 0;
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) tokens += c[i], pages += need[i];
+    return sums_before<THREADS>(tokens, pages, all, shared);
+  };
   Sums total = {0, 0}, all = {0, 0}, before = {0, 0};
-  for (int r0 = 0; r0 < P.rows; r0 += THREADS) {
-    n = c = need = 0;
-    if (r0 + tid < P.rows) bad |= !row_fits(P, r0 + tid, n, c, need);
-    before = sums_before(c, need, all, shared);
+  for (int r0 = 0; r0 < P.rows; r0 += ROUND) {
+    bad |= !load(r0 + tid * ROWS);
+    before = sums(all);
     total.tokens += all.tokens, total.pages += all.pages;
   }
   bad |= taken < 0 || taken + total.pages > P.free_n || (P.packed && total.tokens > P.tokens);
   bad = __syncthreads_or(bad);
-  if (bad && blockIdx.x == 0 && tid == 0 && P.tokens_too) atomicOr(P.status, 4u);
   const bool first = blockIdx.x == 0;
-  const int lo = blockIdx.x * EACH, hi = min(P.tokens, lo + EACH);
+  if (bad && first && tid == 0 && P.tokens_too) atomicOr(P.status, 4u);
+  const int lo = blockIdx.x * P.each, hi = min(P.tokens, lo + P.each);
   if (P.tokens_too) {                  // places of no token (all of them, where the call does not fit)
     const int end = bad ? 0 : P.packed ? (int)total.tokens : P.tokens;
     for (int t = max(lo, end) + tid; t < hi; t += THREADS) P.positions[t] = 0, P.slots[t] = -1;
   }
   Sums front = {0, 0};                 // of the rounds before
-  for (int r0 = 0; r0 < P.rows; r0 += THREADS) {
-    const int r = r0 + tid;
-    if (P.rows > THREADS) {            // (one round: they are still there)
-      n = c = need = 0;
-      if (r < P.rows) row_fits(P, r, n, c, need);
-      before = sums_before(c, need, all, shared);
+  for (int r0 = 0; r0 < P.rows; r0 += ROUND) {
+    const int mine = r0 + tid * ROWS;
+    if (P.rows > ROUND) {              // (one round: they are still there)
+      load(mine);
+      before = sums(all);
     }
-    const int start = (int)(front.tokens + before.tokens);
-    const long long page = taken + front.pages + before.pages;
-    if (P.tokens_too) {
-      if (first && r < P.rows) P.starts[r] = bad ? 0 : P.packed ? start : r;
-      if (!bad && !P.packed) {
-        if (r < P.rows && r >= lo && r < hi) {
-          long long slot = -1;
-          if (c) {
-            int* entry = P.tables + r * P.table_row + (n >> P.shift);
-            const int id = need ? P.free[page] : *entry;
-            if (need) *entry = id;
-            if (id < 0)
-              atomicOr(P.status, 4u);
-            else
-              slot = (long long)id * ps + (n & (ps - 1));
-          }
-          P.positions[r] = c ? n : 0;
-          P.slots[r] = slot;
+    int start = (int)(front.tokens + before.tokens);
+    long long page = taken + front.pages + before.pages;
+    int* entry[ROWS];
+    int id[ROWS];
+    if (P.tokens_too && !bad && !P.packed) {
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i) {
+        const int r = mine + i;
+        entry[i] = nullptr, id[i] = 0;
+        if (r < P.rows && r >= lo && r < hi && c[i]) {
+          entry[i] = P.tables + r * P.table_row + (n[i] >> P.shift);
+          id[i] = need[i] ? P.free[page + (i > 0 ? need[0] : 0) + (i > 1 ? need[1] : 0) + (i > 2 ? need[2] : 0)] : *entry[i];
         }
-      } else if (!bad) {
-        upto[tid] = start + c, had[tid] = n, page_at[tid] = (int)page;
-        __syncthreads();
-        const int from = max(lo, (int)front.tokens), to = min(hi, (int)(front.tokens + all.tokens));
-        for (int t = from + tid; t < to; t += THREADS) {
-          int a = 0, b = THREADS - 1;  // the first row that ends behind t
-          while (a < b) {
-            const int mid = (a + b) >> 1;
-            if (upto[mid] > t)
-              b = mid;
-            else
-              a = mid + 1;
-          }
-          const int at = had[a] + t - (a ? upto[a - 1] : (int)front.tokens);
-          const int used = (had[a] + ps - 1) >> P.shift, place = at >> P.shift;
-          int* entry = P.tables + (r0 + a) * P.table_row + place;
-          const int id = place < used ? *entry : P.free[page_at[a] + place - used];
-          if (place >= used && (at & (ps - 1)) == 0) *entry = id;      // (a new page begins with a new token)
-          if (id < 0) atomicOr(P.status, 4u);
-          P.positions[t] = at;
-          P.slots[t] = id < 0 ? -1 : (long long)id * ps + (at & (ps - 1));
-        }
-        __syncthreads();
       }
     }
-    if (P.rows_too && first && r < P.rows) P.lengths_out[r] = bad ? P.lengths[r] : n + c;
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const int r = mine + i;
+      if (P.tokens_too) {
+        if (first && r < P.rows) P.starts[r] = bad ? 0 : P.packed ? start : r;
+        if (!bad && !P.packed && r < P.rows && r >= lo && r < hi) {
+          if (need[i]) *entry[i] = id[i];
+          if (c[i] && id[i] < 0) atomicOr(P.status, 4u);
+          P.positions[r] = c[i] ? n[i] : 0;
+          P.slots[r] = c[i] && id[i] >= 0 ? (long long)id[i] * ps + (n[i] & (ps - 1)) : -1;
+        }
+        if (!bad && P.packed) upto[tid * ROWS + i] = start + c[i], had[tid * ROWS + i] = n[i], page_at[tid * ROWS + i] = (int)page;
+      }
+      if (P.rows_too && first && r < P.rows) P.lengths_out[r] = bad ? P.lengths[r] : n[i] + c[i];
+      start += c[i], page += need[i];
+    }
+    if (P.tokens_too && !bad && P.packed) {
+      __syncthreads();
+      // four tokens a thread of those of this round's rows that are this workgroup's
+      const int from = max(lo, (int)front.tokens), to = min(hi, (int)(front.tokens + all.tokens)), t0 = lo + tid * ROWS;
+      int a = 0;
+      if (t0 + ROWS > from && t0 < to) {
+        int b = ROUND - 1;             // the first row that ends behind the first of them
+        while (a < b) {
+          const int mid = (a + b) >> 1;
+          if (upto[mid] > max(t0, from))
+            b = mid;
+          else
+            a = mid + 1;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i) {
+        const int t = t0 + i;
+        if (t < from || t >= to) continue;
+        while (upto[a] <= t) ++a;      // (some row ends behind t)
+        const int at = had[a] + t - (a ? upto[a - 1] : (int)front.tokens);
+        const int used = (had[a] + ps - 1) >> P.shift, place = at >> P.shift;
+        int* to_entry = P.tables + (r0 + a) * P.table_row + place;
+        const int page_id = place < used ? *to_entry : P.free[page_at[a] + place - used];
+        if (place >= used && (at & (ps - 1)) == 0) *to_entry = page_id;    // (a new page begins with a new token)
+        if (page_id < 0) atomicOr(P.status, 4u);
+        P.positions[t] = at;
+        P.slots[t] = page_id < 0 ? -1 : (long long)page_id * ps + (at & (ps - 1));
+      }
+      __syncthreads();
+    }
     front.tokens += all.tokens, front.pages += all.pages;
   }
   if (first && tid == 0) {
@@ -167,14 +205,26 @@ int dz_extend_tables(const dz_extend_args* a, void* stream) {
   P.positions = (long long*)a->positions, P.slots = (long long*)a->slots, P.status = a->status;
   P.table_row = a->table_row;
   P.rows = a->rows, P.width = a->pages_per_row, P.shift = __builtin_ctz(a->page_size), P.free_n = a->free_n, P.tokens = a->tokens, P.packed = a->packed != 0;
-  const int grid = a->tokens > EACH ? (a->tokens + EACH - 1) / EACH : 1;
+  // threads for all rows in one round, where these are enough (16 rows 6.3 us with 1024, 5.0 with 64); of a token a row each few a workgroup, as
+  // their pages lie apart (1777 rows 8.1 -> 7.4 us), of others four a thread
+  const int threads = a->rows <= 64 * ROWS && a->tokens <= 64 * ROWS ? 64 : a->rows <= 256 * ROWS ? 256 : 1024;
+  P.each = a->packed ? threads * ROWS : 256;
+  const int grid = a->tokens > P.each ? (a->tokens + P.each - 1) / P.each : 1;
   const bool over = a->lengths_out == a->lengths || a->taken_out == a->taken;
   P.tokens_too = 1, P.rows_too = grid == 1 || !over;
   const hipStream_t st = (hipStream_t)stream;
-  hipLaunchKernelGGL(dz_extend_kernel, dim3(grid), dim3(THREADS), 0, st, P);
+  auto launch = [&](int workgroups) {
+    if (threads == 64)
+      hipLaunchKernelGGL(dz_extend_kernel<64>, dim3(workgroups), dim3(64), 0, st, P);
+    else if (threads == 256)
+      hipLaunchKernelGGL(dz_extend_kernel<256>, dim3(workgroups), dim3(256), 0, st, P);
+    else
+      hipLaunchKernelGGL(dz_extend_kernel<1024>, dim3(workgroups), dim3(1024), 0, st, P);
+  };
+  launch(grid);
   if (!P.rows_too) {
     P.tokens_too = 0, P.rows_too = 1;
-    hipLaunchKernelGGL(dz_extend_kernel, dim3(1), dim3(THREADS), 0, st, P);
+    launch(1);
   }
   return hipGetLastError() == hipSuccess ? DZ_OK : DZ_ELAUNCH;
 }

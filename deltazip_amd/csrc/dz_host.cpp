@@ -199,9 +199,9 @@ PyObject* prefix(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// A piece of a tensor's memory as a tensor.
-at::Tensor piece_of(const at::Tensor& t, int64_t from, int64_t n) {
-  at::Tensor y = at::detail::make_tensor<c10::TensorImpl>(c10::TensorImpl::VIEW, c10::Storage(t.storage()), t.key_set(), t.dtype());
+// A piece of a tensor's memory as a tensor, from and n in its elements.
+at::Tensor piece_of(const at::Tensor& t, int64_t from, int64_t n, at::ScalarType type) {
+  at::Tensor y = at::detail::make_tensor<c10::TensorImpl>(c10::TensorImpl::VIEW, c10::Storage(t.storage()), t.key_set(), c10::scalarTypeToTypeMeta(type));
   y.unsafeGetTensorImpl()->set_storage_offset(from);
   y.unsafeGetTensorImpl()->set_sizes_contiguous({n});
   return y;
@@ -226,13 +226,13 @@ PyObject* extend(PyObject*, PyObject* const* a, Py_ssize_t n) {
       !index_on(*taken, 1, at::kInt, dev))
     Py_RETURN_NONE;
   if (!ends_apart(*tables, *lengths) || !ends_apart(*tables, *counts) || !ends_apart(*tables, *free) || !ends_apart(*tables, *taken)) Py_RETURN_NONE;
-  const at::Tensor both = at::empty({2 * tokens}, tables->options().dtype(at::kLong)), rest = at::empty({2 * rows + 2}, tables->options());
+  const at::Tensor room = at::empty({4 * tokens + 2 * rows + 2}, tables->options());      // positions, slots; lengths, pages taken, starts
   dz_extend_args c{};
   c.bytes = sizeof(c);
   c.tables = (int32_t*)tables->data_ptr(), c.lengths = (const int32_t*)lengths->data_ptr(), c.counts = (const int32_t*)counts->data_ptr();
   c.free_pages = (const int32_t*)free->data_ptr(), c.taken = (const int32_t*)taken->data_ptr();
-  c.lengths_out = (int32_t*)rest.data_ptr(), c.taken_out = c.lengths_out + rows, c.starts = c.taken_out + 1;
-  c.positions = (int64_t*)both.data_ptr(), c.slots = c.positions + tokens, c.status = here.status;
+  c.positions = (int64_t*)room.data_ptr(), c.slots = c.positions + tokens, c.status = here.status;
+  c.lengths_out = (int32_t*)(c.slots + tokens), c.taken_out = c.lengths_out + rows, c.starts = c.taken_out + 1;
   c.table_row = step(*tables, 0);
   c.rows = (int)rows, c.pages_per_row = (int)width, c.page_size = (int)ps, c.free_n = (int)pages, c.tokens = (int)tokens, c.packed = a[6] != Py_None;
   int rc;
@@ -242,11 +242,12 @@ PyObject* extend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (rc) Py_RETURN_NONE;
   PyObject* made = PyTuple_New(5);
   if (!made) return nullptr;
-  PyTuple_SET_ITEM(made, 0, THPVariable_Wrap(piece_of(rest, 0, rows)));
-  PyTuple_SET_ITEM(made, 1, THPVariable_Wrap(piece_of(rest, rows, 1)));
-  PyTuple_SET_ITEM(made, 2, THPVariable_Wrap(piece_of(rest, rows + 1, rows + 1)));
-  PyTuple_SET_ITEM(made, 3, THPVariable_Wrap(piece_of(both, 0, tokens)));
-  PyTuple_SET_ITEM(made, 4, THPVariable_Wrap(piece_of(both, tokens, tokens)));
+  const int64_t at = 4 * tokens;
+  PyTuple_SET_ITEM(made, 0, THPVariable_Wrap(piece_of(room, at, rows, at::kInt)));
+  PyTuple_SET_ITEM(made, 1, THPVariable_Wrap(piece_of(room, at + rows, 1, at::kInt)));
+  PyTuple_SET_ITEM(made, 2, THPVariable_Wrap(piece_of(room, at + rows + 1, rows + 1, at::kInt)));
+  PyTuple_SET_ITEM(made, 3, THPVariable_Wrap(piece_of(room, 0, tokens, at::kLong)));
+  PyTuple_SET_ITEM(made, 4, THPVariable_Wrap(piece_of(room, tokens, tokens, at::kLong)));
   return made;
   END_HANDLE_TH_ERRORS
 }
