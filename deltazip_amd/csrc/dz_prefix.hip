@@ -41,6 +41,12 @@ struct Unit {
   long long part;                      // records of its sums, or -1: it has one piece, and nothing else to join
   int causal, pad;
 };
+// What the join needs of a row, its group's part of it among that.
+struct Row {
+  int tok0, ntok, n, np;
+  long long part, pre_part;
+  int pre_tok0, pre_ntok, pre_np, pad;
+};
 struct Item {
   Unit unit;
   int tile, piece, pad[2];
@@ -51,11 +57,12 @@ struct PrefixParams {
   const int *tables, *lengths, *starts, *groups, *prefixes;
   uint16_t* out;
   unsigned* status;
-  int* head;                           // [0]: how many items there are, of them the groups' [2]; [1]: whether keys and values are more than
+  int* head;                           // [0]: how many items there are, [1]: whether keys and values are more than
                                        // the caches keep; [3]: whether no row has any tokens, as what says so does not fit; [4]: items of short
                                        // units, in a list from the end, and [5] how many of them a workgroup takes; [6]: whether outputs are
                                        // left to the join
-  Unit* units;                         // the groups', the rows'
+  Unit* units;                         // the groups'
+  Row* row;                            // the rows'
   Item* items;
   float* parts;                        // records of dim + 4 floats: values, maximum, sum
   long long q_row, q_head, k_page, k_head, k_token, v_page, v_head, v_token, out_row, out_head, table_row;   // bytes; out, table: elements
@@ -81,8 +88,8 @@ __device__ __forceinline__ int last_upto(const T* at, int n, T x) {
   return lo - 1;
 }
 
-// The plan, as N threads of a workgroup make it together.  KEPT: rows, and groups and rows together, are no more than these, and what is known of
-// them stays in LDS.
+// The plan, as N threads of a workgroup make it together.  KEPT: rows and groups together are no more than these, and what is known of them stays in
+// LDS.  The code runs once and from memory: what it need not do is left out of it.
 template <int N, bool KEPT>
 struct PlanRoom {
   static constexpr int G = KEPT ? N : GROUPS;
@@ -118,6 +125,8 @@ struct Planner {
   // Checks what the device alone knows and finds the prefixes that are taken apart from their rows; tell: reports it.
   __device__ __forceinline__ void begin(bool tell) {
     int bad = 0, bad_groups = 0, beyond = 0;
+    int group[3] = {0, 0, 0};          // (asked for together with the rows')
+    if (tid < P.ngroups) group[0] = P.groups[tid], group[1] = P.groups[tid + 1], group[2] = P.prefixes[tid];
     for (int r = tid; r < P.rows; r += N) {
       const int n = P.lengths[r], a = P.starts ? P.starts[r] : r, b = P.starts ? P.starts[r + 1] : r + 1;
       bad |= a < 0 || b < a || b > P.tokens;
@@ -125,10 +134,11 @@ struct Planner {
       if (KEPT) S.length[r] = max(0, min(n, room)), S.start[r] = a, S.start[r + 1] = b;      // (neighbours write the same)
     }
     for (int g = tid; g < P.ngroups; g += N) {
-      const int a = P.groups[g], b = P.groups[g + 1];
+      if (g >= N) group[0] = P.groups[g], group[1] = P.groups[g + 1], group[2] = P.prefixes[g];
+      const int a = group[0], b = group[1];
       bad_groups |= a < 0 || b < a || b > P.rows;
       S.first[g] = a, S.first[g + 1] = b;
-      S.cut[g] = min(P.prefixes[g], room);
+      S.cut[g] = min(group[2], room);
       S.leader[g] = P.rows;
       S.alone[g] = 0;
     }
@@ -185,11 +195,12 @@ struct Planner {
 
   __device__ __forceinline__ bool few(const Unit& x) const { return (long long)x.ntok * P.share <= FEW; }
 
-  // How long pieces are: tokens times tiles, over the pieces aimed at.
-  __device__ __forceinline__ void lengths_of_pieces() {
+  // How long pieces are: tokens times tiles, over the pieces aimed at.  x: this thread's unit, of the last N of them.
+  __device__ __forceinline__ void lengths_of_pieces(Unit& x) {
     float all = 0.0f, of_few = 0.0f, tiles = 0.0f;
-    for (int u = tid; u < units(); u += N) {
-      const Unit x = unit_of(u);
+#pragma unroll 1
+    for (int u0 = 0; u0 < units(); u0 += N) {
+      x = unit_of(u0 + tid);
       const float w = (float)x.tiles * (float)(x.n - x.k0);
       all += w;
       if (few(x))
@@ -201,7 +212,7 @@ struct Planner {
     if (lane == 63) S.wave_work[wave] = all, S.wave_few[wave] = of_few, S.wave_tiles[wave] = tiles;
     __syncthreads();
     all = of_few = tiles = 0.0f;
-#pragma unroll
+#pragma unroll 2
     for (int w = 0; w < N / 64; ++w) all += S.wave_work[w], of_few += S.wave_few[w], tiles += S.wave_tiles[w];
     // in whole steps (sums above 2^24 are rounded: a piece is a little longer)
     auto each_of = [&](float work, int target, int least) {
@@ -231,16 +242,20 @@ struct Planner {
     const long long records = x.np > 1 || x.k0 > 0 || !x.causal ? (long long)x.np * x.ntok * P.heads : 0;
     const int upto = scan_add(mine), shorts_upto = scan_add(mine_short);
     long long records_upto = records;
+    if (KEPT) {                        // (fewer than 2^31)
+      records_upto = scan_add((int)records);
+    } else {
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const long long y = __shfl_up(records_upto, d);
-      if (lane >= d) records_upto += y;
+      for (int d = 1; d < 64; d *= 2) {
+        const long long y = __shfl_up(records_upto, d);
+        if (lane >= d) records_upto += y;
+      }
     }
     if (lane == 63) S.wave_items[wave] = upto, S.wave_shorts[wave] = shorts_upto, S.wave_parts[wave] = records_upto;
     __syncthreads();
     int before = items, shorts_before = shorts;
     long long parts_before = parts;
-#pragma unroll
+#pragma unroll 2
     for (int w = 0; w < N / 64; ++w) {
       if (w < wave) before += S.wave_items[w], shorts_before += S.wave_shorts[w], parts_before += S.wave_parts[w];
       items += S.wave_items[w], shorts += S.wave_shorts[w], parts += S.wave_parts[w];
@@ -262,46 +277,59 @@ struct Planner {
     P.head[4] = fits() ? shorts : 0;
     P.head[5] = (long long)shorts * P.kv_heads > TARGET ? 4 : 1;
   }
-
-  // Where unit u's entry is: the groups', then the rows'.
-  __device__ __forceinline__ int entry_of(int u) const { return u < groups ? u : P.ngroups + u - groups; }
 };
 
 // One workgroup.
 template <int N, bool KEPT>
 __global__ __launch_bounds__(N) void dz_prefix_plan_kernel(const PrefixParams P) {
   __shared__ PlanRoom<N, KEPT> room;
-  __shared__ int upto[N];
+  __shared__ int upto[N], of_groups;
   __shared__ __attribute__((aligned(16))) Unit made[N];        // a round's units
   Planner<N, KEPT> plan(P, room);
   const int tid = threadIdx.x;
   int unfinished = 0;                    // whether anything is left to the join
   plan.begin(true);
-  plan.lengths_of_pieces();
+  Unit x = {0, 0, 0, 0, 0, 0, 0, -1, -1, 0, 0};
+  plan.lengths_of_pieces(x);
   for (int u0 = 0; u0 < plan.units(); u0 += N) {
     const int u = u0 + tid, begin = plan.items;
-    Unit x = plan.unit_of(u);
+    if (!KEPT) x = plan.unit_of(u);
     upto[tid] = plan.place(x);
     made[tid] = x;
-    if (u < plan.units()) {
-      P.units[plan.entry_of(u)] = x;
-      unfinished |= u >= plan.groups && x.ntok > 0 && (x.np != 1 || x.part >= 0);
-    }
-    if (u == plan.groups - 1) P.head[2] = upto[tid];
+    if (!KEPT && u < plan.groups) P.units[u] = x;
+    // Items in the order in which they are taken: prefixes' pieces, which keep the matrix cores busy, and rows' own, which wait for memory, a compute
+    // unit each of both, then the others (where rows and groups are few).
+    if (u == plan.groups - 1) of_groups = upto[tid];
     __syncthreads();
+    if (u >= plan.groups && u < plan.units()) {
+      unfinished |= x.ntok > 0 && (x.np != 1 || x.part >= 0);
+      Row row = {x.tok0, x.ntok, x.n, x.np, x.part, -1, 0, 0, 0, 0};
+      if (x.pref >= 0) {
+        const Unit pre = KEPT ? made[x.pref] : P.units[x.pref];
+        row.pre_part = pre.part, row.pre_tok0 = pre.tok0, row.pre_ntok = pre.ntok, row.pre_np = pre.np;
+      }
+      P.row[u - plan.groups] = row;
+    }
+    const int shared = KEPT && plan.groups ? of_groups : 0, round = max(1, 256 / P.kv_heads), pairs = min(shared, plan.items - shared) / round;
+    auto place_of = [&](int i) {
+      if (!pairs) return i;
+      const int k = i < shared ? i : i - shared;
+      return k < pairs * round ? k / round * 2 * round + (i < shared ? 0 : round) + k % round : i < shared ? i + pairs * round : i;
+    };
     for (int i = begin + tid; i < plan.items; i += N) {
       const int at = last_upto(upto, N, i) + 1;                // the first unit that ends behind i
       const Unit& y = made[at];
       const int tiles = y.tiles, rest = i - (upto[at] - tiles * y.np);
       // tiles that share keys and values next to each other; of a row's, those that see most first
-      if (i < P.room_items) P.items[i] = Item{y, tiles - 1 - rest % tiles, rest / tiles, {0, 0}};
+      const int to = place_of(i);
+      if (to < P.room_items) P.items[to] = Item{y, tiles - 1 - rest % tiles, rest / tiles, {0, 0}};
     }
+    if (KEPT) break;
     __syncthreads();
   }
   unfinished = __syncthreads_or(unfinished);
   if (tid == 0) {
     plan.tell();
-    if (!plan.groups) P.head[2] = 0;
     P.head[6] = unfinished || !plan.fits() || plan.rows < P.rows || !P.rows || plan.start_of(0) > 0 || plan.start_of(P.rows) < P.tokens;
   }
 }
@@ -420,23 +448,16 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void dz_prefix_kernel(const P
   constexpr unsigned BAD = BF ? 0x7f80u : 0x7c00u;     // exponent of what is not finite
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
-  const int turn = blockIdx.x / P.kv_heads, kvh = blockIdx.x % P.kv_heads, all = P.head[0], shared = P.head[2], shorts = P.head[4], together = P.head[5];
+  const int turn = blockIdx.x / P.kv_heads, kvh = blockIdx.x % P.kv_heads;
+  Item item = P.items[turn];           // (asked for together with what says whether it is one; there are as many places as turns)
+  const int all = P.head[0], shorts = P.head[4], together = P.head[5];
   const bool once = P.head[1] != 0, is_short = turn >= all;
-  int nth = turn;
   if (is_short) {
     // four at once, where there are many of them: each waits by itself for what it asks for
     const int at = (turn - all) * together + (together > 1 ? wave : 0);
     if (at >= shorts) return;
-    nth = P.room_items - 1 - at;
-  } else {
-    // prefixes' pieces, which keep the matrix cores busy, and rows' own, which wait for memory: a compute unit each of both, then the others
-    const int round = max(1, 256 / P.kv_heads), pairs = min(shared, all - shared) / round, at = turn % (2 * round);
-    if (turn < pairs * 2 * round)
-      nth = turn / (2 * round) * round + (at < round ? at : shared + at - round);
-    else if (turn - pairs * round < shared)
-      nth = turn - pairs * round;
+    item = P.items[P.room_items - 1 - at];
   }
-  const Item item = P.items[nth];
   const Unit U = item.unit;
   const int tile = item.tile, piece = item.piece;
   const int queries = U.ntok * P.share, x0 = tile * ROWS, in_tile = min(ROWS, queries - x0);
@@ -514,6 +535,7 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void dz_prefix_kernel(const P
       }
     }
   };
+
   if (begin < hi) issue(begin, 0);
 
   auto work = [&](auto cols) __attribute__((always_inline)) {
@@ -730,21 +752,20 @@ __global__ __launch_bounds__(256) void dz_prefix_join_kernel(const PrefixParams 
       }
     }
     if (none) row = -1;
-    Unit own = {0, 0, 0, 0, 0, 0, 0, -1, -1, 0, 0}, pre = own;
+    Row own = {0, 0, 0, 0, -1, -1, 0, 0, 0, 0};
     bool sees = false;
     if (row >= 0) {
-      own = P.units[P.ngroups + row];
+      own = P.row[row];
       sees = own.n - (own.ntok - 1 - (t - own.tok0)) > 0;
-      if (sees && own.pref >= 0) pre = P.units[own.pref];
     }
     if (sees && own.np == 1 && own.part < 0) continue;    // (stored already)
     const int quads = P.dim / 4, places = P.heads * quads;
-    const long long stride = P.dim + 4, pre_queries = (long long)pre.ntok * P.share, own_queries = (long long)own.ntok * P.share;
-    const int pieces = sees ? pre.np + own.np : 0;
+    const long long stride = P.dim + 4, pre_queries = (long long)own.pre_ntok * P.share, own_queries = (long long)own.ntok * P.share;
+    const int pieces = sees ? own.pre_np + own.np : 0;
     const int slice = threadIdx.x / SPOTS;
     for (int x0 = blockIdx.y * SPOTS; x0 < places; x0 += gridDim.y * SPOTS) {
       const int x = x0 + threadIdx.x % SPOTS, h = min(x, places - 1) / quads, d = x % quads * 4, kvh = h / P.share, hs = h % P.share;
-      const float* from_pre = P.parts + (pre.part + kvh * pre_queries + (long long)(t - pre.tok0) * P.share + hs) * stride;
+      const float* from_pre = P.parts + (own.pre_part + kvh * pre_queries + (long long)(t - own.pre_tok0) * P.share + hs) * stride;
       const float* from_own = P.parts + (own.part + kvh * own_queries + (long long)(t - own.tok0) * P.share + hs) * stride;
       float m = -INFINITY, l = 0.0f;
       f4_t o = {0, 0, 0, 0};
@@ -755,7 +776,7 @@ __global__ __launch_bounds__(256) void dz_prefix_join_kernel(const PrefixParams 
 #pragma unroll
         for (int i = 0; i < AT_ONCE; ++i) {
           const int p = min(p0 + i * SLICES, pieces - 1);
-          const float* record = p < pre.np ? from_pre + p * (P.kv_heads * pre_queries * stride) : from_own + (p - pre.np) * (P.kv_heads * own_queries * stride);
+          const float* record = p < own.pre_np ? from_pre + p * (P.kv_heads * pre_queries * stride) : from_own + (p - own.pre_np) * (P.kv_heads * own_queries * stride);
           w[i] = *(const f4_t*)(record + d);
           ml[i] = *(const f2_t*)(record + P.dim);
         }
@@ -821,7 +842,7 @@ inline bool shapes_fit(int tokens, int rows, int groups, int heads, int kv_heads
 // What a call's plan comes to at most.
 struct Room {
   long long items, tiles, parts;       // items of one key head, in so many tiles; records
-  size_t units_at, items_at, parts_at, bytes;
+  size_t units_at, rows_at, items_at, parts_at, bytes;
 };
 inline Room room_of(int tokens, int rows, int groups, int heads, int kv_heads, int dim) {
   Room m;
@@ -833,7 +854,8 @@ inline Room room_of(int tokens, int rows, int groups, int heads, int kv_heads, i
   m.parts = both * tokens * heads + (long long)ROWS * (TARGET + kv_heads) + (long long)FEW * (TARGET_FEW + kv_heads);
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
   m.units_at = 256;
-  m.items_at = up(m.units_at + sizeof(Unit) * (size_t)(rows + groups));
+  m.rows_at = up(m.units_at + sizeof(Unit) * (size_t)groups);
+  m.items_at = up(m.rows_at + sizeof(Row) * (size_t)rows);
   m.parts_at = up(m.items_at + sizeof(Item) * (size_t)m.items);
   m.bytes = m.parts_at + (size_t)m.parts * (dim + 4) * 4;
   return m;
@@ -876,7 +898,7 @@ int dz_prefix_attention(const dz_prefix_args* a, void* stream) {
   P.q = (const char*)a->q, P.k = (const char*)a->k_pages, P.v = (const char*)a->v_pages;
   P.tables = a->tables, P.lengths = a->lengths, P.starts = a->starts, P.groups = a->groups, P.prefixes = a->prefixes;
   P.out = (uint16_t*)a->out, P.status = a->status;
-  P.head = (int*)work, P.units = (Unit*)(work + m.units_at), P.items = (Item*)(work + m.items_at),
+  P.head = (int*)work, P.units = (Unit*)(work + m.units_at), P.row = (Row*)(work + m.rows_at), P.items = (Item*)(work + m.items_at),
   P.parts = (float*)(work + m.parts_at);
   P.q_row = 2 * a->q_row, P.q_head = 2 * a->q_head;
   P.k_page = 2 * a->k_page, P.k_head = 2 * a->k_head, P.k_token = 2 * a->k_token;
@@ -898,12 +920,12 @@ int dz_prefix_attention(const dz_prefix_args* a, void* stream) {
   static std::atomic<unsigned long long> attr_done[36];        // one per kernel
   if (lds > 65536 && !dz_lds_limit_once(attr_done[which], (const void*)kern, (int)lds)) return DZ_ELAUNCH;
   const hipStream_t st = (hipStream_t)stream;
-  const int most_units = a->rows > a->groups_n ? a->rows : a->groups_n;
-  if (a->rows + a->groups_n <= 64)
+  const int units = m.parts < (1ll << 31) ? a->rows + a->groups_n : 1 << 30;
+  if (units <= 64)
     hipLaunchKernelGGL((dz_prefix_plan_kernel<64, true>), dim3(1), dim3(64), 0, st, P);
-  else if (most_units <= 256)
+  else if (units <= 256)
     hipLaunchKernelGGL((dz_prefix_plan_kernel<256, true>), dim3(1), dim3(256), 0, st, P);
-  else if (most_units <= 1024)
+  else if (units <= 1024)
     hipLaunchKernelGGL((dz_prefix_plan_kernel<1024, true>), dim3(1), dim3(1024), 0, st, P);
   else
     hipLaunchKernelGGL((dz_prefix_plan_kernel<1024, false>), dim3(1), dim3(1024), 0, st, P);
