@@ -220,7 +220,7 @@ struct Planner {
       return STEP * (int)fminf(fmaxf(want, (float)(least / STEP)), (float)(1 << 24));
     };
     // (whole tiles that are enough by themselves are spared the join)
-    each = each_of(all, TARGET, tiles * (float)P.kv_heads >= TARGET ? ENOUGH : LEAST);
+    each = each_of(all, TARGET, tiles * (float)P.kv_heads >= TARGET / 2 ? ENOUGH : LEAST);
     each_few = min(each, each_of(of_few, TARGET_FEW, LEAST));
     once = all * (float)P.kv_heads * (4.0f * (float)P.dim) > CACHED;
   }
@@ -573,6 +573,7 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void dz_prefix_kernel(const P
       const char* keys = at + col * ROW;
       const int turn_k = swizzled<KC>(col);
       f4_t sc[NC][4];
+      constexpr bool AHEAD = KC <= 6;  // (heads of 256: no registers for it)
       v8 kw[2][KC];
       auto load_keys = [&](int a) __attribute__((always_inline)) {
 #pragma unroll
@@ -581,7 +582,8 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void dz_prefix_kernel(const P
       load_keys(0);
 #pragma unroll
       for (int a = 0; a < 4; ++a) {
-        if (a < 3) load_keys(a + 1);
+        if (!AHEAD && a) load_keys(a);
+        if (AHEAD && a < 3) load_keys(a + 1);
 #pragma unroll
         for (int n = 0; n < NC; ++n) sc[n][a] = f4_t{0, 0, 0, 0};
 #pragma unroll
@@ -933,7 +935,7 @@ int dz_prefix_attention(const dz_prefix_args* a, void* stream) {
   // of few outputs the pieces, too, are shared out; of many tokens, most of which are stored already, a workgroup takes all heads
   const long long values = (long long)a->tokens * a->heads * (a->dim / 4);
   const bool few = values <= (1 << 17);
-  const long long sets = ((long long)a->heads * (a->dim / 4) * (few ? 8 : 1) + 255) / 256, most = 1 + 8192 / a->tokens;
+  const long long sets = ((long long)a->heads * (a->dim / 4) * (few ? 8 : 1) + 255) / 256, most = 1 + 2048 / a->tokens;
   const kernel_t join = few ? (a->dtype == DZ_BF16 ? dz_prefix_join_kernel<8, true> : dz_prefix_join_kernel<8, false>)
                             : (a->dtype == DZ_BF16 ? dz_prefix_join_kernel<1, true> : dz_prefix_join_kernel<1, false>);
   hipLaunchKernelGGL(join, dim3(a->tokens < 2048 ? a->tokens : 2048, (unsigned)(sets < most ? sets : most)), dim3(256), 0, st, P);
