@@ -150,10 +150,11 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// prefix(q, k_pages, v_pages, tables, lengths, starts, groups, prefixes (None: there are none), scale or None)
+// prefix(q, k_pages, v_pages, tables, lengths, starts, groups, prefixes (None: there are none), scale or None, bytes of tables up to which rows of one
+// token go one by one)
 PyObject* prefix(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (n != 9) Py_RETURN_NONE;
+  if (n != 10 || !PyLong_CheckExact(a[9])) Py_RETURN_NONE;
   const at::Tensor *q = tensor(a[0]), *k = tensor(a[1]), *v = tensor(a[2]), *tables = tensor(a[3]), *lengths = tensor(a[4]);
   if (!q || !k || !v || !tables || !lengths || !(a[8] == Py_None || PyFloat_CheckExact(a[8])) || !q->is_cuda()) Py_RETURN_NONE;
   const at::Tensor *starts = tensor(a[5]), *groups = tensor(a[6]), *prefixes = tensor(a[7]);
@@ -171,6 +172,14 @@ PyObject* prefix(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!index_on(*lengths, rows, at::kInt, dev) || (starts && !index_on(*starts, rows + 1, at::kInt, dev)) ||
       (prefixes && (!index_on(*prefixes, ngroups, at::kInt, dev) || !index_on(*groups, ngroups + 1, at::kInt, dev))))
     Py_RETURN_NONE;
+  if (!starts && (!ngroups || rows * width * ps * kv_heads * dim * 4 <= PyLong_AsLongLong(a[9]))) {
+    PyObject* const zero = PyLong_FromLong(0);
+    if (!zero) return nullptr;
+    PyObject* const as[] = {a[0], a[1], a[2], a[3], a[4], a[8], zero, ngroups ? Py_True : Py_False};
+    PyObject* const made = attend(nullptr, as, 8);
+    Py_DECREF(zero);
+    return made;
+  }
   const size_t need = dz_prefix_attention_bytes((int)tokens, (int)rows, (int)ngroups, (int)heads, (int)kv_heads, (int)dim);
   if (!need || dz_capture_id(here.stream)) Py_RETURN_NONE;       // (a graph has its own room)
   const Space space = space_of(here, need, *q);

@@ -37,6 +37,9 @@ _EXTEND = struct.Struct("=q11Qq6i")               # dz_extend_args
 MAX_DIM = 256
 COUNTERS = 32768                  # DZ_ATTENTION_COUNTERS
 MAX_GROUPS = 2048                 # DZ_PREFIX_GROUPS
+# Bytes of keys and values that all rows' tables have room for, up to which a call of one new token a row goes row by row: 4 rows of 292 tokens of 32 key
+# heads (20 MB) 8 us and 16 behind their prefix, 32 of 1124 of 8 (149) 22 and 23, 16 of 612 of 32 (164) 26 and 20, 8 of 2148 (283) 28 and 21.
+ROW_BY_ROW = 128 << 20
 
 
 class RotaryPositions:
@@ -351,9 +354,9 @@ def prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     block_tables [rows, n], lengths [rows], scale and strides as for `paged_attention`.
 
     Rows groups[g] .. groups[g + 1] - 1 (int32 [n + 1], rising, up to 2048 groups) have their first prefixes[g] (int32 [n]) tokens in common: samples of
-    one prompt, chats with one system prompt, questions about one document.  They are read through the table of the
-    first of these rows that has tokens; what is longer than the first new token of any of them sees is each row's own.  None: nothing
-    is shared.
+    one prompt, chats with one system prompt, questions about one document.  All of their tables name these pages, or pages that hold the same (one of them
+    is read); what is longer than the first new token of any of them sees is each row's own.  None: nothing is shared.  Where it is one
+    token of each row, and nothing is shared or the tables have little room, rows are taken one by one, as `paged_attention` does.
 
     Tokens of no row (in front of starts[0], behind starts[rows]) and those of rows of length 0 give zeros; nothing that a token
     does not see reaches its output, whatever is there.  Starts that do not rise within q leave all rows without tokens, groups
@@ -361,7 +364,7 @@ def prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     status word.  The weights of 17 and more queries a key (tokens times heads that share one) are rounded to q's type, as their products with the values take
     them.  The same call gives the same bits; they depend on the lengths of all of its rows."""
     if out is None:
-        made = _lib.host().prefix(q, k_pages, v_pages, block_tables, lengths, starts, groups, prefixes, scale)
+        made = _lib.host().prefix(q, k_pages, v_pages, block_tables, lengths, starts, groups, prefixes, scale, ROW_BY_ROW)
         if made is not None:
             return made
     ops._need_cuda(q, k_pages, v_pages, block_tables, lengths, starts, groups, prefixes, out)
@@ -398,6 +401,10 @@ def prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     if prefixes is not None:
         _index("prefixes", prefixes, ngroups, torch.int32)
         _index("groups", groups, ngroups + 1, torch.int32)
+    if starts is None and (not ngroups or rows * width * page_size * kv_heads * dim * 4 <= ROW_BY_ROW):
+        if out is not None:
+            _apart("out", out, groups, prefixes)
+        return paged_attention(q, k_pages, v_pages, block_tables, lengths, scale, out=out, shared=ngroups > 0)
     if out is None:
         out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=q.device)
     else:

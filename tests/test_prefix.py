@@ -428,10 +428,11 @@ HEADS = [(4, 4, 128), (8, 2, 64), (7, 1, 80), (20, 1, 128), (6, 3, 256), (33, 1,
 def test_prefix_of_single_tokens(dev, dtype, heads, kv, dim, ps):
     suffixes = [1, 5, None, 9, 64, 65, 300, 1, 1, 130, None, 7, 40, 3]
     p = _problem(dev, dtype, [96, 333, 64], suffixes, [1] * 14, [0, 7, 10, 13], heads, kv, dim, ps)
-    got = _run(p, single=True)
-    _hold(got, *p)
-    assert torch.equal(got, _run(p, single=True))
-    assert torch.equal(got, _run(p))                               # starts that say the same
+    for single in (True, False):                                   # (starts that say the same; without them so few rows go one by one)
+        got = _run(p, single=single)
+        _hold(got, *p)
+        assert torch.equal(got, _run(p, single=single))
+    assert torch.equal(_run(p, single=True, shared=False), _run(p[:3] + [p[3].clone()] + p[4:], single=True))
 
 
 @pytest.mark.gpu
@@ -452,6 +453,7 @@ def test_prefix_of_several_tokens(dev, dtype, heads, kv, dim, ps):
 def test_prefix_of_long_contexts(dev, dtype, rows, prefix, heads, kv, dim, ps):
     rng = random.Random(rows)
     p = _problem(dev, dtype, [prefix], [rng.randrange(1, 600) for _ in range(rows)], [1] * rows, [0, rows], heads, kv, dim, ps)
+    _hold(_run(p), *p)
     _hold(_run(p, single=True), *p)
 
 
@@ -468,6 +470,7 @@ def test_prompts(dev, dtype, new, earlier, heads, kv, dim):
 def test_prefix_of_any_number_of_rows(dev, rows):
     rng = random.Random(rows)
     p = _problem(dev, torch.float16, [48], [rng.choice([None, 1, 2, 30]) for _ in range(rows)], [1] * rows, [0, rows], 2, 1, 32, 8)
+    _hold(_run(p), *p, most_rows=200)
     _hold(_run(p, single=True), *p, most_rows=200)
 
 
@@ -576,7 +579,7 @@ def test_prefix_far_into_a_large_pool(dev):
     q = torch.randn(2, 4, dim, generator=g).to(dev).bfloat16()
     i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)
     from deltazip_amd import prefix_attention
-    got = prefix_attention(q, k, k, tables, i32(200, 256), groups=i32(0, 2), prefixes=i32(192))
+    got = prefix_attention(q, k, k, tables, i32(200, 256), starts=i32(0, 1, 2), groups=i32(0, 2), prefixes=i32(192))
     _hold(got, q, k, k, tables, i32(200, 256), i32(0, 1, 2), i32(0, 2), i32(192))
 
 
@@ -714,14 +717,14 @@ def test_captured_calls_replay_beside_eager_ones(dev):
 @pytest.mark.gpu
 def test_calls_on_two_streams_do_not_meet(dev):
     ps = [_problem(dev, torch.float16, [1500], [30] * 40, [1] * 40, [0, 40], 8, 8, 64, 16, seed=s) for s in range(2)]
-    want = [_run(p, single=True) for p in ps]
+    want = [_run(p) for p in ps]
     streams = [torch.cuda.Stream(), torch.cuda.Stream()]
     torch.cuda.synchronize()
     for _ in range(20):
         got = []
         for s, p in zip(streams, ps):
             with torch.cuda.stream(s):
-                got.append(_run(p, single=True))
+                got.append(_run(p))
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
 
@@ -742,7 +745,9 @@ def test_prefix_over_drawn_sizes(dev, seed):
     suffixes = [None if s == 0 else s for s in suffixes]
     prefixes = [rng.choice([0, 1, ps, int(2 ** rng.uniform(0, 11))]) for _ in range(n)]
     p = _problem(dev, dtype, prefixes, suffixes, news, groups, heads, kv, dim, ps, seed=seed)
-    _hold(_run(p, single=not many), *p, most_rows=200)
+    _hold(_run(p), *p, most_rows=200)
+    if not many:
+        _hold(_run(p, single=True), *p, most_rows=200)
 
 
 @pytest.mark.gpu
