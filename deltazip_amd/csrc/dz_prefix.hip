@@ -490,18 +490,14 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void dz_prefix_kernel(const P
     for (int i = threadIdx.x; i < 2 * STAGE / 16; i += 256) *(u4_t*)(lds + 16 * i) = u4_t{0, 0, 0, 0};
     __syncthreads();
   }
-  // a wavefront brings in 16 tokens of each step; request i of a lane is for token (64 i + lane) / (4 KC) of them
-  int req_token[KC], req_at[KC];
-  unsigned req_k[KC], req_v[KC];       // bytes from the first of the 16 in their page
-#pragma unroll
-  for (int i = 0; i < KC; ++i) {
-    const int at = 64 * i + lane;
-    req_token[i] = at / (4 * KC);
-    const int c = at % (4 * KC) ^ swizzled<KC>(req_token[i]);
-    req_at[i] = FULL || c < per_row ? 16 * c : -1;
-    req_k[i] = req_token[i] * (unsigned)P.k_token + 16 * c;
-    req_v[i] = req_token[i] * (unsigned)P.v_token + 16 * c;
-  }
+  // A wavefront brings in 16 tokens of each step; request i of a lane is for token (64 i + lane) / (4 KC) of them.
+  struct Request {
+    int token, at;                     // bytes into the token's row, -1: behind the head's end
+  };
+  auto request = [&](int i, int of_lane) __attribute__((always_inline)) {
+    const int token = (64 * i + of_lane) / (4 * KC), c = (64 * i + of_lane) % (4 * KC) ^ swizzled<KC>(token);
+    return Request{token, FULL || c < per_row ? 16 * c : -1};
+  };
   auto bring = [&](const char* from, char* to) __attribute__((always_inline)) {
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (__attribute__((address_space(3))) void*)to, 16, 0, 0);
   };
@@ -513,29 +509,33 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void dz_prefix_kernel(const P
     }
     char* to = lds + buf * STAGE + wave * 16 * ROW;
     const int t0 = s + 16 * wave;
+    int of_lane = lane;
+    if (KC == 8) asm volatile("" : "+v"(of_lane));         // (worked out anew for each step: no registers to keep it)
     if (P.near && t0 + 16 <= hi) {     // all of one page: its place is the wavefront's
       const long long id = __builtin_amdgcn_readlane(ids, (t0 >> P.shift) - page0);
       const char* k = P.k + id * P.k_page + kvh * P.k_head + (t0 & in_page) * P.k_token;
       const char* v = P.v + id * P.v_page + kvh * P.v_head + (t0 & in_page) * P.v_token;
 #pragma unroll
-      for (int i = 0; i < KC; ++i)
-        if (FULL || req_at[i] >= 0) {
-          bring(k + req_k[i], to + i * 1024);
-          bring(v + req_v[i], to + HALF + i * 1024);
+      for (int i = 0; i < KC; ++i) {
+        const Request r = request(i, of_lane);
+        if (FULL || r.at >= 0) {
+          bring(k + (unsigned)(r.token * (unsigned)P.k_token + r.at), to + i * 1024);
+          bring(v + (unsigned)(r.token * (unsigned)P.v_token + r.at), to + HALF + i * 1024);
         }
+      }
     } else {
 #pragma unroll
       for (int i = 0; i < KC; ++i) {
-        const int t = min(t0 + req_token[i], hi - 1);      // (behind the end: the last one again)
+        const Request r = request(i, of_lane);
+        const int t = min(t0 + r.token, hi - 1);           // (behind the end: the last one again)
         const unsigned id = __shfl(ids, (t >> P.shift) - page0);
-        if (FULL || req_at[i] >= 0) {
-          bring(P.k + id * P.k_page + kvh * P.k_head + (t & in_page) * P.k_token + req_at[i], to + i * 1024);
-          bring(P.v + id * P.v_page + kvh * P.v_head + (t & in_page) * P.v_token + req_at[i], to + HALF + i * 1024);
+        if (FULL || r.at >= 0) {
+          bring(P.k + id * P.k_page + kvh * P.k_head + (t & in_page) * P.k_token + r.at, to + i * 1024);
+          bring(P.v + id * P.v_page + kvh * P.v_head + (t & in_page) * P.v_token + r.at, to + HALF + i * 1024);
         }
       }
     }
   };
-
   if (begin < hi) issue(begin, 0);
 
   auto work = [&](auto cols) __attribute__((always_inline)) {
@@ -545,7 +545,11 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void dz_prefix_kernel(const P
     v8 q[NC][KC];
     int lim[NC];
     f4_t acc[NC][2 * KC];
-    float top[NC], sum[NC];
+    float top[NC];
+    f4_t sum[NC];                      // of the weights as they are rounded (a product with ones: what rounding does to a large weight is gone when it is divided by)
+    v8 ones;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ones[e] = Ty::one(1.0f);
     const float scale = fabsf(P.scale);
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
@@ -562,7 +566,7 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void dz_prefix_kernel(const P
         for (int c = 0; c < KC; ++c) q[n][c] = -q[n][c];
       }
       lim[n] = min(limit_of(xx), hi);
-      top[n] = -INFINITY, sum[n] = 0.0f;
+      top[n] = -INFINITY, sum[n] = f4_t{0, 0, 0, 0};
 #pragma unroll
       for (int j = 0; j < 2 * KC; ++j) acc[n][j] = f4_t{0, 0, 0, 0};
     }
@@ -645,10 +649,9 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void dz_prefix_kernel(const P
         const float ref = top[n] == -INFINITY ? 0.0f : Ty::BIAS - top[n];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][e >> 2][e & 3], scale, ref));
-          sum[n] += x;
-          p[n][e >> 3][e & 7] = Ty::one(x);
+          p[n][e >> 3][e & 7] = Ty::one(__builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][e >> 2][e & 3], scale, ref)));
         }
+        sum[n] = Ty::mma(ones, p[n][1], Ty::mma(ones, p[n][0], sum[n]));
       }
       if (__builtin_expect(spoilt, 0)) {
         // a weight of 0 would take what is not finite to queries that do not see it: left out of the products, and added where it is seen
@@ -697,8 +700,6 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void dz_prefix_kernel(const P
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
       const int x = mine + 16 * n + col;
-      sum[n] += __shfl_xor(sum[n], 16);
-      sum[n] += __shfl_xor(sum[n], 32);
       if (x >= in_tile) continue;
       const int xx = x0 + x;
       if (U.part >= 0) {
@@ -706,11 +707,11 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void dz_prefix_kernel(const P
 #pragma unroll
         for (int j = 0; j < 2 * KC; ++j)
           if (FULL || 16 * j + 4 * g < P.dim) *(f4_t*)(record + 16 * j + 4 * g) = acc[n][j];
-        if (g == 0) *(f2_t*)(record + P.dim) = f2_t{top[n], sum[n]};
+        if (g == 0) *(f2_t*)(record + P.dim) = f2_t{top[n], sum[n][0]};
       } else {
         uint16_t* to = P.out + (U.tok0 + xx / P.share) * P.out_row + (kvh * P.share + xx % P.share) * P.out_head;
         const bool sees = limit_of(xx) > 0;
-        const float part = 1.0f / sum[n];
+        const float part = 1.0f / sum[n][0];
 #pragma unroll
         for (int j = 0; j < 2 * KC; ++j) {
           const f4_t y = sees ? acc[n][j] * part : f4_t{0, 0, 0, 0};

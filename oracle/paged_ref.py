@@ -81,11 +81,12 @@ def tokens_as_rows(starts, lengths, tables, groups=None, prefixes=None, page_siz
 
 
 def prefix_bound(want, size, most, dtype, dim, tokens, largest):
-    """attention_bound for weights that are rounded to the type, as 2^(s - m + 14) in float16, which keeps those above 2^-28 of the
-    largest to half a step and of the others all but 2^-39 each."""
+    """attention_bound for weights p that are rounded to the type, p (1 + d) with d up to half a step, in the sum of values and in that of weights:
+    sum p (1 + d) v / sum p (1 + d) is off from sum p v / sum p = o by  sum p d (v - o) / sum p (1 + d),  at most half a step of the sum of
+    p |v| and |o|, over 1 - half a step.  float16 holds 2^(s - m + 14): those above 2^-28 of the largest to half a step, and of the others all but 2^-39 each."""
     half = torch.finfo(dtype).eps / 2
     lost = tokens * 2.0 ** -39 * largest if dtype == torch.float16 else 0.0
-    return attention_bound(want, size, most, dtype, dim, tokens) + half * (1 + half) * size + lost
+    return attention_bound(want, size, most, dtype, dim, tokens) + half * (1 + 2 * half) * (size + want.abs()) + lost
 
 
 def extend_tables(tables, lengths, counts, free, taken, page_size, tokens=None):
