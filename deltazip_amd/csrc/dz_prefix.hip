@@ -10,6 +10,24 @@
 // The work is units (a group's prefix; a row's own tokens) of tiles of 128 queries (a token and one of the heads that share a key)
 // times pieces of the tokens that these see.  dz_prefix_plan_kernel, one workgroup, makes the list of them from the lengths, which only
 // the device knows; a workgroup of dz_prefix_kernel takes one of them for one key head; dz_prefix_join_kernel joins.
+//
+// A tile's workgroup brings 64 tokens' keys and values into LDS (two steps' room, loads that pass the registers by) and has 32 queries a
+// wavefront.  As in dz_attend.h scores are C[token, query] = K Q^T, so that a lane's weights are just what the second product's
+// operand wants of it; the values' operand is read from LDS by the transposing read.  A query tile's operand from LDS serves two
+// matrix instructions; with more queries a wavefront their sums fill the registers that a second workgroup on the compute unit needs.
+// Weights are held in one value of the type, times 2^14 in fp16: two, as for few queries, would be half as many matrix instructions again, where these are the
+// bound.  Outputs are 2.1e-3 (bf16) off in the root mean square where their own rounding is 1.7e-3, 2.4e-4 and 2.1e-4 in fp16.
+//
+// What bounds it: reading keys and values once up to some 180 queries a key, the matrix cores above.  Measured, a pass among others:
+//   a prompt of 8192 tokens of 32 heads of 128, 8 key heads     552 us, 997 TFLOP/s (a library product of 8192^3 1171 to 1220)
+//   16 rows behind 131072 tokens of 8 key heads                 119 us, 4.7 TB/s; 5.8 while all workgroups read
+//   128 rows in 4 groups behind 4096 tokens of 32 key heads     234 us, 5.8 TB/s
+//   203 rows of 64 heads in 3 groups behind 20000 of 8          359 us, 4.0 TB/s and 376 TFLOP/s: neither one's bound; a compute unit's two workgroups are
+//                                                               too few to wait for memory and to multiply at the same time
+//   32 rows behind 2048 of 32                                   32 us: plan 5, pieces 22 (a piece takes 14: memory is waited for in turn), join 5
+// What did not pay: the exponentials of 32 tokens beside the products of the next 32 (more instructions, 560 -> 621 us for 8192 tokens) or of one
+// query tile beside the other's (680: operands read twice); priorities of wavefronts (the same); a queue of items that workgroups which stay take from (203 rows 360 -> 588:
+// registers to keep the plan, and no two tiles of a key head at once); 768 to 1536 pieces (16 rows 122 -> 133 to 147, 128 rows 238 -> 245).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -24,7 +42,9 @@ typedef short s4_t __attribute__((ext_vector_type(4)));
 typedef short s8_t __attribute__((ext_vector_type(8)));
 
 constexpr int ROWS = 128;              // queries of a workgroup
-constexpr int FEW = 16;                // queries of a unit up to which wavefronts share out its tokens and not its queries
+// Queries of a unit up to which wavefronts share out its tokens and not its queries: they wait for memory by themselves and hold weights in two
+// values (128 rows behind 4096 tokens, one query a row's own, 256 -> 239 us).
+constexpr int FEW = 16;
 constexpr int SHORT = 256;             // tokens of such a unit up to which a wavefront may take it alone
 constexpr float CACHED = 64 << 20;     // bytes of keys and values up to which they may be in the last cache
 constexpr int STEP = 64;               // tokens of a step
@@ -854,7 +874,11 @@ inline Room room_of(int tokens, int rows, int groups, int heads, int kv_heads, i
   // a unit's tiles: the last one is not full; pieces: of those aimed at one more of each tile
   m.tiles = both * whole + some + (groups < tokens ? groups : tokens);
   m.items = m.tiles + (TARGET + TARGET_FEW) / kv_heads + 2;
-  m.parts = both * tokens * heads + (long long)ROWS * (TARGET + kv_heads) + (long long)FEW * (TARGET_FEW + kv_heads);
+  // Records: a unit in several pieces has one more than aimed at for each of its queries; in groups every query has one for its row and one for its group.
+  // Units that are longer than a piece have fewer tiles together than there are pieces (a piece is as long as all tiles' tokens over the pieces
+  // aimed at): of them no more than two times as many queries.
+  const long long cut = 2 * ((long long)ROWS * (TARGET + kv_heads) + (long long)FEW * (TARGET_FEW + kv_heads));
+  m.parts = (groups ? 2ll * tokens * heads : (long long)tokens * heads < cut ? (long long)tokens * heads : cut) + cut / 2;
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
   m.units_at = 256;
   m.rows_at = up(m.units_at + sizeof(Unit) * (size_t)groups);
@@ -895,6 +919,7 @@ int dz_prefix_attention(const dz_prefix_args* a, void* stream) {
   // (what tables hold may allow fewer)
   const long long cuts = ((long long)a->pages_per_row * a->page_size + LEAST - 1) / LEAST, fewer = m.tiles * (cuts < 1 ? 1 : cuts);
   const long long grid = (m.items < fewer ? m.items : fewer) * a->kv_heads;
+  if (grid > 0xffffff) return DZ_EPAGES;                       // (of 256 threads each)
 
   PrefixParams P;
   char* work = (char*)a->work;
