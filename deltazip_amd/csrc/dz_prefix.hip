@@ -485,12 +485,13 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void dz_prefix_kernel(const P
   const int end = max(limit_of(x0 + in_tile - 1), U.k0);
   const long long len = end - U.k0;
   // pieces meet between steps, and steps lie in whole pages or hold whole pages
-  auto bound = [&](int p) { return p == U.np ? end : max(U.k0, (U.k0 + (int)(len * p / U.np)) & ~(STEP - 1)); };
+  auto bound = [&](int p) { return p == U.np ? end : p == 0 ? U.k0 : max(U.k0, (U.k0 + (int)(len * p / U.np)) & ~(STEP - 1)); };
   const int lo = bound(piece), hi = bound(piece + 1), begin = lo < hi ? lo & ~(STEP - 1) : hi;
 
   if (queries <= FEW) {
     few_queries<KC, FULL, BF>(P, U, piece, kvh, lo, hi, once, is_short && together > 1, (float*)lds);
-  } else {
+    return;
+  }
   const int last_page = (hi - 1) >> P.shift, in_page = (1 << P.shift) - 1;
   const int* table = P.tables + U.row * P.table_row;
   int page0 = begin >> P.shift;        // of the 64 page numbers that the lanes hold
@@ -745,7 +746,6 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void dz_prefix_kernel(const P
     work(std::integral_constant<int, 2>());
   else
     work(std::integral_constant<int, 1>());
-  }
 }
 
 // The pieces of a token's row's sums and of its group's joined, or zeros.  A thread takes four values of a head over every SLICES-th
