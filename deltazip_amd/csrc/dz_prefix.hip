@@ -19,12 +19,12 @@
 // bound.  Outputs are 2.1e-3 (bf16) off in the root mean square where their own rounding is 1.7e-3, 2.4e-4 and 2.1e-4 in fp16.
 //
 // What bounds it: reading keys and values once up to some 180 queries a key, the matrix cores above.  Measured, a pass among others:
-//   a prompt of 8192 tokens of 32 heads of 128, 8 key heads     552 us, 997 TFLOP/s (a library product of 8192^3 1171 to 1220)
+//   a prompt of 8192 tokens of 32 heads of 128, 8 key heads     555 us, 990 TFLOP/s (a library product of 8192^3 1171 to 1220)
 //   16 rows behind 131072 tokens of 8 key heads                 119 us, 4.7 TB/s; 5.8 while all workgroups read
-//   128 rows in 4 groups behind 4096 tokens of 32 key heads     234 us, 5.8 TB/s
+//   128 rows in 4 groups behind 4096 tokens of 32 key heads     230 us, 5.9 TB/s
 //   203 rows of 64 heads in 3 groups behind 20000 of 8          359 us, 4.0 TB/s and 376 TFLOP/s: neither one's bound; a compute unit's two workgroups are
 //                                                               too few to wait for memory and to multiply at the same time
-//   32 rows behind 2048 of 32                                   32 us: plan 5, pieces 22 (a piece takes 14: memory is waited for in turn), join 5
+//   32 rows behind 2048 of 32                                   31 us: plan 5, pieces 22 (a piece takes 14: memory is waited for in turn), join 5
 // What did not pay: the exponentials of 32 tokens beside the products of the next 32 (more instructions, 560 -> 621 us for 8192 tokens) or of one
 // query tile beside the other's (680: operands read twice); priorities of wavefronts (the same); a queue of items that workgroups which stay take from (203 rows 360 -> 588:
 // registers to keep the plan, and no two tiles of a key head at once); 768 to 1536 pieces (16 rows 122 -> 133 to 147, 128 rows 238 -> 245).
@@ -142,8 +142,8 @@ struct Planner {
     return g >= 0 && r < S.first[g + 1] ? g : -1;
   }
 
-  // Checks what the device alone knows and finds the prefixes that are taken apart from their rows; tell: reports it.
-  __device__ __forceinline__ void begin(bool tell) {
+  // Checks what the device alone knows and finds the prefixes that are taken apart from their rows.
+  __device__ __forceinline__ void begin() {
     int bad = 0, bad_groups = 0, beyond = 0;
     int group[3] = {0, 0, 0};          // (asked for together with the rows')
     if (tid < P.ngroups) group[0] = P.groups[tid], group[1] = P.groups[tid + 1], group[2] = P.prefixes[tid];
@@ -162,10 +162,10 @@ struct Planner {
       S.leader[g] = P.rows;
       S.alone[g] = 0;
     }
-    if (tell && beyond) atomicOr(P.status, 4u);
+    if (beyond) atomicOr(P.status, 4u);
     bad = __syncthreads_or(bad);
     if (P.ngroups) bad_groups = __syncthreads_or(bad_groups);
-    if (tell && (bad || bad_groups) && tid == 0) atomicOr(P.status, 4u);
+    if ((bad || bad_groups) && tid == 0) atomicOr(P.status, 4u);
     rows = bad ? 0 : P.rows, groups = bad || bad_groups ? 0 : P.ngroups;
     if (!groups) return;
     // a prefix ends where the first of its rows' new tokens sees no more of it
@@ -308,7 +308,7 @@ __global__ __launch_bounds__(N) void dz_prefix_plan_kernel(const PrefixParams P)
   Planner<N, KEPT> plan(P, room);
   const int tid = threadIdx.x;
   int unfinished = 0;                    // whether anything is left to the join
-  plan.begin(true);
+  plan.begin();
   Unit x = {0, 0, 0, 0, 0, 0, 0, -1, -1, 0, 0};
   plan.lengths_of_pieces(x);
   for (int u0 = 0; u0 < plan.units(); u0 += N) {
@@ -660,7 +660,8 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void dz_prefix_kernel(const P
         if (__any(most > top[n] + 1.0f)) {
           most = fmaxf(most, __shfl_xor(most, 16));
           most = fmaxf(most, __shfl_xor(most, 32));
-          const float up = fmaxf(most, top[n]);
+          // (each query's by its own scores: another's change nothing of it)
+          const float up = most > top[n] + 1.0f ? most : top[n];
           const float f = top[n] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top[n] - up);
           top[n] = up;
           sum[n] *= f;

@@ -123,6 +123,23 @@ def test_neighbours_that_share_pages_are_groups(monkeypatch):
             cache.batch([1, None, "z", 2], **bad)
 
 
+def test_more_groups_than_a_call_takes(monkeypatch):
+    from deltazip_amd import kv_cache
+    monkeypatch.setattr(kv_cache, "MAX_GROUPS", 2)
+    cache = _cache(monkeypatch=monkeypatch)
+    for i in range(3):
+        cache.add(("p", i), 16)
+        for j in range(2):
+            cache.fork(("p", i), (i, j))
+    seqs = [(i, j) for i in range(3) for j in range(2)]
+    run = cache.run(seqs, 1, prefix=True)
+    b = run.step()
+    assert b.groups.tolist() == [0, 2, 4] and b.prefixes.tolist() == [16, 16]            # (the others read their own)
+    run.finish()
+    b = cache.batch(seqs, prefix=True)
+    assert b.groups.tolist() == [0, 2, 4] and b.prefixes.tolist() == [16, 16]
+
+
 @pytest.mark.parametrize("seed", range(10))
 def test_groups_hold_what_their_rows_share(seed):
     cache, rng = _cache(), random.Random(seed)
@@ -522,6 +539,25 @@ def test_what_a_token_does_not_see_does_not_reach_it(dev, dtype, heads, kv, dim,
             assert torch.equal(torch.isnan(mine[..., 3]), torch.full_like(mine[..., 3], bad != bad, dtype=torch.bool))
         elif bad != bad or which == "both":
             assert torch.isnan(mine).any(-1).all() or which == "both"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv,dim", [(4, 2, 64), (40, 2, 128), (6, 3, 200)])
+def test_queries_that_are_not_finite_stay_with_themselves(dev, dtype, heads, kv, dim):
+    """Those of padded rows and behind the last row, and one head of one token among the others of its tile."""
+    p = _problem(dev, dtype, [300], [5, None, 9, 70, None, 3], [2, 1, 1, 30, 3, 3], [0, 6], heads, kv, dim, 8)
+    p[0] = torch.cat((p[0], p[0][:4]))
+    want = _run(p)
+    assert (want[40:] == 0).all() and (want[2:3] == 0).all() and (want[34:37] == 0).all()
+    for bad in (float("nan"), float("inf")):
+        p[0][40:], p[0][2:3], p[0][34:37] = bad, bad, -bad
+        assert torch.equal(_run(p), want)
+    p[0][8, 1] = float("nan")
+    got = _run(p)
+    assert torch.isnan(got[8, 1]).all()
+    got[8, 1] = want[8, 1]
+    assert torch.equal(got, want)
 
 
 @pytest.mark.gpu
