@@ -146,7 +146,7 @@ __global__ __launch_bounds__(THREADS) void dz_extend_kernel(const ExtendParams P
     }
     if (P.tokens_too && !bad && P.packed) {
       __syncthreads();
-      // four tokens a thread of those of this round's rows that are this workgroup's
+      // four tokens a thread of those that are this workgroup's, of the rows at hand
       const int from = max(lo, (int)front.tokens), to = min(hi, (int)(front.tokens + all.tokens)), t0 = lo + tid * ROWS;
       int a = 0;
       if (t0 + ROWS > from && t0 < to) {
