@@ -360,7 +360,7 @@ def prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
 
     Tokens of no row (in front of starts[0], behind starts[rows]) and those of rows of length 0 give zeros; nothing that a token
     does not see reaches its output, whatever is there.  Starts that do not rise within q leave all rows without tokens, groups
-    that do not rise within the rows share nothing; these, lengths beyond the tables and page numbers outside the pool are reported through the
+    that do not rise within the rows share nothing; these (where they are looked at), lengths beyond the tables and page numbers outside the pool are reported through the
     status word.  The weights of 17 and more queries a key (tokens times heads that share one) are rounded to q's type, as their products with the values take
     them.  The same call gives the same bits; they depend on the lengths of all of its rows."""
     if out is None:

@@ -328,6 +328,22 @@ def test_tables_that_do_not_fit_are_left_as_they_were(dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows", [256, 512, 1024])
+def test_tables_of_counts_whose_sum_passes_32_bits(dev, rows):
+    """2^24 tokens a row: 256 rows' sum is 2^32, which 32 bits would take for 0, and there are pages for them."""
+    from deltazip_amd import extend_tables, ops
+    most, ps = 1 << 24, 1024
+    tables = torch.full((rows, most // ps), -7, dtype=torch.int32, device=dev)
+    lengths, counts = (torch.full((rows,), x, dtype=torch.int32, device=dev) for x in (0, most))
+    free, taken = torch.arange(rows * (most // ps), dtype=torch.int32, device=dev), _i32([0], dev)
+    got = extend_tables(tables, lengths, counts, free, taken, ps, tokens=most)
+    with pytest.raises(ops.DeltaKernelError, match="paged"):
+        ops.poll_status(wait=True)
+    assert bool((tables == -7).all()) and got.lengths.tolist() == [0] * rows and got.taken.tolist() == [0]
+    assert got.starts.tolist() == [0] * (rows + 1) and not bool(got.positions.any()) and bool((got.slots == -1).all())
+
+
+@pytest.mark.gpu
 def test_tables_a_page_below_zero_stores_nothing(dev):
     from deltazip_amd import extend_tables, ops
     tables = _i32([[-3, 0], [1, 0]], dev)
