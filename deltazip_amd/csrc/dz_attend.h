@@ -21,6 +21,8 @@ struct Type<false> {
   static __device__ __forceinline__ f4_t mma(v8 a, v8 b, f4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
   static __device__ __forceinline__ uint16_t round(float x) { return __builtin_bit_cast(uint16_t, (_Float16)x); }
   static __device__ __forceinline__ _Float16 one(float x) { return (_Float16)x; }
+  static __device__ __forceinline__ _Float16 cut(float x) { return __builtin_amdgcn_cvt_pkrtz(x, 0.0f)[0]; }        // towards zero
+  static constexpr float MORE = 0x1p-12f;
 };
 template <>
 struct Type<true> {
@@ -29,6 +31,8 @@ struct Type<true> {
   static __device__ __forceinline__ f4_t mma(v8 a, v8 b, f4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
   static __device__ __forceinline__ uint16_t round(float x) { return __builtin_bit_cast(uint16_t, (__bf16)x); }
   static __device__ __forceinline__ __bf16 one(float x) { return (__bf16)x; }
+  static __device__ __forceinline__ __bf16 cut(float x) { return __builtin_bit_cast(__bf16, (uint16_t)(__builtin_bit_cast(unsigned, x) >> 16)); }
+  static constexpr float MORE = 0x1p-9f;
 };
 
 // Sums over the lanes in front of and at each, by shifts within the wavefront's rows of 16 lanes and broadcasts of their last ones.

@@ -15,8 +15,10 @@
 // wavefront.  As in dz_attend.h scores are C[token, query] = K Q^T, so that a lane's weights are just what the second product's
 // operand wants of it; the values' operand is read from LDS by the transposing read.  A query tile's operand from LDS serves two
 // matrix instructions; with more queries a wavefront their sums fill the registers that a second workgroup on the compute unit needs.
-// Weights are held in one value of the type, times 2^14 in fp16: two, as for few queries, would be half as many matrix instructions again, where these are the
-// bound.  Outputs are 2.1e-3 (bf16) off in the root mean square where their own rounding is 1.7e-3, 2.4e-4 and 2.1e-4 in fp16.
+// A weight is held in two values of the type in tiles of up to 64 queries, as for few queries: half as many matrix instructions again, which cost nothing there (32
+// rows 31.2 and 30.8 us, 128 rows in 4 groups 230 and 230, 48 rows of drafted tokens 32.0 and 32.6), and outputs are off by their own rounding.  In larger ones they
+// would cost (two values: 80 queries behind 131072 tokens 120 -> 130 us, 203 rows of 8 heads a key 361 -> 390, nine prompts 32.5 -> 36.8, 8192 tokens 567 -> 742): there it is one
+// value, times 2^14 in fp16.  Outputs are then 2.0e-3 to 2.1e-3 (bf16) off in the root mean square where their own rounding is 1.65e-3, 2.2e-4 and 2.0e-4 in fp16.
 //
 // What bounds it: reading keys and values once up to some 180 queries a key, the matrix cores above.  Measured, a pass among others:
 //   a prompt of 8192 tokens of 32 heads of 128, 8 key heads     555 us, 990 TFLOP/s (a library product of 8192^3 1171 to 1220)
@@ -561,6 +563,7 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void dz_prefix_kernel(const P
 
   auto work = [&](auto cols) __attribute__((always_inline)) {
     constexpr int NC = decltype(cols)::value;          // tiles of 16 queries of a wavefront
+    constexpr bool TWO = NC == 1;                      // weights held in two values
     const int mine = wave * 16 * NC;                   // its first query in the tile
     const bool active = mine < in_tile;
     v8 q[NC][KC];
@@ -649,7 +652,7 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void dz_prefix_kernel(const P
             if (hidden(n, e)) sc[n][e >> 2][e & 3] = -INFINITY;
       }
       load_values(0);
-      v8 p[NC][2];
+      v8 p[NC][2], low[TWO ? NC : 1][2];
 #pragma unroll
       for (int n = 0; n < NC; ++n) {
         float most = sc[n][0][0];
@@ -671,9 +674,18 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void dz_prefix_kernel(const P
         const float ref = top[n] == -INFINITY ? 0.0f : Ty::BIAS - top[n];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          p[n][e >> 3][e & 7] = Ty::one(__builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][e >> 2][e & 3], scale, ref)));
+          const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][e >> 2][e & 3], scale, ref));
+          if (TWO) {
+            // the second is above zero where the weight is, so that infinity times it is no NaN: all weights are 1 + MORE times what they are
+            const auto high = Ty::cut(w);
+            p[n][e >> 3][e & 7] = high;
+            low[n][e >> 3][e & 7] = Ty::one(__builtin_fmaf(w, 1.0f + Ty::MORE, -(float)high));
+          } else {
+            p[n][e >> 3][e & 7] = Ty::one(w);
+          }
         }
         sum[n] = Ty::mma(ones, p[n][1], Ty::mma(ones, p[n][0], sum[n]));
+        if (TWO) sum[n] = Ty::mma(ones, low[n][1], Ty::mma(ones, low[n][0], sum[n]));
       }
       if (__builtin_expect(spoilt, 0)) {
         // a weight of 0 would take what is not finite to queries that do not see it: left out of the products, and added where it is seen
@@ -706,6 +718,13 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void dz_prefix_kernel(const P
 #pragma unroll
           for (int n = 0; n < NC; ++n)
             acc[n][2 * jj + (x >> 1)] = Ty::mma(__builtin_bit_cast(v8, vw[jj & 1][x]), p[n][x & 1], acc[n][2 * jj + (x >> 1)]);
+        if (TWO) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+#pragma unroll
+            for (int n = 0; n < NC; ++n)
+              acc[n][2 * jj + (x >> 1)] = Ty::mma(__builtin_bit_cast(v8, vw[jj & 1][x]), low[n][x & 1], acc[n][2 * jj + (x >> 1)]);
+        }
         __builtin_amdgcn_sched_barrier(0);
       }
     };
@@ -725,11 +744,13 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void dz_prefix_kernel(const P
       if (x >= in_tile) continue;
       const int xx = x0 + x;
       if (U.part >= 0) {
+        // (other units' weights, which these are joined with, are what they are)
+        constexpr float less = TWO ? 1.0f / (1.0f + Ty::MORE) : 1.0f;
         float* record = P.parts + (U.part + ((long long)piece * P.kv_heads + kvh) * queries + xx) * (P.dim + 4);
 #pragma unroll
         for (int j = 0; j < 2 * KC; ++j)
-          if (FULL || 16 * j + 4 * g < P.dim) *(f4_t*)(record + 16 * j + 4 * g) = acc[n][j];
-        if (g == 0) *(f2_t*)(record + P.dim) = f2_t{top[n], sum[n][0]};
+          if (FULL || 16 * j + 4 * g < P.dim) *(f4_t*)(record + 16 * j + 4 * g) = acc[n][j] * less;
+        if (g == 0) *(f2_t*)(record + P.dim) = f2_t{top[n], sum[n][0] * less};
       } else {
         uint16_t* to = P.out + (U.tok0 + xx / P.share) * P.out_row + (kvh * P.share + xx % P.share) * P.out_head;
         const bool sees = limit_of(xx) > 0;

@@ -361,8 +361,8 @@ def prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     Tokens of no row (in front of starts[0], behind starts[rows]) and those of rows of length 0 give zeros; nothing that a token
     does not see reaches its output, whatever is there.  Starts that do not rise within q leave all rows without tokens, groups
     that do not rise within the rows share nothing; these (where they are looked at), lengths beyond the tables and page numbers outside the pool are reported through the
-    status word.  The weights of 17 and more queries a key (tokens times heads that share one) are rounded to q's type, as their products with the values take
-    them.  The same call gives the same bits; they depend on the lengths of all of its rows."""
+    status word.  Where more than 64 queries (tokens times heads that share a key) go together, weights are rounded to q's type, as their products with the
+    values take them: outputs are off by up to 1.3 times their own rounding in the root mean square.  The same call gives the same bits; they depend on the lengths of all of its rows."""
     if out is None:
         made = _lib.host().prefix(q, k_pages, v_pages, block_tables, lengths, starts, groups, prefixes, scale, ROW_BY_ROW)
         if made is not None:

@@ -1,0 +1,42 @@
+"""Attention behind prefixes, batches and runs of the paged cache: what tests/test_prefix.py leaves open."""
+import random
+
+import pytest
+import torch
+
+from oracle import paged_ref as ref
+from test_prefix import HEADS, TYPES, _problem, _run
+
+
+# ---------------------------------------------------------------------------------------------
+# attention: weights
+# ---------------------------------------------------------------------------------------------
+
+
+def _two_values_bound(want, size, most, dtype, dim, tokens, largest):
+    """How far outputs may be off where weights are held in two values of the type.  A weight p (1 + m) is cut to the type and what is left, at most
+    a step (eps) and m of p, rounded to half a step of itself: p (1 + m) (1 + d) with d up to half (eps + m), in the sum of values and in
+    that of weights, so that m cancels and d counts for the sum of p |v| and |o|.  m is eps / 4; below 2^-39 of the largest float16 holds nothing."""
+    half = torch.finfo(dtype).eps / 2
+    d = half * (2 * half + half / 2) * (1 + 2 * half)
+    lost = 2 * tokens * 2.0 ** -39 * largest if dtype == torch.float16 else 0.0
+    return ref.attention_bound(want, size, most, dtype, dim, tokens) + d * (size + want.abs()) + lost
+
+
+def _hold_two_values(got, q, k, v, tables, lengths, starts, groups=None, prefixes=None):
+    row, length, tab = ref.tokens_as_rows(starts, lengths, tables, groups, prefixes, k.shape[2])
+    want, size, most = ref.attention(q, k, v, tab, length, q.shape[2] ** -0.5)
+    bound = _two_values_bound(want, size, most, q.dtype, q.shape[2], int(length.max()), float(v.nan_to_num(0, 0, 0).abs().max()))
+    off = (got.double().cpu() - want).abs()
+    assert (off <= bound).all(), f"off by up to {(off / bound).max():.2f} of the bound"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,new,heads,kv,dim,prefix", [(32, 1, 2, 2, 128, 700), (64, 1, 3, 3, 64, 3000), (17, 1, 2, 2, 80, 90), (5, 3, 12, 3, 96, 400), (13, 1, 8, 2, 256, 1000),
+                                                          (3, 20, 2, 2, 192, 64), (1, 64, 2, 2, 128, 0)])
+def test_weights_of_up_to_64_queries_are_held_in_two_values(dev, dtype, rows, new, heads, kv, dim, prefix):
+    """Units of few queries and tiles alike, and the join of both."""
+    rng = random.Random(rows)
+    p = _problem(dev, dtype, [prefix], [new + rng.randrange(0, 90) for _ in range(rows)], [new] * rows, [0, rows], heads, kv, dim, 16)
+    _hold_two_values(_run(p), *p)
