@@ -437,9 +437,12 @@ class PagedRun:
         return self._batch
 
     def finish(self) -> None:
-        """Gives the cache its sequences back, as long as they have become, and the pages that were not needed.  Waits for the device."""
+        """Gives the cache its sequences back, as long as they have become, and the pages that were not needed.  Waits for the device: for steps and
+        replays on every stream."""
         if self._finished:
             return
+        if self.cache.pool.is_cuda:
+            torch.cuda.synchronize(self.cache.pool.device)
         lengths, tables = self._lengths.cpu().numpy(), self._tables.cpu().numpy()
         cache, taken = self.cache, set()
         for r, x in enumerate(self._seqs):

@@ -1,11 +1,12 @@
 """Attention behind prefixes, batches and runs of the paged cache: what tests/test_prefix.py leaves open."""
 import random
+import types
 
 import pytest
 import torch
 
 from oracle import paged_ref as ref
-from test_prefix import HEADS, TYPES, _problem, _run
+from test_prefix import HEADS, TYPES, _cache, _problem, _run
 
 
 # ---------------------------------------------------------------------------------------------
@@ -40,3 +41,51 @@ def test_weights_of_up_to_64_queries_are_held_in_two_values(dev, dtype, rows, ne
     rng = random.Random(rows)
     p = _problem(dev, dtype, [prefix], [new + rng.randrange(0, 90) for _ in range(rows)], [new] * rows, [0, rows], heads, kv, dim, 16)
     _hold_two_values(_run(p), *p)
+
+
+# ---------------------------------------------------------------------------------------------
+# runs
+# ---------------------------------------------------------------------------------------------
+
+
+def test_a_run_is_finished_once_the_device_is_done(monkeypatch):
+    """Not when the current stream is: steps may be on others."""
+    cache = _cache(monkeypatch=monkeypatch)
+    cache.add("a", 8)
+    run = cache.run(["a"], 9)
+    run.step()
+    before = run._lengths.clone()
+
+    def wait(device):
+        if (run._lengths == before).all():
+            run.step()                                 # (what was still under way)
+    monkeypatch.setattr(torch.cuda, "synchronize", wait)
+    cache.pool = types.SimpleNamespace(is_cuda=True, device="cuda:0")
+    run.finish()
+    assert cache.length("a") == 10 and len(cache.pages("a")) == 2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("captured", [False, True])
+def test_runs_whose_steps_are_on_another_stream(dev, captured):
+    """Behind long work on that stream, finished from the current one."""
+    from deltazip_amd import PagedKVCache
+    cache = PagedKVCache(1, 60, 8, 1, 8, max_tokens=200, device=dev)
+    for x, n in (("a", 7), ("b", 16)):
+        cache.add(x, n)
+    run = cache.run(["a", "b"], 20)
+    work, side, graph = torch.randn(4096, 4096, device=dev), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        run.step()
+        if captured:
+            with torch.cuda.graph(graph, stream=side):
+                run.step()
+        for _ in range(20):
+            work = work @ work / 64.0
+        for _ in range(19):
+            graph.replay() if captured else run.step()
+    run.finish()
+    assert cache.length("a") == 27 and cache.length("b") == 36 and cache.free_pages == 60 - 4 - 5
+    held = [p for x in "ab" for p in cache.pages(x)]
+    assert len(set(held)) == 9 and sorted(held + cache._free) == list(range(60))
