@@ -78,8 +78,9 @@ __device__ __forceinline__ u4_t load16(const char* at) {
 // (fp16) so that they use the type's range, at most 2^15, and are split in two values of the type, high and low: a
 // weight then has 16 (bf16) or 22 (fp16) bits, and the output's error is its own rounding.  Sums are fp32.
 //
-// SEVERAL: the columns are queries that see tokens up to limits of their own, `limit` the lane's, `seen_by_all` the least of them.
-template <int KC, bool FULL, bool BF>
+// QUERIES: the columns are queries of their own, of several tokens or rows, and a maximum moves by its own scores alone: another's change nothing of it.
+// SEVERAL: they see tokens up to limits of their own, `limit` the lane's, `seen_by_all` the least of them.
+template <int KC, bool FULL, bool BF, bool QUERIES>
 struct Walk {
   typedef Type<BF> Ty;
   typedef typename Ty::v8 v8;
@@ -232,7 +233,7 @@ struct Walk {
       most = fmaxf(most, __shfl_xor(most, 16));
       most = fmaxf(most, __shfl_xor(most, 32));
       if (__any(most > top + 1.0f)) {
-        const float up = fmaxf(most, top);
+        const float up = QUERIES ? (most > top + 1.0f ? most : top) : fmaxf(most, top);
         const float f = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - up);
         top = up;
         sum *= f;

@@ -180,7 +180,7 @@ __global__ __launch_bounds__(64 * WAVES, KC == 8 && !FULL ? 1 : 2) void dz_atten
   const int t1 = tile0 + lo + (hi - lo) * (wave + 1) / WAVES;
 
   // queries: lane holds dims 32 c + 8 g .. + 7 of head `col`
-  Walk<KC, FULL, BF> walk;
+  Walk<KC, FULL, BF, false> walk;
 #pragma unroll
   for (int c = 0; c < KC; ++c) {
     u4_t w = {0, 0, 0, 0};

@@ -372,7 +372,7 @@ __device__ __forceinline__ void few_queries(const PrefixParams& P, const Unit& U
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
   const int queries = U.ntok * P.share;
   auto limit_of = [&](int x) { return U.causal ? max(U.n - (U.ntok - 1 - x / P.share), 0) : U.n; };
-  Walk<KC, FULL, BF> walk;
+  Walk<KC, FULL, BF, true> walk;
   const int mine = min(col, queries - 1);
   const char* from = P.q + (U.tok0 + mine / P.share) * P.q_row + (kvh * P.share + mine % P.share) * P.q_head;
 #pragma unroll

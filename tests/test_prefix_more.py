@@ -44,6 +44,35 @@ def test_weights_of_up_to_64_queries_are_held_in_two_values(dev, dtype, rows, ne
 
 
 # ---------------------------------------------------------------------------------------------
+# attention: what others hold
+# ---------------------------------------------------------------------------------------------
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv,dim", [(2, 2, 128), (4, 2, 64), (3, 1, 200)])
+@pytest.mark.parametrize("news,groups,prefix", [([1] * 4, [0, 4], 2000), ([2, 1], [0, 2], 900), ([3], [0, 1], 0), ([5], [0, 1], 0), ([1] * 30, [0, 30], 1500)])
+def test_finite_queries_and_keys_of_others_change_no_bit(dev, dtype, heads, kv, dim, news, groups, prefix):
+    """Of units of few queries and of tiles: a query's sums go by its own scores."""
+    p = _problem(dev, dtype, [prefix], [c + 700 for c in news], news, groups, heads, kv, dim, 16)
+    want, last = _run(p), sum(news)
+    for token, factor in ((0, 9.0), (last - 1, 0.0), (last // 2, -30.0)):
+        q = p[0].clone()
+        q[token] = q[token] * factor
+        got = _run([q] + p[1:])
+        keep = torch.arange(last, device=dev) != token
+        assert torch.equal(got[keep], want[keep]) and not torch.equal(got[token], want[token])
+    if news[0] > 1:
+        # the newest key of row 0, which its other tokens do not see
+        n = int(p[4][0])
+        k = p[1].clone()
+        k[int(p[3][0, (n - 1) // 16]), :, (n - 1) % 16] *= 20.0
+        got = _run([p[0], k] + p[2:])
+        keep = torch.arange(last, device=dev) != news[0] - 1
+        assert torch.equal(got[keep], want[keep]) and not torch.equal(got[news[0] - 1], want[news[0] - 1])
+
+
+# ---------------------------------------------------------------------------------------------
 # runs
 # ---------------------------------------------------------------------------------------------
 
