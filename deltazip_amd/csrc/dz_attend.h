@@ -86,6 +86,7 @@ struct Walk {
   typedef typename Ty::v8 v8;
   static constexpr int NB = (KC + 3) / 4;     // blocks of 128 dims
   static constexpr bool AHEAD = KC <= 6;      // (heads of 256: no registers for it)
+  static constexpr unsigned BAD = BF ? 0x7f80u : 0x7c00u;      // exponent of what is not finite
   v8 q[KC];
   f4_t acc[8 * NB];
   float top, sum;                      // of column lane % 16: the reference maximum, this lane's share of the sum
@@ -168,10 +169,10 @@ struct Walk {
 #pragma unroll
         for (int i = 0; i < 4; ++i) s[4 * a + i] = c4[i] * P.scale;
       }
+      bool spoilt = false;
       if (SEVERAL && (tok < first || tok + TILE > seen_by_all)) {
         // what is not finite and not seen by all must not reach the others as 0 * infinity: left out of the products, and
-        // added where it is seen
-        constexpr unsigned BAD = BF ? 0x7f80u : 0x7c00u;
+        // added below where it is seen
         unsigned found = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -182,7 +183,8 @@ struct Walk {
 #pragma unroll
             for (int x = 0; x < 4; ++x) found |= (vw[b][e][x] & (BAD | BAD << 16)) + ((0x8000u - BAD) | (0x8000u - BAD) << 16);
         }
-        if (__builtin_expect(__any(found & 0x80008000u), 0)) {
+        spoilt = __any(found & 0x80008000u);
+        if (__builtin_expect(spoilt, 0)) {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
 #pragma unroll
@@ -192,23 +194,6 @@ struct Walk {
                 if ((vw[b][e][x] & BAD) == BAD) vw[b][e][x] &= 0xffff0000u;
                 if ((vw[b][e][x] >> 16 & BAD) == BAD) vw[b][e][x] &= 0xffffu;
               }
-#pragma unroll 1
-          for (int t = max(tok, first); t < min(tok + TILE, end); ++t) {
-            const char* at = place(P.v, P.v_page, P.v_head, P.v_token, t, false);
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int d = 128 * b + 8 * (4 * g + i);
-                const u4_t w = *(const u4_t*)(at + (d < P.dim ? 2 * d : 0));
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                  const uint16_t one = (uint16_t)(w[j >> 1] >> 16 * (j & 1));
-                  const float y = BF ? __builtin_bit_cast(float, (unsigned)one << 16) : (float)__builtin_bit_cast(_Float16, one);
-                  acc[8 * b + j][i] += (one & BAD) == BAD && t < limit ? y : 0.0f;
-                }
-              }
-          }
         }
       }
       // the next step's keys are on their way while this one's values come in
@@ -239,6 +224,26 @@ struct Walk {
         sum *= f;
 #pragma unroll
         for (int j = 0; j < 8 * NB; ++j) acc[j] *= f;
+      }
+      if (SEVERAL && __builtin_expect(spoilt, 0)) {        // (now that sums are what these are added to: a first maximum takes them times 0)
+#pragma unroll 1
+        for (int t = max(tok, first); t < min(tok + TILE, end); ++t) {
+          const unsigned page = (unsigned)table[t >> P.shift];             // (the lanes may hold the next ones)
+          const char* at = P.v + (page < P.num_pages ? page : 0u) * P.v_page + kvh * P.v_head + (t & in_page) * P.v_token;
+#pragma unroll
+          for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int d = 128 * b + 8 * (4 * g + i);
+              const u4_t w = *(const u4_t*)(at + (d < P.dim ? 2 * d : 0));
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const uint16_t one = (uint16_t)(w[j >> 1] >> 16 * (j & 1));
+                const float y = BF ? __builtin_bit_cast(float, (unsigned)one << 16) : (float)__builtin_bit_cast(_Float16, one);
+                acc[8 * b + j][i] += (one & BAD) == BAD && t < limit ? y : 0.0f;
+              }
+            }
+        }
       }
       const float ref = top == -INFINITY ? 0.0f : top - Ty::BIAS;
       v8 ph, pl;

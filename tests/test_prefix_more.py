@@ -72,6 +72,92 @@ def test_finite_queries_and_keys_of_others_change_no_bit(dev, dtype, heads, kv, 
         assert torch.equal(got[keep], want[keep]) and not torch.equal(got[news[0] - 1], want[news[0] - 1])
 
 
+SMALL = [([3], [3], [0], [0, 1]), ([4], [90], [0], [0, 1]), ([2] * 4, [2, 30, 2, 9], [64], [0, 4]), ([5, 1], [5, 1], [40], [0, 2]), ([1] * 8, [1, None, 7, 1, 3, None, 1, 90], [200], [0, 8])]
+LARGE = [([40, 3], [70, 9], [64], [0, 2]), ([200], [200], [0], [0, 1]), ([20] * 9, [20] * 9, [128], [0, 9])]
+
+
+def _hold_not_finite(got, p, spoilt):
+    """Outputs of keys or values that are not finite: not finite where the definition says so, and elsewhere within the bound of the scores that are."""
+    q, k, v, tables, lengths, starts, groups, prefixes = p
+    row, length, tab = ref.tokens_as_rows(starts, lengths, tables, groups, prefixes, k.shape[2])
+    _, _, most = ref.attention(q, k, v, tab, length, q.shape[2] ** -0.5)
+    _, size, _ = ref.attention(q, spoilt[0], v, tab, length, q.shape[2] ** -0.5)
+    want, _, _ = ref.attention(q, *spoilt, tab, length, q.shape[2] ** -0.5)
+    bound = ref.prefix_bound(want, size, most, q.dtype, q.shape[2], int(length.max()), float(v.nan_to_num(0, 0, 0).abs().max()))
+    got = got.double().cpu()
+    finite = torch.isfinite(want)
+    assert torch.equal(torch.isfinite(got), finite) and ((got - want).abs()[finite] <= bound[finite]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv,dim", [(2, 2, 64), (4, 2, 128), (6, 3, 200), (3, 1, 256)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_values_that_are_not_finite_reach_who_sees_them(dev, dtype, heads, kv, dim, bad):
+    """In the newest token of a row, one of the older new ones and one that all of its new ones see; units of few queries and tiles."""
+    for news, suffixes, prefixes, groups in SMALL + LARGE:
+        p = _problem(dev, dtype, prefixes, suffixes, news, groups, heads, kv, dim, 8)
+        clean = _run(p)
+        n, c, share = int(p[4][0]), news[0], heads // kv
+        for t in {n - 1, n - c, n - (c + 1) // 2, max(prefixes[0], n - c - 1)}:
+            v = p[2].clone()
+            v[int(p[3][0, t // 8]), 0, t % 8, 3] = bad
+            got = _run([p[0], p[1], v] + p[3:])
+            first = max(0, t - (n - c))                            # the first of row 0's new tokens that sees it
+            seen = torch.zeros_like(clean, dtype=torch.bool)
+            seen[first:c, :share, 3] = True
+            assert torch.equal(got[~seen], clean[~seen]) and not torch.isfinite(got[seen]).any()
+            if t > n - c:                                          # (in a step that some do not see: as it is)
+                assert torch.equal(torch.isnan(got[seen]), torch.full_like(got[seen], bad != bad, dtype=torch.bool))
+                assert bad != bad or (got[seen] == bad).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv,dim", [(4, 2, 128), (6, 3, 200)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("which", ["keys", "both"])
+def test_keys_that_are_not_finite_reach_who_sees_them(dev, dtype, heads, kv, dim, bad, which):
+    """As scores that are not finite do in the definition: NaN, or, far below all others, no weight."""
+    for news, suffixes, prefixes, groups in SMALL + LARGE:
+        p = _problem(dev, dtype, prefixes, suffixes, news, groups, heads, kv, dim, 8, poison=False)
+        clean = _run(p)
+        n, c, share = int(p[4][0]), news[0], heads // kv
+        for t in {n - 1, n - (c + 1) // 2, max(prefixes[0], n - c - 1)}:
+            if n == 1 or (t == 0 and bad == bad):
+                continue                                           # (a token's only score)
+            k, v = p[1].clone(), p[2].clone()
+            for x in (k, v)[:1 if which == "keys" else 2]:
+                x[int(p[3][0, t // 8]), 0, t % 8, 3] = bad
+            got = _run([p[0], k, v] + p[3:])
+            first = max(0, t - (n - c))
+            assert torch.equal(got[:first], clean[:first]) and torch.equal(got[c:], clean[c:]) and torch.equal(got[:, share:], clean[:, share:])
+            if bad != bad:
+                assert torch.isnan(got[first:c, :share]).all()
+            _hold_not_finite(got, p, (k, v))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv,dim", [(2, 2, 64), (4, 2, 128), (3, 3, 200)])
+def test_queries_of_padded_rows_that_are_not_finite_stay_with_themselves(dev, dtype, heads, kv, dim):
+    """In a group's unit of few queries, among the others of a matrix instruction."""
+    for prefix in (40, 700):
+        p = _problem(dev, dtype, [prefix], [1, None, 7, 1, 3, None, 1, 90], [1] * 8, [0, 8], heads, kv, dim, 8)
+        want = _run(p)
+        assert (want[[1, 5]] == 0).all()
+        for bad in (float("nan"), float("inf")):
+            p[0][1], p[0][5] = bad, -bad
+            assert torch.equal(_run(p), want)
+        for bad in (float("nan"), float("inf"), 6e4):
+            q = p[0].clone()
+            q[6] = bad
+            got = _run([q] + p[1:])
+            keep = torch.arange(8, device=dev) != 6
+            assert torch.equal(got[keep], want[keep])
+            assert bad == 6e4 or torch.isnan(got[6]).all()
+
+
 # ---------------------------------------------------------------------------------------------
 # runs
 # ---------------------------------------------------------------------------------------------
