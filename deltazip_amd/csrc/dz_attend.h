@@ -56,6 +56,9 @@ __device__ __forceinline__ T scan_add(T x) {
 __device__ __forceinline__ float weight_of(float top, float up) { return top == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - up); }
 
 constexpr int TILE = 32;               // tokens of a step of a wavefront
+// Maxima beyond which 32 bits no longer hold what a score, or a weight's 2^14, is apart from them by: differences are taken by themselves there.
+constexpr float FAR = 4096.0f;
+__device__ __forceinline__ bool is_far(float top) { return fabsf(top) > FAR && top != -INFINITY; }
 
 // Keys and values of a call pass through once: loads that keep nothing in the caches read 7.1 TB/s where others read 6.2.  Not so
 // where rows share pages: 16 rows of one sequence's 4096 tokens of 32 key heads 130 -> 81 us with the others.
@@ -98,6 +101,7 @@ struct Walk {
 #pragma unroll
     for (int j = 0; j < 8 * NB; ++j) acc[j] = f4_t{0, 0, 0, 0};
     top = -INFINITY, sum = 0.0f;
+    bool far = false;                  // of any column's maximum, where weights are held times 2^14
     const int last_page = (end - 1) >> P.shift;
     int page0 = t0 * TILE >> P.shift;  // of the 64 page numbers that the lanes hold
     auto fetch = [&](int base) {
@@ -221,6 +225,7 @@ struct Walk {
         const float up = QUERIES ? (most > top + 1.0f ? most : top) : fmaxf(most, top);
         const float f = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - up);
         top = up;
+        if (Ty::BIAS != 0.0f) far |= __any(is_far(up));
         sum *= f;
 #pragma unroll
         for (int j = 0; j < 8 * NB; ++j) acc[j] *= f;
@@ -245,7 +250,12 @@ struct Walk {
             }
         }
       }
-      const float ref = top == -INFINITY ? 0.0f : top - Ty::BIAS;
+      float ref = top == -INFINITY ? 0.0f : top - Ty::BIAS;
+      if (Ty::BIAS != 0.0f && __builtin_expect(far, 0) && is_far(top)) {
+        ref = -Ty::BIAS;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e] -= top;
+      }
       v8 ph, pl;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {

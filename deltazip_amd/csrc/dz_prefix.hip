@@ -569,12 +569,13 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void dz_prefix_kernel(const P
     v8 q[NC][KC];
     int lim[NC];
     f4_t acc[NC][2 * KC];
-    float top[NC];
+    float top[NC], ref[NC], by[NC];    // maximum; a weight is 2^(score by + ref)
     f4_t sum[NC];                      // of the weights as they are rounded (a product with ones: what rounding does to a large weight is gone when it is divided by)
     v8 ones;
 #pragma unroll
     for (int e = 0; e < 8; ++e) ones[e] = Ty::one(1.0f);
     const float scale = fabsf(P.scale);
+    bool far = false;                  // of any query's maximum
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
       const int x = mine + 16 * n + col, xx = x0 + min(x, in_tile - 1);
@@ -590,7 +591,7 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void dz_prefix_kernel(const P
         for (int c = 0; c < KC; ++c) q[n][c] = -q[n][c];
       }
       lim[n] = min(limit_of(xx), hi);
-      top[n] = -INFINITY, sum[n] = f4_t{0, 0, 0, 0};
+      top[n] = -INFINITY, ref[n] = 0.0f, by[n] = scale, sum[n] = f4_t{0, 0, 0, 0};
 #pragma unroll
       for (int j = 0; j < 2 * KC; ++j) acc[n][j] = f4_t{0, 0, 0, 0};
     }
@@ -660,7 +661,7 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void dz_prefix_kernel(const P
         for (int e = 1; e < 16; ++e) most = fmaxf(most, sc[n][e >> 2][e & 3]);
         most *= scale;
         // the reference moves only where a score is more than twice above it
-        if (__any(most > top[n] + 1.0f)) {
+        if (__any(most > top[n] + 1.0f) || far) {
           most = fmaxf(most, __shfl_xor(most, 16));
           most = fmaxf(most, __shfl_xor(most, 32));
           // (each query's by its own scores: another's change nothing of it)
@@ -670,11 +671,19 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void dz_prefix_kernel(const P
           sum[n] *= f;
 #pragma unroll
           for (int j = 0; j < 2 * KC; ++j) acc[n][j] *= f;
+          ref[n] = up == -INFINITY ? 0.0f : Ty::BIAS - up;
+          far |= __any(is_far(up));
+          if (__builtin_expect(far, 0) && is_far(up)) {
+            // (the maximum is a rounded product: the scores, too, before it is taken from them)
+#pragma clang fp contract(off)
+            by[n] = 1.0f, ref[n] = Ty::BIAS;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) sc[n][e >> 2][e & 3] = sc[n][e >> 2][e & 3] * scale - up;
+          }
         }
-        const float ref = top[n] == -INFINITY ? 0.0f : Ty::BIAS - top[n];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][e >> 2][e & 3], scale, ref));
+          const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][e >> 2][e & 3], by[n], ref[n]));
           if (TWO) {
             // the second is above zero where the weight is, so that infinity times it is no NaN: all weights are 1 + MORE times what they are
             const auto high = Ty::cut(w);

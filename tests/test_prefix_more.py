@@ -72,6 +72,63 @@ def test_finite_queries_and_keys_of_others_change_no_bit(dev, dtype, heads, kv, 
         assert torch.equal(got[keep], want[keep]) and not torch.equal(got[news[0] - 1], want[news[0] - 1])
 
 
+def _one_sided(dev, dtype, tokens, scores, extra=None):
+    """Tokens of 300 (256 of them a prefix) whose keys hold `scores` in their first value and `extra` in their second, which queries of ones pick."""
+    from deltazip_amd import paged_attention, prefix_attention
+    g = torch.Generator().manual_seed(tokens)
+    k, v = torch.zeros(38 * 8, 2, 64, dtype=dtype), torch.randn(38 * 8, 2, 64, generator=g).to(dtype)
+    k[:300, :, 0] = scores.to(dtype)[:, None]
+    if extra is not None:
+        k[:300, :, 1] = extra.to(dtype)[:, None]
+    k, v = (x.view(38, 8, 2, 64).transpose(1, 2).contiguous().to(dev) for x in (k, v))
+    q = torch.zeros(tokens, 2, 64, dtype=dtype)
+    q[..., :2] = 1.0
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)
+    p = [q.to(dev), k, v, i32([list(range(38))] * tokens), i32([300] * tokens), i32(list(range(tokens + 1))), i32([0, tokens]), i32([256])]
+    return p, lambda scale: prefix_attention(*p[:5], starts=p[5], groups=p[6], prefixes=p[7], scale=scale), lambda scale: paged_attention(*p[:5], scale=scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens", [1, 3, 40, 64, 100, 300])
+def test_scores_of_any_size(dev, dtype, tokens):
+    """Of 2^11 to 2^126: four tokens have the largest, alike, and their values' mean is the output, or all but four have it.  (Weights alike are rounded
+    alike; sums of 300 are off by 300 2^-24 twice.)"""
+    g = torch.Generator().manual_seed(5)
+    for e in list(range(11, 40)) + [60, 90, 124]:
+        top = torch.empty(1).uniform_(1.0, 1.9, generator=g).to(dtype)
+        scores = (top / 2).repeat(300)
+        where = [5, 77, 190, 290]
+        scores[where] = top
+        p, behind, single = _one_sided(dev, dtype, tokens, scores)
+        v = p[2].transpose(1, 2).reshape(304, 2, 64)[:300].double().cpu()
+        for sign in (1.0, -1.0):
+            pick = torch.zeros(300, dtype=torch.bool)
+            pick[where] = True
+            want = v[pick if sign > 0 else ~pick].mean(0)
+            for y in (behind(sign * 0.7123 * 2.0 ** e), single(sign * 0.7123 * 2.0 ** e)):
+                off = (y.double().cpu() - want).abs()
+                assert (off <= torch.finfo(dtype).eps / 2 * want.abs() + 600 * 2.0 ** -24 * v.abs().max() + 2.0 ** -24).all(), (e, sign)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens", [3, 40, 100])
+@pytest.mark.parametrize("base", [1000, 2830, 2840, 2848, -2848, 20000])
+def test_scores_around_where_differences_are_taken_by_themselves(dev, dtype, tokens, base):
+    """Large sums with small differences, maxima of pieces on either side of the border: a score is rounded by up to 2^-23 of its size twice, whichever way it goes."""
+    g = torch.Generator().manual_seed(base % 97)
+    for extra in (torch.randn(300, generator=g), torch.linspace(-6, 6, 300), torch.linspace(6, -6, 300)):
+        scores = torch.full((300,), float(base))
+        p, behind, single = _one_sided(dev, dtype, tokens, scores, extra)
+        q, k, v, tables, lengths = p[:5]
+        want, size, most = ref.attention(q[:1], k, v, tables[:1], lengths[:1], 1.0)
+        bound = ref.prefix_bound(want, size, most / 17, dtype, 64, 300, float(v.abs().max()))           # (4 roundings of a score, not 68)
+        for y in (behind(1.0), single(1.0)):
+            off = (y.double().cpu() - want).abs()
+            assert (off <= bound).all(), float((off / bound).max())
+
+
 SMALL = [([3], [3], [0], [0, 1]), ([4], [90], [0], [0, 1]), ([2] * 4, [2, 30, 2, 9], [64], [0, 4]), ([5, 1], [5, 1], [40], [0, 2]), ([1] * 8, [1, None, 7, 1, 3, None, 1, 90], [200], [0, 8])]
 LARGE = [([40, 3], [70, 9], [64], [0, 2]), ([200], [200], [0], [0, 1]), ([20] * 9, [20] * 9, [128], [0, 9])]
 
