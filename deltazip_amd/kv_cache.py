@@ -335,24 +335,34 @@ class PagedKVCache:
 
     def _groups_of(self, tables: np.ndarray, used: np.ndarray) -> Tuple[List[int], List[int]]:
         """(rows where groups of neighbours begin and the last one ends, tokens that each group's rows have in common).  A row joins the group in front of
-        it where that spares as many pages as the group spared without it."""
+        it where that spares as many pages as the group spared without it; rows without pages between two of a group are among it."""
+        alive = np.flatnonzero(used)
         columns = np.arange(tables.shape[1])
-        same = (tables[1:] == tables[:-1]) & (columns < np.minimum(used[1:], used[:-1])[:, None])
-        common = np.where(same.all(1), len(columns), same.argmin(1)).tolist()        # pages, with the row in front
+        rows, pages = tables[alive], used[alive]
+        same = (rows[1:] == rows[:-1]) & (columns < np.minimum(pages[1:], pages[:-1])[:, None])
+        common = np.where(same.all(1), len(columns), same.argmin(1)).tolist() if len(alive) > 1 else []        # pages, with the one in front
         bounds, sizes, first = [0], [], 0
-        while first < len(used):
+
+        def close(end: int, pages: int) -> None:
+            if end == bounds[-1]:
+                return
+            if pages == 0 and sizes and sizes[-1] == 0:
+                bounds[-1] = end
+            else:
+                sizes.append(pages * self.page_size)
+                bounds.append(end)
+
+        while first < len(alive):
             last, cut = first + 1, 0
-            while last < len(used):
+            while last < len(alive):
                 c = min(cut, common[last - 1]) if cut else common[last - 1]
                 if not c or c * (last - first) < cut * (last - first - 1):
                     break
                 last, cut = last + 1, c
-            if cut == 0 and sizes and sizes[-1] == 0:
-                bounds[-1] = last
-            else:
-                sizes.append(cut * self.page_size)
-                bounds.append(last)
+            close(int(alive[first]), 0)
+            close(int(alive[last - 1]) + 1, cut)
             first = last
+        close(len(used), 0)
         return bounds, sizes
 
     # -- steps that the device goes by itself ---------------------------------------------------
@@ -420,7 +430,8 @@ class PagedRun:
         if rows:
             # (the page that a row's tokens go on in is its own: no group has it)
             bounds, sizes = cache._groups_of(tables, used)
-            shared = 2 * sum(n // cache.page_size * (b - a - 1) for a, b, n in zip(bounds, bounds[1:], sizes)) > int(used.sum())
+            holders = [int(np.count_nonzero(used[a:b])) for a, b in zip(bounds, bounds[1:])]
+            shared = 2 * sum(n // cache.page_size * (h - 1) for h, n in zip(holders, sizes) if n) > int(used.sum())
             if prefix:
                 n = min(len(sizes), MAX_GROUPS)
                 both = torch.from_numpy(np.asarray(bounds[:n + 1] + sizes[:n], dtype=np.int32)).to(cache.pool.device)

@@ -216,6 +216,57 @@ def test_queries_of_padded_rows_that_are_not_finite_stay_with_themselves(dev, dt
 
 
 # ---------------------------------------------------------------------------------------------
+# groups
+# ---------------------------------------------------------------------------------------------
+
+
+def test_padded_rows_do_not_cut_a_group(monkeypatch):
+    cache = _cache(monkeypatch=monkeypatch, pages=400)
+    cache.add("p", 80)
+    rows = [None if i % 16 == 15 else i for i in range(60)]
+    for i in rows:
+        if i is not None:
+            cache.fork("p", i)
+    cache.extend([i for i in rows if i is not None])
+    for seqs, bounds, sizes in ((rows, [0, 60], [80]), ([None, None] + rows + [None] * 3, [0, 2, 62, 65], [0, 80, 0]), ([None, 1, None], [0, 3], [0]), ([None] * 3, [0, 3], [0])):
+        b = cache.batch(seqs, prefix=True)
+        n = len(bounds)
+        assert b.groups.tolist()[:n] == bounds and set(b.groups.tolist()[n:]) <= {len(seqs)}
+        assert b.prefixes.tolist()[:n - 1] == sizes and not any(b.prefixes.tolist()[n - 1:])
+    assert cache.batch([None, None], width=0, prefix=True).prefixes.tolist() == [0, 0]
+    run = cache.run([0, None, None, 1, 2], 1, prefix=True)
+    b = run.step()
+    assert b.groups.tolist() == [0, 5] and b.prefixes.tolist() == [80] and b.shared
+    run.finish()
+    run = cache.run([0] + [None] * 40, 1, prefix=True)
+    assert not run.step().shared
+    run.finish()
+
+
+@pytest.mark.parametrize("seed", range(20))
+def test_groups_over_padded_rows_hold_what_their_rows_share(seed):
+    """And are those of the rows without the padded ones."""
+    import numpy as np
+    cache, rng = _cache(), random.Random(seed)
+    rows, w = rng.randrange(1, 30), 6
+    used = np.array([rng.choice([0, rng.randrange(1, w + 1)]) for _ in range(rows)])
+    tables, last = np.zeros((rows, w), dtype=np.int32), None
+    for r in np.flatnonzero(used):
+        keep = 0 if last is None else min(rng.randrange(0, w + 1), used[r], used[last])
+        tables[r, :used[r]] = [tables[last, i] if i < keep else 100 * r + i + 1 for i in range(used[r])]
+        last = r
+    bounds, sizes = cache._groups_of(tables, used)
+    assert bounds[0] == 0 and bounds[-1] == rows and len(sizes) == len(bounds) - 1 and (np.diff(bounds) > 0).all()
+    alive = np.flatnonzero(used)
+    for a, b, n in zip(bounds, bounds[1:], sizes):
+        mine = [r for r in range(a, b) if used[r]]
+        assert n % 8 == 0 and (n == 0 or (len(mine) > 1 and used[a] and used[b - 1] and all(used[r] >= n // 8 and (tables[r, :n // 8] == tables[a, :n // 8]).all() for r in mine)))
+    packed, shares = cache._groups_of(tables[alive], used[alive])
+    assert [(list(alive[a:b]), n) for a, b, n in zip(packed, packed[1:], shares) if n] == [
+        ([r for r in range(a, b) if used[r]], n) for a, b, n in zip(bounds, bounds[1:], sizes) if n]
+
+
+# ---------------------------------------------------------------------------------------------
 # runs
 # ---------------------------------------------------------------------------------------------
 
