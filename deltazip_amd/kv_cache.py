@@ -25,22 +25,34 @@ class OutOfPages(RuntimeError):
     """The pool has too few free pages for the call; nothing was changed."""
 
 
-class PagedBatch(NamedTuple):
+class _Batch(NamedTuple):
+    positions: torch.Tensor
+    slots: torch.Tensor
+    block_tables: torch.Tensor
+    lengths: torch.Tensor
+    shared: bool = False
+
+
+class PagedBatch(_Batch):
     """What a step of one new token per row needs of the cache, on the device: the newest token's position and slot
     (int64 [rows]), the tables (int32 [rows, pages]) and lengths (int32 [rows], the new token counted); and, on the host, whether
     most of its rows' pages are another of its rows', too (for `paged_attention`, which takes no notice of it for one row; of
     one row: whether sharing spares the cache most of as many pages).  A captured step keeps what it was captured with.
 
     With several new tokens of a row, `starts` (int32 [rows + 1]) says where each row's begin among positions and slots; with prefixes that
-    neighbouring rows share, `groups` (int32 [n + 1]) and `prefixes` (int32 [n]) say which: both as `prefix_attention` takes them."""
-    positions: torch.Tensor
-    slots: torch.Tensor
-    block_tables: torch.Tensor
-    lengths: torch.Tensor
-    shared: bool = False
+    neighbouring rows share, `groups` (int32 [n + 1]) and `prefixes` (int32 [n]) say which: both as `prefix_attention` takes them.  (These three are
+    no items of the tuple.)"""
     starts: Optional[torch.Tensor] = None
     groups: Optional[torch.Tensor] = None
     prefixes: Optional[torch.Tensor] = None
+
+    def __new__(cls, positions, slots, block_tables, lengths, shared=False, starts=None, groups=None, prefixes=None):
+        batch = super().__new__(cls, positions, slots, block_tables, lengths, shared)
+        batch.starts, batch.groups, batch.prefixes = starts, groups, prefixes
+        return batch
+
+    def _replace(self, **changes) -> "PagedBatch":
+        return PagedBatch(**{**self._asdict(), "starts": self.starts, "groups": self.groups, "prefixes": self.prefixes, **changes})
 
 
 class _Sequence:
@@ -328,8 +340,8 @@ class PagedKVCache:
                           made[4] if tokens is not None else None, made[-2] if prefix else None, made[-1] if prefix else None)
         if out is None:
             return made
-        for to, t in zip(out, made):
-            if isinstance(t, torch.Tensor):
+        for to, t in zip((*out[:4], out.groups, out.prefixes), (*made[:4], made.groups, made.prefixes)):
+            if t is not None:
                 to.copy_(t)
         return out._replace(shared=made.shared)
 

@@ -267,6 +267,35 @@ def test_groups_over_padded_rows_hold_what_their_rows_share(seed):
 
 
 # ---------------------------------------------------------------------------------------------
+# batches
+# ---------------------------------------------------------------------------------------------
+
+
+def test_a_batch_is_five_items_whatever_it_holds_besides():
+    import copy
+    import pickle
+    from deltazip_amd import PagedBatch
+    cache = _cache()
+    cache.add("a", 21)
+    cache.add("b", 4)
+    for kw in (dict(), dict(prefix=True), dict(tokens=[3, 2]), dict(tokens=[1, 0], prefix=True)):
+        b = cache.batch(["a", "b"], **kw)
+        positions, slots, tables, lengths, shared = b
+        assert positions is b.positions and lengths.tolist() == [21, 4] and shared is False and len(b) == 5
+        assert (b.starts is not None) == ("tokens" in kw) and (b.groups is not None) == (b.prefixes is not None) == ("prefix" in kw)
+        other = b._replace(shared=True)
+        assert type(other) is PagedBatch and other.shared and other.starts is b.starts and other.groups is b.groups and other.slots is slots
+        for same in (pickle.loads(pickle.dumps(b)), copy.copy(b), copy.deepcopy(b)):
+            for name in ("positions", "slots", "block_tables", "lengths", "starts", "groups", "prefixes"):
+                x, y = getattr(b, name), getattr(same, name)
+                assert (x is None and y is None) or torch.equal(x, y)
+    b = cache.batch(["a", None], prefix=True)
+    again = cache.batch([None, "b"], prefix=True, out=b)
+    assert again.groups is b.groups and again.lengths is b.lengths and b.lengths.tolist() == [0, 4]
+    assert PagedBatch(positions, slots, tables, lengths, True, b.starts, b.groups, b.prefixes).prefixes is b.prefixes
+
+
+# ---------------------------------------------------------------------------------------------
 # runs
 # ---------------------------------------------------------------------------------------------
 
