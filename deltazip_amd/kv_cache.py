@@ -85,11 +85,17 @@ class PagedKVCache:
         self._seqs: Dict[Hashable, _Sequence] = {}
         self._rows = np.zeros((8, self.max_pages), dtype=np.int32)                 # tables, a row per sequence
         self._free_rows = list(range(8))[::-1]
+        self._runs: List["PagedRun"] = []           # not finished
 
     # -- what there is ---------------------------------------------------------------------
     @property
     def free_pages(self) -> int:
         return len(self._free)
+
+    @property
+    def runs(self) -> Tuple["PagedRun", ...]:
+        """Runs that are not finished, those among them that the caller has lost: their sequences come back with `finish`."""
+        return tuple(self._runs)
 
     def __contains__(self, seq: Hashable) -> bool:
         return seq in self._seqs
@@ -108,7 +114,7 @@ class PagedKVCache:
         if s is None:
             raise ValueError(f"no sequence {seq!r} in the cache")
         if s.running:
-            raise ValueError(f"sequence {seq!r} is in a run: what it holds is known when that is finished")
+            raise ValueError(f"sequence {seq!r} is in a run: what it holds is known when that (one of `runs`) is finished")
         return s
 
     # -- sequences that come, grow, fork and go ----------------------------------------------
@@ -407,10 +413,9 @@ class PagedKVCache:
 class PagedRun:
     """Steps of a batch whose tables, lengths and free pages stay on the device (`PagedKVCache.run`):
 
-        run = cache.run(seqs, steps=64)
-        for _ in range(64):
-            logits = model.paged_step(tokens, cache, run.step())       # or captured once and replayed
-        run.finish()
+        with cache.run(seqs, steps=64) as run:                         # (finished at its end, whatever happens in it)
+            for _ in range(64):
+                logits = model.paged_step(tokens, cache, run.step())   # or captured once and replayed
 
     `step` makes room for each row's next token and returns the batch of it, the same tensors every time; `counts` (int32 [rows]: 1, or 0
     of a row that gets no more tokens) may be written between steps.  A step that needs more pages than were set aside stores
@@ -452,6 +457,13 @@ class PagedRun:
         for s in found:
             if s is not None:
                 s.running = True
+        cache._runs.append(self)
+
+    def __enter__(self) -> "PagedRun":
+        return self
+
+    def __exit__(self, *error) -> None:
+        self.finish()
 
     def step(self) -> PagedBatch:
         if self._finished:
@@ -480,4 +492,5 @@ class PagedRun:
         for page in self._pages:
             if page not in taken:
                 cache._release(page)
+        cache._runs.remove(self)
         self._finished = True

@@ -341,3 +341,25 @@ def test_runs_whose_steps_are_on_another_stream(dev, captured):
     assert cache.length("a") == 27 and cache.length("b") == 36 and cache.free_pages == 60 - 4 - 5
     held = [p for x in "ab" for p in cache.pages(x)]
     assert len(set(held)) == 9 and sorted(held + cache._free) == list(range(60))
+
+
+def test_a_run_that_is_dropped_gives_its_sequences_back(monkeypatch):
+    cache = _cache(monkeypatch=monkeypatch)
+    cache.add("a", 10)
+    cache.add("b", 3)
+    with pytest.raises(KeyError):
+        with cache.run(["a"], 20) as run:
+            run.step()
+            raise KeyError
+    assert cache.length("a") == 11 and cache.runs == () and cache.free_pages == 200 - 3
+    cache.run(["a", None], 20).step()
+    cache.run(["b"], 1)
+    with pytest.raises(ValueError, match="runs"):
+        cache.free("a")
+    for run in cache.runs:
+        run.finish()
+        run.finish()
+    assert cache.runs == () and cache.length("a") == 12 and cache.length("b") == 3
+    cache.free("a")
+    cache.free("b")
+    assert cache.free_pages == 200
