@@ -91,6 +91,7 @@ struct PrefixParams {
   long long room_parts;
   unsigned num_pages;
   int tokens, rows, ngroups, heads, kv_heads, share, dim, shift, pages_per_row, room_items, near;
+  unsigned line;                       // workgroups of a line of the grid
   float scale;
 };
 
@@ -470,7 +471,9 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void dz_prefix_kernel(const P
   constexpr unsigned BAD = BF ? 0x7f80u : 0x7c00u;     // exponent of what is not finite
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
-  const int turn = blockIdx.x / P.kv_heads, kvh = blockIdx.x % P.kv_heads;
+  const unsigned id = blockIdx.y * P.line + blockIdx.x;
+  const int turn = id / P.kv_heads, kvh = id % P.kv_heads;
+  if (turn >= P.room_items) return;    // (behind a grid's last line)
   Item item = P.items[turn];           // (asked for together with what says whether it is one; there are as many places as turns)
   const int all = P.head[0], shorts = P.head[4], together = P.head[5];
   const bool once = P.head[1] != 0, is_short = turn >= all;
@@ -946,11 +949,10 @@ int dz_prefix_attention(const dz_prefix_args* a, void* stream) {
   if (a->table_row < 0) return DZ_EPAGES;
   const Room m = room_of(a->tokens, a->rows, a->groups_n, a->heads, a->kv_heads, a->dim);
   if (!a->work || (size_t)a->work_bytes < m.bytes || ((uintptr_t)a->work & 15)) return DZ_EWORKSPACE;
-  if (m.items * a->kv_heads > 0x7fffffffll) return DZ_EPAGES;
   // (what tables hold may allow fewer)
   const long long cuts = ((long long)a->pages_per_row * a->page_size + LEAST - 1) / LEAST, fewer = m.tiles * (cuts < 1 ? 1 : cuts);
   const long long grid = (m.items < fewer ? m.items : fewer) * a->kv_heads;
-  if (grid > 0xffffff) return DZ_EPAGES;                       // (of 256 threads each)
+  const long long lines = (grid + 0xfffffe) / 0xffffff, line = (grid + lines - 1) / lines;       // (a line has less than 2^32 threads; under 2^32 workgroups in all)
 
   PrefixParams P;
   char* work = (char*)a->work;
@@ -963,7 +965,7 @@ int dz_prefix_attention(const dz_prefix_args* a, void* stream) {
   P.k_page = 2 * a->k_page, P.k_head = 2 * a->k_head, P.k_token = 2 * a->k_token;
   P.v_page = 2 * a->v_page, P.v_head = 2 * a->v_head, P.v_token = 2 * a->v_token;
   P.out_row = a->out_row, P.out_head = a->out_head, P.table_row = a->table_row;
-  P.room_parts = m.parts, P.room_items = (int)m.items;
+  P.room_parts = m.parts, P.room_items = (int)m.items, P.line = (unsigned)line;
   P.num_pages = (unsigned)a->num_pages;
   P.tokens = a->tokens, P.rows = a->rows, P.ngroups = a->groups_n, P.heads = a->heads, P.kv_heads = a->kv_heads, P.share = a->heads / a->kv_heads;
   P.dim = a->dim, P.shift = __builtin_ctz(a->page_size), P.pages_per_row = a->pages_per_row;
@@ -972,7 +974,6 @@ int dz_prefix_attention(const dz_prefix_args* a, void* stream) {
   // 16 tokens that a wavefront asks for lie in one page, within 32 bits
   P.near = a->page_size >= 16 && P.k_token < (1 << 27) && P.v_token < (1 << 27);
   const int kc = chunks_of(a->dim), which = kc * 4 + (a->dim == 32 * kc) * 2 + a->dtype;
-  // two steps' keys and values; or the sums of four wavefronts and their maxima
   // two steps' keys and values; or the sums of four wavefronts and their maxima
   const size_t steps = 2 * (size_t)(8 * kc) * 1024, sums = (4 * FEW * (size_t)(a->dim + 4) + 8 * FEW) * 4, lds = steps > sums ? steps : sums;
   const kernel_t kern = a->dtype == DZ_BF16 ? kernel_for<true>(a->dim) : kernel_for<false>(a->dim);
@@ -988,7 +989,7 @@ int dz_prefix_attention(const dz_prefix_args* a, void* stream) {
     hipLaunchKernelGGL((dz_prefix_plan_kernel<1024, true>), dim3(1), dim3(1024), 0, st, P);
   else
     hipLaunchKernelGGL((dz_prefix_plan_kernel<1024, false>), dim3(1), dim3(1024), 0, st, P);
-  hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(256), lds, st, P);
+  hipLaunchKernelGGL(kern, dim3((unsigned)line, (unsigned)lines), dim3(256), lds, st, P);
   // of few outputs the pieces, too, are shared out (16 rows of 40 heads in 60 pieces 128 -> 119 us; 144 tokens of 20 in 4 32 -> 34); of many tokens, most of which
   // are stored already, a workgroup takes more of the heads
   const long long values = (long long)a->tokens * a->heads * (a->dim / 4);

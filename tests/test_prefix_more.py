@@ -215,6 +215,26 @@ def test_queries_of_padded_rows_that_are_not_finite_stay_with_themselves(dev, dt
             assert bad == 6e4 or torch.isnan(got[6]).all()
 
 
+@pytest.mark.gpu
+def test_more_workgroups_than_a_line_of_a_grid_has(dev):
+    """Rows times key heads beyond 2^24: every output, against the same in 32 bits."""
+    from deltazip_amd import prefix_attention
+    rows, heads, dim, ps = 530001, 32, 8, 8
+    g = torch.Generator(device=dev).manual_seed(0)
+    k, v = (torch.randn(3, heads, ps, dim, generator=g, device=dev).half() for _ in range(2))
+    q = torch.randn(rows, heads, dim, generator=g, device=dev).half()
+    lengths = torch.randint(0, ps + 1, (rows,), generator=g, device=dev, dtype=torch.int32)
+    tables = torch.tensor([[2]], dtype=torch.int32, device=dev).expand(rows, 1)
+    got = prefix_attention(q, k, v, tables, lengths, starts=torch.arange(rows + 1, dtype=torch.int32, device=dev))
+    half = torch.finfo(torch.float16).eps / 2
+    for h in range(heads):
+        s = dim ** -0.5 * (q[:, h].float() @ k[2, h].float().t().contiguous())
+        p = torch.softmax(s.masked_fill(torch.arange(ps, device=dev) >= lengths[:, None], -1e30), 1)
+        want = (p @ v[2, h].float()) * (lengths > 0)[:, None]
+        # (both sides' sums of 8 in 32 bits, and exponentials: 2^-19 of the largest value)
+        assert ((got[:, h].float() - want).abs() <= half * want.abs() + 2.0 ** -19 * 5 + 2.0 ** -24).all(), h
+
+
 # ---------------------------------------------------------------------------------------------
 # groups
 # ---------------------------------------------------------------------------------------------
