@@ -12,6 +12,7 @@ front of that still read it.
 from __future__ import annotations
 
 import heapq
+from itertools import accumulate
 from typing import Dict, Hashable, Iterable, List, NamedTuple, Optional, Sequence, Tuple
 
 import numpy as np
@@ -304,7 +305,7 @@ class PagedKVCache:
         length = np.fromiter((0 if s is None else s.length for s in found), np.int64, rows)
         real = length > 0
         if tokens is None:
-            n, row, position = rows, slice(None), np.maximum(length - 1, 0)
+            n, position = rows, np.maximum(length - 1, 0)
         else:
             new = np.asarray(list(tokens), dtype=np.int64)
             if new.shape != (rows,) or (new < 0).any() or (new > length).any():
@@ -314,17 +315,18 @@ class PagedKVCache:
             position = (length - new - begin[:-1])[row] + np.arange(n)
         groups = min(rows, MAX_GROUPS) if prefix else 0
         parts = [2 * n, 2 * n, rows, rows * width] + ([rows + 1] if tokens is not None else []) + ([groups + 1, groups] if prefix else [])     # words
-        ends = np.cumsum(parts)
-        host = np.zeros(int(ends[-1]), dtype=np.int32)                               # one transfer for all of it
+        ends = list(accumulate(parts))
+        host = np.zeros(ends[-1], dtype=np.int32)                                    # one transfer for all of it
         pieces = [host[e - p:e] for e, p in zip(ends, parts)]
         place, slot = pieces[0].view(np.int64), pieces[1].view(np.int64)
         lengths, tables = pieces[2], pieces[3].reshape(rows, width)
-        page = self._rows[at[row], position // self.page_size]
-        mine = real[row] if tokens is None else np.ones(n, dtype=bool)
-        if any(self._users[p] > 1 for p in set(page[mine].tolist())):
+        page = self._rows[at if tokens is None else at[row], position // self.page_size]
+        if any([self._users[p] > 1 for p in (page[real].tolist() if tokens is None else set(page.tolist()))]):
             raise ValueError("a row's newest token lies in a page that other sequences hold too: extend makes it its own")
         place[:], lengths[:] = position, length
-        slot[:] = np.where(mine, page.astype(np.int64) * self.page_size + position % self.page_size, -1)
+        slot[:] = page.astype(np.int64) * self.page_size + position % self.page_size
+        if tokens is None:
+            slot[~real] = -1
         columns = np.arange(min(width, self.max_pages))
         inside = columns < -(-length // self.page_size)[:, None]
         tables[:, :len(columns)] = np.where(inside, self._rows[at, :len(columns)], 0)
@@ -341,7 +343,7 @@ class PagedKVCache:
             pieces[-2][:] = rows
             pieces[-2][:len(bounds[:groups + 1])], pieces[-1][:len(sizes[:groups])] = bounds[:groups + 1], sizes[:groups]
         dev = torch.from_numpy(host).to(self.pool.device)
-        made = [dev[e - p:e] for e, p in zip(ends.tolist(), parts)]
+        made = [dev[e - p:e] for e, p in zip(ends, parts)]
         made = PagedBatch(made[0].view(torch.int64), made[1].view(torch.int64), made[3].view(rows, width), made[2], shared,
                           made[4] if tokens is not None else None, made[-2] if prefix else None, made[-1] if prefix else None)
         if out is None:
@@ -349,7 +351,7 @@ class PagedKVCache:
         for to, t in zip((*out[:4], out.groups, out.prefixes), (*made[:4], made.groups, made.prefixes)):
             if t is not None:
                 to.copy_(t)
-        return out._replace(shared=made.shared)
+        return PagedBatch(*out[:4], made.shared, None, out.groups, out.prefixes)
 
     def _groups_of(self, tables: np.ndarray, used: np.ndarray) -> Tuple[List[int], List[int]]:
         """(rows where groups of neighbours begin and the last one ends, tokens that each group's rows have in common).  A row joins the group in front of
