@@ -383,3 +383,46 @@ def test_a_run_that_is_dropped_gives_its_sequences_back(monkeypatch):
     cache.free("a")
     cache.free("b")
     assert cache.free_pages == 200
+
+
+# ---------------------------------------------------------------------------------------------
+# tables
+# ---------------------------------------------------------------------------------------------
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [256, 257, 600, 1025, 1777])
+def test_steps_of_many_rows_over_their_inputs(dev, rows):
+    """A place a row, as a run steps: more than one workgroup, lengths and pages taken left to a launch of their own; by calls and by replays, until the
+    pages are at an end and nothing goes on."""
+    from deltazip_amd import TableStep, extend_tables, ops
+    rng = random.Random(rows)
+    ps, width, steps = 8, 8, 12
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)
+    lengths, counts = [rng.randrange(0, 40) for _ in range(rows)], [rng.choice([0, 1, 1, 1]) for _ in range(rows)]
+    tables = [[100000 + width * r + i if i < -(-n // ps) else -7 for i in range(width)] for r, n in enumerate(lengths)]
+    state, free = (tables, lengths, 0), rng.sample(range(90000), 2 * rows)
+    for _ in range(steps):
+        state = ref.extend_tables(state[0], state[1], counts, free, state[2], ps)
+    free = free[:state[2]]                             # (just enough for so many steps)
+    tab, ln, ct, fr, tk = (i32(x) for x in (tables, lengths, counts, free, [0]))
+    out = TableStep(ln, tk, torch.empty(rows + 1, dtype=torch.int32, device=dev), *torch.empty(2, rows, dtype=torch.int64, device=dev))
+    step = lambda: extend_tables(tab, ln, ct, fr, tk, ps, out=out)
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    state = ref.extend_tables(tables, lengths, counts, free, 0, ps)
+    for i in range(1, steps + 30):
+        assert tab.tolist() == state[0] and ln.tolist() == state[1] and tk.tolist() == [state[2]]
+        if i <= steps:
+            assert [out.starts.tolist(), out.positions.tolist(), out.slots.tolist()] == list(state[3:])
+        graph.replay() if i % 2 else step()
+        after = ref.extend_tables(state[0], state[1], counts, free, state[2], ps)
+        if after is None:
+            assert i >= steps and out.slots.tolist() == [-1] * rows and ln.tolist() == state[1] and tab.tolist() == state[0] and tk.tolist() == [state[2]]
+            with pytest.raises(ops.DeltaKernelError, match="paged"):
+                ops.poll_status(wait=True)
+            return
+        state = after
+    raise AssertionError("steps without an end")
