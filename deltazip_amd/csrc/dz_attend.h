@@ -252,6 +252,7 @@ struct Walk {
       }
       float ref = top == -INFINITY ? 0.0f : top - Ty::BIAS;
       if (Ty::BIAS != 0.0f && __builtin_expect(far, 0) && is_far(top)) {
+#pragma clang fp contract(off)
         ref = -Ty::BIAS;
 #pragma unroll
         for (int e = 0; e < 8; ++e) s[e] -= top;

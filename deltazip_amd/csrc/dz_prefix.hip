@@ -674,7 +674,7 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void dz_prefix_kernel(const P
           sum[n] *= f;
 #pragma unroll
           for (int j = 0; j < 2 * KC; ++j) acc[n][j] *= f;
-          ref[n] = up == -INFINITY ? 0.0f : Ty::BIAS - up;
+          ref[n] = up == -INFINITY ? 0.0f : Ty::BIAS - up, by[n] = scale;
           far |= __any(is_far(up));
           if (__builtin_expect(far, 0) && is_far(up)) {
             // (the maximum is a rounded product: the scores, too, before it is taken from them)

@@ -129,6 +129,24 @@ def test_scores_around_where_differences_are_taken_by_themselves(dev, dtype, tok
             assert (off <= bound).all(), float((off / bound).max())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens", [3, 40, 100, 300])
+@pytest.mark.parametrize("first,then", [(-30000.0, 0.0), (-4000.0, 3.0), (-50.0, 4000.0), (-20000.0, -3000.0), (-30000.0, 30000.0)])
+def test_scores_that_come_from_where_differences_are_taken_by_themselves(dev, dtype, tokens, first, then):
+    """The first 130 tokens' far below the others', whose differences are small: maxima pass the border within a piece."""
+    g = torch.Generator().manual_seed(3)
+    scores = torch.where(torch.arange(300) < 130, torch.tensor(first), torch.tensor(then))
+    p, behind, single = _one_sided(dev, dtype, tokens, scores, torch.randn(300, generator=g))
+    q, k, v, tables, lengths = p[:5]
+    want, size, most = ref.attention(q[:1], k, v, tables[:1], lengths[:1], 1.0)
+    most = torch.full_like(most, 2 * abs(then) + 20.0)             # (of the scores that count)
+    bound = ref.prefix_bound(want, size, most / 17, dtype, 64, 300, float(v.abs().max()))
+    for y in (behind(1.0), single(1.0)):
+        off = (y.double().cpu() - want).abs()
+        assert (off <= bound).all(), float((off / bound).max())
+
+
 SMALL = [([3], [3], [0], [0, 1]), ([4], [90], [0], [0, 1]), ([2] * 4, [2, 30, 2, 9], [64], [0, 4]), ([5, 1], [5, 1], [40], [0, 2]), ([1] * 8, [1, None, 7, 1, 3, None, 1, 90], [200], [0, 8])]
 LARGE = [([40, 3], [70, 9], [64], [0, 2]), ([200], [200], [0], [0, 1]), ([20] * 9, [20] * 9, [128], [0, 9])]
 
