@@ -17,7 +17,7 @@
 // Measured (keys and values over the time of a call among others): 128 rows of 1025 tokens of 32 key heads of 128 325 us, 6.6 TB/s;
 // 32 of 1024 84 us, 6.4; one of 131071 tokens of 8 94 us, 5.7, of which 76 at the rate of a kernel that only reads (7.1 TB/s with
 // loads that keep nothing in the caches, 6.2 with others; a copy moves 4.9 to 5.4); one of 17 tokens 5 us, of which an empty
-// launch takes 2.5.  32 rows of 1024 tokens of 16 key heads of 256 93 us, 5.8 TB/s; of 200 205 us, 2.0: the form of heads of 200 to 248 takes
+// launch takes 2.5.  32 rows of 1024 tokens of 16 key heads of 256 89 us, 6.0 TB/s; of 200 185 us, 2.3: the form of heads of 200 to 248 takes
 // more than half of the registers, so one wavefront a SIMD asks for keys no step ahead.  A compute unit has some 64 KB on their way at most, which at 2 us is 30 GB/s: what long
 // rows lose is the uneven ends of their parts (63 to 86 us) and the two joins (9 us).
 #include <hip/hip_runtime.h>

@@ -21,10 +21,11 @@
 // value, times 2^14 in fp16.  Outputs are then 2.0e-3 to 2.1e-3 (bf16) off in the root mean square where their own rounding is 1.65e-3, 2.2e-4 and 2.0e-4 in fp16.
 //
 // What bounds it: reading keys and values once up to some 180 queries a key, the matrix cores above.  Measured, a pass among others:
-//   a prompt of 8192 tokens of 32 heads of 128, 8 key heads     555 us, 990 TFLOP/s (a library product of 8192^3 1171 to 1220)
+//   a prompt of 8192 tokens of 32 heads of 128, 8 key heads     573 to 591 us from one card to another, 930 to 960 TFLOP/s (a library product of 8192^3
+//                                                               1171 to 1220)
 //   16 rows behind 131072 tokens of 8 key heads                 119 us, 4.7 TB/s; 5.8 while all workgroups read
 //   128 rows in 4 groups behind 4096 tokens of 32 key heads     230 us, 5.9 TB/s
-//   203 rows of 64 heads in 3 groups behind 20000 of 8          359 us, 4.0 TB/s and 376 TFLOP/s: neither one's bound; a compute unit's two workgroups are
+//   203 rows of 64 heads in 3 groups behind 20000 of 8          365 us, 3.9 TB/s and 376 TFLOP/s: neither one's bound; a compute unit's two workgroups are
 //                                                               too few to wait for memory and to multiply at the same time
 //   32 rows behind 2048 of 32                                   31 us: plan 5, pieces 22 (a piece takes 14: memory is waited for in turn), join 5
 // What did not pay: the exponentials of 32 tokens beside the products of the next 32 (more instructions, 560 -> 621 us for 8192 tokens) or of one
@@ -253,7 +254,8 @@ struct Planner {
     return x.tiles ? (x.n - x.k0 + most - 1) / most : 0;
   }
 
-  // (queries that see as much as each other: 32 rows of up to 200 tokens of their own 34 -> 32 us; 48 of several new ones 34 -> 42)
+  // (queries that see as much as each other: 32 rows of up to 200 tokens of their own 34 -> 32 us.  Of several new tokens it goes by how unlike the rows are: 48 of up
+  // to 333 tokens of their own 34 -> 42, 64 of 3 behind their 200 each 55 -> 58, 32 of 128 31 -> 31, but 64 of 2 of 64 37 -> 33, 128 of 32 57 -> 38)
   __device__ __forceinline__ bool is_short(const Unit& x) const { return few(x) && x.np == 1 && x.n - x.k0 <= SHORT && (x.ntok == 1 || !x.causal); }
 
   // The pieces of this thread's unit, of the next N of them: its items (those of short units in a list of their own) end at what is returned, its
@@ -990,8 +992,9 @@ int dz_prefix_attention(const dz_prefix_args* a, void* stream) {
   else
     hipLaunchKernelGGL((dz_prefix_plan_kernel<1024, false>), dim3(1), dim3(1024), 0, st, P);
   hipLaunchKernelGGL(kern, dim3((unsigned)line, (unsigned)lines), dim3(256), lds, st, P);
-  // of few outputs the pieces, too, are shared out (16 rows of 40 heads in 60 pieces 128 -> 119 us; 144 tokens of 20 in 4 32 -> 34); of many tokens, most of which
-  // are stored already, a workgroup takes more of the heads
+  // of few outputs the pieces, too, are shared out (without and with, heads of 128: 16 rows of 40 behind 131072 tokens 128 and 119 us; of 32, 4 behind 65536 102 and
+  // 73, 8 behind 4096 28.8 and 26.6, 31 behind 2048 26.4 and 26.2; 32 25.9 and 26.3, 64 34.9 and 37.3, 128 behind 4096 52 and 57, 128 behind 32768 of 8 key heads
+  // 104 and 107; but 32 behind 32768 of 8 54 and 49: many pieces are what it misses); of many tokens, most of which are stored already, a workgroup takes more of the heads
   const long long values = (long long)a->tokens * a->heads * (a->dim / 4);
   const bool few = values < (1 << 15);
   const long long sets = ((long long)a->heads * (a->dim / 4) * (few ? 8 : 1) + 255) / 256, most = 1 + 2048 / a->tokens;

@@ -37,8 +37,11 @@ _EXTEND = struct.Struct("=q11Qq6i")               # dz_extend_args
 MAX_DIM = 256
 COUNTERS = 32768                  # DZ_ATTENTION_COUNTERS
 MAX_GROUPS = 2048                 # DZ_PREFIX_GROUPS
-# Bytes of keys and values that all rows' tables have room for, up to which a call of one new token a row goes row by row: 4 rows of 292 tokens of 32 key
-# heads (20 MB) 8 us and 16 behind their prefix, 32 of 1124 of 8 (149) 22 and 23, 16 of 612 of 32 (164) 26 and 20, 8 of 2148 (283) 28 and 21.
+# Bytes of keys and values that all rows' tables have room for, up to which a call of one new token a row goes row by row.  Row by row and behind the prefix, us, where most of the
+# tokens are shared: 4 rows of 32 key heads 15.3 and 16.2 at 71 MB, 19.4 and 18.6 at 138, 28 and 24 at 273; 8 of 32 16.5 and 16.8 at 109, 18.8 and 17.3 at 143; 16 of 32 10.5 and
+# 21.5 at 71, 21.4 and 18.1 at 117, 25.7 and 20.1 at 164; 32 of 32 14.1 and 17.3 at 117, 17.8 and 18.8 at 151, 29 and 21 at 302; 32 of 8 20.5 and 22.2 at 115, 27.6 and 24.0 at 216; 64 of
+# 8 10.7 and 22.5 at 75, 25.5 and 21.8 at 109.  The host knows the tables' room, not the lengths: tables of twice the pages that rows of 272 tokens use, 16 of 32, take 21.6 at
+# 143 where row by row is 11.1; and of rows that share little (64 of 576 tokens) row by row is the faster one everywhere (151 MB 29 and 35, 285 47 and 56).
 ROW_BY_ROW = 128 << 20
 
 
@@ -441,7 +444,8 @@ class TableStep(NamedTuple):
 
 def extend_tables(block_tables: torch.Tensor, lengths: torch.Tensor, counts: torch.Tensor, free_pages: torch.Tensor, taken: torch.Tensor,
                   page_size: int, tokens: Optional[int] = None, out: Optional[TableStep] = None) -> TableStep:
-    """Room for the tokens that rows get next, made on the device: what `PagedKVCache.extend` and `batch` do on the host.
+    """Room for the tokens that rows get next, made on the device: what `PagedKVCache.extend` and `batch` do on the host.  (Every workgroup adds up all
+    rows: 8 us for 4096 of them, 0.12 ms for 65536, 27 ms for the most, 2^20.)
 
     Row r has lengths[r] tokens and gets counts[r] more (int32 [rows]); the pages that it needs for them are the next of
     free_pages (int32 [n]) behind the first taken[0] (int32 [1]), in the order of the rows, and are written into its row of block_tables
