@@ -1,13 +1,24 @@
 // What the attention kernels over a paged cache share: element types, sums over a wavefront, the joining of pieces.
 #pragma once
 #include <hip/hip_runtime.h>
+#include <pthread.h>
 #include <stdint.h>
 
 #include <type_traits>
 
 #include "dz_device.h"
 
+extern __attribute__((visibility("hidden"))) pthread_mutex_t dz_attention_launches;
+
 namespace {
+
+// Held while a call of attention launches: room for plans and parts is a stream's, so that nothing that another thread launches on that stream may come
+// between the launches of a call.
+struct Launches {
+  Launches() { pthread_mutex_lock(&dz_attention_launches); }
+  ~Launches() { pthread_mutex_unlock(&dz_attention_launches); }
+  Launches(const Launches&) = delete;
+};
 
 typedef float f2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 b8_t __attribute__((ext_vector_type(8)));

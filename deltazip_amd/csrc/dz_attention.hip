@@ -28,6 +28,8 @@
 #include "../../include/dz_amd.h"
 #include "dz_attend.h"
 
+pthread_mutex_t dz_attention_launches = PTHREAD_MUTEX_INITIALIZER;
+
 namespace {
 
 constexpr int WAVES = 4;               // wavefronts of a workgroup
@@ -444,6 +446,7 @@ int dz_paged_attention(const dz_attention_args* a, void* stream) {
   if (lds > 65536 && !dz_lds_limit_once(attr_done[which], (const void*)kern, (int)LDS_MOST)) return DZ_ELAUNCH;
   const hipStream_t st = (hipStream_t)stream;
   const int together = group_rows(items);
+  const Launches held;
   for (long long row = 0; row < a->rows; row += together) {
     P.rows = a->rows - row < together ? (int)(a->rows - row) : together;
     P.q = (const char*)a->q + row * P.q_row;

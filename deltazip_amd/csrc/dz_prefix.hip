@@ -983,6 +983,7 @@ int dz_prefix_attention(const dz_prefix_args* a, void* stream) {
   if (lds > 65536 && !dz_lds_limit_once(attr_done[which], (const void*)kern, (int)lds)) return DZ_ELAUNCH;
   const hipStream_t st = (hipStream_t)stream;
   const int units = m.parts < (1ll << 31) ? a->rows + a->groups_n : 1 << 30;
+  const Launches held;
   if (units <= 64)
     hipLaunchKernelGGL((dz_prefix_plan_kernel<64, true>), dim3(1), dim3(64), 0, st, P);
   else if (units <= 256)

@@ -513,7 +513,8 @@ int dz_paged_attention(const dz_attention_args* args, void* stream);
  * the first new token of each sees), which are read through the table of the first of them that has tokens.  groups_n 0: nothing is shared.
  * Tokens of no row, and those that see nothing, give zeros; lengths, tables and pages as in dz_paged_attention.  Starts that do
  * not rise from 0 or more to `tokens` or less leave no row any token, groups that do not rise within the rows share nothing; either
- * sets bit 2 of *status.  work: dz_prefix_attention_bytes() bytes, any contents, that no call overlapping in time uses.  rows <= 2^20,
+ * sets bit 2 of *status.  work: dz_prefix_attention_bytes() bytes, any contents, that no call overlapping in time uses (calls on
+ * one stream, of dz_paged_attention too, launch one after the other, whichever threads make them).  rows <= 2^20,
  * groups_n <= DZ_PREFIX_GROUPS, tokens * heads < 2^31. */
 typedef struct dz_prefix_args {
   int64_t bytes;

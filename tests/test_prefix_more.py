@@ -253,6 +253,34 @@ def test_more_workgroups_than_a_line_of_a_grid_has(dev):
         assert ((got[:, h].float() - want).abs() <= half * want.abs() + 2.0 ** -19 * 5 + 2.0 ** -24).all(), h
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("into", [False, True])
+def test_calls_of_several_threads_on_one_stream(dev, into):
+    """Plans, sums and joins of a call lie in the stream's room: no other's launch may come between them."""
+    import threading
+    from deltazip_amd import paged_attention
+    few = _problem(dev, torch.float16, [600], [30] * 5, [1] * 5, [0, 5], 4, 2, 64, 16, seed=1)
+    many = _problem(dev, torch.float16, [40, 900], [9] * 300, [2] * 300, [0, 200, 300], 8, 2, 64, 16, seed=2)
+    long = _problem(dev, torch.float16, [0], [9000] * 3, [1] * 3, [0, 3], 8, 2, 64, 16, seed=3)
+    calls = [lambda out: _run(few, out=out), lambda out: _run(many, out=out), lambda out: paged_attention(*long[:5], out=out)]
+    want = [call(None) for call in calls]
+    stream, got = torch.cuda.Stream(), [[] for _ in calls]
+    torch.cuda.synchronize()
+
+    def repeat(call, like, kept):
+        with torch.cuda.stream(stream):
+            for _ in range(150):
+                kept.append(call(torch.empty_like(like) if into else None))
+
+    threads = [threading.Thread(target=repeat, args=x) for x in zip(calls, want, got)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert all(len(kept) == 150 and all(torch.equal(x, w) for x in kept) for kept, w in zip(got, want))
+
+
 # ---------------------------------------------------------------------------------------------
 # groups
 # ---------------------------------------------------------------------------------------------
